@@ -505,6 +505,83 @@ int sn_rotary_kv_append(const void *qkv, void *q, void *k_cache, void *v_cache, 
                         int batch, int nheads, int nheads_kv, int head_dim, int max_seqlen, int pos, void *stream);
 int sn_swiglu(const void *h, void *y, int batch, int d, void *stream);
 
+/*
+ * Mamba2 over prompts: the causal convolution and the selective state space
+ * scan of ragged prompts, the many-token form of sn_mamba2_split_conv +
+ * sn_selective_state_update (no counterpart kernel in the reference, whose
+ * prompts run inside the mamba_ssm library).  zxbcdt [tokens, ld]: the
+ * in_proj rows [z | x B C | dt] of all prompts, packed; prompt i holds rows
+ * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32 [batch + 1] on the device;
+ * NULL: one prompt of all tokens, batch 1; empty prompts are fine).
+ *   xBC_t = SiLU(conv_bias + sum_k conv_weight[d, k] u_{t - d_conv + 1 + k}[d])
+ *   dt_t  = softplus(dt + dt_bias)
+ *   S_t   = exp(dt_t A) S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t + D x_t
+ * and y_t *= SiLU(z_t) when gate.  conv_state [batch, conv_dim, d_conv] and
+ * ssm_state [batch, nheads, headdim, d_state] hold each prompt's state before
+ * its first token (zeros for a new stream) and are left as the state after
+ * its last one, so a prompt may be taken in pieces.  A fp32 [nheads]; D and
+ * dt_bias bf16 [nheads] or NULL; y [tokens, nheads, headdim].  d_conv <= 8,
+ * d_state <= 256.  workspace: sn_mamba2_prompt_workspace_size bytes, free to
+ * reuse when the call's work on the stream is done.
+ */
+size_t sn_mamba2_prompt_workspace_size(int tokens, int batch, int d_inner, int ngroups, int d_state, int nheads);
+int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const void *conv_weight,
+                     const void *conv_bias, void *ssm_state, const float *A, const void *D, const void *dt_bias,
+                     void *y, const int *cu_seqlens, int batch, int tokens, int d_inner, int ngroups, int d_state,
+                     int nheads, int headdim, int d_conv, int gate, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
+/*
+ * Paged KV cache (no counterpart in the reference, whose cache is one dense
+ * tensor at one position).  k_pages / v_pages: bf16 [num_pages, nheads_kv,
+ * page_size, head_dim] given by page, head and token strides (elements, the
+ * last axis dense).  page_table int32 [batch, max_pages] (row stride
+ * table_stride): the page of each block of page_size positions.  seq_lens
+ * int32 [batch].  All three are on the device.  A page or length out of range
+ * is skipped (clamped) and recorded as SN_ERR_INVALID_ARGUMENT in the device
+ * status word.
+ *
+ * sn_rotary_paged_append: qkv [tokens, ld] = [q | k | v] rows of the new
+ * tokens; stream b's are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (NULL:
+ * one token a stream) and end at position seq_lens[b] - 1 (seq_lens counts
+ * them).  The first rot_dim elements of every q and k head are rotated by
+ * the table row of the token's position (cos, sin fp32 [max_pos, rot_dim /
+ * 2]): pairs (j, j + rot_dim / 2), or (2j, 2j + 1) when interleaved.  q goes
+ * to q [tokens, nheads, head_dim], k and v to their pages.  Products and
+ * sums in fp32, rounded separately, as sn_rotary_kv_append.
+ *
+ * sn_paged_decode_attention: out[b, h] = sum_t softmax_t(scale q[b, h] .
+ * k[t]) v[t] over the stream's positions t < seq_lens[b]; nheads / nheads_kv
+ * query heads share a key/value head.  q [batch, nheads, head_dim] by batch
+ * and head strides, out dense; lse fp32 [batch, nheads] (log of the sum of
+ * exponentials, -inf for an empty stream) or NULL.  An empty stream gives
+ * zeros.  head_dim <= 256.  workspace: sn_paged_decode_workspace_size bytes,
+ * 16-byte aligned, zero before the first call and left ready for the next;
+ * calls that share it must not overlap.
+ *
+ * sn_copy_pages: page dst[i] = page src[i] (i < pairs, int32 on the device)
+ * for each of `outer` pools outer_stride_bytes apart (layers, and k and v);
+ * a page is page_bytes dense bytes, page_stride_bytes apart.  No page may be
+ * both copied from and copied to in one call, nor copied to twice.
+ */
+int sn_rotary_paged_append(const void *qkv, int64_t ld, void *q, void *k_pages, int64_t k_page_stride,
+                           int64_t k_head_stride, int64_t k_tok_stride, void *v_pages, int64_t v_page_stride,
+                           int64_t v_head_stride, int64_t v_tok_stride, int num_pages, int page_size,
+                           const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens,
+                           const int *cu_seqlens, const float *cos, const float *sin, int max_pos, int tokens,
+                           int batch, int nheads, int nheads_kv, int head_dim, int rot_dim, int interleaved,
+                           void *stream);
+size_t sn_paged_decode_workspace_size(int batch, int nheads, int head_dim);
+int sn_paged_decode_attention(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_pages,
+                              int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
+                              const void *v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                              int64_t v_tok_stride, int num_pages, int page_size, const int *page_table,
+                              int64_t table_stride, int max_pages, const int *seq_lens, void *out, float *lse,
+                              float scale, int batch, int nheads, int nheads_kv, int head_dim, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_bytes, int64_t page_bytes, int outer,
+                  int num_pages, const int *src, const int *dst, int pairs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,6 +72,14 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "sn_mamba2_conv_ssu": ([_P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P], _I),
     "sn_rotary_kv_append": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
     "sn_swiglu": ([_P, _P, _I, _I, _P], _I),
+    "sn_mamba2_prompt_workspace_size": ([_I] * 6, ctypes.c_size_t),
+    "sn_mamba2_prompt": ([_P, _I64] + [_P] * 9 + [_I] * 9 + [_P, ctypes.c_size_t, _P], _I),
+    "sn_rotary_paged_append": ([_P, _I64, _P] + [_P, _I64, _I64, _I64] * 2 + [_I, _I, _P, _I64, _I, _P, _P, _P, _P]
+                               + [_I] * 8 + [_P], _I),
+    "sn_paged_decode_workspace_size": ([_I, _I, _I], ctypes.c_size_t),
+    "sn_paged_decode_attention": ([_P, _I64, _I64] + [_P, _I64, _I64, _I64] * 2 + [_I, _I, _P, _I64, _I, _P, _P, _P,
+                                  ctypes.c_float, _I, _I, _I, _I, _P, ctypes.c_size_t, _P], _I),
+    "sn_copy_pages": ([_P, _I64, _I64, _I64, _I, _I, _P, _P, _I, _P], _I),
     "sn_snake1d": ([_P, _P, _P, _I, _I, _I64, ctypes.c_float, _P], _I),
     "sn_diag_bounded_wait": ([ctypes.c_uint64, _P], _I),
     "sn_snake_conv_transpose1d_pack": ([_P, _I, _I, _I, _I, _P, ctypes.c_size_t, _P], _I),

@@ -22,6 +22,8 @@ __global__ void bounded_wait_probe_kernel(uint64_t limit_ns) {
 int tu_status_gemv(bool reset, cudaStream_t st, int* out);
 int tu_status_bmm(bool reset, cudaStream_t st, int* out);
 int tu_status_snake(bool reset, cudaStream_t st, int* out);
+int tu_status_paged(bool reset, cudaStream_t st, int* out);
+int tu_status_prompt(bool reset, cudaStream_t st, int* out);
 }  // namespace sn
 
 extern "C" {
@@ -29,7 +31,7 @@ extern "C" {
 int sn_device_status(int reset, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int (*units[])(bool, cudaStream_t, int*) = {sn::tu_status_gemv, sn::tu_status_bmm, sn::tu_status_snake,
-                                              sn::read_tu_status};
+                                              sn::tu_status_paged, sn::tu_status_prompt, sn::read_tu_status};
   int first = SN_OK;
   for (auto f : units) {
     int v = SN_OK;

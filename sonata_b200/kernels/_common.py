@@ -1,6 +1,8 @@
 """Tensor / stream plumbing shared by the kernel wrappers."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .. import _lib
@@ -18,6 +20,27 @@ def stream_handle(stream=None) -> int:
     if h is not None:
         return int(h)
     raise TypeError(f"cannot interpret {type(stream).__name__} as a CUDA stream")
+
+
+@contextlib.contextmanager
+def on_stream(stream=None):
+    """Makes `stream` (as stream_handle takes it) torch's current stream, so
+    that what a wrapper allocates belongs to the stream its kernels run on,
+    and yields the raw handle."""
+    h = stream_handle(stream)
+    if stream is None or h == torch.cuda.current_stream().cuda_stream:
+        yield h
+        return
+    with torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(h)):
+        yield h
+
+
+def same_device(**tensors) -> None:
+    """Every given tensor (or None) is on torch's current CUDA device, where the kernels launch."""
+    cur = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.device.index != cur:
+            raise ValueError(f"{name} is on {t.device}, but the current CUDA device is cuda:{cur}")
 
 
 def require_cuda(name: str, t: torch.Tensor, dtype=None, dim=None) -> None:
