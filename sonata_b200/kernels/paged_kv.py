@@ -149,7 +149,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     with on_stream(stream) as st:
         out = torch.empty(batch, nheads, hd, device=q.device, dtype=_BF16)
         lse = torch.empty(batch, nheads, device=q.device, dtype=torch.float32) if return_lse else None
-        ws = workspace if workspace is not None else torch.zeros(need, device=q.device, dtype=torch.uint8)
+        ws = workspace
+        if ws is None:  # only the arrival counters at its start have to be zero
+            ws = torch.empty(need, device=q.device, dtype=torch.uint8)
+            ws[:4 * batch * nheads].zero_()
         call("sn_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), *args, out.data_ptr(),
              lse.data_ptr() if return_lse else None, float(hd ** -0.5 if scale is None else scale), batch, nheads, hkv,
              hd, ws.data_ptr(), ws.numel(), st)
