@@ -13,8 +13,11 @@
 // offsets are on the device, so every CTA finds its own prompt.  Offsets out
 // of [0, tokens] or falling are clamped and recorded as
 // SN_ERR_INVALID_ARGUMENT in the status word.
-#include "common.cuh"
+#include "tc.cuh"
 
+#include <cuda_fp16.h>
+
+#include <algorithm>
 #include <climits>
 
 namespace sn {
@@ -34,22 +37,35 @@ struct PromptBlock {
   int blocks;  // blocks of the prompt
 };
 
+// Tokens [s, e) of prompt b0 + lane (empty past the last), called by whole
+// warps for b0 = 0, 32, ... in turn with `upto` = 0 before the first.  Offsets
+// are clamped and never fall, so that prompts cannot overlap whatever the
+// tensor holds; true when they had to be changed.
+__device__ __forceinline__ bool prompt_bounds(const Prompts& p, int b0, int& upto, int& s, int& e) {
+  const int lane = threadIdx.x & 31, b = b0 + lane;
+  const bool on = b < p.batch;
+  const int s0 = on && p.cu ? p.cu[b] : 0, e0 = !on ? 0 : p.cu ? p.cu[b + 1] : p.tokens;
+  s = max(min(max(s0, 0), p.tokens), upto);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s = max(s, v);
+  }
+  e = max(min(e0, p.tokens), s);
+  upto = __shfl_sync(0xffffffffu, e, 31);
+  return on && (s != s0 || e != e0);
+}
+
 // The index-th block, where every prompt is cut into blocks of `rows` tokens
 // (at least `least` of them, so that an empty prompt still has one where its
 // state has to be handled).  Called by whole warps; every lane gets the answer.
 __device__ __forceinline__ PromptBlock find_block(const Prompts& p, int rows, int least, int index) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
+  int before = 0, last = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int b = b0 + lane;
-    int s = 0, e = 0, n = 0;
-    if (b < p.batch) {
-      const int s0 = p.cu ? p.cu[b] : 0, e0 = p.cu ? p.cu[b + 1] : p.tokens;
-      s = min(max(s0, 0), p.tokens);
-      e = min(max(e0, s), p.tokens);
-      if (s != s0 || e != e0) record_status(SN_ERR_INVALID_ARGUMENT);
-      n = max((e - s + rows - 1) / rows, least);
-    }
+    int s, e;
+    if (prompt_bounds(p, b0, last, s, e)) record_status(SN_ERR_INVALID_ARGUMENT);
+    const int n = b0 + lane < p.batch ? max((e - s + rows - 1) / rows, least) : 0;
     int upto = n;  // inclusive scan over the warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -214,6 +230,782 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
   }
 }
 
+// ---------------------------------------------------------------------------
+// The tensor-core form: headdim 64, d_state 128, convolution widths 2 to 4.
+//
+// Mathematics.  In a chunk of L = 128 tokens, with a_i = sum_{k <= i} dt_k A
+// counted from the chunk's start,
+//   Y = M X + diag(exp a_i) C S_in,   M_ij = (C B^T)_ij exp(a_i - a_j) dt_j  (j <= i)
+//   S_out = exp(a_L) S_in + sum_j exp(a_L - a_j) dt_j B_j (x) x_j
+// so a chunk is four products of 128 rows: C B^T, shared by the heads of a
+// group, then C S, M X and B^T (w x) of each head; only the states go from
+// chunk to chunk.  A long prompt is cut into segments of whole chunks: one
+// launch finds each segment's own contribution to the state, the next joins
+// those before a segment and does its outputs.
+//
+// Numbers.  The products are kind::f16 with fp32 accumulators.  Operands in
+// fp16 (11 significant bits) instead of bf16 (8) keep their roundings below
+// that of the bf16 results; their range is kept by exact powers of two: every
+// 128-channel block of a chunk (x of two heads, B, C) is scaled to below 2,
+// dt to below 2 by its largest value, and the state operand by a bound of the
+// state carried along with it.  States and sums stay in fp32.
+//
+// Layout.  The convolution writes its results as the shared-memory images the
+// products read (128-byte swizzle, 128 tokens by 64 channels, 16 KB), padded
+// with zero rows to whole chunks of a prompt, so a chunk's operands come in
+// three bulk copies and no product sees another prompt's tokens.
+// ---------------------------------------------------------------------------
+constexpr int kChunk = 128;
+constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 64 channels of fp16
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ChunkWork {  // workspace arrays; chunks are counted over all prompts
+  unsigned char* x;  // [chunks][nh] tiles
+  unsigned char* b;  // [chunks][ng] pairs of tiles (128 states)
+  unsigned char* c;  // [chunks][ng] pairs of tiles
+  float* cum;        // [chunks][nh][128] cumulative dt A / ln 2
+  float* dt;         // [chunks][nh][128], 0 past the prompt's end
+  float2* meta;      // [chunks][nh] largest dt; sum of dt exp(a_L - a_j)
+  float* scale;      // [chunks][blocks] power of two of each 128-channel block
+  float* state;      // [slots][nh][64][128] see prompt_scan_mma_kernel
+  float* total;      // [slots][nh] sum of dt A / ln 2 over a segment
+  int xblocks, blocks;  // 128-channel blocks of x; of x, B and C together
+  int seg;              // chunks a segment
+};
+
+// The power of two at or below |v| (at least 2^-24); 1 for 0, infinities and NaN.
+__device__ __forceinline__ float pow2_floor(float v) {
+  const uint32_t e = (__float_as_uint(v) >> 23) & 255u;
+  return e == 0 || e == 255 ? 1.f : __uint_as_float(max(e, 127u - 24u) << 23);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// One 128-channel block of one chunk (blockIdx.x < blocks), or the chunk's dt
+// and decays (blockIdx.x == blocks).  Thread: 8 channels, 8 tokens.
+template <int W>
+__global__ void __launch_bounds__(256) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+  __shared__ float s_dt[64 * 129];
+  __shared__ float s_max[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int conv_dim = p.di + 2 * p.gds;
+  const int blk = blockIdx.x;
+  // this thread's channels, tokens and weights (the weights are the layer's: no need to wait for them)
+  const int c8 = tid & 15, r0 = (tid >> 4) * 8;
+  int d = blk * 128 + c8 * 8;  // channel of the convolution
+  if (blk >= wk.xblocks) d = p.di + (blk - wk.xblocks) * 128 + c8 * 8;
+  const bool on = blk < wk.xblocks ? d < p.di : blk < wk.blocks;
+  float w[8][W], bias[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PromptBlock pb = find_block(p.prompts, kChunk, 0, blockIdx.y);
+  if (pb.seq < 0) return;
+  const int t0 = pb.block * kChunk;
+  const int64_t chunk = blockIdx.y;
+
+  if (blk == wk.blocks) {  // dt and decays: 64 heads at a time
+    for (int h0 = 0; h0 < p.nh; h0 += 64) {
+      const int64_t at = 2 * static_cast<int64_t>(p.di) + 2 * p.gds + h0;
+      for (int e = tid; e < 64 * kChunk; e += 256) {
+        const int h = e & 63, r = e >> 6;
+        float v = 0.f;
+        if (h0 + h < p.nh && t0 + r < pb.len) {
+          v = __bfloat162float(p.zx[(pb.start + t0 + r) * p.ld + at + h]);
+          if (p.dt_bias) v += __bfloat162float(p.dt_bias[h0 + h]);
+          v = v <= 20.f ? log1pf(expf(v)) : v;
+        }
+        s_dt[h * 129 + r] = v;
+      }
+      __syncthreads();
+      for (int h = warp; h < 64 && h0 + h < p.nh; h += 8) {
+        const float a2 = p.A[h0 + h] * kLog2e;
+        float v[4], c[4], run = 0.f, top = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = s_dt[h * 129 + lane * 4 + k];
+          run = fmaf(v[k], a2, run);
+          c[k] = run;
+          top = fmaxf(top, v[k]);
+        }
+        float upto = run;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float u = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += u;
+        }
+        const float before = upto - run, all = __shfl_sync(0xffffffffu, upto, 31);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          c[k] += before;
+          sum = fmaf(v[k], exp2_approx(all - c[k]), sum);
+        }
+        if (lane == 31) c[3] = all;  // the state's decay and the last token's are the same number
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int64_t row = chunk * p.nh + h0 + h;
+        reinterpret_cast<float4*>(wk.cum + row * kChunk)[lane] = make_float4(c[0], c[1], c[2], c[3]);
+        reinterpret_cast<float4*>(wk.dt + row * kChunk)[lane] = make_float4(v[0], v[1], v[2], v[3]);
+        if (lane == 0) wk.meta[row] = make_float2(top, sum);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+
+  float top = 0.f;
+  float out[8][8];  // [token][channel]
+  if (on) {
+    const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
+    __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
+    uint4 raw[W + 7];  // inputs t0 + r0 - W + 1 .. t0 + r0 + 7
+#pragma unroll
+    for (int k = 0; k < W + 7; ++k) {
+      const int t = t0 + r0 + k - (W - 1);
+      raw[k] = make_uint4(0, 0, 0, 0);
+      if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u + t * p.ld);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      bias[c] = p.bias ? __bfloat162float(p.bias[d + c]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[c][k] = __bfloat162float(p.w[static_cast<int64_t>(d + c) * W + k]);
+    }
+    if (t0 + r0 == 0) {  // the prompt's first tokens: inputs before them are the state's columns 1 .. W - 1
+      __nv_bfloat16 old[8][W], moved[8][W];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) old[c][k] = st[c * W + k];
+      }
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k) {
+        uint32_t v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          v[c] = static_cast<uint32_t>(__bfloat16_as_ushort(old[2 * c][k + 1])) |
+                 static_cast<uint32_t>(__bfloat16_as_ushort(old[2 * c + 1][k + 1])) << 16;
+        raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      // and the state after the prompt, its last W inputs (only this thread reads or writes these channels' state)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          const int t = pb.len - W + k;  // < 0: the old state's column W + t = k + len
+          __nv_bfloat16 v = t >= 0 ? u[t * p.ld + c] : old[c][W - 1];
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (t < 0 && j == pb.len + k) v = old[c][j];
+          moved[c][k] = v;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) st[c * W + k] = moved[c][k];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const bool live = t0 + r0 + r < pb.len;
+      float acc[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] = bias[c];
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint32_t v[4] = {raw[r + k].x, raw[r + k].y, raw[r + k].z, raw[r + k].w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          acc[2 * c] = fmaf(bf16lo(v[c]), w[2 * c][k], acc[2 * c]);
+          acc[2 * c + 1] = fmaf(bf16hi(v[c]), w[2 * c + 1][k], acc[2 * c + 1]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        out[r][c] = live ? __fdividef(acc[c], 1.f + __expf(-acc[c])) : 0.f;
+        top = fmaxf(top, fabsf(out[r][c]));
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_max[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, s_max[k]);
+  const float sc = pow2_floor(top);
+  if (tid == 0) wk.scale[chunk * wk.blocks + blk] = sc;
+  if (!on) return;
+  const float inv = 1.f / sc;  // exact
+  // tile of these channels, chunk c8 % 8 of its rows
+  unsigned char* tile;
+  if (blk < wk.xblocks) {
+    tile = wk.x + (chunk * p.nh + blk * 2 + (c8 >> 3)) * kTileBytes;
+  } else {
+    const int g = blk - wk.xblocks;
+    tile = (g < p.ng ? wk.b + (chunk * p.ng + g) * 2 * kTileBytes : wk.c + (chunk * p.ng + g - p.ng) * 2 * kTileBytes) +
+           (c8 >> 3) * kTileBytes;
+  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const int row = r0 + r;  // row % 8 == r
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((c8 & 7) ^ r) << 4)) =
+        make_uint4(pack_f16(out[r][0] * inv, out[r][1] * inv), pack_f16(out[r][2] * inv, out[r][3] * inv),
+                   pack_f16(out[r][4] * inv, out[r][5] * inv), pack_f16(out[r][6] * inv, out[r][7] * inv));
+  }
+}
+
+// ---- tcgen05 pieces of this kernel ----
+// Operand whose rows run along the contraction (K): 64 elements of the other
+// axis a 128-byte row, 8-row groups 1024 bytes apart, the next 64 elements of
+// that axis `next` bytes on.
+__device__ __forceinline__ uint64_t desc_k_rows(uint32_t addr, uint32_t next) {
+  uint64_t d = 0;
+  d |= (static_cast<uint64_t>(addr) >> 4) & 0x3FFFull;
+  d |= static_cast<uint64_t>(next >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
+  return d;
+}
+// kind::f16, fp16 operands, fp32 accumulator; a_k_rows / b_k_rows: the operand is laid out as above.
+constexpr uint32_t idesc_f16(int M, int N, bool a_k_rows, bool b_k_rows) {
+  return (1u << 4) | (a_k_rows ? 1u << 15 : 0u) | (b_k_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+// The same product with A in tensor memory (two fp16 a column).
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  uint32_t lo[16], hi[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    lo[i] = __float_as_uint(v[i]);
+    hi[i] = __float_as_uint(v[16 + i]);
+  }
+  tmem_st16(taddr, lo);
+  tmem_st16(taddr + 16, hi);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+struct Segment {
+  int seq, start, len, index, count;  // prompt, its tokens; segment of it, of how many
+  int chunk0;                         // the prompt's first chunk, over all prompts
+  int slot0;                          // its first state slot (prompts of several segments have one a segment)
+};
+__device__ __forceinline__ Segment find_segment(const Prompts& p, int seg, int index) {
+  const int lane = threadIdx.x & 31;
+  int before = 0, chunks = 0, slots = 0, last = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    int s, e;
+    prompt_bounds(p, b0, last, s, e);
+    const int nc = (e - s + kChunk - 1) / kChunk;
+    const int n = (nc + seg - 1) / seg, ns = n > 1 ? n : 0;
+    int u = n, uc = nc, us = ns;  // inclusive scans
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, u, o), vc = __shfl_up_sync(0xffffffffu, uc, o);
+      const int vs = __shfl_up_sync(0xffffffffu, us, o);
+      if (lane >= o) {
+        u += v;
+        uc += vc;
+        us += vs;
+      }
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, index - before < u && n > 0);
+    if (here) {
+      const int l = __ffs(here) - 1;
+      Segment r;
+      r.seq = b0 + l;
+      r.start = __shfl_sync(0xffffffffu, s, l);
+      r.len = __shfl_sync(0xffffffffu, e, l) - r.start;
+      r.count = __shfl_sync(0xffffffffu, n, l);
+      r.index = index - before - (__shfl_sync(0xffffffffu, u, l) - r.count);
+      r.chunk0 = chunks + __shfl_sync(0xffffffffu, uc - nc, l);
+      r.slot0 = slots + __shfl_sync(0xffffffffu, us - ns, l);
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, u, 31);
+    chunks += __shfl_sync(0xffffffffu, uc, 31);
+    slots += __shfl_sync(0xffffffffu, us, 31);
+  }
+  return {-1, 0, 0, 0, 0, 0, 0};
+}
+
+// Shared memory (from a 1024-byte boundary): two stages of B, C (32 KB each)
+// and X of two heads, the heads' state / weighted-x operands, then per head
+// the factors of the tokens.
+constexpr uint32_t kStageBytes = 6 * kTileBytes;
+constexpr uint32_t kOperandAt = 2 * kStageBytes;
+constexpr uint32_t kFactorsAt = kOperandAt + 2 * kTileBytes;
+constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 64;  // + cend
+constexpr uint32_t kScanSmem = kScanBytes + 128 /* barriers */ + 512;
+// Tensor memory columns: S of two heads, C B^T, M of two heads, Y of two heads.
+constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
+
+// One segment of one pair of heads of a group (blockIdx.x: pair, blockIdx.y:
+// segment).  Warps 0-3 have the first head, 4-7 the second, a thread one row
+// (token i, or state n) of every product; warp 8 loads the operands and issues
+// C B^T.  With kStatesOnly, the segment's state from nothing (from the
+// prompt's state for its first segment) goes to slot index + 1 of the prompt,
+// and the prompt's state itself to slot 0; the last segment has nothing to do.
+template <bool kStatesOnly>
+__global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptParams p, const ChunkWork wk) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  if (pad > 512) {  // does not happen: dynamic shared memory starts on a 1024-byte boundary
+    record_status(SN_ERR_MISALIGNED);
+    return;
+  }
+  unsigned char* smem = smem_raw + pad;
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScanBytes);
+  uint64_t *full = bars, *empty = bars + 2, *bar_g = bars + 4, *gfree = bars + 5, *bar_y2 = bars + 6, *bar_y = bars + 8,
+           *bar_s = bars + 10;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 12);
+  pdl_launch_dependents();
+  pdl_wait();
+  // heads: pairs within a group
+  const int ppg = (p.hpg + 1) / 2;
+  const int g = blockIdx.x / ppg, h0 = g * p.hpg + (blockIdx.x - g * ppg) * 2;
+  const int heads = min(2, (g + 1) * p.hpg - h0);
+  const Segment sg = find_segment(p.prompts, wk.seg, blockIdx.y);
+  if (sg.seq < 0 || (kStatesOnly && sg.index + 1 >= sg.count)) return;  // the same in every warp
+  const int c0 = sg.index * wk.seg;
+  const int nchunks = min(wk.seg, (sg.len + kChunk - 1) / kChunk - c0);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, heads);
+      mbar_init(bar_y2 + i, 1);
+      mbar_init(bar_y + i, 1);
+      mbar_init(bar_s + i, 1);
+    }
+    mbar_init(bar_g, 1);
+    mbar_init(gfree, 4 * heads);
+    fence_barrier_init();
+  }
+  if (warp == 8) tc::tmem_alloc(tslot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tslot;
+  bool dead = false;  // a wait ran out: no further waits but for what is in flight
+  auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+    if (!dead && !mbar_wait_bounded(bar, parity)) {
+      record_status(SN_ERR_TIMEOUT);
+      dead = true;
+    }
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // whole warps
+    wait_one(bar, parity);
+    dead = __any_sync(0xffffffffu, dead);
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t bytes = (kStatesOnly ? 2 : 4) * kTileBytes + heads * kTileBytes;
+      auto load = [&](int c) {
+        const uint32_t st = sbase + (c & 1) * kStageBytes;
+        const int64_t chunk = sg.chunk0 + c0 + c;
+        mbar_arrive_expect_tx(full + (c & 1), bytes);
+        bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+        if (!kStatesOnly) bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+        bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
+      };
+      int loaded = 0;
+      for (; loaded < min(2, nchunks); ++loaded) load(loaded);
+      constexpr uint32_t id_g = idesc_f16(128, 128, false, false);
+      for (int c = 0; c < nchunks && !dead; ++c) {
+        wait_one(full + (c & 1), (c >> 1) & 1);
+        if (!kStatesOnly) {
+          if (c > 0) wait_one(gfree, (c - 1) & 1);
+          if (!dead) {
+            tc::fence_after_sync();
+            const unsigned char* st = smem + (c & 1) * kStageBytes;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
+              tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id_g, k > 0);
+            }
+            tc::mma_commit(bar_g);
+          }
+        }
+        if (c > 0 && c + 1 < nchunks) {  // chunk c - 1's stage, once its products are done
+          wait_one(empty + ((c + 1) & 1), ((c - 1) >> 1) & 1);
+          if (!dead) {
+            load(c + 1);
+            ++loaded;
+          }
+        }
+      }
+      if (dead)  // copies in flight land before the CTA leaves
+        for (int c = max(0, loaded - 2); c < loaded; ++c) mbar_wait_bounded(full + (c & 1), (c >> 1) & 1);
+    }
+  } else if ((warp >> 2) < heads) {
+    const int wg = warp >> 2, q = warp & 3, i = tid & 127, h = h0 + wg;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tS = tmem + kColS + wg * 64 + lanes, tG = tmem + kColG + lanes, tM = tmem + kColM + wg * 64 + lanes,
+                   tY = tmem + kColY + wg * 64 + lanes;
+    const uint32_t opnd = sbase + kOperandAt + wg * kTileBytes;
+    float* lg = reinterpret_cast<float*>(smem + kFactorsAt) + wg * 2 * kChunk;  // a_j - log2 dt_j
+    float* ej = lg + kChunk;                                                     // exp2(a_end(block of j) - lg_j)
+    float* cend = reinterpret_cast<float*>(smem + kFactorsAt + 2 * 2 * kChunk * 4) + wg * 4;
+    const uint32_t row = i * 128, sw = i & 7;
+    const int bar_id = 1 + wg;
+    const float D = !kStatesOnly && p.D ? __bfloat162float(p.D[h]) : 0.f;
+
+    // ---- the state before the segment: row n = i of S^T, true values ----
+    float unit = 1.f, bound = 0.f;  // S = unit * tensor memory; |S| <= bound
+    {
+      const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + i;
+      const float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + i;
+      const int64_t slot = static_cast<int64_t>(p.nh) * 64 * 128;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        if (sg.count == 1 || (kStatesOnly && sg.index == 0)) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = __bfloat162float(st[(32 * half + k) * 128]);
+          if (kStatesOnly) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) wk.state[(static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + (32 * half + k) * 128 + i] = v[k];
+          }
+        } else if (kStatesOnly) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = 0.f;
+        } else {  // slot 0, or the segments before this one joined
+          const int first = min(sg.index, 1);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = ws[first * slot + (32 * half + k) * 128];
+          for (int j = 2; j <= sg.index; ++j) {
+            const float dec = exp2_approx(wk.total[static_cast<int64_t>(sg.slot0 + j) * p.nh + h]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], dec, ws[j * slot + (32 * half + k) * 128]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) bound = fmaxf(bound, fabsf(v[k]));
+        tmem_st32(tS + 32 * half, v);
+      }
+      tmem_wait_st();
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+      if (lane == 0) cend[q] = bound;
+      named_bar_sync(bar_id, 128);
+      bound = fmaxf(fmaxf(cend[0], cend[1]), fmaxf(cend[2], cend[3]));
+      named_bar_sync(bar_id, 128);
+    }
+
+    float total = 0.f;  // log2 of the segment's decay
+    for (int c = 0; c < nchunks; ++c) {
+      const int64_t chunk = sg.chunk0 + c0 + c;
+      const unsigned stage = c & 1, ph = (c >> 1) & 1;
+      const uint32_t sst = sbase + stage * kStageBytes;
+      const int64_t th = chunk * p.nh + h;
+      const float a_i = wk.cum[th * kChunk + i], dt_i = wk.dt[th * kChunk + i];
+      const float a_end = wk.cum[th * kChunk + kChunk - 1];
+      const float2 meta = wk.meta[th];
+      const float sx = wk.scale[chunk * wk.blocks + h / 2], sB = wk.scale[chunk * wk.blocks + wk.xblocks + g];
+      const float sC = wk.scale[chunk * wk.blocks + wk.xblocks + p.ng + g];
+      const float sdt = pow2_floor(meta.x), dec = exp2_approx(a_end);
+      const float unit_in = unit, unit_new = sB * sx * sdt;
+      const float dtn = dt_i / sdt;  // exact scaling
+      if (c > 0) {  // the last chunk's products are done: its stage, the operand buffer and S are free
+        wait(bar_s + wg, (c - 1) & 1);
+        tc::fence_after_sync();
+        if (i == 0) mbar_arrive(empty + ((c - 1) & 1));
+        __syncwarp();
+      }
+      // ---- S: operand of C S, and decayed, in the new unit ----
+      const float sS = pow2_floor(bound) * (1.f / 8192.f);  // |S / sS| < 2^14
+      const float f_op = unit_in / sS, f_dec = dec * (unit_in / unit_new);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        tc::tmem_ld32(tS + 32 * half, v);
+        if (!kStatesOnly) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            sts128(opnd + row + (((4 * half + k) ^ sw) << 4), pack_f16(v[8 * k] * f_op, v[8 * k + 1] * f_op),
+                   pack_f16(v[8 * k + 2] * f_op, v[8 * k + 3] * f_op), pack_f16(v[8 * k + 4] * f_op, v[8 * k + 5] * f_op),
+                   pack_f16(v[8 * k + 6] * f_op, v[8 * k + 7] * f_op));
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= f_dec;
+        tmem_st32(tS + 32 * half, v);
+      }
+      unit = unit_new;
+      bound = fmaf(dec, bound, unit_new * 4.f * (meta.y / sdt));
+      total += a_end;
+      wait(full + stage, ph);
+      uint4 x[8];  // this token's row of X
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = lds128(sst + (4 + wg) * kTileBytes + row + ((k ^ sw) << 4));
+      const float wj = dtn * exp2_approx(a_end - a_i);
+      if (!kStatesOnly) {
+        const float l = a_i - log2f(dtn);  // +inf where dt is 0
+        lg[i] = l;
+        const float e = __shfl_sync(0xffffffffu, a_i, 31);  // the last token of the row's 32-token block
+        ej[i] = exp2_approx(e - l);
+        if (lane == 31) cend[q] = a_i;
+        __syncwarp();
+        tmem_wait_st();
+        tc::fence_before_sync();
+        tc::fence_proxy_async_smem();
+        named_bar_sync(bar_id, 128);
+        if (i == 0 && !dead) {  // Y = C S
+          tc::fence_after_sync();
+          constexpr uint32_t id = idesc_f16(128, 64, false, true);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tc::mma_bf16(tmem + kColY + wg * 64, tc::smem_desc_sw128(smem + stage * kStageBytes + (2 + (k >> 2)) * kTileBytes + (k & 3) * 32),
+                         desc_k_rows(opnd + k * 2048, 16), id, k > 0);
+          tc::mma_commit(bar_y2 + wg);
+        }
+        __syncwarp();
+        // ---- M from C B^T ----
+        wait(bar_g, c & 1);
+        tc::fence_after_sync();
+#pragma unroll
+        for (int jb = 0; jb < 4; ++jb) {
+          uint32_t m[16];
+          if (jb <= q) {
+            float v[32];
+            tc::tmem_ld32(tG + 32 * jb, v);
+            if (jb < q) {  // all of these tokens are earlier: exp(a_i - a_end) exp(a_end - a_j) dt_j, both at most 1
+              const float r = exp2_approx(a_i - cend[jb]);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) m[k] = pack_f16(v[2 * k] * (r * ej[32 * jb + 2 * k]), v[2 * k + 1] * (r * ej[32 * jb + 2 * k + 1]));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const float e0 = exp2_approx(a_i - lg[32 * jb + 2 * k]), e1 = exp2_approx(a_i - lg[32 * jb + 2 * k + 1]);
+                m[k] = pack_f16(2 * k <= lane ? v[2 * k] * e0 : 0.f, 2 * k + 1 <= lane ? v[2 * k + 1] * e1 : 0.f);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) m[k] = 0;
+          }
+          tmem_st16(tM + 16 * jb, m);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(gfree);
+        __syncwarp();
+        // ---- Y = exp(a_i) C S, in the unit of M X ----
+        wait(bar_y2 + wg, c & 1);
+        tc::fence_after_sync();
+        const float f_y = exp2_approx(a_i) * (sS / unit_new);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float v[32];
+          tc::tmem_ld32(tY + 32 * half, v);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] *= f_y;
+          tmem_st32(tY + 32 * half, v);
+        }
+      }
+      // ---- weighted x ----
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack_f16(u[j]);
+          o[j] = pack_f16(f.x * wj, f.y * wj);
+        }
+        sts128(opnd + row + ((k ^ sw) << 4), o[0], o[1], o[2], o[3]);
+      }
+      tmem_wait_st();
+      tc::fence_before_sync();
+      tc::fence_proxy_async_smem();
+      named_bar_sync(bar_id, 128);
+      if (i == 0 && !dead) {
+        tc::fence_after_sync();
+        if (!kStatesOnly) {  // Y += M X
+          constexpr uint32_t id = idesc_f16(128, 64, false, true);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_f16_ts(tmem + kColY + wg * 64, tmem + kColM + wg * 64 + 8 * k, desc_k_rows(sst + (4 + wg) * kTileBytes + k * 2048, 16), id, 1);
+          tc::mma_commit(bar_y + wg);
+        }
+        constexpr uint32_t id = idesc_f16(128, 64, true, true);  // S += B^T (w x)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          tc::mma_bf16(tmem + kColS + wg * 64, desc_k_rows(sst + k * 2048, kTileBytes), desc_k_rows(opnd + k * 2048, 16), id, 1);
+        tc::mma_commit(bar_s + wg);
+      }
+      __syncwarp();
+      if (!kStatesOnly) {
+        wait(bar_y + wg, c & 1);
+        tc::fence_after_sync();
+        const int t = (c0 + c) * kChunk + i;
+        const float f = sC * unit_new, dx = D * sx;
+        const bool live = t < sg.len;
+        const int64_t token = sg.start + t;
+        const __nv_bfloat16* z = p.zx + token * p.ld + h * 64;
+        __nv_bfloat16* out = p.y + (token * p.nh + h) * 64;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float v[32];
+          tc::tmem_ld32(tY + 32 * half, v);
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 xv = x[4 * half + k];
+              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+              uint32_t o[4];
+              uint4 zv = make_uint4(0, 0, 0, 0);
+              if (p.gate) zv = *reinterpret_cast<const uint4*>(z + 32 * half + 8 * k);
+              const uint32_t zu[4] = {zv.x, zv.y, zv.z, zv.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 xf = unpack_f16(u[j]);
+                float y0 = fmaf(v[8 * k + 2 * j], f, xf.x * dx), y1 = fmaf(v[8 * k + 2 * j + 1], f, xf.y * dx);
+                if (p.gate) {
+                  const float z0 = bf16lo(zu[j]), z1 = bf16hi(zu[j]);
+                  y0 *= __fdividef(z0, 1.f + __expf(-z0));
+                  y1 *= __fdividef(z1, 1.f + __expf(-z1));
+                }
+                const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
+                o[j] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+              *reinterpret_cast<uint4*>(out + 32 * half + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          }
+          __syncwarp();
+        }
+        tc::fence_before_sync();
+      }
+    }
+    // ---- the state after the segment ----
+    wait(bar_s + wg, (nchunks - 1) & 1);
+    tc::fence_after_sync();
+    if (dead) mbar_wait_bounded(bar_s + wg, (nchunks - 1) & 1);
+    const bool last = sg.index + 1 == sg.count;
+    if (kStatesOnly || last) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        tc::tmem_ld32(tS + 32 * half, v);
+        if (kStatesOnly) {
+          float* ws = wk.state + (static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h) * 64 * 128 + i;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) ws[(32 * half + k) * 128] = v[k] * unit;
+        } else {
+          __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + i;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) st[(32 * half + k) * 128] = __float2bfloat16_rn(v[k] * unit);
+        }
+      }
+      if (kStatesOnly && i == 0) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+}
+
+// ---- host: sizes of the tensor-core form ----
+struct ScanPlan {
+  int64_t chunks;    // at most, over all prompts
+  int64_t slots;     // state slots
+  int64_t segments;  // at most
+  int seg, pairs, xblocks, blocks;
+  size_t x, b, c, cum, dt, meta, scale, state, total, bytes;  // offsets
+};
+inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, int nh, ScanPlan* out) {
+  if (d_state != 128 || d_inner != static_cast<int64_t>(nh) * 64) return false;
+  ScanPlan r;
+  r.chunks = tokens / kChunk + static_cast<int64_t>(batch);
+  const int hpg = nh / ng;
+  r.pairs = ng * ((hpg + 1) / 2);
+  r.xblocks = (d_inner + 127) / 128;
+  r.blocks = r.xblocks + 2 * ng;
+  // Chunks a segment: the fewest chunk steps over the SMs' waves.  A step of the second launch costs about twice one of the
+  // first, a CTA's start and end about one step.
+  const int sms = 148;
+  const int64_t nc = std::max<int64_t>(1, (tokens + kChunk - 1) / kChunk);
+  const int64_t each = (nc + batch - 1) / batch;  // of a prompt, if they are alike
+  int64_t best = INT64_MAX;
+  r.seg = static_cast<int>(each);
+  for (int64_t n = 1; n <= std::min<int64_t>(each, 32); ++n) {  // segments of such a prompt
+    const int64_t seg = (each + n - 1) / n;
+    const int64_t waves = (batch * ((each + seg - 1) / seg) * r.pairs + sms - 1) / sms;
+    const int64_t waves1 = n == 1 ? 0 : (batch * ((each + seg - 1) / seg - 1) * r.pairs + sms - 1) / sms;
+    const int64_t cost = waves * (2 * seg + 2) + waves1 * (seg + 2);
+    if (cost < best) {
+      best = cost;
+      r.seg = static_cast<int>(seg);
+    }
+  }
+  r.segments = nc / r.seg + batch;
+  r.slots = std::min<int64_t>(r.segments, 2 * (nc / r.seg) + 2);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t here = at;
+    at += (n + 255) / 256 * 256;
+    return here;
+  };
+  const size_t nch = static_cast<size_t>(r.chunks);
+  r.x = take(nch * nh * kTileBytes);
+  r.b = take(nch * ng * 2 * kTileBytes);
+  r.c = take(nch * ng * 2 * kTileBytes);
+  r.cum = take(nch * nh * kChunk * 4);
+  r.dt = take(nch * nh * kChunk * 4);
+  r.meta = take(nch * nh * 8);
+  r.scale = take(nch * r.blocks * 4);
+  r.state = take(static_cast<size_t>(r.slots) * nh * 64 * 128 * 4);
+  r.total = take(static_cast<size_t>(r.slots) * nh * 4);
+  r.bytes = at;
+  *out = r;
+  return true;
+}
+
 }  // namespace
 
 int tu_status_prompt(bool reset, cudaStream_t st, int* out) { return read_tu_status(reset, st, out); }
@@ -224,8 +1016,11 @@ extern "C" {
 
 size_t sn_mamba2_prompt_workspace_size(int tokens, int batch, int d_inner, int ngroups, int d_state, int nheads) {
   if (tokens < 0 || batch < 1 || d_inner < 1 || ngroups < 1 || d_state < 1 || nheads < 1) return 0;
-  return (static_cast<size_t>(tokens) * (d_inner + 2 * static_cast<size_t>(ngroups) * d_state) * 2 + 255) / 256 * 256 +
-         256;
+  size_t n = static_cast<size_t>(tokens) * (d_inner + 2 * static_cast<size_t>(ngroups) * d_state) * 2;
+  sn::ScanPlan plan;
+  if (nheads % ngroups == 0 && sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan))
+    n = std::max(n, plan.bytes);
+  return (n + 255) / 256 * 256 + 256;
 }
 
 int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const void* conv_weight, const void* conv_bias,
@@ -267,6 +1062,42 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
   p.W = d_conv;
   p.gate = gate ? 1 : 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  sn::ScanPlan plan;
+  const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y);
+  // 64-element heads, 128 states, 16-byte rows: the tensor-core form
+  if (d_conv >= 2 && d_conv <= 4 && rows16 &&
+      sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan) && plan.chunks <= 65535 && plan.segments <= 65535) {
+    unsigned char* base = reinterpret_cast<unsigned char*>(p.xbc);
+    sn::ChunkWork wk;
+    wk.x = base + plan.x;
+    wk.b = base + plan.b;
+    wk.c = base + plan.c;
+    wk.cum = reinterpret_cast<float*>(base + plan.cum);
+    wk.dt = reinterpret_cast<float*>(base + plan.dt);
+    wk.meta = reinterpret_cast<float2*>(base + plan.meta);
+    wk.scale = reinterpret_cast<float*>(base + plan.scale);
+    wk.state = reinterpret_cast<float*>(base + plan.state);
+    wk.total = reinterpret_cast<float*>(base + plan.total);
+    wk.xblocks = plan.xblocks;
+    wk.blocks = plan.blocks;
+    wk.seg = plan.seg;
+    auto conv = d_conv == 4 ? sn::prompt_conv_tile_kernel<4> : d_conv == 3 ? sn::prompt_conv_tile_kernel<3> : sn::prompt_conv_tile_kernel<2>;
+    int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + 1), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
+    if (rc != SN_OK) return rc;
+    const dim3 grid(static_cast<unsigned>(plan.pairs), static_cast<unsigned>(plan.segments));
+    auto scan = [&](auto kern) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sn::kScanSmem)) != cudaSuccess) {
+        cudaGetLastError();
+        return SN_ERR_LAUNCH;
+      }
+      return sn::launch(kern, grid, dim3(288), sn::kScanSmem, st, true, p, wk);
+    };
+    if (tokens > static_cast<int64_t>(plan.seg) * sn::kChunk) {  // a prompt may have several segments
+      rc = scan(sn::prompt_scan_mma_kernel<true>);
+      if (rc != SN_OK) return rc;
+    }
+    return scan(sn::prompt_scan_mma_kernel<false>);
+  }
   const int64_t rows = static_cast<int64_t>(batch) * d_inner;
   const int64_t blocks = tokens / sn::kConvRows + static_cast<int64_t>(batch);
   if (blocks > 65535 || rows > INT32_MAX / 16) return SN_ERR_UNSUPPORTED;
