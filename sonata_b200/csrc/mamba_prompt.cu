@@ -292,84 +292,131 @@ __device__ __forceinline__ float exp2_approx(float v) {
   return r;
 }
 
-// One 128-channel block of one chunk (blockIdx.x < blocks), or the chunk's dt
-// and decays (blockIdx.x == blocks).  Thread: 8 channels, 8 tokens.
+// Two fp32 products in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+__device__ __forceinline__ float2 unpack_bf16(uint32_t v) { return make_float2(bf16lo(v), bf16hi(v)); }
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / v of a power of two, exactly.
+__device__ __forceinline__ float rcp_pow2(float v) { return __uint_as_float((254u << 23) - __float_as_uint(v)); }
+__device__ __forceinline__ float2 silu2(float2 v) {
+  const float2 z = mul2(v, splat(-kLog2e));
+  return mul2(v, make_float2(rcp_approx(1.f + exp2_approx(z.x)), rcp_approx(1.f + exp2_approx(z.y))));
+}
+
+// dt and decays of 16 heads of one chunk.
+constexpr int kDtHeads = 16;
+__device__ __forceinline__ void prompt_dt(const PromptParams& p, const ChunkWork& wk, const PromptBlock& pb, int64_t chunk, int h0,
+                                          float* s_dt) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t0 = pb.block * kChunk;
+  const int r = tid >> 1, e0 = (tid & 1) * 8;  // token; the first of 8 heads
+  const int64_t at = 2 * static_cast<int64_t>(p.di) + 2 * p.gds + h0 + e0;
+  const __nv_bfloat16* src = p.zx + (pb.start + t0 + r) * p.ld + at;
+  const bool live = t0 + r < pb.len;
+  float v[8];
+  if (live && h0 + e0 + 8 <= p.nh && (at & 7) == 0) {
+    const uint4 u = *reinterpret_cast<const uint4*>(src);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = bf16lo(w[k]);
+      v[2 * k + 1] = bf16hi(w[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = live && h0 + e0 + k < p.nh ? __bfloat162float(src[k]) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (p.dt_bias && h0 + e0 + k < p.nh) v[k] += __bfloat162float(p.dt_bias[h0 + e0 + k]);
+    v[k] = v[k] <= 20.f ? log1pf(__expf(v[k])) : v[k];
+    s_dt[(e0 + k) * 129 + r] = live ? v[k] : 0.f;
+  }
+  __syncthreads();
+  for (int h = warp; h < kDtHeads && h0 + h < p.nh; h += 8) {
+    const float a2 = p.A[h0 + h] * kLog2e;
+    float c[4], run = 0.f, top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = s_dt[h * 129 + lane * 4 + k];
+      run = fmaf(v[k], a2, run);
+      c[k] = run;
+      top = fmaxf(top, v[k]);
+    }
+    float upto = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    const float before = upto - run, all = __shfl_sync(0xffffffffu, upto, 31);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      c[k] += before;
+      sum = fmaf(v[k], exp2_approx(all - c[k]), sum);
+    }
+    if (lane == 31) c[3] = all;  // the state's decay and the last token's are the same number
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int64_t row = chunk * p.nh + h0 + h;
+    reinterpret_cast<float4*>(wk.cum + row * kChunk)[lane] = make_float4(c[0], c[1], c[2], c[3]);
+    reinterpret_cast<float4*>(wk.dt + row * kChunk)[lane] = make_float4(v[0], v[1], v[2], v[3]);
+    if (lane == 0) wk.meta[row] = make_float2(top, sum);
+  }
+}
+
+// One 128-channel block of one chunk (blockIdx.x < blocks), or 16 heads' dt
+// and decays.  Thread: 8 channels, 8 tokens.  Reads the inputs and writes the
+// tiles once: bounded by HBM (and, half as much, by the two special functions
+// of a SiLU).
 template <int W>
-__global__ void __launch_bounds__(256) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
-  __shared__ float s_dt[64 * 129];
+__global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+  __shared__ float s_dt[kDtHeads * 129];
   __shared__ float s_max[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int conv_dim = p.di + 2 * p.gds;
   const int blk = blockIdx.x;
-  // this thread's channels, tokens and weights (the weights are the layer's: no need to wait for them)
   const int c8 = tid & 15, r0 = (tid >> 4) * 8;
   int d = blk * 128 + c8 * 8;  // channel of the convolution
   if (blk >= wk.xblocks) d = p.di + (blk - wk.xblocks) * 128 + c8 * 8;
   const bool on = blk < wk.xblocks ? d < p.di : blk < wk.blocks;
-  float w[8][W], bias[8];
   pdl_launch_dependents();
   pdl_wait();
   const PromptBlock pb = find_block(p.prompts, kChunk, 0, blockIdx.y);
   if (pb.seq < 0) return;
   const int t0 = pb.block * kChunk;
   const int64_t chunk = blockIdx.y;
-
-  if (blk == wk.blocks) {  // dt and decays: 64 heads at a time
-    for (int h0 = 0; h0 < p.nh; h0 += 64) {
-      const int64_t at = 2 * static_cast<int64_t>(p.di) + 2 * p.gds + h0;
-      for (int e = tid; e < 64 * kChunk; e += 256) {
-        const int h = e & 63, r = e >> 6;
-        float v = 0.f;
-        if (h0 + h < p.nh && t0 + r < pb.len) {
-          v = __bfloat162float(p.zx[(pb.start + t0 + r) * p.ld + at + h]);
-          if (p.dt_bias) v += __bfloat162float(p.dt_bias[h0 + h]);
-          v = v <= 20.f ? log1pf(expf(v)) : v;
-        }
-        s_dt[h * 129 + r] = v;
-      }
-      __syncthreads();
-      for (int h = warp; h < 64 && h0 + h < p.nh; h += 8) {
-        const float a2 = p.A[h0 + h] * kLog2e;
-        float v[4], c[4], run = 0.f, top = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[k] = s_dt[h * 129 + lane * 4 + k];
-          run = fmaf(v[k], a2, run);
-          c[k] = run;
-          top = fmaxf(top, v[k]);
-        }
-        float upto = run;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float u = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += u;
-        }
-        const float before = upto - run, all = __shfl_sync(0xffffffffu, upto, 31);
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          c[k] += before;
-          sum = fmaf(v[k], exp2_approx(all - c[k]), sum);
-        }
-        if (lane == 31) c[3] = all;  // the state's decay and the last token's are the same number
-        sum = warp_sum(sum);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int64_t row = chunk * p.nh + h0 + h;
-        reinterpret_cast<float4*>(wk.cum + row * kChunk)[lane] = make_float4(c[0], c[1], c[2], c[3]);
-        reinterpret_cast<float4*>(wk.dt + row * kChunk)[lane] = make_float4(v[0], v[1], v[2], v[3]);
-        if (lane == 0) wk.meta[row] = make_float2(top, sum);
-      }
-      __syncthreads();
-    }
+  if (blk >= wk.blocks) {
+    prompt_dt(p, wk, pb, chunk, (blk - wk.blocks) * kDtHeads, s_dt);
     return;
   }
 
   float top = 0.f;
-  float out[8][8];  // [token][channel]
+  float2 out[8][4];  // [token][pair of channels]
   if (on) {
     const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
-    __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
     uint4 raw[W + 7];  // inputs t0 + r0 - W + 1 .. t0 + r0 + 7
 #pragma unroll
     for (int k = 0; k < W + 7; ++k) {
@@ -377,66 +424,87 @@ __global__ void __launch_bounds__(256) prompt_conv_tile_kernel(const PromptParam
       raw[k] = make_uint4(0, 0, 0, 0);
       if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u + t * p.ld);
     }
+    float2 w[W][4], bias[4];
+    {
+      const __nv_bfloat16* wr = p.w + static_cast<int64_t>(d) * W;  // [8][W], 16 W bytes from a 16-byte boundary
+      uint32_t wu[4 * W];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      bias[c] = p.bias ? __bfloat162float(p.bias[d + c]) : 0.f;
+      for (int k = 0; k < W; ++k) *reinterpret_cast<uint4*>(wu + 4 * k) = reinterpret_cast<const uint4*>(wr)[k];
+      auto at = [&](int e) { return e & 1 ? bf16hi(wu[e / 2]) : bf16lo(wu[e / 2]); };
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[c][k] = __bfloat162float(p.w[static_cast<int64_t>(d + c) * W + k]);
+      for (int k = 0; k < W; ++k) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[k][c] = make_float2(at(2 * c * W + k), at((2 * c + 1) * W + k));
+      }
+      uint4 bu = make_uint4(0, 0, 0, 0);
+      if (p.bias) bu = *reinterpret_cast<const uint4*>(p.bias + d);
+      bias[0] = unpack_bf16(bu.x);
+      bias[1] = unpack_bf16(bu.y);
+      bias[2] = unpack_bf16(bu.z);
+      bias[3] = unpack_bf16(bu.w);
     }
     if (t0 + r0 == 0) {  // the prompt's first tokens: inputs before them are the state's columns 1 .. W - 1
-      __nv_bfloat16 old[8][W], moved[8][W];
+      __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
+      uint32_t old[4 * W];  // element c * W + k
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) old[c][k] = st[c * W + k];
-      }
+      for (int k = 0; k < W; ++k) *reinterpret_cast<uint4*>(old + 4 * k) = reinterpret_cast<const uint4*>(st)[k];
+      auto at = [&](int e) { return (old[e / 2] >> (16 * (e & 1))) & 0xFFFFu; };
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) {
         uint32_t v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          v[c] = static_cast<uint32_t>(__bfloat16_as_ushort(old[2 * c][k + 1])) |
-                 static_cast<uint32_t>(__bfloat16_as_ushort(old[2 * c + 1][k + 1])) << 16;
+        for (int c = 0; c < 4; ++c) v[c] = at(2 * c * W + k + 1) | at((2 * c + 1) * W + k + 1) << 16;
         raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
       }
       // and the state after the prompt, its last W inputs (only this thread reads or writes these channels' state)
+      uint32_t moved[8 * W];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int k = 0; k < W; ++k) {
+        const int t = pb.len - W + k;  // < 0: the old state's column W + t = k + len
+        if (t >= 0) {
+          const uint4 v = *reinterpret_cast<const uint4*>(u + t * p.ld);
+          const uint32_t vu[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const int t = pb.len - W + k;  // < 0: the old state's column W + t = k + len
-          __nv_bfloat16 v = t >= 0 ? u[t * p.ld + c] : old[c][W - 1];
+          for (int c = 0; c < 8; ++c) moved[c * W + k] = (vu[c / 2] >> (16 * (c & 1))) & 0xFFFFu;
+        } else {
 #pragma unroll
-          for (int j = 0; j < W; ++j)
-            if (t < 0 && j == pb.len + k) v = old[c][j];
-          moved[c][k] = v;
+          for (int c = 0; c < 8; ++c) {
+            moved[c * W + k] = at(c * W + W - 1);
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j)
+              if (j == pb.len + k) moved[c * W + k] = at(c * W + j);
+          }
         }
       }
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int k = 0; k < W; ++k)
+        reinterpret_cast<uint4*>(st)[k] =
+            make_uint4(moved[8 * k] | moved[8 * k + 1] << 16, moved[8 * k + 2] | moved[8 * k + 3] << 16,
+                       moved[8 * k + 4] | moved[8 * k + 5] << 16, moved[8 * k + 6] | moved[8 * k + 7] << 16);
+    }
 #pragma unroll
-        for (int k = 0; k < W; ++k) st[c * W + k] = moved[c][k];
+    for (int r = 0; r < 8; ++r) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) out[r][c] = bias[c];
+    }
+#pragma unroll
+    for (int k = 0; k < W + 7; ++k) {  // each input once, into the outputs it belongs to
+      const float2 v[4] = {unpack_bf16(raw[k].x), unpack_bf16(raw[k].y), unpack_bf16(raw[k].z), unpack_bf16(raw[k].w)};
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int r = k - j;  // tap j of output r
+        if (r < 0 || r > 7) continue;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) out[r][c] = fma2(v[c], w[j][c], out[r][c]);
       }
     }
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const bool live = t0 + r0 + r < pb.len;
-      float acc[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) acc[c] = bias[c];
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const uint32_t v[4] = {raw[r + k].x, raw[r + k].y, raw[r + k].z, raw[r + k].w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          acc[2 * c] = fmaf(bf16lo(v[c]), w[2 * c][k], acc[2 * c]);
-          acc[2 * c + 1] = fmaf(bf16hi(v[c]), w[2 * c + 1][k], acc[2 * c + 1]);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        out[r][c] = live ? __fdividef(acc[c], 1.f + __expf(-acc[c])) : 0.f;
-        top = fmaxf(top, fabsf(out[r][c]));
+      for (int c = 0; c < 4; ++c) {
+        out[r][c] = live ? silu2(out[r][c]) : make_float2(0.f, 0.f);
+        top = fmaxf(fmaxf(top, fabsf(out[r][c].x)), fabsf(out[r][c].y));
       }
     }
   }
@@ -449,7 +517,7 @@ __global__ void __launch_bounds__(256) prompt_conv_tile_kernel(const PromptParam
   const float sc = pow2_floor(top);
   if (tid == 0) wk.scale[chunk * wk.blocks + blk] = sc;
   if (!on) return;
-  const float inv = 1.f / sc;  // exact
+  const float2 inv = splat(rcp_pow2(sc));
   // tile of these channels, chunk c8 % 8 of its rows
   unsigned char* tile;
   if (blk < wk.xblocks) {
@@ -462,9 +530,13 @@ __global__ void __launch_bounds__(256) prompt_conv_tile_kernel(const PromptParam
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int row = r0 + r;  // row % 8 == r
-    *reinterpret_cast<uint4*>(tile + row * 128 + (((c8 & 7) ^ r) << 4)) =
-        make_uint4(pack_f16(out[r][0] * inv, out[r][1] * inv), pack_f16(out[r][2] * inv, out[r][3] * inv),
-                   pack_f16(out[r][4] * inv, out[r][5] * inv), pack_f16(out[r][6] * inv, out[r][7] * inv));
+    uint32_t o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float2 v = mul2(out[r][c], inv);
+      o[c] = pack_f16(v.x, v.y);
+    }
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((c8 & 7) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -578,19 +650,22 @@ __device__ __forceinline__ Segment find_segment(const Prompts& p, int seg, int i
 constexpr uint32_t kStageBytes = 6 * kTileBytes;
 constexpr uint32_t kOperandAt = 2 * kStageBytes;
 constexpr uint32_t kFactorsAt = kOperandAt + 2 * kTileBytes;
-constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 64;  // + cend
+constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 128;  // and their block ends
 constexpr uint32_t kScanSmem = kScanBytes + 128 /* barriers */ + 512;
 // Tensor memory columns: S of two heads, C B^T, M of two heads, Y of two heads.
+constexpr int kScanThreads = 2 * 256;
 constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 
 // One segment of one pair of heads of a group (blockIdx.x: pair, blockIdx.y:
-// segment).  Warps 0-3 have the first head, 4-7 the second, a thread one row
-// (token i, or state n) of every product; warp 8 loads the operands and issues
+// segment).  Warps 0-7 have the first head, 8-15 the second, a thread one row
+// (token i, or state n) and half of the columns of every product: 16 warps with
+// 128 registers each (a 17th for the copies would leave 96).  The first thread
+// of a head issues its products, that of the first head also the copies and
 // C B^T.  With kStatesOnly, the segment's state from nothing (from the
 // prompt's state for its first segment) goes to slot index + 1 of the prompt,
 // and the prompt's state itself to slot 0; the last segment has nothing to do.
 template <bool kStatesOnly>
-__global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptParams p, const ChunkWork wk) {
+__global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const PromptParams p, const ChunkWork wk) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -617,185 +692,204 @@ __global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptPar
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, heads);
+      mbar_init(empty + i, 8 * heads);
       mbar_init(bar_y2 + i, 1);
       mbar_init(bar_y + i, 1);
       mbar_init(bar_s + i, 1);
     }
     mbar_init(bar_g, 1);
-    mbar_init(gfree, 4 * heads);
+    mbar_init(gfree, 8 * heads);
     fence_barrier_init();
   }
-  if (warp == 8) tc::tmem_alloc(tslot, 512);
+  if (warp == 0) tc::tmem_alloc(tslot, 512);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tslot;
   bool dead = false;  // a wait ran out: no further waits but for what is in flight
-  auto wait_one = [&](uint64_t* bar, uint32_t parity) {
-    if (!dead && !mbar_wait_bounded(bar, parity)) {
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // whole warps
+    if (!__all_sync(0xffffffffu, dead || mbar_wait_bounded(bar, parity))) {
       record_status(SN_ERR_TIMEOUT);
       dead = true;
     }
   };
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // whole warps
-    wait_one(bar, parity);
-    dead = __any_sync(0xffffffffu, dead);
-  };
 
-  if (warp == 8) {
-    if (lane == 0) {
-      const uint32_t bytes = (kStatesOnly ? 2 : 4) * kTileBytes + heads * kTileBytes;
-      auto load = [&](int c) {
-        const uint32_t st = sbase + (c & 1) * kStageBytes;
-        const int64_t chunk = sg.chunk0 + c0 + c;
-        mbar_arrive_expect_tx(full + (c & 1), bytes);
-        bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-        if (!kStatesOnly) bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-        bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
-      };
-      int loaded = 0;
-      for (; loaded < min(2, nchunks); ++loaded) load(loaded);
-      constexpr uint32_t id_g = idesc_f16(128, 128, false, false);
-      for (int c = 0; c < nchunks && !dead; ++c) {
-        wait_one(full + (c & 1), (c >> 1) & 1);
-        if (!kStatesOnly) {
-          if (c > 0) wait_one(gfree, (c - 1) & 1);
-          if (!dead) {
-            tc::fence_after_sync();
-            const unsigned char* st = smem + (c & 1) * kStageBytes;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
-              tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id_g, k > 0);
-            }
-            tc::mma_commit(bar_g);
-          }
-        }
-        if (c > 0 && c + 1 < nchunks) {  // chunk c - 1's stage, once its products are done
-          wait_one(empty + ((c + 1) & 1), ((c - 1) >> 1) & 1);
-          if (!dead) {
-            load(c + 1);
-            ++loaded;
-          }
-        }
-      }
-      if (dead)  // copies in flight land before the CTA leaves
-        for (int c = max(0, loaded - 2); c < loaded; ++c) mbar_wait_bounded(full + (c & 1), (c >> 1) & 1);
-    }
-  } else if ((warp >> 2) < heads) {
-    const int wg = warp >> 2, q = warp & 3, i = tid & 127, h = h0 + wg;
+  // the copies of a chunk's operands into its stage (one thread)
+  auto load = [&](int c) {
+    const uint32_t st = sbase + (c & 1) * kStageBytes;
+    const int64_t chunk = sg.chunk0 + c0 + c;
+    mbar_arrive_expect_tx(full + (c & 1), ((kStatesOnly ? 2 : 4) + heads) * kTileBytes);
+    bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+    if (!kStatesOnly) bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+    bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
+  };
+  int loaded = min(2, nchunks);  // chunks whose copies have been issued
+  if (tid == 0) {
+    for (int c = 0; c < loaded; ++c) load(c);
+  }
+  if ((warp >> 3) < heads) {
+    const int wg = warp >> 3, half = (warp >> 2) & 1, q = warp & 3, i = q * 32 + lane, h = h0 + wg;
+    const bool lead = half == 0 && i == 0;  // issues the head's products
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tS = tmem + kColS + wg * 64 + lanes, tG = tmem + kColG + lanes, tM = tmem + kColM + wg * 64 + lanes,
-                   tY = tmem + kColY + wg * 64 + lanes;
+    const uint32_t tS = tmem + kColS + wg * 64 + 32 * half + lanes, tG = tmem + kColG + lanes,
+                   tM = tmem + kColM + wg * 64 + lanes, tY = tmem + kColY + wg * 64 + 32 * half + lanes;
     const uint32_t opnd = sbase + kOperandAt + wg * kTileBytes;
-    float* lg = reinterpret_cast<float*>(smem + kFactorsAt) + wg * 2 * kChunk;  // a_j - log2 dt_j
-    float* ej = lg + kChunk;                                                     // exp2(a_end(block of j) - lg_j)
-    float* cend = reinterpret_cast<float*>(smem + kFactorsAt + 2 * 2 * kChunk * 4) + wg * 4;
+    float* fj = reinterpret_cast<float*>(smem + kFactorsAt) + wg * 2 * kChunk;  // of token j within its block, see below
+    float* ej = fj + kChunk;                                                     // exp2(a_last(block) - a_j) dt_j
+    float* cend = reinterpret_cast<float*>(smem + kFactorsAt + 2 * 2 * kChunk * 4) + wg * 16;  // [4]; first [8] maxima
     const uint32_t row = i * 128, sw = i & 7;
     const int bar_id = 1 + wg;
     const float D = !kStatesOnly && p.D ? __bfloat162float(p.D[h]) : 0.f;
 
-    // ---- the state before the segment: row n = i of S^T, true values ----
+    // ---- the state before the segment: row n = i of S^T, this half's 32 columns, true values ----
     float unit = 1.f, bound = 0.f;  // S = unit * tensor memory; |S| <= bound
     {
-      const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + i;
-      const float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + i;
-      const int64_t slot = static_cast<int64_t>(p.nh) * 64 * 128;
+      const int64_t at = static_cast<int64_t>(32 * half) * 128 + i, slot = static_cast<int64_t>(p.nh) * 64 * 128;
+      const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
+      float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + at;
+      float v[32];
+      if (sg.count == 1 || (kStatesOnly && sg.index == 0)) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float v[32];
-        if (sg.count == 1 || (kStatesOnly && sg.index == 0)) {
+        for (int k = 0; k < 32; ++k) v[k] = __bfloat162float(st[k * 128]);
+        if (kStatesOnly) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = __bfloat162float(st[(32 * half + k) * 128]);
-          if (kStatesOnly) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) wk.state[(static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + (32 * half + k) * 128 + i] = v[k];
-          }
-        } else if (kStatesOnly) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = 0.f;
-        } else {  // slot 0, or the segments before this one joined
-          const int first = min(sg.index, 1);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = ws[first * slot + (32 * half + k) * 128];
-          for (int j = 2; j <= sg.index; ++j) {
-            const float dec = exp2_approx(wk.total[static_cast<int64_t>(sg.slot0 + j) * p.nh + h]);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], dec, ws[j * slot + (32 * half + k) * 128]);
-          }
+          for (int k = 0; k < 32; ++k) ws[k * 128] = v[k];
         }
+      } else if (kStatesOnly) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) bound = fmaxf(bound, fabsf(v[k]));
-        tmem_st32(tS + 32 * half, v);
+        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+      } else {  // slot 0, or the segments before this one joined
+        const int first = min(sg.index, 1);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = ws[first * slot + k * 128];
+        for (int j = 2; j <= sg.index; ++j) {
+          const float dec = exp2_approx(wk.total[static_cast<int64_t>(sg.slot0 + j) * p.nh + h]);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], dec, ws[j * slot + k * 128]);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 32; ++k) bound = fmaxf(bound, fabsf(v[k]));
+      tmem_st32(tS, v);
       tmem_wait_st();
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
-      if (lane == 0) cend[q] = bound;
-      named_bar_sync(bar_id, 128);
-      bound = fmaxf(fmaxf(cend[0], cend[1]), fmaxf(cend[2], cend[3]));
-      named_bar_sync(bar_id, 128);
+      if (lane == 0) cend[warp & 7] = bound;
+      named_bar_sync(bar_id, 256);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) bound = fmaxf(bound, cend[k]);
+      named_bar_sync(bar_id, 256);
     }
 
+    // a chunk's factors, loaded one chunk ahead
+    struct Factors {
+      float a_i, dt_i, a_end, sx, sB, sC;
+      float2 meta;
+    } next;
+    const int chunk0 = sg.chunk0 + c0;
+    auto fetch = [&](int c) {
+      const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
+      const float* cum = wk.cum + th * kChunk;
+      const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * wk.blocks;
+      next.a_i = cum[i];
+      next.a_end = cum[kChunk - 1];
+      next.dt_i = wk.dt[th * kChunk + i];
+      next.meta = wk.meta[th];
+      next.sx = sc[h / 2];
+      next.sB = sc[wk.xblocks + g];
+      next.sC = sc[wk.xblocks + p.ng + g];
+    };
+    fetch(0);
     float total = 0.f;  // log2 of the segment's decay
     for (int c = 0; c < nchunks; ++c) {
-      const int64_t chunk = sg.chunk0 + c0 + c;
       const unsigned stage = c & 1, ph = (c >> 1) & 1;
       const uint32_t sst = sbase + stage * kStageBytes;
-      const int64_t th = chunk * p.nh + h;
-      const float a_i = wk.cum[th * kChunk + i], dt_i = wk.dt[th * kChunk + i];
-      const float a_end = wk.cum[th * kChunk + kChunk - 1];
-      const float2 meta = wk.meta[th];
-      const float sx = wk.scale[chunk * wk.blocks + h / 2], sB = wk.scale[chunk * wk.blocks + wk.xblocks + g];
-      const float sC = wk.scale[chunk * wk.blocks + wk.xblocks + p.ng + g];
-      const float sdt = pow2_floor(meta.x), dec = exp2_approx(a_end);
-      const float unit_in = unit, unit_new = sB * sx * sdt;
-      const float dtn = dt_i / sdt;  // exact scaling
+      const uint32_t xrow = sst + (4 + wg) * kTileBytes + row;
+      const Factors f = next;
+      if (c + 1 < nchunks) fetch(c + 1);
+      // every scale is a power of two: products and reciprocals of them are exact
+      const float sdt = pow2_floor(f.meta.x), rdt = rcp_pow2(sdt), dec = exp2_approx(f.a_end);
+      const float unit_new = f.sB * f.sx * sdt, runit = rcp_pow2(f.sB) * rcp_pow2(f.sx) * rdt;
+      const float dtn = f.dt_i * rdt;
+      const float sb = pow2_floor(bound), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
+      const float f_op = unit * (rcp_pow2(sb) * 8192.f), f_dec = dec * (unit * runit);
+      unit = unit_new;
+      bound = fmaf(dec, bound, unit_new * 4.f * (f.meta.y * rdt));
+      total += f.a_end;
       if (c > 0) {  // the last chunk's products are done: its stage, the operand buffer and S are free
         wait(bar_s + wg, (c - 1) & 1);
         tc::fence_after_sync();
-        if (i == 0) mbar_arrive(empty + ((c - 1) & 1));
+        if (lane == 0) mbar_arrive(empty + ((c - 1) & 1));
         __syncwarp();
       }
-      // ---- S: operand of C S, and decayed, in the new unit ----
-      const float sS = pow2_floor(bound) * (1.f / 8192.f);  // |S / sS| < 2^14
-      const float f_op = unit_in / sS, f_dec = dec * (unit_in / unit_new);
+      if (!kStatesOnly && warp == 0) {  // C B^T, once both heads have read the last chunk's
+        wait(full + stage, ph);
+        if (c > 0) wait(gfree, (c - 1) & 1);
+        if (lane == 0 && !dead) {
+          tc::fence_after_sync();
+          constexpr uint32_t id = idesc_f16(128, 128, false, false);
+          const unsigned char* st = smem + stage * kStageBytes;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
+            tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id, k > 0);
+          }
+          tc::mma_commit(bar_g);
+        }
+        __syncwarp();
+      }
+      auto refill = [&]() {  // warp 0: the next chunk's copies, into the last one's stage
+        if (warp == 0 && c > 0 && c + 1 < nchunks) {
+          wait(empty + ((c - 1) & 1), ((c - 1) >> 1) & 1);
+          if (lane == 0 && !dead) load(c + 1);
+          if (!dead) loaded = c + 2;
+          __syncwarp();
+        }
+      };
+      // ---- S: operand of C S, and decayed, in the new unit ----
+      {
         float v[32];
-        tc::tmem_ld32(tS + 32 * half, v);
+        tc::tmem_ld32(tS, v);
         if (!kStatesOnly) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            sts128(opnd + row + (((4 * half + k) ^ sw) << 4), pack_f16(v[8 * k] * f_op, v[8 * k + 1] * f_op),
-                   pack_f16(v[8 * k + 2] * f_op, v[8 * k + 3] * f_op), pack_f16(v[8 * k + 4] * f_op, v[8 * k + 5] * f_op),
-                   pack_f16(v[8 * k + 6] * f_op, v[8 * k + 7] * f_op));
+          for (int k = 0; k < 4; ++k) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 m = mul2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), make_float2(f_op, f_op));
+              o[j] = pack_f16(m.x, m.y);
+            }
+            sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= f_dec;
-        tmem_st32(tS + 32 * half, v);
+        for (int k = 0; k < 32; k += 2) {
+          const float2 m = mul2(make_float2(v[k], v[k + 1]), make_float2(f_dec, f_dec));
+          v[k] = m.x;
+          v[k + 1] = m.y;
+        }
+        tmem_st32(tS, v);
       }
-      unit = unit_new;
-      bound = fmaf(dec, bound, unit_new * 4.f * (meta.y / sdt));
-      total += a_end;
-      wait(full + stage, ph);
-      uint4 x[8];  // this token's row of X
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = lds128(sst + (4 + wg) * kTileBytes + row + ((k ^ sw) << 4));
-      const float wj = dtn * exp2_approx(a_end - a_i);
+      const float wj = dtn * exp2_approx(f.a_end - f.a_i);
+      uint4 x[4];  // this half of this token's row of X
       if (!kStatesOnly) {
-        const float l = a_i - log2f(dtn);  // +inf where dt is 0
-        lg[i] = l;
-        const float e = __shfl_sync(0xffffffffu, a_i, 31);  // the last token of the row's 32-token block
-        ej[i] = exp2_approx(e - l);
-        if (lane == 31) cend[q] = a_i;
+        // of the row's 32-token block: first and last token
+        const float a_first = __shfl_sync(0xffffffffu, f.a_i, 0), a_last = __shfl_sync(0xffffffffu, f.a_i, 31);
+        if (half == 0) {
+          // within the block exp(a_i - a_j) = exp(a_i - a_first) exp(a_first - a_j) as long as the second stays far
+          // from overflow; with more decay than 2^-100 in 32 tokens the exponents are subtracted first
+          fj[i] = a_first - a_last < 100.f ? exp2_approx(a_first - f.a_i) * dtn : f.a_i - __log2f(dtn);
+          if (lane == 31) cend[q] = f.a_i;
+        } else {
+          ej[i] = exp2_approx(a_last - f.a_i) * dtn;
+        }
         __syncwarp();
         tmem_wait_st();
         tc::fence_before_sync();
         tc::fence_proxy_async_smem();
-        named_bar_sync(bar_id, 128);
-        if (i == 0 && !dead) {  // Y = C S
+        named_bar_sync(bar_id, 256);
+        if (half == 0 && q == 0) wait(full + stage, ph);
+        if (lead && !dead) {  // Y = C S
           tc::fence_after_sync();
           constexpr uint32_t id = idesc_f16(128, 64, false, true);
 #pragma unroll
@@ -805,29 +899,55 @@ __global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptPar
           tc::mma_commit(bar_y2 + wg);
         }
         __syncwarp();
-        // ---- M from C B^T ----
-        wait(bar_g, c & 1);
+        refill();
+        // ---- M from C B^T: blocks half and half + 2 of 32 columns ----
+        wait(bar_g, c & 1);  // the chunk's operands are there too
         tc::fence_after_sync();
 #pragma unroll
-        for (int jb = 0; jb < 4; ++jb) {
+        for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int jb = 2 * jj + half;
           uint32_t m[16];
-          if (jb <= q) {
-            float v[32];
-            tc::tmem_ld32(tG + 32 * jb, v);
-            if (jb < q) {  // all of these tokens are earlier: exp(a_i - a_end) exp(a_end - a_j) dt_j, both at most 1
-              const float r = exp2_approx(a_i - cend[jb]);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) m[k] = pack_f16(v[2 * k] * (r * ej[32 * jb + 2 * k]), v[2 * k + 1] * (r * ej[32 * jb + 2 * k + 1]));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const float e0 = exp2_approx(a_i - lg[32 * jb + 2 * k]), e1 = exp2_approx(a_i - lg[32 * jb + 2 * k + 1]);
-                m[k] = pack_f16(2 * k <= lane ? v[2 * k] * e0 : 0.f, 2 * k + 1 <= lane ? v[2 * k + 1] * e1 : 0.f);
-              }
-            }
-          } else {
+          if (jb > q) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) m[k] = 0;
+            tmem_st16(tM + 16 * jb, m);
+            continue;
+          }
+          float v[32];
+          tc::tmem_ld32(tG + 32 * jb, v);
+          auto scaled = [&](const float* e, float2 r) {
+            const float4* e4 = reinterpret_cast<const float4*>(e + 32 * jb);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 f4 = e4[k];
+              const float2 m0 = mul2(mul2(make_float2(v[4 * k], v[4 * k + 1]), r), make_float2(f4.x, f4.y));
+              const float2 m1 = mul2(mul2(make_float2(v[4 * k + 2], v[4 * k + 3]), r), make_float2(f4.z, f4.w));
+              m[2 * k] = pack_f16(m0.x, m0.y);
+              m[2 * k + 1] = pack_f16(m1.x, m1.y);
+            }
+          };
+          if (jb < q) {  // an earlier block: exp(a_i - a_last) exp(a_last - a_j) dt_j, both at most 1
+            scaled(ej, splat(exp2_approx(f.a_i - cend[jb])));
+          } else {
+            if (a_first - a_last < 100.f) {
+              // v r first: r <= 1, and fj may be as large as 2^101
+              scaled(fj, splat(exp2_approx(f.a_i - a_first)));
+            } else {
+              const float4* l4 = reinterpret_cast<const float4*>(fj + 32 * jb);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float4 l = l4[k];
+                m[2 * k] = pack_f16(v[4 * k] * exp2_approx(f.a_i - l.x), v[4 * k + 1] * exp2_approx(f.a_i - l.y));
+                m[2 * k + 1] = pack_f16(v[4 * k + 2] * exp2_approx(f.a_i - l.z), v[4 * k + 3] * exp2_approx(f.a_i - l.w));
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {  // causal: columns up to the row's own
+              const uint32_t keep = 2 * k < lane ? 0xFFFFFFFFu : 2 * k == lane ? 0xFFFFu : 0u;
+              m[k] &= keep;
+            }
           }
           tmem_st16(tM + 16 * jb, m);
         }
@@ -838,33 +958,39 @@ __global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptPar
         // ---- Y = exp(a_i) C S, in the unit of M X ----
         wait(bar_y2 + wg, c & 1);
         tc::fence_after_sync();
-        const float f_y = exp2_approx(a_i) * (sS / unit_new);
+        const float f_y = exp2_approx(f.a_i) * (sS * runit);
+        float v[32];
+        tc::tmem_ld32(tY, v);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float v[32];
-          tc::tmem_ld32(tY + 32 * half, v);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] *= f_y;
-          tmem_st32(tY + 32 * half, v);
+        for (int k = 0; k < 32; k += 2) {
+          const float2 m = mul2(make_float2(v[k], v[k + 1]), make_float2(f_y, f_y));
+          v[k] = m.x;
+          v[k + 1] = m.y;
         }
+        tmem_st32(tY, v);
+      } else {
+        refill();
+        wait(full + stage, ph);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
       }
       // ---- weighted x ----
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_f16(u[j]);
-          o[j] = pack_f16(f.x * wj, f.y * wj);
+          const float2 m = mul2(unpack_f16(u[j]), make_float2(wj, wj));
+          o[j] = pack_f16(m.x, m.y);
         }
-        sts128(opnd + row + ((k ^ sw) << 4), o[0], o[1], o[2], o[3]);
+        sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
       }
       tmem_wait_st();
       tc::fence_before_sync();
       tc::fence_proxy_async_smem();
-      named_bar_sync(bar_id, 128);
-      if (i == 0 && !dead) {
+      named_bar_sync(bar_id, 256);
+      if (lead && !dead) {
         tc::fence_after_sync();
         if (!kStatesOnly) {  // Y += M X
           constexpr uint32_t id = idesc_f16(128, 64, false, true);
@@ -881,73 +1007,83 @@ __global__ void __launch_bounds__(288, 1) prompt_scan_mma_kernel(const PromptPar
       }
       __syncwarp();
       if (!kStatesOnly) {
+        // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
+        // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
+        const float2 fy = splat(f.sC * unit_new), dx = splat(D * f.sx);
+        const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
+        const int64_t tok = sg.start + tw;
+        const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
+        const int piece = 4 * half + (lane & 3), psw = (lane >> 2) & 7;  // rows 8 apart swizzle alike
+        uint4 zv[4];
+        if (p.gate) {
+          const __nv_bfloat16* z = p.zx + tok * p.ld + h * 64 + 8 * piece;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            zv[k] = tw + 8 * k < sg.len ? *reinterpret_cast<const uint4*>(z + 8 * k * p.ld) : make_uint4(0, 0, 0, 0);
+        }
         wait(bar_y + wg, c & 1);
         tc::fence_after_sync();
-        const int t = (c0 + c) * kChunk + i;
-        const float f = sC * unit_new, dx = D * sx;
-        const bool live = t < sg.len;
-        const int64_t token = sg.start + t;
-        const __nv_bfloat16* z = p.zx + token * p.ld + h * 64;
-        __nv_bfloat16* out = p.y + (token * p.nh + h) * 64;
+        if (p.gate) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float v[32];
-          tc::tmem_ld32(tY + 32 * half, v);
-          if (live) {
+          for (int k = 0; k < 4; ++k) sts128(stg + k * 1024 + ((piece ^ psw) << 4), zv[k].x, zv[k].y, zv[k].z, zv[k].w);
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint4 xv = x[4 * half + k];
-              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
-              uint32_t o[4];
-              uint4 zv = make_uint4(0, 0, 0, 0);
-              if (p.gate) zv = *reinterpret_cast<const uint4*>(z + 32 * half + 8 * k);
-              const uint32_t zu[4] = {zv.x, zv.y, zv.z, zv.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 xf = unpack_f16(u[j]);
-                float y0 = fmaf(v[8 * k + 2 * j], f, xf.x * dx), y1 = fmaf(v[8 * k + 2 * j + 1], f, xf.y * dx);
-                if (p.gate) {
-                  const float z0 = bf16lo(zu[j]), z1 = bf16hi(zu[j]);
-                  y0 *= __fdividef(z0, 1.f + __expf(-z0));
-                  y1 *= __fdividef(z1, 1.f + __expf(-z1));
-                }
-                const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
-                o[j] = *reinterpret_cast<const uint32_t*>(&b);
-              }
-              *reinterpret_cast<uint4*>(out + 32 * half + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-          }
+          for (int k = 0; k < 4; ++k) zv[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
           __syncwarp();
         }
+        float v[32];
+        tc::tmem_ld32(tY, v);
         tc::fence_before_sync();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, zu[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 y = fma2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), fy, mul2(unpack_f16(u[j]), dx));
+            if (p.gate) y = mul2(y, silu2(unpack_bf16(zu[j])));
+            const __nv_bfloat162 b = __floats2bfloat162_rn(y.x, y.y);
+            o[j] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          sts128(xrow + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+        }
+        __syncwarp();
+        __nv_bfloat16* out = p.y + (tok * p.nh + h) * 64 + 8 * piece;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 o = lds128(stg + k * 1024 + ((piece ^ psw) << 4));
+          if (tw + 8 * k < sg.len) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(8 * k) * p.nh * 64) = o;
+        }
+        tc::fence_proxy_async_smem();  // before the stage is handed back to the copies
+        __syncwarp();
       }
     }
     // ---- the state after the segment ----
     wait(bar_s + wg, (nchunks - 1) & 1);
-    tc::fence_after_sync();
     if (dead) mbar_wait_bounded(bar_s + wg, (nchunks - 1) & 1);
-    const bool last = sg.index + 1 == sg.count;
-    if (kStatesOnly || last) {
+    __syncwarp();
+    tc::fence_after_sync();
+    if (kStatesOnly || sg.index + 1 == sg.count) {
+      const int64_t at = static_cast<int64_t>(32 * half) * 128 + i;
+      float v[32];
+      tc::tmem_ld32(tS, v);
+      if (kStatesOnly) {
+        float* ws = wk.state + (static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h) * 64 * 128 + at;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float v[32];
-        tc::tmem_ld32(tS + 32 * half, v);
-        if (kStatesOnly) {
-          float* ws = wk.state + (static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h) * 64 * 128 + i;
+        for (int k = 0; k < 32; ++k) ws[k * 128] = v[k] * unit;
+        if (lead) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
+      } else {
+        __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) ws[(32 * half + k) * 128] = v[k] * unit;
-        } else {
-          __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + i;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) st[(32 * half + k) * 128] = __float2bfloat16_rn(v[k] * unit);
-        }
+        for (int k = 0; k < 32; ++k) st[k * 128] = __float2bfloat16_rn(v[k] * unit);
       }
-      if (kStatesOnly && i == 0) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
     }
   }
+  if (dead && tid == 0)  // copies in flight land before the CTA leaves
+    for (int c = max(0, loaded - 2); c < loaded; ++c) mbar_wait_bounded(full + (c & 1), (c >> 1) & 1);
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
 // ---- host: sizes of the tensor-core form ----
@@ -1063,7 +1199,8 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
   p.gate = gate ? 1 : 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   sn::ScanPlan plan;
-  const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y);
+  const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y) && sn::aligned16(conv_state) &&
+                      sn::aligned16(conv_weight) && (!conv_bias || sn::aligned16(conv_bias));
   // 64-element heads, 128 states, 16-byte rows: the tensor-core form
   if (d_conv >= 2 && d_conv <= 4 && rows16 &&
       sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan) && plan.chunks <= 65535 && plan.segments <= 65535) {
@@ -1082,7 +1219,7 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
     wk.blocks = plan.blocks;
     wk.seg = plan.seg;
     auto conv = d_conv == 4 ? sn::prompt_conv_tile_kernel<4> : d_conv == 3 ? sn::prompt_conv_tile_kernel<3> : sn::prompt_conv_tile_kernel<2>;
-    int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + 1), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
+    int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
     if (rc != SN_OK) return rc;
     const dim3 grid(static_cast<unsigned>(plan.pairs), static_cast<unsigned>(plan.segments));
     auto scan = [&](auto kern) {
@@ -1090,7 +1227,7 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
         cudaGetLastError();
         return SN_ERR_LAUNCH;
       }
-      return sn::launch(kern, grid, dim3(288), sn::kScanSmem, st, true, p, wk);
+      return sn::launch(kern, grid, dim3(sn::kScanThreads), sn::kScanSmem, st, true, p, wk);
     };
     if (tokens > static_cast<int64_t>(plan.seg) * sn::kChunk) {  // a prompt may have several segments
       rc = scan(sn::prompt_scan_mma_kernel<true>);
