@@ -781,11 +781,20 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       named_bar_sync(bar_id, 256);
     }
 
-    // a chunk's factors, loaded one chunk ahead
-    struct Factors {
+    // A chunk's inputs, loaded two chunks ahead, and what it needs of them, worked out one chunk ahead while the warp
+    // would wait for M X.
+    struct Inputs {
       float a_i, dt_i, a_end, sx, sB, sC;
       float2 meta;
     } next;
+    struct Factors {
+      float a_i, dtn;    // cumulative decay; dt / sdt
+      float dec, wj;     // the chunk's decay; the token's weight in the state
+      float f_op, f_dec;  // S to its operand; S to the new unit, decayed
+      float f_y;         // exp(a_i) C S from its operand's unit to that of M X
+      float fy, dx;      // M X and x' to outputs
+    } f;
+    float total = 0.f;  // log2 of the segment's decay
     const int chunk0 = sg.chunk0 + c0;
     auto fetch = [&](int c) {
       const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
@@ -799,43 +808,53 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       next.sB = sc[wk.xblocks + g];
       next.sC = sc[wk.xblocks + p.ng + g];
     };
+    auto derive = [&]() {
+      // every scale is a power of two: products and reciprocals of them are exact
+      const float sdt = pow2_floor(next.meta.x), rdt = rcp_pow2(sdt);
+      const float unit_new = next.sB * next.sx * sdt, runit = rcp_pow2(next.sB) * rcp_pow2(next.sx) * rdt;
+      const float sb = pow2_floor(bound), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
+      f.a_i = next.a_i;
+      f.dec = exp2_approx(next.a_end);
+      f.dtn = next.dt_i * rdt;
+      f.wj = f.dtn * exp2_approx(next.a_end - next.a_i);
+      f.f_op = unit * (rcp_pow2(sb) * 8192.f);
+      f.f_dec = f.dec * (unit * runit);
+      f.f_y = exp2_approx(next.a_i) * (sS * runit);
+      f.fy = next.sC * unit_new;
+      f.dx = D * next.sx;
+      unit = unit_new;
+      bound = fmaf(f.dec, bound, unit_new * 4.f * (next.meta.y * rdt));
+      total += next.a_end;
+    };
+    // C B^T of chunk c (warp 0), once both heads have read the last chunk's
+    auto issue_g = [&](int c) {
+      wait(full + (c & 1), (c >> 1) & 1);
+      if (c > 0) wait(gfree, (c - 1) & 1);
+      if (lane == 0 && !dead) {
+        tc::fence_after_sync();
+        constexpr uint32_t id = idesc_f16(128, 128, false, false);
+        const unsigned char* st = smem + (c & 1) * kStageBytes;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
+          tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id, k > 0);
+        }
+        tc::mma_commit(bar_g);
+      }
+      __syncwarp();
+    };
     fetch(0);
-    float total = 0.f;  // log2 of the segment's decay
+    derive();
+    if (nchunks > 1) fetch(1);
+    if (!kStatesOnly && warp == 0) issue_g(0);
     for (int c = 0; c < nchunks; ++c) {
       const unsigned stage = c & 1, ph = (c >> 1) & 1;
       const uint32_t sst = sbase + stage * kStageBytes;
       const uint32_t xrow = sst + (4 + wg) * kTileBytes + row;
-      const Factors f = next;
-      if (c + 1 < nchunks) fetch(c + 1);
-      // every scale is a power of two: products and reciprocals of them are exact
-      const float sdt = pow2_floor(f.meta.x), rdt = rcp_pow2(sdt), dec = exp2_approx(f.a_end);
-      const float unit_new = f.sB * f.sx * sdt, runit = rcp_pow2(f.sB) * rcp_pow2(f.sx) * rdt;
-      const float dtn = f.dt_i * rdt;
-      const float sb = pow2_floor(bound), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
-      const float f_op = unit * (rcp_pow2(sb) * 8192.f), f_dec = dec * (unit * runit);
-      unit = unit_new;
-      bound = fmaf(dec, bound, unit_new * 4.f * (f.meta.y * rdt));
-      total += f.a_end;
       if (c > 0) {  // the last chunk's products are done: its stage, the operand buffer and S are free
         wait(bar_s + wg, (c - 1) & 1);
         tc::fence_after_sync();
         if (lane == 0) mbar_arrive(empty + ((c - 1) & 1));
-        __syncwarp();
-      }
-      if (!kStatesOnly && warp == 0) {  // C B^T, once both heads have read the last chunk's
-        wait(full + stage, ph);
-        if (c > 0) wait(gfree, (c - 1) & 1);
-        if (lane == 0 && !dead) {
-          tc::fence_after_sync();
-          constexpr uint32_t id = idesc_f16(128, 128, false, false);
-          const unsigned char* st = smem + stage * kStageBytes;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
-            tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id, k > 0);
-          }
-          tc::mma_commit(bar_g);
-        }
         __syncwarp();
       }
       auto refill = [&]() {  // warp 0: the next chunk's copies, into the last one's stage
@@ -856,7 +875,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
             uint32_t o[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 m = mul2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), make_float2(f_op, f_op));
+              const float2 m = mul2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), splat(f.f_op));
               o[j] = pack_f16(m.x, m.y);
             }
             sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
@@ -864,13 +883,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         }
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float2 m = mul2(make_float2(v[k], v[k + 1]), make_float2(f_dec, f_dec));
+          const float2 m = mul2(make_float2(v[k], v[k + 1]), splat(f.f_dec));
           v[k] = m.x;
           v[k + 1] = m.y;
         }
         tmem_st32(tS, v);
       }
-      const float wj = dtn * exp2_approx(f.a_end - f.a_i);
       uint4 x[4];  // this half of this token's row of X
       if (!kStatesOnly) {
         // of the row's 32-token block: first and last token
@@ -878,10 +896,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         if (half == 0) {
           // within the block exp(a_i - a_j) = exp(a_i - a_first) exp(a_first - a_j) as long as the second stays far
           // from overflow; with more decay than 2^-100 in 32 tokens the exponents are subtracted first
-          fj[i] = a_first - a_last < 100.f ? exp2_approx(a_first - f.a_i) * dtn : f.a_i - __log2f(dtn);
+          fj[i] = a_first - a_last < 100.f ? exp2_approx(a_first - f.a_i) * f.dtn : f.a_i - __log2f(f.dtn);
           if (lane == 31) cend[q] = f.a_i;
         } else {
-          ej[i] = exp2_approx(a_last - f.a_i) * dtn;
+          ej[i] = exp2_approx(a_last - f.a_i) * f.dtn;
         }
         __syncwarp();
         tmem_wait_st();
@@ -958,12 +976,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         // ---- Y = exp(a_i) C S, in the unit of M X ----
         wait(bar_y2 + wg, c & 1);
         tc::fence_after_sync();
-        const float f_y = exp2_approx(f.a_i) * (sS * runit);
         float v[32];
         tc::tmem_ld32(tY, v);
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float2 m = mul2(make_float2(v[k], v[k + 1]), make_float2(f_y, f_y));
+          const float2 m = mul2(make_float2(v[k], v[k + 1]), splat(f.f_y));
           v[k] = m.x;
           v[k + 1] = m.y;
         }
@@ -981,7 +998,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 m = mul2(unpack_f16(u[j]), make_float2(wj, wj));
+          const float2 m = mul2(unpack_f16(u[j]), splat(f.wj));
           o[j] = pack_f16(m.x, m.y);
         }
         sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
@@ -1009,7 +1026,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       if (!kStatesOnly) {
         // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
         // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
-        const float2 fy = splat(f.sC * unit_new), dx = splat(D * f.sx);
+        const float2 fy = splat(f.fy), dx = splat(f.dx);
         const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
         const int64_t tok = sg.start + tw;
         const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
@@ -1020,6 +1037,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             zv[k] = tw + 8 * k < sg.len ? *reinterpret_cast<const uint4*>(z + 8 * k * p.ld) : make_uint4(0, 0, 0, 0);
+        }
+        if (c + 1 < nchunks) {
+          if (warp == 0) issue_g(c + 1);
+          derive();
+          if (c + 2 < nchunks) fetch(c + 2);
         }
         wait(bar_y + wg, c & 1);
         tc::fence_after_sync();
@@ -1056,6 +1078,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         }
         tc::fence_proxy_async_smem();  // before the stage is handed back to the copies
         __syncwarp();
+      } else if (c + 1 < nchunks) {
+        derive();
+        if (c + 2 < nchunks) fetch(c + 2);
       }
     }
     // ---- the state after the segment ----
