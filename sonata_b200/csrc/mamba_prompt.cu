@@ -650,18 +650,20 @@ __device__ __forceinline__ Segment find_segment(const Prompts& p, int seg, int i
 constexpr uint32_t kStageBytes = 6 * kTileBytes;
 constexpr uint32_t kOperandAt = 2 * kStageBytes;
 constexpr uint32_t kFactorsAt = kOperandAt + 2 * kTileBytes;
-constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 128;  // and their block ends
+constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 256;  // and their block ends, the chunks' factors
 constexpr uint32_t kScanSmem = kScanBytes + 128 /* barriers */ + 512;
 // Tensor memory columns: S of two heads, C B^T, M of two heads, Y of two heads.
 constexpr int kScanThreads = 2 * 256;
+constexpr int kServe = 4;  // the serving warp of a head's eight
 constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 
 // One segment of one pair of heads of a group (blockIdx.x: pair, blockIdx.y:
 // segment).  Warps 0-7 have the first head, 8-15 the second, a thread one row
 // (token i, or state n) and half of the columns of every product: 16 warps with
-// 128 registers each (a 17th for the copies would leave 96).  The first thread
-// of a head issues its products, that of the first head also the copies and
-// C B^T.  With kStatesOnly, the segment's state from nothing (from the
+// 128 registers each (a 17th for the copies would leave 96).  Of a head's warps
+// the one with the first 32 rows and the later columns has no part of M (it is
+// all above the diagonal), so it serves the others: it issues the products and
+// copies and works out the chunk's common factors.  With kStatesOnly, the segment's state from nothing (from the
 // prompt's state for its first segment) goes to slot index + 1 of the prompt,
 // and the prompt's state itself to slot 0; the last segment has nothing to do.
 template <bool kStatesOnly>
@@ -724,12 +726,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
   };
   int loaded = min(2, nchunks);  // chunks whose copies have been issued
-  if (tid == 0) {
+  if (tid == kServe * 32) {
     for (int c = 0; c < loaded; ++c) load(c);
   }
   if ((warp >> 3) < heads) {
     const int wg = warp >> 3, half = (warp >> 2) & 1, q = warp & 3, i = q * 32 + lane, h = h0 + wg;
-    const bool lead = half == 0 && i == 0;  // issues the head's products
+    const bool serving = (warp & 7) == kServe;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS = tmem + kColS + wg * 64 + 32 * half + lanes, tG = tmem + kColG + lanes,
                    tM = tmem + kColM + wg * 64 + lanes, tY = tmem + kColY + wg * 64 + 32 * half + lanes;
@@ -739,7 +741,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     float* cend = reinterpret_cast<float*>(smem + kFactorsAt + 2 * 2 * kChunk * 4) + wg * 16;  // [4]; first [8] maxima
     const uint32_t row = i * 128, sw = i & 7;
     const int bar_id = 1 + wg;
-    const float D = !kStatesOnly && p.D ? __bfloat162float(p.D[h]) : 0.f;
+    // the chunk's common factors, two buffers: 1 / sdt, a_end, S to its operand, S to the new unit and decayed;
+    // C S from its operand's unit to that of M X, M X to outputs, x' to D x
+    float4* common = reinterpret_cast<float4*>(smem + kFactorsAt + 2 * 2 * kChunk * 4 + 128) + wg * 4;
 
     // ---- the state before the segment: row n = i of S^T, this half's 32 columns, true values ----
     float unit = 1.f, bound = 0.f;  // S = unit * tensor memory; |S| <= bound
@@ -778,75 +782,92 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       named_bar_sync(bar_id, 256);
 #pragma unroll
       for (int k = 0; k < 8; ++k) bound = fmaxf(bound, cend[k]);
-      named_bar_sync(bar_id, 256);
     }
 
-    // A chunk's inputs, loaded two chunks ahead, and what it needs of them, worked out one chunk ahead while the warp
-    // would wait for M X.
-    struct Inputs {
-      float a_i, dt_i, a_end, sx, sB, sC;
-      float2 meta;
-    } next;
-    struct Factors {
-      float a_i, dtn;    // cumulative decay; dt / sdt
-      float dec, wj;     // the chunk's decay; the token's weight in the state
-      float f_op, f_dec;  // S to its operand; S to the new unit, decayed
-      float f_y;         // exp(a_i) C S from its operand's unit to that of M X
-      float fy, dx;      // M X and x' to outputs
-    } f;
-    float total = 0.f;  // log2 of the segment's decay
+    // Inputs of a chunk: a token's own for every thread, the head's for the serving warp; loaded a chunk ahead.
     const int chunk0 = sg.chunk0 + c0;
+    float next_a, next_dt;
     auto fetch = [&](int c) {
+      const int64_t at = (static_cast<int64_t>(chunk0 + c) * p.nh + h) * kChunk + i;
+      next_a = wk.cum[at];
+      next_dt = wk.dt[at];
+    };
+    struct {
+      float a_end, sx, sB, sC;
+      float2 meta;
+    } head;
+    auto fetch_head = [&](int c) {
       const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
-      const float* cum = wk.cum + th * kChunk;
       const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * wk.blocks;
-      next.a_i = cum[i];
-      next.a_end = cum[kChunk - 1];
-      next.dt_i = wk.dt[th * kChunk + i];
-      next.meta = wk.meta[th];
-      next.sx = sc[h / 2];
-      next.sB = sc[wk.xblocks + g];
-      next.sC = sc[wk.xblocks + p.ng + g];
+      head.a_end = wk.cum[th * kChunk + kChunk - 1];
+      head.meta = wk.meta[th];
+      head.sx = sc[h / 2];
+      head.sB = sc[wk.xblocks + g];
+      head.sC = sc[wk.xblocks + p.ng + g];
     };
-    auto derive = [&]() {
-      // every scale is a power of two: products and reciprocals of them are exact
-      const float sdt = pow2_floor(next.meta.x), rdt = rcp_pow2(sdt);
-      const float unit_new = next.sB * next.sx * sdt, runit = rcp_pow2(next.sB) * rcp_pow2(next.sx) * rdt;
+    const float D = serving && !kStatesOnly && p.D ? __bfloat162float(p.D[h]) : 0.f;
+    float total = 0.f;  // log2 of the segment's decay
+    auto derive_head = [&](int c) {  // every scale is a power of two: products and reciprocals of them are exact
+      const float sdt = pow2_floor(head.meta.x), rdt = rcp_pow2(sdt), dec = exp2_approx(head.a_end);
+      const float unit_new = head.sB * head.sx * sdt, runit = rcp_pow2(head.sB) * rcp_pow2(head.sx) * rdt;
       const float sb = pow2_floor(bound), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
-      f.a_i = next.a_i;
-      f.dec = exp2_approx(next.a_end);
-      f.dtn = next.dt_i * rdt;
-      f.wj = f.dtn * exp2_approx(next.a_end - next.a_i);
-      f.f_op = unit * (rcp_pow2(sb) * 8192.f);
-      f.f_dec = f.dec * (unit * runit);
-      f.f_y = exp2_approx(next.a_i) * (sS * runit);
-      f.fy = next.sC * unit_new;
-      f.dx = D * next.sx;
+      if (lane == 0) {
+        common[2 * (c & 1)] = make_float4(rdt, head.a_end, unit * (rcp_pow2(sb) * 8192.f), dec * (unit * runit));
+        common[2 * (c & 1) + 1] = make_float4(sS * runit, head.sC * unit_new, D * head.sx, unit_new);
+      }
       unit = unit_new;
-      bound = fmaf(f.dec, bound, unit_new * 4.f * (next.meta.y * rdt));
-      total += next.a_end;
+      bound = fmaf(dec, bound, unit_new * 4.f * (head.meta.y * rdt));
+      total += head.a_end;
     };
-    // C B^T of chunk c (warp 0), once both heads have read the last chunk's
+    struct Factors {
+      float a_i, dtn;     // cumulative decay; dt / sdt
+      float wj;           // the token's weight in the state
+      float f_op, f_dec;  // as common
+      float f_y;          // exp(a_i) C S, likewise
+      float fy, dx;
+    } f;
+    float unit_last = 1.f;
+    auto take = [&](int c) {
+      const float4 u = common[2 * (c & 1)], w = common[2 * (c & 1) + 1];
+      f.a_i = next_a;
+      f.dtn = next_dt * u.x;
+      f.wj = f.dtn * exp2_approx(u.y - next_a);
+      f.f_op = u.z;
+      f.f_dec = u.w;
+      f.f_y = exp2_approx(next_a) * w.x;
+      f.fy = w.y;
+      f.dx = w.z;
+      unit_last = w.w;
+    };
+    // C B^T of chunk c (the second head's serving warp, if there is one), once both heads have read the last chunk's
     auto issue_g = [&](int c) {
       wait(full + (c & 1), (c >> 1) & 1);
       if (c > 0) wait(gfree, (c - 1) & 1);
       if (lane == 0 && !dead) {
         tc::fence_after_sync();
         constexpr uint32_t id = idesc_f16(128, 128, false, false);
-        const unsigned char* st = smem + (c & 1) * kStageBytes;
+        const uint64_t db = tc::smem_desc_sw128(smem + (c & 1) * kStageBytes), dc = db + 2 * kTileBytes / 16;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t at = (k >> 2) * kTileBytes + (k & 3) * 32;
-          tc::mma_bf16(tmem + kColG, tc::smem_desc_sw128(st + 2 * kTileBytes + at), tc::smem_desc_sw128(st + at), id, k > 0);
+          const uint32_t at = ((k >> 2) * kTileBytes + (k & 3) * 32) / 16;
+          tc::mma_bf16(tmem + kColG, dc + at, db + at, id, k > 0);
         }
         tc::mma_commit(bar_g);
       }
       __syncwarp();
     };
+    const bool issues_g = !kStatesOnly && serving && wg == heads - 1;
     fetch(0);
-    derive();
+    if (serving) {
+      fetch_head(0);
+      derive_head(0);
+      if (nchunks > 1) fetch_head(1);
+    }
+    named_bar_sync(bar_id, 256);
+    take(0);
     if (nchunks > 1) fetch(1);
-    if (!kStatesOnly && warp == 0) issue_g(0);
+    if (issues_g) issue_g(0);
+    const uint64_t d_op = desc_k_rows(opnd, 16);
     for (int c = 0; c < nchunks; ++c) {
       const unsigned stage = c & 1, ph = (c >> 1) & 1;
       const uint32_t sst = sbase + stage * kStageBytes;
@@ -857,8 +878,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         if (lane == 0) mbar_arrive(empty + ((c - 1) & 1));
         __syncwarp();
       }
-      auto refill = [&]() {  // warp 0: the next chunk's copies, into the last one's stage
-        if (warp == 0 && c > 0 && c + 1 < nchunks) {
+      auto refill = [&]() {  // the next chunk's copies, into the last one's stage
+        if (warp == kServe && c > 0 && c + 1 < nchunks) {
           wait(empty + ((c - 1) & 1), ((c - 1) >> 1) & 1);
           if (lane == 0 && !dead) load(c + 1);
           if (!dead) loaded = c + 2;
@@ -906,18 +927,24 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         tc::fence_before_sync();
         tc::fence_proxy_async_smem();
         named_bar_sync(bar_id, 256);
-        if (half == 0 && q == 0) wait(full + stage, ph);
-        if (lead && !dead) {  // Y = C S
-          tc::fence_after_sync();
-          constexpr uint32_t id = idesc_f16(128, 64, false, true);
+        if (serving) {
+          wait(full + stage, ph);
+          if (lane == 0 && !dead) {  // Y = C S
+            tc::fence_after_sync();
+            constexpr uint32_t id = idesc_f16(128, 64, false, true);
+            const uint64_t dc = tc::smem_desc_sw128(smem + stage * kStageBytes + 2 * kTileBytes);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            tc::mma_bf16(tmem + kColY + wg * 64, tc::smem_desc_sw128(smem + stage * kStageBytes + (2 + (k >> 2)) * kTileBytes + (k & 3) * 32),
-                         desc_k_rows(opnd + k * 2048, 16), id, k > 0);
-          tc::mma_commit(bar_y2 + wg);
+            for (int k = 0; k < 8; ++k)
+              tc::mma_bf16(tmem + kColY + wg * 64, dc + ((k >> 2) * kTileBytes + (k & 3) * 32) / 16, d_op + k * 128, id, k > 0);
+            tc::mma_commit(bar_y2 + wg);
+          }
+          __syncwarp();
+          refill();
+          if (c + 1 < nchunks) {
+            derive_head(c + 1);
+            if (c + 2 < nchunks) fetch_head(c + 2);
+          }
         }
-        __syncwarp();
-        refill();
         // ---- M from C B^T: blocks half and half + 2 of 32 columns ----
         wait(bar_g, c & 1);  // the chunk's operands are there too
         tc::fence_after_sync();
@@ -987,6 +1014,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         tmem_st32(tY, v);
       } else {
         refill();
+        if (serving && c + 1 < nchunks) {
+          derive_head(c + 1);
+          if (c + 2 < nchunks) fetch_head(c + 2);
+        }
         wait(full + stage, ph);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
@@ -1007,22 +1038,26 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       tc::fence_before_sync();
       tc::fence_proxy_async_smem();
       named_bar_sync(bar_id, 256);
-      if (lead && !dead) {
-        tc::fence_after_sync();
-        if (!kStatesOnly) {  // Y += M X
-          constexpr uint32_t id = idesc_f16(128, 64, false, true);
+      if (serving) {
+        if (lane == 0 && !dead) {
+          tc::fence_after_sync();
+          if (!kStatesOnly) {  // Y += M X
+            constexpr uint32_t id = idesc_f16(128, 64, false, true);
+            const uint64_t dx = desc_k_rows(sst + (4 + wg) * kTileBytes, 16);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_f16_ts(tmem + kColY + wg * 64, tmem + kColM + wg * 64 + 8 * k, desc_k_rows(sst + (4 + wg) * kTileBytes + k * 2048, 16), id, 1);
-          tc::mma_commit(bar_y + wg);
+            for (int k = 0; k < 8; ++k)
+              mma_f16_ts(tmem + kColY + wg * 64, tmem + kColM + wg * 64 + 8 * k, dx + k * 128, id, 1);
+            tc::mma_commit(bar_y + wg);
+          }
+          constexpr uint32_t id = idesc_f16(128, 64, true, true);  // S += B^T (w x)
+          const uint64_t db = desc_k_rows(sst, kTileBytes);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) tc::mma_bf16(tmem + kColS + wg * 64, db + k * 128, d_op + k * 128, id, 1);
+          tc::mma_commit(bar_s + wg);
         }
-        constexpr uint32_t id = idesc_f16(128, 64, true, true);  // S += B^T (w x)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          tc::mma_bf16(tmem + kColS + wg * 64, desc_k_rows(sst + k * 2048, kTileBytes), desc_k_rows(opnd + k * 2048, 16), id, 1);
-        tc::mma_commit(bar_s + wg);
+        __syncwarp();
+        if (issues_g && c + 1 < nchunks) issue_g(c + 1);
       }
-      __syncwarp();
       if (!kStatesOnly) {
         // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
         // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
@@ -1039,8 +1074,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
             zv[k] = tw + 8 * k < sg.len ? *reinterpret_cast<const uint4*>(z + 8 * k * p.ld) : make_uint4(0, 0, 0, 0);
         }
         if (c + 1 < nchunks) {
-          if (warp == 0) issue_g(c + 1);
-          derive();
+          take(c + 1);
           if (c + 2 < nchunks) fetch(c + 2);
         }
         wait(bar_y + wg, c & 1);
@@ -1079,7 +1113,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         tc::fence_proxy_async_smem();  // before the stage is handed back to the copies
         __syncwarp();
       } else if (c + 1 < nchunks) {
-        derive();
+        take(c + 1);
         if (c + 2 < nchunks) fetch(c + 2);
       }
     }
@@ -1095,16 +1129,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       if (kStatesOnly) {
         float* ws = wk.state + (static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h) * 64 * 128 + at;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) ws[k * 128] = v[k] * unit;
-        if (lead) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
+        for (int k = 0; k < 32; ++k) ws[k * 128] = v[k] * unit_last;
+        if (serving && lane == 0) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
       } else {
         __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) st[k * 128] = __float2bfloat16_rn(v[k] * unit);
+        for (int k = 0; k < 32; ++k) st[k * 128] = __float2bfloat16_rn(v[k] * unit_last);
       }
     }
   }
-  if (dead && tid == 0)  // copies in flight land before the CTA leaves
+  if (dead && tid == kServe * 32)  // copies in flight land before the CTA leaves
     for (int c = max(0, loaded - 2); c < loaded; ++c) mbar_wait_bounded(full + (c & 1), (c >> 1) & 1);
   tc::fence_before_sync();
   __syncthreads();
