@@ -62,6 +62,10 @@ __device__ __forceinline__ bool prompt_bounds(const Prompts& p, int b0, int& upt
 __device__ __forceinline__ PromptBlock find_block(const Prompts& p, int rows, int least, int index) {
   const int lane = threadIdx.x & 31;
   int before = 0, last = 0;
+  if (p.batch == 1 && !p.cu) {
+    const int n = max((p.tokens + rows - 1) / rows, least);
+    return {index < n ? 0 : -1, 0, p.tokens, index, n};
+  }
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     int s, e;
     if (prompt_bounds(p, b0, last, s, e)) record_status(SN_ERR_INVALID_ARGUMENT);
@@ -273,10 +277,10 @@ struct ChunkWork {  // workspace arrays; chunks are counted over all prompts
   int seg;              // chunks a segment
 };
 
-// The power of two at or below |v| (at least 2^-24); 1 for 0, infinities and NaN.
-__device__ __forceinline__ float pow2_floor(float v) {
+// The power of two at or below |v| (at least 2^-least); 1 for 0, infinities and NaN.
+__device__ __forceinline__ float pow2_floor(float v, uint32_t least = 24) {
   const uint32_t e = (__float_as_uint(v) >> 23) & 255u;
-  return e == 0 || e == 255 ? 1.f : __uint_as_float(max(e, 127u - 24u) << 23);
+  return e == 0 || e == 255 ? 1.f : __uint_as_float(max(e, 127u - least) << 23);
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
@@ -387,12 +391,23 @@ __device__ __forceinline__ void prompt_dt(const PromptParams& p, const ChunkWork
   }
 }
 
+// Column k of 8 channels' convolution state [8][W].
+template <int W>
+__device__ __forceinline__ uint4 state_column(const __nv_bfloat16* st, int k) {
+  uint32_t v[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    v[c] = static_cast<uint32_t>(__bfloat16_as_ushort(st[2 * c * W + k])) |
+           static_cast<uint32_t>(__bfloat16_as_ushort(st[(2 * c + 1) * W + k])) << 16;
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // One 128-channel block of one chunk (blockIdx.x < blocks), or 16 heads' dt
 // and decays.  Thread: 8 channels, 8 tokens.  Reads the inputs and writes the
 // tiles once: bounded by HBM (and, half as much, by the two special functions
 // of a SiLU).
 template <int W>
-__global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+__global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ float s_dt[kDtHeads * 129];
   __shared__ float s_max[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -414,9 +429,11 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
   }
 
   float top = 0.f;
-  float2 out[8][4];  // [token][pair of channels]
+  uint32_t out[4][8];  // [pair of channels][token], fp16 over the pair's own power of two
+  float own[4];
   if (on) {
     const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
+    const __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
     uint4 raw[W + 7];  // inputs t0 + r0 - W + 1 .. t0 + r0 + 7
 #pragma unroll
     for (int k = 0; k < W + 7; ++k) {
@@ -424,87 +441,50 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
       raw[k] = make_uint4(0, 0, 0, 0);
       if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u + t * p.ld);
     }
-    float2 w[W][4], bias[4];
-    {
-      const __nv_bfloat16* wr = p.w + static_cast<int64_t>(d) * W;  // [8][W], 16 W bytes from a 16-byte boundary
-      uint32_t wu[4 * W];
+    uint32_t wu[4 * W];  // [8][W] taps, 16 W bytes from a 16-byte boundary
 #pragma unroll
-      for (int k = 0; k < W; ++k) *reinterpret_cast<uint4*>(wu + 4 * k) = reinterpret_cast<const uint4*>(wr)[k];
-      auto at = [&](int e) { return e & 1 ? bf16hi(wu[e / 2]) : bf16lo(wu[e / 2]); };
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) w[k][c] = make_float2(at(2 * c * W + k), at((2 * c + 1) * W + k));
-      }
-      uint4 bu = make_uint4(0, 0, 0, 0);
-      if (p.bias) bu = *reinterpret_cast<const uint4*>(p.bias + d);
-      bias[0] = unpack_bf16(bu.x);
-      bias[1] = unpack_bf16(bu.y);
-      bias[2] = unpack_bf16(bu.z);
-      bias[3] = unpack_bf16(bu.w);
-    }
+    for (int k = 0; k < W; ++k)
+      *reinterpret_cast<uint4*>(wu + 4 * k) = reinterpret_cast<const uint4*>(p.w + static_cast<int64_t>(d) * W)[k];
+    uint4 bu = make_uint4(0, 0, 0, 0);
+    if (p.bias) bu = *reinterpret_cast<const uint4*>(p.bias + d);
     if (t0 + r0 == 0) {  // the prompt's first tokens: inputs before them are the state's columns 1 .. W - 1
-      __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
-      uint32_t old[4 * W];  // element c * W + k
 #pragma unroll
-      for (int k = 0; k < W; ++k) *reinterpret_cast<uint4*>(old + 4 * k) = reinterpret_cast<const uint4*>(st)[k];
-      auto at = [&](int e) { return (old[e / 2] >> (16 * (e & 1))) & 0xFFFFu; };
-#pragma unroll
-      for (int k = 0; k < W - 1; ++k) {
-        uint32_t v[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = at(2 * c * W + k + 1) | at((2 * c + 1) * W + k + 1) << 16;
-        raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
-      }
-      // and the state after the prompt, its last W inputs (only this thread reads or writes these channels' state)
-      uint32_t moved[8 * W];
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int t = pb.len - W + k;  // < 0: the old state's column W + t = k + len
-        if (t >= 0) {
-          const uint4 v = *reinterpret_cast<const uint4*>(u + t * p.ld);
-          const uint32_t vu[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int c = 0; c < 8; ++c) moved[c * W + k] = (vu[c / 2] >> (16 * (c & 1))) & 0xFFFFu;
-        } else {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            moved[c * W + k] = at(c * W + W - 1);
-#pragma unroll
-            for (int j = 0; j < W - 1; ++j)
-              if (j == pb.len + k) moved[c * W + k] = at(c * W + j);
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-        reinterpret_cast<uint4*>(st)[k] =
-            make_uint4(moved[8 * k] | moved[8 * k + 1] << 16, moved[8 * k + 2] | moved[8 * k + 3] << 16,
-                       moved[8 * k + 4] | moved[8 * k + 5] << 16, moved[8 * k + 6] | moved[8 * k + 7] << 16);
+      for (int k = 0; k < W - 1; ++k) raw[k] = state_column<W>(st, k + 1);
     }
+    const bool partial = t0 + kChunk > pb.len;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int c = 0; c < 4; ++c) {  // a pair of channels: few registers live at a time
+      auto tap = [&](int k) {
+        const int e0 = 2 * c * W + k, e1 = e0 + W;
+        return make_float2(e0 & 1 ? bf16hi(wu[e0 / 2]) : bf16lo(wu[e0 / 2]), e1 & 1 ? bf16hi(wu[e1 / 2]) : bf16lo(wu[e1 / 2]));
+      };
+      auto word = [&](const uint4& v) { return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w; };
+      float2 w[W], o[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) out[r][c] = bias[c];
-    }
+      for (int k = 0; k < W; ++k) w[k] = tap(k);
 #pragma unroll
-    for (int k = 0; k < W + 7; ++k) {  // each input once, into the outputs it belongs to
-      const float2 v[4] = {unpack_bf16(raw[k].x), unpack_bf16(raw[k].y), unpack_bf16(raw[k].z), unpack_bf16(raw[k].w)};
+      for (int r = 0; r < 8; ++r) o[r] = unpack_bf16(word(bu));
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int r = k - j;  // tap j of output r
-        if (r < 0 || r > 7) continue;
+      for (int k = 0; k < W + 7; ++k) {  // each input once, into the outputs it belongs to
+        const float2 v = unpack_bf16(word(raw[k]));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) out[r][c] = fma2(v[c], w[j][c], out[r][c]);
+        for (int j = 0; j < W; ++j)
+          if (k - j >= 0 && k - j < 8) o[k - j] = fma2(v, w[j], o[k - j]);
       }
-    }
+      float most = 0.f;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const bool live = t0 + r0 + r < pb.len;
+      for (int r = 0; r < 8; ++r) {
+        o[r] = silu2(o[r]);
+        if (partial && t0 + r0 + r >= pb.len) o[r] = make_float2(0.f, 0.f);
+        most = fmaxf(fmaxf(most, fabsf(o[r].x)), fabsf(o[r].y));
+      }
+      top = fmaxf(top, most);
+      own[c] = most == 0.f ? 0.f : pow2_floor(most);
+      const float2 inv = splat(most == 0.f ? 1.f : rcp_pow2(own[c]));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        out[r][c] = live ? silu2(out[r][c]) : make_float2(0.f, 0.f);
-        top = fmaxf(fmaxf(top, fabsf(out[r][c].x)), fabsf(out[r][c].y));
+      for (int r = 0; r < 8; ++r) {
+        const float2 v = mul2(o[r], inv);
+        out[c][r] = pack_f16(v.x, v.y);
       }
     }
   }
@@ -517,7 +497,6 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
   const float sc = pow2_floor(top);
   if (tid == 0) wk.scale[chunk * wk.blocks + blk] = sc;
   if (!on) return;
-  const float2 inv = splat(rcp_pow2(sc));
   // tile of these channels, chunk c8 % 8 of its rows
   unsigned char* tile;
   if (blk < wk.xblocks) {
@@ -527,16 +506,38 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
     tile = (g < p.ng ? wk.b + (chunk * p.ng + g) * 2 * kTileBytes : wk.c + (chunk * p.ng + g - p.ng) * 2 * kTileBytes) +
            (c8 >> 3) * kTileBytes;
   }
+  // to the block's power of two: exact but for what falls below 2^-24 of it
+  __half2 f[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) f[c] = __float2half2_rn(own[c] * rcp_pow2(sc));
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int row = r0 + r;  // row % 8 == r
     uint32_t o[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float2 v = mul2(out[r][c], inv);
-      o[c] = pack_f16(v.x, v.y);
+      const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[c][r]), f[c]);
+      o[c] = *reinterpret_cast<const uint32_t*>(&v);
     }
     *reinterpret_cast<uint4*>(tile + row * 128 + (((c8 & 7) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  if (t0 + r0 == 0) {  // the state after the prompt, its last W inputs; no other thread reads or writes these channels'
+    __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;
+    const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
+    uint4 col[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const int t = pb.len - W + k;  // < 0: the old state's column W + t
+      col[k] = t >= 0 ? *reinterpret_cast<const uint4*>(u + t * p.ld) : state_column<W>(st, W + t);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint32_t v = c / 2 == 0 ? col[k].x : c / 2 == 1 ? col[k].y : c / 2 == 2 ? col[k].z : col[k].w;
+        st[c * W + k] = __ushort_as_bfloat16(static_cast<unsigned short>(c & 1 ? v >> 16 : v & 0xFFFFu));
+      }
+    }
   }
 }
 
@@ -607,6 +608,12 @@ struct Segment {
 };
 __device__ __forceinline__ Segment find_segment(const Prompts& p, int seg, int index) {
   const int lane = threadIdx.x & 31;
+  if (p.batch == 1) {
+    const int s = min(max(p.cu ? p.cu[0] : 0, 0), p.tokens), e = max(min(p.cu ? p.cu[1] : p.tokens, p.tokens), s);
+    const int n = ((e - s + kChunk - 1) / kChunk + seg - 1) / seg;
+    if (index >= n) return {-1, 0, 0, 0, 0, 0, 0};
+    return {0, s, e - s, index, n, 0, 0};
+  }
   int before = 0, chunks = 0, slots = 0, last = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     int s, e;
@@ -644,6 +651,231 @@ __device__ __forceinline__ Segment find_segment(const Prompts& p, int seg, int i
   return {-1, 0, 0, 0, 0, 0, 0};
 }
 
+constexpr int kScanThreads = 512;
+// What both kernels of the scan start with: their heads (a pair within a
+// group), segment and chunks, and a place on a 1024-byte boundary.
+struct ScanWork {
+  Segment sg;
+  int g, h0, heads, c0, chunks;
+};
+__device__ __forceinline__ ScanWork scan_work(const PromptParams& p, const ChunkWork& wk) {
+  ScanWork r;
+  const int ppg = (p.hpg + 1) / 2;
+  r.g = blockIdx.x / ppg;
+  r.h0 = r.g * p.hpg + (blockIdx.x - r.g * ppg) * 2;
+  r.heads = min(2, (r.g + 1) * p.hpg - r.h0);
+  r.sg = find_segment(p.prompts, wk.seg, blockIdx.y);
+  r.c0 = r.sg.index * wk.seg;
+  r.chunks = min(wk.seg, (r.sg.len + kChunk - 1) / kChunk - r.c0);
+  return r;
+}
+__device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
+  const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u;
+  if (pad > 512) {  // does not happen: dynamic shared memory starts on a 1024-byte boundary
+    record_status(SN_ERR_MISALIGNED);
+    return nullptr;
+  }
+  return raw + pad;
+}
+
+// ---------------------------------------------------------------------------
+// The states of segments.  From the last chunk of a segment backwards every
+// token's weight to the segment's end is known as it comes, so the whole
+// segment is one accumulation S += B^T (w x) in tensor memory, with nothing
+// to wait for between chunks: 16 warps scale x in place, a 17th copies and
+// issues.  The segment's state from nothing goes to slot index + 1 of the
+// prompt; the first segment's starts from the prompt's state, which itself
+// goes to slot 0 (the last segment's CTAs of the next launch overwrite it).
+// The last segment has nothing to do.  Bounded by the reads of x.
+// ---------------------------------------------------------------------------
+constexpr int kStateStages = 3;
+constexpr uint32_t kStateStage = 4 * kTileBytes;  // B, then x of two heads
+constexpr uint32_t kStateBytes = kStateStages * kStateStage;
+constexpr uint32_t kStateSmem = kStateBytes + 128 /* barriers */ + 512;
+
+__global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(const PromptParams p, const ChunkWork wk) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned char* smem = aligned_smem(smem_raw);
+  if (!smem) return;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStateBytes);
+  uint64_t *full = bars, *ready = bars + kStateStages, *empty = bars + 2 * kStateStages, *done = bars + 3 * kStateStages;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+  float *s_unit = reinterpret_cast<float*>(done + 2), *s_total = s_unit + 2;
+  pdl_launch_dependents();
+  pdl_wait();
+  const ScanWork w = scan_work(p, wk);
+  const Segment& sg = w.sg;
+  if (sg.seq < 0 || sg.index + 1 >= sg.count) return;  // the same in every warp
+  const int last = sg.chunk0 + w.c0 + w.chunks - 1;  // chunks go from here down
+  auto load = [&](int k) {  // one thread
+    const int st = k % kStateStages;
+    const int64_t chunk = last - k;
+    const uint32_t at = smem_u32(smem) + st * kStateStage;
+    mbar_arrive_expect_tx(full + st, (2 + w.heads) * kTileBytes);
+    bulk_load(at, wk.b + (chunk * p.ng + w.g) * 2 * kTileBytes, 2 * kTileBytes, full + st);
+    bulk_load(at + 2 * kTileBytes, wk.x + (chunk * p.nh + w.h0) * kTileBytes, w.heads * kTileBytes, full + st);
+  };
+  int loaded = 0;
+  if (tid == 16 * 32) {
+    for (int i = 0; i < kStateStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(ready + i, 16);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+    for (; loaded < min(kStateStages, w.chunks); ++loaded) load(loaded);
+  }
+  __syncwarp();
+  if (warp == 16) tc::tmem_alloc(tslot, 128);
+  if (warp < w.heads) {
+    // the unit of the sum: the largest of the chunks' units, decayed to the segment's end
+    const int h = w.h0 + warp;
+    float after = 0.f, top = 0.f;
+    for (int k0 = 0; k0 < w.chunks; k0 += 32) {
+      const int k = k0 + lane;
+      float a = 0.f, u = 0.f;
+      if (k < w.chunks) {
+        const int64_t chunk = last - k, th = chunk * p.nh + h;
+        a = wk.cum[th * kChunk + kChunk - 1];
+        u = wk.scale[chunk * wk.blocks + h / 2] * wk.scale[chunk * wk.blocks + wk.xblocks + w.g] * pow2_floor(wk.meta[th].x);
+      }
+      float upto = a;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      top = fmaxf(top, u * exp2_approx(after + upto - a));
+      after += __shfl_sync(0xffffffffu, upto, 31);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) {
+      s_unit[warp] = pow2_floor(top, 100);
+      s_total[warp] = after;
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tslot;
+  bool dead = false;
+
+  if (warp == 16) {
+    if (lane == 0) {
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait_bounded(bar, parity)) {
+          record_status(SN_ERR_TIMEOUT);
+          dead = true;
+        }
+      };
+      constexpr uint32_t id = idesc_f16(128, 64, true, true);  // S^T += B^T (w x)
+      for (int k = 0; k < w.chunks && !dead; ++k) {
+        const int st = k % kStateStages;
+        wait(ready + st, (k / kStateStages) & 1);
+        if (dead) break;
+        tc::fence_after_sync();
+        const uint32_t at = smem_u32(smem) + st * kStateStage;
+        const uint64_t db = desc_k_rows(at, kTileBytes);
+        for (int h = 0; h < w.heads; ++h) {
+          const uint64_t dx = desc_k_rows(at + (2 + h) * kTileBytes, 16);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) tc::mma_bf16(tmem + 64 * h, db + j * 128, dx + j * 128, id, k > 0 || j > 0);
+        }
+        tc::mma_commit(empty + st);
+        if (k + 1 == w.chunks) tc::mma_commit(done);
+        // the stage of the chunk before this one is free once its products are done: this one's run meanwhile
+        if (k > 0 && loaded < w.chunks) {
+          wait(empty + (k - 1) % kStateStages, ((k - 1) / kStateStages) & 1);
+          if (!dead) load(loaded++);
+        }
+      }
+      if (dead)  // copies in flight land before the CTA leaves
+        for (int k = max(0, loaded - kStateStages); k < loaded; ++k)
+          mbar_wait_bounded(full + k % kStateStages, (k / kStateStages) & 1);
+    }
+    __syncwarp();
+  } else {
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!__all_sync(0xffffffffu, dead || mbar_wait_bounded(bar, parity))) {
+        record_status(SN_ERR_TIMEOUT);
+        dead = true;
+      }
+    };
+    // token, head and half of its 64 elements
+    const int i = tid >> 2, hh = (tid >> 1) & 1, half = tid & 1, h = w.h0 + min(hh, w.heads - 1);
+    const bool on = hh < w.heads;
+    float a_i, a_end, dt, sx, sB;
+    auto fetch = [&](int k) {
+      const int64_t chunk = last - k, th = chunk * p.nh + h;
+      a_i = wk.cum[th * kChunk + i];
+      a_end = wk.cum[th * kChunk + kChunk - 1];
+      dt = wk.dt[th * kChunk + i];
+      sx = wk.scale[chunk * wk.blocks + h / 2];
+      sB = wk.scale[chunk * wk.blocks + wk.xblocks + w.g];
+    };
+    fetch(0);
+    const float runit = rcp_pow2(s_unit[h - w.h0]);
+    float after = 0.f;  // log2 of the decay from the chunk's end to the segment's
+    for (int k = 0; k < w.chunks; ++k) {
+      const float wj = dt * (sx * sB * runit) * exp2_approx(after + a_end - a_i);
+      after += a_end;
+      if (k + 1 < w.chunks) fetch(k + 1);
+      const int st = k % kStateStages;
+      wait(full + st, (k / kStateStages) & 1);
+      if (on) {
+        const uint32_t row = smem_u32(smem) + st * kStateStage + (2 + hh) * kTileBytes + i * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t at = row + (((4 * half + c) ^ (i & 7)) << 4);
+          const uint4 x = lds128(at);
+          const float2 m0 = mul2(unpack_f16(x.x), splat(wj)), m1 = mul2(unpack_f16(x.y), splat(wj));
+          const float2 m2 = mul2(unpack_f16(x.z), splat(wj)), m3 = mul2(unpack_f16(x.w), splat(wj));
+          sts128(at, pack_f16(m0.x, m0.y), pack_f16(m1.x, m1.y), pack_f16(m2.x, m2.y), pack_f16(m3.x, m3.y));
+        }
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ready + st);
+      __syncwarp();
+    }
+    wait(done, 0);
+    tc::fence_after_sync();
+    // row n of S^T; warps of a head and half of its columns
+    const int q = warp & 3, n = q * 32 + lane, wg = warp >> 3, hf = (warp >> 2) & 1;
+    if (wg < w.heads) {
+      float v[32];
+      tc::tmem_ld32(tmem + 64 * wg + 32 * hf + (static_cast<uint32_t>(q * 32) << 16), v);
+      const int hd = w.h0 + wg;
+      const int64_t at = static_cast<int64_t>(32 * hf) * 128 + n, slot = static_cast<int64_t>(p.nh) * 64 * 128;
+      float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + hd) * 64 * 128 + at;
+      const float unit = s_unit[wg], decay = exp2_approx(s_total[wg]);
+      const __nv_bfloat16* s0 = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + hd) * 64 * 128 + at;
+      if (sg.index == 0) {
+        float s[32];  // all loads before the first store, which might be to the same place for all the compiler knows
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s[k] = __bfloat162float(s0[k * 128]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          ws[k * 128] = s[k];
+          v[k] = fmaf(s[k], decay, v[k] * unit);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= unit;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; ++k) ws[(sg.index + 1) * slot + k * 128] = v[k];
+      if (n == 0 && hf == 0) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + hd] = s_total[wg];
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 16) tc::tmem_dealloc(tmem, 128);
+}
+
 // Shared memory (from a 1024-byte boundary): two stages of B, C (32 KB each)
 // and X of two heads, the heads' state / weighted-x operands, then per head
 // the factors of the tokens.
@@ -653,7 +885,6 @@ constexpr uint32_t kFactorsAt = kOperandAt + 2 * kTileBytes;
 constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 256;  // and their block ends, the chunks' factors
 constexpr uint32_t kScanSmem = kScanBytes + 128 /* barriers */ + 512;
 // Tensor memory columns: S of two heads, C B^T, M of two heads, Y of two heads.
-constexpr int kScanThreads = 2 * 256;
 constexpr int kServe = 4;  // the serving warp of a head's eight
 constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 
@@ -663,19 +894,12 @@ constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 // 128 registers each (a 17th for the copies would leave 96).  Of a head's warps
 // the one with the first 32 rows and the later columns has no part of M (it is
 // all above the diagonal), so it serves the others: it issues the products and
-// copies and works out the chunk's common factors.  With kStatesOnly, the segment's state from nothing (from the
-// prompt's state for its first segment) goes to slot index + 1 of the prompt,
-// and the prompt's state itself to slot 0; the last segment has nothing to do.
-template <bool kStatesOnly>
+// copies and works out the chunk's common factors.
 __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const PromptParams p, const ChunkWork wk) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-  if (pad > 512) {  // does not happen: dynamic shared memory starts on a 1024-byte boundary
-    record_status(SN_ERR_MISALIGNED);
-    return;
-  }
-  unsigned char* smem = smem_raw + pad;
+  unsigned char* smem = aligned_smem(smem_raw);
+  if (!smem) return;
   const uint32_t sbase = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScanBytes);
   uint64_t *full = bars, *empty = bars + 2, *bar_g = bars + 4, *gfree = bars + 5, *bar_y2 = bars + 6, *bar_y = bars + 8,
@@ -683,15 +907,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 12);
   pdl_launch_dependents();
   pdl_wait();
-  // heads: pairs within a group
-  const int ppg = (p.hpg + 1) / 2;
-  const int g = blockIdx.x / ppg, h0 = g * p.hpg + (blockIdx.x - g * ppg) * 2;
-  const int heads = min(2, (g + 1) * p.hpg - h0);
-  const Segment sg = find_segment(p.prompts, wk.seg, blockIdx.y);
-  if (sg.seq < 0 || (kStatesOnly && sg.index + 1 >= sg.count)) return;  // the same in every warp
-  const int c0 = sg.index * wk.seg;
-  const int nchunks = min(wk.seg, (sg.len + kChunk - 1) / kChunk - c0);
-  if (tid == 0) {
+  const ScanWork w = scan_work(p, wk);
+  const Segment& sg = w.sg;
+  if (sg.seq < 0) return;  // the same in every warp
+  const int g = w.g, h0 = w.h0, heads = w.heads, c0 = w.c0, nchunks = w.chunks;
+  // the copies of a chunk's operands into its stage (one thread)
+  auto load = [&](int c) {
+    const uint32_t st = sbase + (c & 1) * kStageBytes;
+    const int64_t chunk = sg.chunk0 + c0 + c;
+    mbar_arrive_expect_tx(full + (c & 1), (4 + heads) * kTileBytes);
+    bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+    bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
+    bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
+  };
+  int loaded = min(2, nchunks);  // chunks whose copies have been issued
+  if (tid == kServe * 32) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 8 * heads);
@@ -702,7 +932,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     mbar_init(bar_g, 1);
     mbar_init(gfree, 8 * heads);
     fence_barrier_init();
+    for (int c = 0; c < loaded; ++c) load(c);
   }
+  __syncwarp();
   if (warp == 0) tc::tmem_alloc(tslot, 512);
   tc::fence_before_sync();
   __syncthreads();
@@ -716,19 +948,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     }
   };
 
-  // the copies of a chunk's operands into its stage (one thread)
-  auto load = [&](int c) {
-    const uint32_t st = sbase + (c & 1) * kStageBytes;
-    const int64_t chunk = sg.chunk0 + c0 + c;
-    mbar_arrive_expect_tx(full + (c & 1), ((kStatesOnly ? 2 : 4) + heads) * kTileBytes);
-    bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-    if (!kStatesOnly) bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-    bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
-  };
-  int loaded = min(2, nchunks);  // chunks whose copies have been issued
-  if (tid == kServe * 32) {
-    for (int c = 0; c < loaded; ++c) load(c);
-  }
   if ((warp >> 3) < heads) {
     const int wg = warp >> 3, half = (warp >> 2) & 1, q = warp & 3, i = q * 32 + lane, h = h0 + wg;
     const bool serving = (warp & 7) == kServe;
@@ -752,16 +971,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
       float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + at;
       float v[32];
-      if (sg.count == 1 || (kStatesOnly && sg.index == 0)) {
+      if (sg.count == 1) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = __bfloat162float(st[k * 128]);
-        if (kStatesOnly) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) ws[k * 128] = v[k];
-        }
-      } else if (kStatesOnly) {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = 0.f;
       } else {  // slot 0, or the segments before this one joined
         const int first = min(sg.index, 1);
 #pragma unroll
@@ -805,19 +1017,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       head.sB = sc[wk.xblocks + g];
       head.sC = sc[wk.xblocks + p.ng + g];
     };
-    const float D = serving && !kStatesOnly && p.D ? __bfloat162float(p.D[h]) : 0.f;
-    float total = 0.f;  // log2 of the segment's decay
+    const float D = serving && p.D ? __bfloat162float(p.D[h]) : 0.f;
     auto derive_head = [&](int c) {  // every scale is a power of two: products and reciprocals of them are exact
       const float sdt = pow2_floor(head.meta.x), rdt = rcp_pow2(sdt), dec = exp2_approx(head.a_end);
       const float unit_new = head.sB * head.sx * sdt, runit = rcp_pow2(head.sB) * rcp_pow2(head.sx) * rdt;
-      const float sb = pow2_floor(bound), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
+      const float sb = pow2_floor(bound, 100), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
       if (lane == 0) {
         common[2 * (c & 1)] = make_float4(rdt, head.a_end, unit * (rcp_pow2(sb) * 8192.f), dec * (unit * runit));
         common[2 * (c & 1) + 1] = make_float4(sS * runit, head.sC * unit_new, D * head.sx, unit_new);
       }
       unit = unit_new;
       bound = fmaf(dec, bound, unit_new * 4.f * (head.meta.y * rdt));
-      total += head.a_end;
     };
     struct Factors {
       float a_i, dtn;     // cumulative decay; dt / sdt
@@ -856,7 +1066,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       }
       __syncwarp();
     };
-    const bool issues_g = !kStatesOnly && serving && wg == heads - 1;
+    const bool issues_g = serving && wg == heads - 1;
     fetch(0);
     if (serving) {
       fetch_head(0);
@@ -890,17 +1100,15 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       {
         float v[32];
         tc::tmem_ld32(tS, v);
-        if (!kStatesOnly) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t o[4];
+        for (int k = 0; k < 4; ++k) {
+          uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 m = mul2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), splat(f.f_op));
-              o[j] = pack_f16(m.x, m.y);
-            }
-            sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+          for (int j = 0; j < 4; ++j) {
+            const float2 m = mul2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), splat(f.f_op));
+            o[j] = pack_f16(m.x, m.y);
           }
+          sts128(opnd + row + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
         }
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
@@ -911,117 +1119,106 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         tmem_st32(tS, v);
       }
       uint4 x[4];  // this half of this token's row of X
-      if (!kStatesOnly) {
-        // of the row's 32-token block: first and last token
-        const float a_first = __shfl_sync(0xffffffffu, f.a_i, 0), a_last = __shfl_sync(0xffffffffu, f.a_i, 31);
-        if (half == 0) {
-          // within the block exp(a_i - a_j) = exp(a_i - a_first) exp(a_first - a_j) as long as the second stays far
-          // from overflow; with more decay than 2^-100 in 32 tokens the exponents are subtracted first
-          fj[i] = a_first - a_last < 100.f ? exp2_approx(a_first - f.a_i) * f.dtn : f.a_i - __log2f(f.dtn);
-          if (lane == 31) cend[q] = f.a_i;
-        } else {
-          ej[i] = exp2_approx(a_last - f.a_i) * f.dtn;
-        }
-        __syncwarp();
-        tmem_wait_st();
-        tc::fence_before_sync();
-        tc::fence_proxy_async_smem();
-        named_bar_sync(bar_id, 256);
-        if (serving) {
-          wait(full + stage, ph);
-          if (lane == 0 && !dead) {  // Y = C S
-            tc::fence_after_sync();
-            constexpr uint32_t id = idesc_f16(128, 64, false, true);
-            const uint64_t dc = tc::smem_desc_sw128(smem + stage * kStageBytes + 2 * kTileBytes);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              tc::mma_bf16(tmem + kColY + wg * 64, dc + ((k >> 2) * kTileBytes + (k & 3) * 32) / 16, d_op + k * 128, id, k > 0);
-            tc::mma_commit(bar_y2 + wg);
-          }
-          __syncwarp();
-          refill();
-          if (c + 1 < nchunks) {
-            derive_head(c + 1);
-            if (c + 2 < nchunks) fetch_head(c + 2);
-          }
-        }
-        // ---- M from C B^T: blocks half and half + 2 of 32 columns ----
-        wait(bar_g, c & 1);  // the chunk's operands are there too
-        tc::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          const int jb = 2 * jj + half;
-          uint32_t m[16];
-          if (jb > q) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) m[k] = 0;
-            tmem_st16(tM + 16 * jb, m);
-            continue;
-          }
-          float v[32];
-          tc::tmem_ld32(tG + 32 * jb, v);
-          auto scaled = [&](const float* e, float2 r) {
-            const float4* e4 = reinterpret_cast<const float4*>(e + 32 * jb);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 f4 = e4[k];
-              const float2 m0 = mul2(mul2(make_float2(v[4 * k], v[4 * k + 1]), r), make_float2(f4.x, f4.y));
-              const float2 m1 = mul2(mul2(make_float2(v[4 * k + 2], v[4 * k + 3]), r), make_float2(f4.z, f4.w));
-              m[2 * k] = pack_f16(m0.x, m0.y);
-              m[2 * k + 1] = pack_f16(m1.x, m1.y);
-            }
-          };
-          if (jb < q) {  // an earlier block: exp(a_i - a_last) exp(a_last - a_j) dt_j, both at most 1
-            scaled(ej, splat(exp2_approx(f.a_i - cend[jb])));
-          } else {
-            if (a_first - a_last < 100.f) {
-              // v r first: r <= 1, and fj may be as large as 2^101
-              scaled(fj, splat(exp2_approx(f.a_i - a_first)));
-            } else {
-              const float4* l4 = reinterpret_cast<const float4*>(fj + 32 * jb);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float4 l = l4[k];
-                m[2 * k] = pack_f16(v[4 * k] * exp2_approx(f.a_i - l.x), v[4 * k + 1] * exp2_approx(f.a_i - l.y));
-                m[2 * k + 1] = pack_f16(v[4 * k + 2] * exp2_approx(f.a_i - l.z), v[4 * k + 3] * exp2_approx(f.a_i - l.w));
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {  // causal: columns up to the row's own
-              const uint32_t keep = 2 * k < lane ? 0xFFFFFFFFu : 2 * k == lane ? 0xFFFFu : 0u;
-              m[k] &= keep;
-            }
-          }
-          tmem_st16(tM + 16 * jb, m);
-        }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(gfree);
-        __syncwarp();
-        // ---- Y = exp(a_i) C S, in the unit of M X ----
-        wait(bar_y2 + wg, c & 1);
-        tc::fence_after_sync();
-        float v[32];
-        tc::tmem_ld32(tY, v);
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          const float2 m = mul2(make_float2(v[k], v[k + 1]), splat(f.f_y));
-          v[k] = m.x;
-          v[k + 1] = m.y;
-        }
-        tmem_st32(tY, v);
+      // of the row's 32-token block: first and last token
+      const float a_first = __shfl_sync(0xffffffffu, f.a_i, 0), a_last = __shfl_sync(0xffffffffu, f.a_i, 31);
+      if (half == 0) {
+        // within the block exp(a_i - a_j) = exp(a_i - a_first) exp(a_first - a_j) as long as the second stays far
+        // from overflow; with more decay than 2^-100 in 32 tokens the exponents are subtracted first
+        fj[i] = a_first - a_last < 100.f ? exp2_approx(a_first - f.a_i) * f.dtn : f.a_i - __log2f(f.dtn);
+        if (lane == 31) cend[q] = f.a_i;
       } else {
+        ej[i] = exp2_approx(a_last - f.a_i) * f.dtn;
+      }
+      __syncwarp();
+      tmem_wait_st();
+      tc::fence_before_sync();
+      tc::fence_proxy_async_smem();
+      named_bar_sync(bar_id, 256);
+      if (serving) {
+        wait(full + stage, ph);
+        if (lane == 0 && !dead) {  // Y = C S
+          tc::fence_after_sync();
+          constexpr uint32_t id = idesc_f16(128, 64, false, true);
+          const uint64_t dc = tc::smem_desc_sw128(smem + stage * kStageBytes + 2 * kTileBytes);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tc::mma_bf16(tmem + kColY + wg * 64, dc + ((k >> 2) * kTileBytes + (k & 3) * 32) / 16, d_op + k * 128, id, k > 0);
+          tc::mma_commit(bar_y2 + wg);
+        }
+        __syncwarp();
         refill();
-        if (serving && c + 1 < nchunks) {
+        if (c + 1 < nchunks) {
           derive_head(c + 1);
           if (c + 2 < nchunks) fetch_head(c + 2);
         }
-        wait(full + stage, ph);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
       }
+      // ---- M from C B^T: blocks half and half + 2 of 32 columns ----
+      wait(bar_g, c & 1);  // the chunk's operands are there too
+      tc::fence_after_sync();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int jb = 2 * jj + half;
+        uint32_t m[16];
+        if (jb > q) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) m[k] = 0;
+          tmem_st16(tM + 16 * jb, m);
+          continue;
+        }
+        float v[32];
+        tc::tmem_ld32(tG + 32 * jb, v);
+        auto scaled = [&](const float* e, float2 r) {
+          const float4* e4 = reinterpret_cast<const float4*>(e + 32 * jb);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 f4 = e4[k];
+            const float2 m0 = mul2(mul2(make_float2(v[4 * k], v[4 * k + 1]), r), make_float2(f4.x, f4.y));
+            const float2 m1 = mul2(mul2(make_float2(v[4 * k + 2], v[4 * k + 3]), r), make_float2(f4.z, f4.w));
+            m[2 * k] = pack_f16(m0.x, m0.y);
+            m[2 * k + 1] = pack_f16(m1.x, m1.y);
+          }
+        };
+        if (jb < q) {  // an earlier block: exp(a_i - a_last) exp(a_last - a_j) dt_j, both at most 1
+          scaled(ej, splat(exp2_approx(f.a_i - cend[jb])));
+        } else {
+          if (a_first - a_last < 100.f) {
+            // v r first: r <= 1, and fj may be as large as 2^101
+            scaled(fj, splat(exp2_approx(f.a_i - a_first)));
+          } else {
+            const float4* l4 = reinterpret_cast<const float4*>(fj + 32 * jb);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 l = l4[k];
+              m[2 * k] = pack_f16(v[4 * k] * exp2_approx(f.a_i - l.x), v[4 * k + 1] * exp2_approx(f.a_i - l.y));
+              m[2 * k + 1] = pack_f16(v[4 * k + 2] * exp2_approx(f.a_i - l.z), v[4 * k + 3] * exp2_approx(f.a_i - l.w));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {  // causal: columns up to the row's own
+            const uint32_t keep = 2 * k < lane ? 0xFFFFFFFFu : 2 * k == lane ? 0xFFFFu : 0u;
+            m[k] &= keep;
+          }
+        }
+        tmem_st16(tM + 16 * jb, m);
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(gfree);
+      __syncwarp();
+      // ---- Y = exp(a_i) C S, in the unit of M X ----
+      wait(bar_y2 + wg, c & 1);
+      tc::fence_after_sync();
+      float v[32];
+      tc::tmem_ld32(tY, v);
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) {
+        const float2 m = mul2(make_float2(v[k], v[k + 1]), splat(f.f_y));
+        v[k] = m.x;
+        v[k + 1] = m.y;
+      }
+      tmem_st32(tY, v);
       // ---- weighted x ----
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -1041,7 +1238,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       if (serving) {
         if (lane == 0 && !dead) {
           tc::fence_after_sync();
-          if (!kStatesOnly) {  // Y += M X
+          {  // Y += M X
             constexpr uint32_t id = idesc_f16(128, 64, false, true);
             const uint64_t dx = desc_k_rows(sst + (4 + wg) * kTileBytes, 16);
 #pragma unroll
@@ -1058,84 +1255,71 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         __syncwarp();
         if (issues_g && c + 1 < nchunks) issue_g(c + 1);
       }
-      if (!kStatesOnly) {
-        // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
-        // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
-        const float2 fy = splat(f.fy), dx = splat(f.dx);
-        const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
-        const int64_t tok = sg.start + tw;
-        const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
-        const int piece = 4 * half + (lane & 3), psw = (lane >> 2) & 7;  // rows 8 apart swizzle alike
-        uint4 zv[4];
-        if (p.gate) {
-          const __nv_bfloat16* z = p.zx + tok * p.ld + h * 64 + 8 * piece;
+      // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
+      // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
+      const float2 fy = splat(f.fy), dx = splat(f.dx);
+      const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
+      const int64_t tok = sg.start + tw;
+      const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
+      const int piece = 4 * half + (lane & 3), psw = (lane >> 2) & 7;  // rows 8 apart swizzle alike
+      uint4 zv[4];
+      if (p.gate) {
+        const __nv_bfloat16* z = p.zx + tok * p.ld + h * 64 + 8 * piece;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            zv[k] = tw + 8 * k < sg.len ? *reinterpret_cast<const uint4*>(z + 8 * k * p.ld) : make_uint4(0, 0, 0, 0);
-        }
-        if (c + 1 < nchunks) {
-          take(c + 1);
-          if (c + 2 < nchunks) fetch(c + 2);
-        }
-        wait(bar_y + wg, c & 1);
-        tc::fence_after_sync();
-        if (p.gate) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sts128(stg + k * 1024 + ((piece ^ psw) << 4), zv[k].x, zv[k].y, zv[k].z, zv[k].w);
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) zv[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
-          __syncwarp();
-        }
-        float v[32];
-        tc::tmem_ld32(tY, v);
-        tc::fence_before_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, zu[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float2 y = fma2(make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]), fy, mul2(unpack_f16(u[j]), dx));
-            if (p.gate) y = mul2(y, silu2(unpack_bf16(zu[j])));
-            const __nv_bfloat162 b = __floats2bfloat162_rn(y.x, y.y);
-            o[j] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          sts128(xrow + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
-        }
-        __syncwarp();
-        __nv_bfloat16* out = p.y + (tok * p.nh + h) * 64 + 8 * piece;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 o = lds128(stg + k * 1024 + ((piece ^ psw) << 4));
-          if (tw + 8 * k < sg.len) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(8 * k) * p.nh * 64) = o;
-        }
-        tc::fence_proxy_async_smem();  // before the stage is handed back to the copies
-        __syncwarp();
-      } else if (c + 1 < nchunks) {
+        for (int k = 0; k < 4; ++k)
+          zv[k] = tw + 8 * k < sg.len ? *reinterpret_cast<const uint4*>(z + 8 * k * p.ld) : make_uint4(0, 0, 0, 0);
+      }
+      if (c + 1 < nchunks) {
         take(c + 1);
         if (c + 2 < nchunks) fetch(c + 2);
       }
+      wait(bar_y + wg, c & 1);
+      tc::fence_after_sync();
+      if (p.gate) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sts128(stg + k * 1024 + ((piece ^ psw) << 4), zv[k].x, zv[k].y, zv[k].z, zv[k].w);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) zv[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
+        __syncwarp();
+      }
+      float yv[32];
+      tc::tmem_ld32(tY, yv);
+      tc::fence_before_sync();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, zu[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 y = fma2(make_float2(yv[8 * k + 2 * j], yv[8 * k + 2 * j + 1]), fy, mul2(unpack_f16(u[j]), dx));
+          if (p.gate) y = mul2(y, silu2(unpack_bf16(zu[j])));
+          const __nv_bfloat162 b = __floats2bfloat162_rn(y.x, y.y);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        sts128(xrow + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+      }
+      __syncwarp();
+      __nv_bfloat16* out = p.y + (tok * p.nh + h) * 64 + 8 * piece;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 o = lds128(stg + k * 1024 + ((piece ^ psw) << 4));
+        if (tw + 8 * k < sg.len) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(8 * k) * p.nh * 64) = o;
+      }
+      tc::fence_proxy_async_smem();  // before the stage is handed back to the copies
+      __syncwarp();
     }
     // ---- the state after the segment ----
     wait(bar_s + wg, (nchunks - 1) & 1);
     if (dead) mbar_wait_bounded(bar_s + wg, (nchunks - 1) & 1);
     __syncwarp();
     tc::fence_after_sync();
-    if (kStatesOnly || sg.index + 1 == sg.count) {
-      const int64_t at = static_cast<int64_t>(32 * half) * 128 + i;
+    if (sg.index + 1 == sg.count) {
+      __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + 32 * half * 128 + i;
       float v[32];
       tc::tmem_ld32(tS, v);
-      if (kStatesOnly) {
-        float* ws = wk.state + (static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h) * 64 * 128 + at;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) ws[k * 128] = v[k] * unit_last;
-        if (serving && lane == 0) wk.total[static_cast<int64_t>(sg.slot0 + sg.index + 1) * p.nh + h] = total;
-      } else {
-        __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
-#pragma unroll
-        for (int k = 0; k < 32; ++k) st[k * 128] = __float2bfloat16_rn(v[k] * unit_last);
-      }
+      for (int k = 0; k < 32; ++k) st[k * 128] = __float2bfloat16_rn(v[k] * unit_last);
     }
   }
   if (dead && tid == kServe * 32)  // copies in flight land before the CTA leaves
@@ -1161,8 +1345,8 @@ inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, i
   r.pairs = ng * ((hpg + 1) / 2);
   r.xblocks = (d_inner + 127) / 128;
   r.blocks = r.xblocks + 2 * ng;
-  // Chunks a segment: the fewest chunk steps over the SMs' waves.  A step of the second launch costs about twice one of the
-  // first, a CTA's start and end about one step.
+  // Chunks a segment: the least time over the SMs' waves of both launches, from what was measured (tenths of a
+  // microsecond): 43 a chunk of the outputs and 110 to start and end a CTA of them, 11 and 90 for the states.
   const int sms = 148;
   const int64_t nc = std::max<int64_t>(1, (tokens + kChunk - 1) / kChunk);
   const int64_t each = (nc + batch - 1) / batch;  // of a prompt, if they are alike
@@ -1172,7 +1356,7 @@ inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, i
     const int64_t seg = (each + n - 1) / n;
     const int64_t waves = (batch * ((each + seg - 1) / seg) * r.pairs + sms - 1) / sms;
     const int64_t waves1 = n == 1 ? 0 : (batch * ((each + seg - 1) / seg - 1) * r.pairs + sms - 1) / sms;
-    const int64_t cost = waves * (2 * seg + 2) + waves1 * (seg + 2);
+    const int64_t cost = waves * (43 * seg + 110) + waves1 * (11 * seg + 90);
     if (cost < best) {
       best = cost;
       r.seg = static_cast<int>(seg);
@@ -1281,18 +1465,18 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
     int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
     if (rc != SN_OK) return rc;
     const dim3 grid(static_cast<unsigned>(plan.pairs), static_cast<unsigned>(plan.segments));
-    auto scan = [&](auto kern) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sn::kScanSmem)) != cudaSuccess) {
+    auto scan = [&](auto kern, int threads, uint32_t smem) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
         cudaGetLastError();
         return SN_ERR_LAUNCH;
       }
-      return sn::launch(kern, grid, dim3(sn::kScanThreads), sn::kScanSmem, st, true, p, wk);
+      return sn::launch(kern, grid, dim3(static_cast<unsigned>(threads)), smem, st, true, p, wk);
     };
     if (tokens > static_cast<int64_t>(plan.seg) * sn::kChunk) {  // a prompt may have several segments
-      rc = scan(sn::prompt_scan_mma_kernel<true>);
+      rc = scan(sn::prompt_states_kernel, sn::kScanThreads + 32, sn::kStateSmem);
       if (rc != SN_OK) return rc;
     }
-    return scan(sn::prompt_scan_mma_kernel<false>);
+    return scan(sn::prompt_scan_mma_kernel, sn::kScanThreads, sn::kScanSmem);
   }
   const int64_t rows = static_cast<int64_t>(batch) * d_inner;
   const int64_t blocks = tokens / sn::kConvRows + static_cast<int64_t>(batch);
