@@ -935,6 +935,52 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     for (int c = 0; c < loaded; ++c) load(c);
   }
   __syncwarp();
+  const int wg = warp >> 3, half = (warp >> 2) & 1, q = warp & 3, i = q * 32 + lane, h = h0 + wg;
+  const bool serving = (warp & 7) == kServe;
+  // Inputs of a chunk: a token's own for every thread, the head's for the serving warp; loaded a chunk ahead.
+  const int chunk0 = sg.chunk0 + c0;
+  float next_a, next_dt;
+  auto fetch = [&](int c) {
+    const int64_t at = (static_cast<int64_t>(chunk0 + c) * p.nh + h) * kChunk + i;
+    next_a = wk.cum[at];
+    next_dt = wk.dt[at];
+  };
+  struct {
+    float a_end, sx, sB, sC;
+    float2 meta;
+  } head;
+  auto fetch_head = [&](int c) {
+    const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
+    const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * wk.blocks;
+    head.a_end = wk.cum[th * kChunk + kChunk - 1];
+    head.meta = wk.meta[th];
+    head.sx = sc[h / 2];
+    head.sB = sc[wk.xblocks + g];
+    head.sC = sc[wk.xblocks + p.ng + g];
+  };
+  // The first chunk's inputs and the state before the segment (row n = i of S^T, this half's 32 columns, true values):
+  // all of them on their way before anything waits
+  float v0[32];
+  if (wg < heads) {
+    fetch(0);
+    if (serving) fetch_head(0);
+    const int64_t at = static_cast<int64_t>(32 * half) * 128 + i, slot = static_cast<int64_t>(p.nh) * 64 * 128;
+    const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
+    float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + at;
+    if (sg.count == 1) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v0[k] = __bfloat162float(st[k * 128]);
+    } else {  // slot 0, or the segments before this one joined
+      const int first = min(sg.index, 1);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v0[k] = ws[first * slot + k * 128];
+      for (int j = 2; j <= sg.index; ++j) {
+        const float dec = exp2_approx(wk.total[static_cast<int64_t>(sg.slot0 + j) * p.nh + h]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v0[k] = fmaf(v0[k], dec, ws[j * slot + k * 128]);
+      }
+    }
+  }
   if (warp == 0) tc::tmem_alloc(tslot, 512);
   tc::fence_before_sync();
   __syncthreads();
@@ -948,9 +994,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     }
   };
 
-  if ((warp >> 3) < heads) {
-    const int wg = warp >> 3, half = (warp >> 2) & 1, q = warp & 3, i = q * 32 + lane, h = h0 + wg;
-    const bool serving = (warp & 7) == kServe;
+  if (wg < heads) {
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS = tmem + kColS + wg * 64 + 32 * half + lanes, tG = tmem + kColG + lanes,
                    tM = tmem + kColM + wg * 64 + lanes, tY = tmem + kColY + wg * 64 + 32 * half + lanes;
@@ -964,29 +1008,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     // C S from its operand's unit to that of M X, M X to outputs, x' to D x
     float4* common = reinterpret_cast<float4*>(smem + kFactorsAt + 2 * 2 * kChunk * 4 + 128) + wg * 4;
 
-    // ---- the state before the segment: row n = i of S^T, this half's 32 columns, true values ----
     float unit = 1.f, bound = 0.f;  // S = unit * tensor memory; |S| <= bound
     {
-      const int64_t at = static_cast<int64_t>(32 * half) * 128 + i, slot = static_cast<int64_t>(p.nh) * 64 * 128;
-      const __nv_bfloat16* st = p.ssm_state + (static_cast<int64_t>(sg.seq) * p.nh + h) * 64 * 128 + at;
-      float* ws = wk.state + (static_cast<int64_t>(sg.slot0) * p.nh + h) * 64 * 128 + at;
-      float v[32];
-      if (sg.count == 1) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = __bfloat162float(st[k * 128]);
-      } else {  // slot 0, or the segments before this one joined
-        const int first = min(sg.index, 1);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = ws[first * slot + k * 128];
-        for (int j = 2; j <= sg.index; ++j) {
-          const float dec = exp2_approx(wk.total[static_cast<int64_t>(sg.slot0 + j) * p.nh + h]);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], dec, ws[j * slot + k * 128]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 32; ++k) bound = fmaxf(bound, fabsf(v[k]));
-      tmem_st32(tS, v);
+      for (int k = 0; k < 32; ++k) bound = fmaxf(bound, fabsf(v0[k]));
+      tmem_st32(tS, v0);
       tmem_wait_st();
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
@@ -996,27 +1022,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       for (int k = 0; k < 8; ++k) bound = fmaxf(bound, cend[k]);
     }
 
-    // Inputs of a chunk: a token's own for every thread, the head's for the serving warp; loaded a chunk ahead.
-    const int chunk0 = sg.chunk0 + c0;
-    float next_a, next_dt;
-    auto fetch = [&](int c) {
-      const int64_t at = (static_cast<int64_t>(chunk0 + c) * p.nh + h) * kChunk + i;
-      next_a = wk.cum[at];
-      next_dt = wk.dt[at];
-    };
-    struct {
-      float a_end, sx, sB, sC;
-      float2 meta;
-    } head;
-    auto fetch_head = [&](int c) {
-      const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
-      const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * wk.blocks;
-      head.a_end = wk.cum[th * kChunk + kChunk - 1];
-      head.meta = wk.meta[th];
-      head.sx = sc[h / 2];
-      head.sB = sc[wk.xblocks + g];
-      head.sC = sc[wk.xblocks + p.ng + g];
-    };
     const float D = serving && p.D ? __bfloat162float(p.D[h]) : 0.f;
     auto derive_head = [&](int c) {  // every scale is a power of two: products and reciprocals of them are exact
       const float sdt = pow2_floor(head.meta.x), rdt = rcp_pow2(sdt), dec = exp2_approx(head.a_end);
@@ -1067,9 +1072,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       __syncwarp();
     };
     const bool issues_g = serving && wg == heads - 1;
-    fetch(0);
     if (serving) {
-      fetch_head(0);
       derive_head(0);
       if (nchunks > 1) fetch_head(1);
     }
@@ -1096,6 +1099,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
           __syncwarp();
         }
       };
+      if (p.gate) {  // the gates' lines, on their way to L2
+        const int t = (c0 + c) * kChunk + i;
+        if (half == 0 && t < sg.len)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.zx + (sg.start + t) * p.ld + h * 64));
+      }
       // ---- S: operand of C S, and decayed, in the new unit ----
       {
         float v[32];
