@@ -23,16 +23,25 @@ def stream_handle(stream=None) -> int:
 
 
 @contextlib.contextmanager
-def on_stream(stream=None):
-    """Makes `stream` (as stream_handle takes it) torch's current stream, so
-    that what a wrapper allocates belongs to the stream its kernels run on,
-    and yields the raw handle."""
-    h = stream_handle(stream)
-    if stream is None or h == torch.cuda.current_stream().cuda_stream:
-        yield h
-        return
+def _on_other_stream(stream, h: int):
     with torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(h)):
         yield h
+
+
+def current_handle(device: int) -> int:
+    """stream_handle(None) for the current device `device`, without a Stream
+    object around it (a short call spends most of its time on the host)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def on_stream(stream=None):
+    """A context that makes `stream` (as stream_handle takes it) torch's
+    current stream, so that what a wrapper allocates belongs to the stream its
+    kernels run on, and gives the raw handle."""
+    h = stream_handle(stream)
+    if h == torch.cuda.current_stream().cuda_stream:
+        return contextlib.nullcontext(h)
+    return _on_other_stream(stream, h)
 
 
 def same_device(**tensors) -> None:

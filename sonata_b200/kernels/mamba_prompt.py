@@ -8,18 +8,27 @@ layouts, so that decoding goes on from them (C ABI: ``sn_mamba2_prompt``).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
-from ._common import call, on_stream, require_cuda, same_device
+from ._common import call, current_handle, on_stream, require_cuda, same_device
 
 _BF16 = torch.bfloat16
 
 
 def _dense(name, t, shape, dtype=_BF16):
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous():
+        return
     require_cuda(name, t, dtype)
     if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor, got {tuple(t.shape)}")
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(*sizes: int) -> int:
+    return _lib.lib().sn_mamba2_prompt_workspace_size(*sizes)
 
 
 def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias, ssm_state: torch.Tensor,
@@ -33,7 +42,8 @@ def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     and are updated in place; A fp32 [nheads] (negative), D / dt_bias bf16
     [nheads] or None, weight [conv_dim, W], bias [conv_dim] or None.  Returns
     y [tokens, nheads, headdim] = S_t C_t + D x_t, times SiLU(z_t) with gate."""
-    require_cuda("zxbcdt", zxbcdt, _BF16, 2)
+    if not (isinstance(zxbcdt, torch.Tensor) and zxbcdt.dtype is _BF16 and zxbcdt.is_cuda and zxbcdt.dim() == 2):
+        require_cuda("zxbcdt", zxbcdt, _BF16, 2)
     if zxbcdt.shape[0] > 0 and zxbcdt.stride(1) != 1:
         raise ValueError("zxbcdt must be contiguous along its last dimension")
     tokens = zxbcdt.shape[0]
@@ -48,8 +58,9 @@ def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.
         if cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens must be a contiguous int32 [batch + 1] tensor, batch >= 1")
         batch = cu_seqlens.numel() - 1
-    _dense("conv_state", conv_state, (batch, conv_dim, conv_state.shape[-1]))
-    _dense("weight", weight, (conv_dim, conv_state.shape[-1]))
+    width = conv_state.shape[-1]
+    _dense("conv_state", conv_state, (batch, conv_dim, width))
+    _dense("weight", weight, (conv_dim, width))
     _dense("ssm_state", ssm_state, (batch, nheads, d_inner // nheads, d_state))
     _dense("A", A, (nheads,), torch.float32)
     if bias is not None:
@@ -57,17 +68,26 @@ def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     for name, t in (("D", D), ("dt_bias", dt_bias)):
         if t is not None:
             _dense(name, t, (nheads,))
-    same_device(zxbcdt=zxbcdt, conv_state=conv_state, weight=weight, bias=bias, ssm_state=ssm_state, A=A, D=D,
-                dt_bias=dt_bias, cu_seqlens=cu_seqlens)
-    ptr = lambda t: t.data_ptr() if t is not None else None
-    with on_stream(stream) as st:
-        y = torch.empty(tokens, nheads, d_inner // nheads, device=zxbcdt.device, dtype=_BF16)
+    dev = torch.cuda.current_device()
+    for t in (zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, cu_seqlens):
+        if t is not None and t.get_device() != dev:
+            same_device(zxbcdt=zxbcdt, conv_state=conv_state, weight=weight, bias=bias, ssm_state=ssm_state, A=A, D=D,
+                        dt_bias=dt_bias, cu_seqlens=cu_seqlens)
+
+    def launch(st):
+        y = torch.empty((tokens, nheads, d_inner // nheads), device=zxbcdt.device, dtype=_BF16)
         if tokens == 0:
             return y
-        nbytes = _lib.lib().sn_mamba2_prompt_workspace_size(tokens, batch, d_inner, ngroups, d_state, nheads)
+        nbytes = _workspace_size(tokens, batch, d_inner, ngroups, d_state, nheads)
         ws = torch.empty(nbytes, device=zxbcdt.device, dtype=torch.uint8)
         call("sn_mamba2_prompt", zxbcdt.data_ptr(), zxbcdt.stride(0) if tokens > 1 else zxbcdt.shape[1],
-             conv_state.data_ptr(), weight.data_ptr(), ptr(bias), ssm_state.data_ptr(), A.data_ptr(), ptr(D),
-             ptr(dt_bias), y.data_ptr(), ptr(cu_seqlens), batch, tokens, d_inner, ngroups, d_state, nheads,
-             d_inner // nheads, conv_state.shape[-1], int(bool(gate)), ws.data_ptr(), nbytes, st)
-    return y
+             conv_state.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(), ssm_state.data_ptr(),
+             A.data_ptr(), None if D is None else D.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(),
+             y.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), batch, tokens, d_inner, ngroups, d_state,
+             nheads, d_inner // nheads, conv_state.shape[2], 1 if gate else 0, ws.data_ptr(), nbytes, st)
+        return y
+
+    if stream is None:
+        return launch(current_handle(dev))
+    with on_stream(stream) as st:
+        return launch(st)

@@ -10,13 +10,14 @@ serves growing streams.  C ABI: ``sn_rotary_paged_append``,
 """
 from __future__ import annotations
 
+import functools
 import heapq
 import math
 
 import torch
 
 from .. import _lib
-from ._common import call, on_stream, require_cuda, same_device
+from ._common import call, current_handle, on_stream, require_cuda, same_device
 
 _BF16 = torch.bfloat16
 
@@ -47,12 +48,13 @@ def rotary_table(max_pos: int, rot_dim: int, base: float = 10000.0, factor: floa
     return ang.cos().float().to(device), ang.sin().float().to(device)
 
 
+# A decode step's calls are short, so the checks are two-tiered: one expression that holds for every valid call, and the
+# functions that say what is wrong with the others.
+
 def _pool(name: str, t: torch.Tensor):
     require_cuda(name, t, _BF16, 4)
     if t.stride(3) != 1 or min(t.shape) < 1:
         raise ValueError(f"{name} must be [num_pages, nheads_kv, page_size, head_dim] with a dense last dimension")
-    # an axis of extent 1 is never stepped along: its stride may be anything
-    return [st if n > 1 else max(st, t.shape[3]) for n, st in zip(t.shape[:3], t.stride()[:3])]
 
 
 def _index(name: str, t: torch.Tensor, dim: int = 1):
@@ -61,18 +63,33 @@ def _index(name: str, t: torch.Tensor, dim: int = 1):
         raise ValueError(f"{name} must be a non-empty int32 tensor with a dense last dimension")
 
 
-def _pages(k_pages, v_pages, page_table, seq_lens):
-    """Checked pools and tables: the arguments both kernels take in the same order."""
-    ks, vs = _pool("k_pages", k_pages), _pool("v_pages", v_pages)
+def _check_pages(k_pages, v_pages, page_table, seq_lens):
+    _pool("k_pages", k_pages)
+    _pool("v_pages", v_pages)
     if k_pages.shape != v_pages.shape:
         raise ValueError(f"k_pages and v_pages differ in shape: {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
     _index("page_table", page_table, 2)
     _index("seq_lens", seq_lens)
     if page_table.shape[0] != seq_lens.shape[0]:
         raise ValueError(f"page_table has {page_table.shape[0]} rows for {seq_lens.shape[0]} streams")
-    stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-    return (k_pages.data_ptr(), *ks, v_pages.data_ptr(), *vs, k_pages.shape[0], k_pages.shape[2], page_table.data_ptr(),
-            stride, page_table.shape[1], seq_lens.data_ptr())
+
+
+def _pages(k_pages, v_pages, page_table, seq_lens):
+    """Checked pools and tables: the arguments both kernels take in the same order."""
+    if not (isinstance(k_pages, torch.Tensor) and isinstance(v_pages, torch.Tensor) and
+            isinstance(page_table, torch.Tensor) and isinstance(seq_lens, torch.Tensor)):
+        _check_pages(k_pages, v_pages, page_table, seq_lens)
+    ks, kt, vt, ts, tt = k_pages.shape, k_pages.stride(), v_pages.stride(), page_table.shape, page_table.stride()
+    if not (len(ks) == 4 and ks == v_pages.shape and kt[3] == 1 == vt[3] and k_pages.dtype is _BF16 is v_pages.dtype and
+            k_pages.is_cuda and v_pages.is_cuda and 0 not in ks and len(ts) == 2 and 0 not in ts and tt[1] == 1 and
+            seq_lens.shape == ts[:1] and seq_lens.stride() == (1,) and page_table.dtype is torch.int32 is seq_lens.dtype
+            and page_table.is_cuda and seq_lens.is_cuda):
+        _check_pages(k_pages, v_pages, page_table, seq_lens)
+    n, h, page, hd = ks
+    if n == 1 or h == 1 or page == 1:  # an axis of extent 1 is never stepped along: its stride may be anything
+        kt, vt = ([st if e > 1 else max(st, hd) for e, st in zip(ks, t)] for t in (kt, vt))
+    return (k_pages.data_ptr(), kt[0], kt[1], kt[2], v_pages.data_ptr(), vt[0], vt[1], vt[2], n, page, page_table.data_ptr(),
+            tt[0] if ts[0] > 1 else ts[1], ts[1], seq_lens.data_ptr())
 
 
 def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -86,37 +103,55 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     sin fp32 [max_pos, rot / 2]: halves (j, j + rot/2), or neighbours (2j, 2j
     + 1) when interleaved.  k and v go to their pages; returns q [tokens,
     nheads, head_dim]."""
-    require_cuda("qkv", qkv, _BF16, 2)
+    if not (isinstance(qkv, torch.Tensor) and qkv.dtype is _BF16 and qkv.is_cuda and qkv.dim() == 2):
+        require_cuda("qkv", qkv, _BF16, 2)
     args = _pages(k_pages, v_pages, page_table, seq_lens)
-    tokens, (_, hkv, _, hd), batch = qkv.shape[0], k_pages.shape, seq_lens.shape[0]
-    if qkv.shape[1] != (nheads + 2 * hkv) * hd or tokens > 0 and qkv.stride(1) != 1:
+    (tokens, width), (_, hkv, _, hd), batch = qkv.shape, k_pages.shape, seq_lens.shape[0]
+    if width != (nheads + 2 * hkv) * hd or tokens > 0 and qkv.stride(1) != 1:
         raise ValueError(f"qkv must be [tokens, {(nheads + 2 * hkv) * hd}] with a dense last dimension")
     if cu_seqlens is None:
         if tokens != batch:
             raise ValueError(f"{tokens} tokens for {batch} streams: give cu_seqlens")
-    else:
+    elif not (isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda and cu_seqlens.dtype is torch.int32 and
+              cu_seqlens.shape == (batch + 1,) and cu_seqlens.is_contiguous()):
         _index("cu_seqlens", cu_seqlens)
-        if cu_seqlens.shape[0] != batch + 1:
-            raise ValueError(f"cu_seqlens must hold {batch + 1} offsets")
-    for name, t in (("cos", cos), ("sin", sin)):
-        require_cuda(name, t, torch.float32, 2)
-        if not t.is_contiguous() or t.shape != cos.shape or t.shape[0] < 1 or 2 * t.shape[1] > hd:
-            raise ValueError(f"{name} must be contiguous fp32 [max_pos, rot / 2], rot at most {hd}, both alike")
-    same_device(qkv=qkv, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, cos=cos, sin=sin,
-                cu_seqlens=cu_seqlens)
-    with on_stream(stream) as st:
-        q = torch.empty(tokens, nheads, hd, device=qkv.device, dtype=_BF16)
+        raise ValueError(f"cu_seqlens must hold {batch + 1} contiguous offsets")
+    if not (isinstance(cos, torch.Tensor) and isinstance(sin, torch.Tensor) and cos.dtype is torch.float32 is sin.dtype and
+            cos.is_cuda and sin.is_cuda and cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous() and
+            sin.is_contiguous() and cos.shape[0] > 0 and 2 * cos.shape[1] <= hd):
+        for name, t in (("cos", cos), ("sin", sin)):
+            require_cuda(name, t, torch.float32, 2)
+        raise ValueError(f"cos and sin must be contiguous fp32 [max_pos, rot / 2], rot at most {hd}, both alike")
+    max_pos, half = cos.shape
+    dev = torch.cuda.current_device()
+    if not (dev == qkv.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device() ==
+            seq_lens.get_device() == cos.get_device() == sin.get_device() == (cos if cu_seqlens is None else cu_seqlens).get_device()):
+        same_device(qkv=qkv, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, cos=cos, sin=sin,
+                    cu_seqlens=cu_seqlens)
+
+    def launch(st):
+        q = qkv.new_empty((tokens, nheads, hd))
         if tokens:
-            call("sn_rotary_paged_append", qkv.data_ptr(), qkv.stride(0) if tokens > 1 else qkv.shape[1], q.data_ptr(),
+            call("sn_rotary_paged_append", qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width, q.data_ptr(),
                  *args, cu_seqlens.data_ptr() if cu_seqlens is not None else None, cos.data_ptr(), sin.data_ptr(),
-                 cos.shape[0], tokens, batch, nheads, hkv, hd, 2 * cos.shape[1], int(bool(interleaved)), st)
-    return q
+                 max_pos, tokens, batch, nheads, hkv, hd, 2 * half, 1 if interleaved else 0, st)
+        return q
+
+    if stream is None:
+        return launch(current_handle(dev))
+    with on_stream(stream) as st:
+        return launch(st)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(batch: int, nheads: int, head_dim: int) -> int:
+    return _lib.lib().sn_paged_decode_workspace_size(batch, nheads, head_dim)
 
 
 def decode_workspace(batch: int, nheads: int, head_dim: int, device="cuda") -> torch.Tensor:
     """The workspace of paged_decode_attention for up to `batch` streams: zeroed
     once, kept for every step on one stream of calls."""
-    n = _lib.lib().sn_paged_decode_workspace_size(batch, nheads, head_dim)
+    n = _workspace_size(batch, nheads, head_dim)
     if n == 0:
         raise ValueError("batch, nheads and head_dim must be positive")
     return torch.zeros(n, device=device, dtype=torch.uint8)
@@ -132,31 +167,44 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     the sum of exponentials fp32 [batch, nheads].  `workspace`
     (decode_workspace) saves an allocation and a fill a call; calls that share
     one must not overlap."""
-    require_cuda("q", q, _BF16, 3)
+    if not (isinstance(q, torch.Tensor) and q.dtype is _BF16 and q.is_cuda and q.dim() == 3):
+        require_cuda("q", q, _BF16, 3)
     args = _pages(k_pages, v_pages, page_table, seq_lens)
-    batch, nheads, hd = q.shape
+    (batch, nheads, hd), (qb, qh, qc) = q.shape, q.stride()
     hkv = k_pages.shape[1]
     if batch != seq_lens.shape[0] or hd != k_pages.shape[3] or nheads < 1 or nheads % hkv:
         raise ValueError(f"q {tuple(q.shape)} does not match {seq_lens.shape[0]} streams of {hkv} heads of {k_pages.shape[3]}")
-    if q.stride(2) != 1 and hd > 1:
+    if qc != 1 and hd > 1:
         raise ValueError("q must be dense along its last dimension")
-    need = _lib.lib().sn_paged_decode_workspace_size(batch, nheads, hd)
-    if workspace is not None:
+    need = _workspace_size(batch, nheads, hd)
+    dev = torch.cuda.current_device()
+    if not (dev == q.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device() ==
+            seq_lens.get_device()):
+        same_device(q=q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens)
+    if workspace is not None and not (
+            isinstance(workspace, torch.Tensor) and workspace.dtype is torch.uint8 and workspace.get_device() == dev and
+            workspace.dim() == 1 and workspace.numel() >= need and workspace.is_contiguous()
+            and workspace.data_ptr() % 16 == 0):
         require_cuda("workspace", workspace, torch.uint8, 1)
-        if workspace.numel() < need or not workspace.is_contiguous() or workspace.data_ptr() % 16:
-            raise ValueError(f"workspace must hold {need} contiguous, 16-byte aligned bytes (decode_workspace)")
-    same_device(q=q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, workspace=workspace)
-    with on_stream(stream) as st:
-        out = torch.empty(batch, nheads, hd, device=q.device, dtype=_BF16)
-        lse = torch.empty(batch, nheads, device=q.device, dtype=torch.float32) if return_lse else None
+        same_device(workspace=workspace)
+        raise ValueError(f"workspace must hold {need} contiguous, 16-byte aligned bytes (decode_workspace)")
+
+    def launch(st):
+        out = q.new_empty((batch, nheads, hd))
+        lse = torch.empty((batch, nheads), device=q.device, dtype=torch.float32) if return_lse else None
         ws = workspace
         if ws is None:  # only the arrival counters at its start have to be zero
             ws = torch.empty(need, device=q.device, dtype=torch.uint8)
             ws[:4 * batch * nheads].zero_()
-        call("sn_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), *args, out.data_ptr(),
-             lse.data_ptr() if return_lse else None, float(hd ** -0.5 if scale is None else scale), batch, nheads, hkv,
-             hd, ws.data_ptr(), ws.numel(), st)
-    return (out, lse) if return_lse else out
+        call("sn_paged_decode_attention", q.data_ptr(), qb, qh, *args, out.data_ptr(),
+             lse.data_ptr() if return_lse else None, hd ** -0.5 if scale is None else float(scale), batch, nheads, hkv,
+             hd, ws.data_ptr(), need, st)
+        return (out, lse) if return_lse else out
+
+    if stream is None:
+        return launch(current_handle(dev))
+    with on_stream(stream) as st:
+        return launch(st)
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, stream=None) -> None:
@@ -164,16 +212,141 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, stream=
     type): page dst[i] = page src[i] under every leading index; src, dst int32
     [pairs] on the device.  No page may be both copied from and copied to in
     one call, nor copied to twice."""
-    require_cuda("pool", pool)
-    if pool.dim() < 4 or not pool.is_contiguous() or pool.numel() == 0:
+    if not (isinstance(pool, torch.Tensor) and pool.is_cuda and pool.dim() >= 4 and pool.is_contiguous() and pool.numel()):
+        require_cuda("pool", pool)
         raise ValueError("pool must be a contiguous, non-empty [..., num_pages, nheads_kv, page_size, head_dim] tensor")
-    for name, t in (("src", src), ("dst", dst)):
-        require_cuda(name, t, torch.int32, 1)
-        if not t.is_contiguous() or t.shape != src.shape:
-            raise ValueError("src and dst must be contiguous int32 tensors of one length")
-    same_device(pool=pool, src=src, dst=dst)
-    n = pool.shape[-4]
-    nbytes = pool.shape[-1] * pool.shape[-2] * pool.shape[-3] * pool.element_size()
-    with on_stream(stream) as st:
-        call("sn_copy_pages", pool.data_ptr(), n * nbytes, nbytes, nbytes, pool.numel() * pool.element_size() // (n * nbytes),
-             n, src.data_ptr(), dst.data_ptr(), src.shape[0], st)
+    if not (isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.dtype is torch.int32 is dst.dtype and
+            src.dim() == 1 and src.shape == dst.shape and src.is_contiguous() and dst.is_contiguous()):
+        for name, t in (("src", src), ("dst", dst)):
+            require_cuda(name, t, torch.int32, 1)
+        raise ValueError("src and dst must be contiguous int32 tensors of one length")
+    dev = torch.cuda.current_device()
+    if not dev == pool.get_device() == src.get_device() == dst.get_device():
+        for name, t in (("src", src), ("dst", dst)):
+            require_cuda(name, t)
+        same_device(pool=pool, src=src, dst=dst)
+    n, heads, page, hd = pool.shape[-4:]
+    size = pool.element_size()
+    nbytes = heads * page * hd * size
+    args = (pool.data_ptr(), n * nbytes, nbytes, nbytes, pool.numel() * size // (n * nbytes), n, src.data_ptr(), dst.data_ptr(),
+            src.shape[0])
+    if stream is None:
+        call("sn_copy_pages", *args, current_handle(dev))
+    else:
+        with on_stream(stream) as st:
+            call("sn_copy_pages", *args, st)
+
+
+class PagedKVCache:
+    """The pages of all layers' keys and values, and the host's book-keeping of
+    who owns them: `slots` streams, each a list of pages and a length.
+
+    pool bf16 [n_layers, 2, num_pages, nheads_kv, page_size, head_dim]: a page
+    number means the same page in every layer, so one table serves all of them
+    and one copy_pages call moves a page everywhere.  `page_table` int32
+    [slots, max_pages] and `seq_lens` int32 [slots] are device tensors that
+    reserve / fork / free / compact update in place, so a captured decode step
+    goes on using them.  Full pages may be shared between forked streams (they
+    are never written again); a stream's last, partly filled page never is."""
+
+    def __init__(self, n_layers: int, num_pages: int, nheads_kv: int, head_dim: int, slots: int, max_pages: int,
+                 page_size: int = 16, device="cuda"):
+        if min(n_layers, num_pages, nheads_kv, head_dim, slots, max_pages, page_size) < 1:
+            raise ValueError("every size must be positive")
+        self.pool = torch.zeros(n_layers, 2, num_pages, nheads_kv, page_size, head_dim, device=device, dtype=_BF16)
+        self.page_size, self.num_pages, self.max_pages = page_size, num_pages, max_pages
+        self.page_table = torch.full((slots, max_pages), -1, device=device, dtype=torch.int32)
+        self.seq_lens = torch.zeros(slots, device=device, dtype=torch.int32)
+        self.pages = [[] for _ in range(slots)]  # of each stream, in order
+        self.lens = [0] * slots
+        self._users = [0] * num_pages
+        self._free = list(range(num_pages))  # a heap: the lowest free page first
+
+    def k(self, layer: int) -> torch.Tensor:
+        return self.pool[layer, 0]
+
+    def v(self, layer: int) -> torch.Tensor:
+        return self.pool[layer, 1]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self) -> int:
+        p = heapq.heappop(self._free)
+        self._users[p] = 1
+        return p
+
+    def _drop(self, page: int) -> None:
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            heapq.heappush(self._free, page)
+
+    def _upload(self, slots) -> None:
+        for s in slots:
+            row = self.pages[s] + [-1] * (self.max_pages - len(self.pages[s]))
+            self.page_table[s].copy_(torch.tensor(row, dtype=torch.int32))
+        self.seq_lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
+
+    def reserve(self, counts) -> None:
+        """Room for counts[s] more positions of every slot s (0: unchanged);
+        seq_lens then counts them.  Nothing is changed if there is not enough."""
+        if len(counts) != len(self.lens) or any(c < 0 for c in counts):
+            raise ValueError(f"counts must hold {len(self.lens)} numbers, none negative")
+        want = [-(-(n + c) // self.page_size) for n, c in zip(self.lens, counts)]
+        if max(want) > self.max_pages:
+            raise ValueError(f"a stream would need {max(want)} pages of at most {self.max_pages}")
+        need = sum(w - len(p) for w, p in zip(want, self.pages))
+        if need > len(self._free):
+            raise RuntimeError(f"out of pages: {need} needed, {len(self._free)} free")
+        grown = [s for s, w in enumerate(want) if w > len(self.pages[s])]
+        for s in grown:
+            self.pages[s] += [self._take() for _ in range(want[s] - len(self.pages[s]))]
+        self.lens = [n + c for n, c in zip(self.lens, counts)]
+        self._upload(grown)
+
+    def fork(self, src: int, dst: int) -> None:
+        """The stream of slot `src` once more in the empty slot `dst`: full pages
+        shared, the partly filled last one copied."""
+        if self.pages[dst] or self.lens[dst] or src == dst:
+            raise ValueError(f"slot {dst} is not empty")
+        full = self.lens[src] // self.page_size
+        partial = self.lens[src] % self.page_size > 0
+        if partial and not self._free:
+            raise RuntimeError("out of pages: 1 needed, 0 free")
+        self.pages[dst] = self.pages[src][:full]
+        for p in self.pages[dst]:
+            self._users[p] += 1
+        if partial:
+            self.pages[dst].append(self._take())
+            self._copy([self.pages[src][full]], [self.pages[dst][full]])
+        self.lens[dst] = self.lens[src]
+        self._upload([dst])
+
+    def free(self, slot: int) -> None:
+        """Empties a slot; its pages that no other stream shares are free again."""
+        for p in self.pages[slot]:
+            self._drop(p)
+        self.pages[slot], self.lens[slot] = [], 0
+        self._upload([slot])
+
+    def compact(self) -> int:
+        """Moves used pages to the lowest numbers; returns how many moved.  (The
+        rest of the pool may then be cut off or handed to something else.)"""
+        used = [p for p, n in enumerate(self._users) if n]
+        src = [p for p in used if p >= len(used)]
+        dst = [p for p in range(len(used)) if self._users[p] == 0]  # as many, and none of them a source
+        if not src:
+            return 0
+        self._copy(src, dst)
+        to = dict(zip(src, dst))
+        for a, b in to.items():
+            self._users[a], self._users[b] = 0, self._users[a]
+        self.pages = [[to.get(p, p) for p in pages] for pages in self.pages]
+        self._free = list(range(len(used), self.num_pages))
+        self._upload(range(len(self.pages)))
+        return len(src)
+
+    def _copy(self, src, dst) -> None:
+        dev = self.pool.device
+        copy_pages(self.pool, torch.tensor(src, dtype=torch.int32, device=dev), torch.tensor(dst, dtype=torch.int32, device=dev))
