@@ -1473,18 +1473,13 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
     int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
     if (rc != SN_OK) return rc;
     const dim3 grid(static_cast<unsigned>(plan.pairs), static_cast<unsigned>(plan.segments));
-    auto scan = [&](auto kern, int threads, uint32_t smem) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
-        cudaGetLastError();
-        return SN_ERR_LAUNCH;
-      }
-      return sn::launch(kern, grid, dim3(static_cast<unsigned>(threads)), smem, st, true, p, wk);
-    };
+    if (!sn::smem_room<sn::prompt_scan_mma_kernel>(sn::kScanSmem)) return SN_ERR_LAUNCH;
     if (tokens > static_cast<int64_t>(plan.seg) * sn::kChunk) {  // a prompt may have several segments
-      rc = scan(sn::prompt_states_kernel, sn::kScanThreads + 32, sn::kStateSmem);
+      if (!sn::smem_room<sn::prompt_states_kernel>(sn::kStateSmem)) return SN_ERR_LAUNCH;
+      rc = sn::launch(sn::prompt_states_kernel, grid, dim3(sn::kScanThreads + 32), sn::kStateSmem, st, true, p, wk);
       if (rc != SN_OK) return rc;
     }
-    return scan(sn::prompt_scan_mma_kernel, sn::kScanThreads, sn::kScanSmem);
+    return sn::launch(sn::prompt_scan_mma_kernel, grid, dim3(sn::kScanThreads), sn::kScanSmem, st, true, p, wk);
   }
   const int64_t rows = static_cast<int64_t>(batch) * d_inner;
   const int64_t blocks = tokens / sn::kConvRows + static_cast<int64_t>(batch);

@@ -910,6 +910,15 @@ inline bool pool_map(CUtensorMap* map, const void* base, const PoolStrides& st, 
   return tc::make_map_bf16_sw128(map, base, 5, dims, strides, box);
 }
 
+template <int HD, int NT>
+int launch_decode(int grid, cudaStream_t st, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p,
+                  const AttendSplit& sp) {
+  constexpr int smem = static_cast<int>(ring_bytes<HD>()) + 1024;
+  if (!smem_room<paged_decode_mma_kernel<HD, NT>>(smem)) return SN_ERR_LAUNCH;
+  return launch(paged_decode_mma_kernel<HD, NT>, dim3(static_cast<unsigned>(grid)), dim3(kAttWarps * 32), smem, st, true, km,
+                vm, p, sp);
+}
+
 inline bool pool_ok(int64_t page, int64_t head, int64_t tok, int nheads, int page_size, int hd) {
   // rows dense, axes in any order but not overlapping below the row
   return tok >= hd && head >= hd && page >= hd && nheads >= 1 && page_size >= 1;
@@ -1050,19 +1059,9 @@ int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_h
     const int64_t tiles = static_cast<int64_t>(max_pages) * (page_size / sn::kTile) * batch * sp.sets;
     const int64_t most = std::min<int64_t>((tiles + sn::kAttWarps - 1) / sn::kAttWarps, sn::kAttGridMax);
     const int grid = static_cast<int>(std::min<int64_t>(2 * sn::sm_count(), most));
-    auto go = [&](auto kern, size_t ring) {
-      const size_t smem = ring + 1024;
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
-        cudaGetLastError();
-        return SN_ERR_LAUNCH;
-      }
-      return sn::launch(kern, dim3(static_cast<unsigned>(grid)), dim3(sn::kAttWarps * 32), smem, st, true, km, vm, p, sp);
-    };
     if (head_dim == 64)
-      return two ? go(sn::paged_decode_mma_kernel<64, 2>, sn::ring_bytes<64>())
-                 : go(sn::paged_decode_mma_kernel<64, 1>, sn::ring_bytes<64>());
-    return two ? go(sn::paged_decode_mma_kernel<128, 2>, sn::ring_bytes<128>())
-               : go(sn::paged_decode_mma_kernel<128, 1>, sn::ring_bytes<128>());
+      return two ? sn::launch_decode<64, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<64, 1>(grid, st, km, vm, p, sp);
+    return two ? sn::launch_decode<128, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<128, 1>(grid, st, km, vm, p, sp);
   }
   return sn::launch(sn::paged_decode_rows_kernel, dim3(static_cast<unsigned>(batch * nheads)), dim3(128), 0, st,
                     true, p);

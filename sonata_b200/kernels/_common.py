@@ -2,10 +2,43 @@
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import importlib.machinery
+import importlib.util
 
 import torch
 
 from .. import _lib
+
+_FAST_PATH = _lib.LIB_PATH.with_name("_fastcall.so")
+_FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_copy_pages",
+                 "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size")
+
+
+class _NoFast:
+    """In the place of the short way's functions where it was not built: every
+    call is left to the wrapper."""
+    attend = append = copy = prompt = staticmethod(lambda *args: None)
+
+
+_fast = None
+
+
+def fast():
+    """bind/fastcall.cpp, on the loaded library: its functions return None for
+    what they leave to the wrappers, an int for a status of the C ABI."""
+    global _fast
+    if _fast is None:
+        lib = _lib.lib()
+        if not _FAST_PATH.exists():
+            _fast = _NoFast
+            return _fast
+        loader = importlib.machinery.ExtensionFileLoader("_fastcall", str(_FAST_PATH))
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fastcall", loader))
+        loader.exec_module(m)
+        m.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_SYMBOLS})
+        _fast = m
+    return _fast
 
 
 def stream_handle(stream=None) -> int:

@@ -13,7 +13,7 @@ import functools
 import torch
 
 from .. import _lib
-from ._common import call, current_handle, on_stream, require_cuda, same_device
+from ._common import call, current_handle, fast, on_stream, require_cuda, same_device
 
 _BF16 = torch.bfloat16
 
@@ -26,24 +26,8 @@ def _dense(name, t, shape, dtype=_BF16):
         raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor, got {tuple(t.shape)}")
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_size(*sizes: int) -> int:
-    return _lib.lib().sn_mamba2_prompt_workspace_size(*sizes)
-
-
-def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias, ssm_state: torch.Tensor,
-                  A: torch.Tensor, D, dt_bias, d_inner: int, ngroups: int, d_state: int, nheads: int,
-                  cu_seqlens: torch.Tensor | None = None, gate: bool = False, stream=None) -> torch.Tensor:
-    """zxbcdt [tokens, >= width]: the in_proj rows [z | x B C | dt] of all
-    prompts, packed (row stride taken from the tensor); prompt i holds rows
-    cu_seqlens[i] .. cu_seqlens[i+1]-1 (int32 [batch + 1] on the device;
-    None: one prompt).  conv_state [batch, conv_dim, W] and ssm_state [batch,
-    nheads, headdim, d_state] are each prompt's state before its first token
-    and are updated in place; A fp32 [nheads] (negative), D / dt_bias bf16
-    [nheads] or None, weight [conv_dim, W], bias [conv_dim] or None.  Returns
-    y [tokens, nheads, headdim] = S_t C_t + D x_t, times SiLU(z_t) with gate."""
-    if not (isinstance(zxbcdt, torch.Tensor) and zxbcdt.dtype is _BF16 and zxbcdt.is_cuda and zxbcdt.dim() == 2):
-        require_cuda("zxbcdt", zxbcdt, _BF16, 2)
+def _check(zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, d_inner, ngroups, d_state, nheads, cu_seqlens):
+    require_cuda("zxbcdt", zxbcdt, _BF16, 2)
     if zxbcdt.shape[0] > 0 and zxbcdt.stride(1) != 1:
         raise ValueError("zxbcdt must be contiguous along its last dimension")
     tokens = zxbcdt.shape[0]
@@ -68,23 +52,68 @@ def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     for name, t in (("D", D), ("dt_bias", dt_bias)):
         if t is not None:
             _dense(name, t, (nheads,))
+    same_device(zxbcdt=zxbcdt, conv_state=conv_state, weight=weight, bias=bias, ssm_state=ssm_state, A=A, D=D,
+                dt_bias=dt_bias, cu_seqlens=cu_seqlens)
+    raise ValueError("the arguments of mamba2_prompt do not fit together")
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(*sizes: int) -> int:
+    return _lib.lib().sn_mamba2_prompt_workspace_size(*sizes)
+
+
+def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias, ssm_state: torch.Tensor,
+                  A: torch.Tensor, D, dt_bias, d_inner: int, ngroups: int, d_state: int, nheads: int,
+                  cu_seqlens: torch.Tensor | None = None, gate: bool = False, stream=None) -> torch.Tensor:
+    """zxbcdt [tokens, >= width]: the in_proj rows [z | x B C | dt] of all
+    prompts, packed (row stride taken from the tensor); prompt i holds rows
+    cu_seqlens[i] .. cu_seqlens[i+1]-1 (int32 [batch + 1] on the device;
+    None: one prompt).  conv_state [batch, conv_dim, W] and ssm_state [batch,
+    nheads, headdim, d_state] are each prompt's state before its first token
+    and are updated in place; A fp32 [nheads] (negative), D / dt_bias bf16
+    [nheads] or None, weight [conv_dim, W], bias [conv_dim] or None.  Returns
+    y [tokens, nheads, headdim] = S_t C_t + D x_t, times SiLU(z_t) with gate."""
+    if stream is None:
+        r = fast().prompt(zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, d_inner, ngroups, d_state, nheads,
+                          cu_seqlens, gate)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_mamba2_prompt", r)
+    # one expression that holds for every valid call; _check says what is wrong with the others
     dev = torch.cuda.current_device()
-    for t in (zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, cu_seqlens):
-        if t is not None and t.get_device() != dev:
-            same_device(zxbcdt=zxbcdt, conv_state=conv_state, weight=weight, bias=bias, ssm_state=ssm_state, A=A, D=D,
-                        dt_bias=dt_bias, cu_seqlens=cu_seqlens)
+    conv_dim, heads = d_inner + 2 * ngroups * d_state, (nheads,)
+    try:
+        (tokens, columns), width = zxbcdt.shape, conv_state.shape[-1]
+        batch = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+        ok = (zxbcdt.dtype is conv_state.dtype is weight.dtype is ssm_state.dtype is _BF16 and A.dtype is torch.float32 and
+              d_inner % nheads == 0 and nheads % ngroups == 0 and columns >= d_inner + conv_dim + nheads and batch >= 1 and
+              conv_state.shape == (batch, conv_dim, width) and weight.shape == (conv_dim, width) and
+              ssm_state.shape == (batch, nheads, d_inner // nheads, d_state) and A.shape == heads and
+              (tokens == 0 or zxbcdt.stride(1) == 1) and conv_state.is_contiguous() and weight.is_contiguous() and
+              ssm_state.is_contiguous() and A.is_contiguous() and
+              zxbcdt.get_device() == conv_state.get_device() == weight.get_device() == ssm_state.get_device() ==
+              A.get_device() == dev)
+        for t, shape in ((bias, (conv_dim,)), (D, heads), (dt_bias, heads)):
+            if t is not None:
+                ok = ok and t.dtype is _BF16 and t.shape == shape and t.is_contiguous() and t.get_device() == dev
+        if cu_seqlens is not None:
+            ok = ok and (cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous() and
+                         cu_seqlens.get_device() == dev)
+    except (AttributeError, TypeError, ValueError, IndexError, ZeroDivisionError):
+        ok = False
+    if not ok:
+        _check(zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, d_inner, ngroups, d_state, nheads, cu_seqlens)
 
     def launch(st):
-        y = torch.empty((tokens, nheads, d_inner // nheads), device=zxbcdt.device, dtype=_BF16)
+        y = zxbcdt.new_empty((tokens, nheads, d_inner // nheads))
         if tokens == 0:
             return y
         nbytes = _workspace_size(tokens, batch, d_inner, ngroups, d_state, nheads)
         ws = torch.empty(nbytes, device=zxbcdt.device, dtype=torch.uint8)
-        call("sn_mamba2_prompt", zxbcdt.data_ptr(), zxbcdt.stride(0) if tokens > 1 else zxbcdt.shape[1],
+        call("sn_mamba2_prompt", zxbcdt.data_ptr(), zxbcdt.stride(0) if tokens > 1 else columns,
              conv_state.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(), ssm_state.data_ptr(),
              A.data_ptr(), None if D is None else D.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(),
              y.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), batch, tokens, d_inner, ngroups, d_state,
-             nheads, d_inner // nheads, conv_state.shape[2], 1 if gate else 0, ws.data_ptr(), nbytes, st)
+             nheads, d_inner // nheads, width, 1 if gate else 0, ws.data_ptr(), nbytes, st)
         return y
 
     if stream is None:

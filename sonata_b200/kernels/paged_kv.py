@@ -17,7 +17,7 @@ import math
 import torch
 
 from .. import _lib
-from ._common import call, current_handle, on_stream, require_cuda, same_device
+from ._common import call, current_handle, fast, on_stream, require_cuda, same_device
 
 _BF16 = torch.bfloat16
 
@@ -103,6 +103,10 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     sin fp32 [max_pos, rot / 2]: halves (j, j + rot/2), or neighbours (2j, 2j
     + 1) when interleaved.  k and v go to their pages; returns q [tokens,
     nheads, head_dim]."""
+    if stream is None:
+        r = fast().append(qkv, k_pages, v_pages, page_table, seq_lens, cos, sin, nheads, cu_seqlens, interleaved)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_rotary_paged_append", r)
     if not (isinstance(qkv, torch.Tensor) and qkv.dtype is _BF16 and qkv.is_cuda and qkv.dim() == 2):
         require_cuda("qkv", qkv, _BF16, 2)
     args = _pages(k_pages, v_pages, page_table, seq_lens)
@@ -167,6 +171,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     the sum of exponentials fp32 [batch, nheads].  `workspace`
     (decode_workspace) saves an allocation and a fill a call; calls that share
     one must not overlap."""
+    if stream is None:
+        r = fast().attend(q, k_pages, v_pages, page_table, seq_lens, scale, workspace, return_lse)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_paged_decode_attention", r)
     if not (isinstance(q, torch.Tensor) and q.dtype is _BF16 and q.is_cuda and q.dim() == 3):
         require_cuda("q", q, _BF16, 3)
     args = _pages(k_pages, v_pages, page_table, seq_lens)
@@ -212,6 +220,10 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, stream=
     type): page dst[i] = page src[i] under every leading index; src, dst int32
     [pairs] on the device.  No page may be both copied from and copied to in
     one call, nor copied to twice."""
+    if stream is None:
+        r = fast().copy(pool, src, dst)
+        if r is not None:
+            return None if r is True else _lib.check("sn_copy_pages", r)
     if not (isinstance(pool, torch.Tensor) and pool.is_cuda and pool.dim() >= 4 and pool.is_contiguous() and pool.numel()):
         require_cuda("pool", pool)
         raise ValueError("pool must be a contiguous, non-empty [..., num_pages, nheads_kv, page_size, head_dim] tensor")
