@@ -13,6 +13,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -74,10 +75,13 @@ struct Pages {
       return false;
     n = k->size(0), heads = k->size(1), page = k->size(2), hd = k->size(3);
     streams = table->size(0), width = table->size(1);
-    // axes of extent 1 have strides of their own: the wrapper's case
-    return n > 1 && heads > 1 && page > 1 && hd > 1 && k->stride(3) == 1 && v->stride(3) == 1 && streams > 0 && width > 1 &&
-           table->stride(1) == 1 && lens->size(0) == streams && lens->is_contiguous() && n <= INT32_MAX &&
+    return n > 0 && heads > 0 && page > 0 && hd > 0 && k->stride(3) == 1 && v->stride(3) == 1 && streams > 0 && width > 0 &&
+           (table->stride(1) == 1 || width == 1) && lens->size(0) == streams && lens->is_contiguous() && n <= INT32_MAX &&
            page <= INT32_MAX && width <= INT32_MAX;
+  }
+  // an axis of extent 1 is never stepped along: its stride may be anything
+  int64_t stride(const Tensor* t, int axis) const {
+    return t->size(axis) > 1 ? t->stride(axis) : std::max(t->stride(axis), hd);
   }
   int64_t table_stride() const { return streams > 1 ? table->stride(0) : width; }
 };
@@ -101,8 +105,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const float scale = a[5] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(p.hd)))
                                       : static_cast<float>(PyFloat_AS_DOUBLE(a[5]));
   Tensor out = at::empty({batch, heads, p.hd}, q->options());
-  const int rc = abi.attend(q->data_ptr(), q->stride(0), q->stride(1), p.k->data_ptr(), p.k->stride(0), p.k->stride(1),
-                            p.k->stride(2), p.v->data_ptr(), p.v->stride(0), p.v->stride(1), p.v->stride(2),
+  const int rc = abi.attend(q->data_ptr(), q->stride(0), q->stride(1), p.k->data_ptr(), p.stride(p.k, 0), p.stride(p.k, 1),
+                            p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1), p.stride(p.v, 2),
                             static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(), p.table_stride(),
                             static_cast<int>(p.width), p.lens->data_ptr<int>(), out.data_ptr(), nullptr, scale,
                             static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(p.heads),
@@ -128,8 +132,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   Tensor q = at::empty({tokens, heads, p.hd}, qkv->options());
   const int rc = abi.append(qkv->data_ptr(), tokens > 1 ? qkv->stride(0) : width, q.data_ptr(), p.k->data_ptr(),
-                            p.k->stride(0), p.k->stride(1), p.k->stride(2), p.v->data_ptr(), p.v->stride(0), p.v->stride(1),
-                            p.v->stride(2), static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(),
+                            p.stride(p.k, 0), p.stride(p.k, 1), p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1),
+                            p.stride(p.v, 2), static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(),
                             p.table_stride(), static_cast<int>(p.width), p.lens->data_ptr<int>(),
                             cu ? cu->data_ptr<int>() : nullptr, cos->data_ptr<float>(), sin->data_ptr<float>(),
                             static_cast<int>(cos->size(0)), static_cast<int>(tokens), static_cast<int>(p.streams), heads,

@@ -407,7 +407,7 @@ __device__ __forceinline__ uint4 state_column(const __nv_bfloat16* st, int k) {
 // tiles once: bounded by HBM (and, half as much, by the two special functions
 // of a SiLU).
 template <int W>
-__global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+__global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ float s_dt[kDtHeads * 129];
   __shared__ float s_max[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

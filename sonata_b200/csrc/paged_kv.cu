@@ -358,7 +358,8 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
 //   64.3; six in two: 85.4 and 65.9.)
 // ---------------------------------------------------------------------------
 constexpr int kAttWarps = 6;
-constexpr int kUncutSteps = 7;
+constexpr int kCutGain = 14;   // steps that a cut has to save
+constexpr int kCutSteps = 2;   // and the least a CTA takes of one
 constexpr int kTile = 16;
 constexpr int kAttHeadsMax = 16;   // heads a CTA takes together
 constexpr int kAttGridMax = 640;   // partial results the workspace holds, two a CTA
@@ -368,6 +369,7 @@ struct AttendSplit {
   unsigned* ticket;  // [batch * sets] arrivals, zero between calls
   int group, sets;   // query heads per key/value head; head sets of a stream (hkv * sets per kv head)
   int sets_per_kv, heads_per_set;
+  int slots;  // CTAs that are on the device together: no more take part in a cut
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -425,11 +427,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   constexpr int BOX = kTile * 128;  // bytes of one TMA box: 16 positions of 64 elements
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kAttWarps][S];
-  __shared__ float s_f[kAttWarps][H], s_lt[H];
+  __shared__ float s_f[kAttWarps][H], s_mt[H];
   __shared__ long long s_sum[kAttWarps];
   __shared__ int s_max[kAttWarps], s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int grid = gridDim.x, me = blockIdx.x;
+  const int me = blockIdx.x;
   unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   auto s_o = [&](int w) { return reinterpret_cast<float*>(ring + w * (S * stage_bytes<HD>())); };  // [H][HD]
   if (lane == 0) {
@@ -453,16 +455,16 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
 
   // ---- this CTA's share of all tiles: [at, stop) ----
   long long total = 0;
-  int longest = 0;
+  int longest = 0, tiles = 0;  // up to 32 streams: tiles of stream `lane`, in every warp
   for (int b = p.batch <= 32 ? lane : tid; b < p.batch; b += kAttWarps * 32) {
-    const int n = tiles_of(stream_len(p, b));
-    total += n;
-    longest = max(longest, n);
+    tiles = tiles_of(stream_len(p, b));
+    total += tiles;
+    longest = max(longest, tiles);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  if (p.batch > 32) {  // up to 32 streams every warp has summed all of them
+  if (p.batch > 32) {
     if (lane == 0) {
       s_sum[warp] = total;
       s_max[warp] = longest;
@@ -476,28 +478,39 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
     }
   }
   total *= sp.sets;
-  for (int b = me; b < p.batch; b += grid) {
-    if (stream_len(p, b) > 0) continue;  // an empty stream: zeros
+  for (int b = me; b < p.batch; b += gridDim.x) {
+    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : tiles_of(stream_len(p, b));
+    if (n > 0) continue;  // an empty stream: zeros
     for (int c = tid; c < p.hq * HD; c += kAttWarps * 32)
       p.out[static_cast<int64_t>(b) * p.hq * HD + c] = __float2bfloat16_rn(0.f);
     if (p.lse)
       for (int h = tid; h < p.hq; h += kAttWarps * 32) p.lse[static_cast<int64_t>(b) * p.hq + h] = -INFINITY;
   }
-  // Cutting a (stream, head) over CTAs costs its partial results and the last CTA's join, about 3 us; a step of a
-  // CTA's warps over their tiles about 0.45 us.  So where every stream is done in a few steps the cuts move to
-  // where a (stream, head) starts.
-  const bool cut = longest > kUncutSteps * kAttWarps;
-  const long long share = max((total + grid - 1) / grid, 1LL);
+  // Cutting a (stream, head set) over CTAs costs its partial results, the last CTA's join and a second start in most
+  // CTAs, as much as about 14 steps of a CTA's warps over their tiles.  So nothing is cut unless the longest one is that
+  // much above the even share: a CTA takes one (stream, head set), or, with more of them than CTAs, those that start in
+  // its share of the tiles.  Measured, cut / not: 4 streams of 2000 positions 13.5 / 20.5 us, 2 of 1500 13.9 / 14.3, 50 of
+  // 931 to 1863 31.5 / 28.9, 86 of up to 906 with one key/value head 34.8 / 19.3.
+  const int grid = min(static_cast<int>(gridDim.x), sp.slots);  // CTAs with a share
+  const bool cut = longest - total / grid > kCutGain * kAttWarps;
+  const bool single = !cut && static_cast<long long>(p.batch) * sp.sets <= gridDim.x;
+  const long long share = max((total + grid - 1) / grid, cut ? static_cast<long long>(kCutSteps) * kAttWarps : 1LL);
   long long at = me * share;
-  const long long stop = min(at + share, total);
+  const long long stop = single ? at + 1 : me < grid ? min(at + share, total) : 0;
   if (at >= stop) return;
   int b = 0;
   long long in_b = 0;  // place of `at` within the stream's tiles, head set by head set
-  {
+  if (single) {
+    b = me / sp.sets;
+    if (b >= p.batch) return;
+    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : tiles_of(stream_len(p, b));
+    if (n == 0) return;
+    in_b = static_cast<long long>(me - b * sp.sets) * n;
+  } else {
     long long before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {  // every warp for itself
-      const long long n =
-          b0 + lane < p.batch ? static_cast<long long>(tiles_of(stream_len(p, b0 + lane))) * sp.sets : 0;
+      if (p.batch > 32) tiles = b0 + lane < p.batch ? tiles_of(stream_len(p, b0 + lane)) : 0;
+      const long long n = static_cast<long long>(tiles) * sp.sets;
       long long upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -741,42 +754,41 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
     __syncthreads();
     const bool whole = lo == 0 && hi == nt;
     float* part = sp.part + (static_cast<int64_t>(2) * me + (first_piece ? 0 : 1)) * (H * (HD + 2));
-    if (tid < nh) {  // each warp's factor
-      float mt = s_m[0][tid], lt = 0.f;
+    if (tid < kAttWarps * H) {  // each warp's factor
+      const int w = tid / H, h = tid - w * H;
+      float mt = s_m[0][h];
 #pragma unroll
-      for (int w = 1; w < kAttWarps; ++w) mt = fmaxf(mt, s_m[w][tid]);
-#pragma unroll
-      for (int w = 0; w < kAttWarps; ++w) {
-        s_f[w][tid] = s_m[w][tid] == -INFINITY ? 0.f : exp2_approx(s_m[w][tid] - mt);
-        lt = fmaf(s_f[w][tid], s_l[w][tid], lt);
-      }
-      s_lt[tid] = lt == 0.f ? 0.f : 1.f / lt;
-      if (whole) {
-        if (p.lse) p.lse[static_cast<int64_t>(b) * p.hq + h0 + tid] = (mt + log2f(lt)) * 0.6931471805599453f;
-      } else {
-        part[tid] = mt;
-        part[H + tid] = lt;
-      }
+      for (int k = 1; k < kAttWarps; ++k) mt = fmaxf(mt, s_m[k][h]);
+      s_f[w][h] = s_m[w][h] == -INFINITY ? 0.f : exp2_approx(s_m[w][h] - mt);
+      if (w == 0) s_mt[h] = mt;
     }
     __syncthreads();
     for (int e = tid; e < nh * (HD / 4); e += kAttWarps * 32) {  // four elements of a head
       const int h = e / (HD / 4);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float lt = 0.f;
 #pragma unroll
       for (int w = 0; w < kAttWarps; ++w) {
         const float4 x = reinterpret_cast<const float4*>(s_o(w))[e];
         const float f = s_f[w][h];
+        lt = fmaf(f, s_l[w][h], lt);
         v.x = fmaf(f, x.x, v.x);
         v.y = fmaf(f, x.y, v.y);
         v.z = fmaf(f, x.z, v.z);
         v.w = fmaf(f, x.w, v.w);
       }
       if (whole) {
-        const float inv = s_lt[h];
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
         *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(b) * p.hq + h0) * HD + 4 * e) =
             make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+        if (p.lse && e % (HD / 4) == 0)
+          p.lse[static_cast<int64_t>(b) * p.hq + h0 + h] = (s_mt[h] + log2f(lt)) * 0.6931471805599453f;
       } else {
         reinterpret_cast<float4*>(part + 2 * H)[e] = v;
+        if (e % (HD / 4) == 0) {
+          part[h] = s_mt[h];
+          part[H + h] = lt;
+        }
       }
     }
     if (!whole) {
@@ -784,9 +796,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       const long long i0 = at - lo;
       const int first = static_cast<int>(i0 / share), last = static_cast<int>((i0 + nt - 1) / share);
       unsigned* ticket = sp.ticket + static_cast<int64_t>(b) * sp.sets + set;
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();  // the whole CTA's partial result (the barrier above) before its arrival
         const unsigned before = atomicAdd(ticket, 1u);
         s_last = before == static_cast<unsigned>(last - first);
         if (s_last) *ticket = 0;  // ready for the next call
@@ -798,10 +810,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
         const int n = last - first + 1;
         float* pm = reinterpret_cast<float*>(ring);  // [n][nh], the piece's factor in the end
         float* pl = pm + n * nh;                     // [n][nh]
-        auto piece = [&](int k) {  // in its CTA the piece comes first unless the set starts inside that CTA's share
-          const long long cta = first + k;
-          return sp.part + (2 * cta + (i0 > cta * share ? 1 : 0)) * (H * (HD + 2));
-        };
+        // in its CTA the piece comes first, but for a set that starts inside the first CTA's share
+        constexpr int kPart = H * (HD + 2);
+        const float* pieces = sp.part + static_cast<int64_t>(2) * first * kPart;
+        const int skip = i0 > first * share ? kPart : 0;
+        auto piece = [&](int k) { return pieces + (k == 0 ? skip : 2 * k * kPart); };
         for (int e = tid; e < n * nh; e += kAttWarps * 32) {
           const int k = e / nh, h = e - k * nh;
           const float* q = piece(k);
@@ -1057,8 +1070,10 @@ int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_h
     const bool two = sp.heads_per_set > 8;  // the operand takes 8 heads
     // two CTAs an SM, and no more than the page tables have tiles for
     const int64_t tiles = static_cast<int64_t>(max_pages) * (page_size / sn::kTile) * batch * sp.sets;
-    const int64_t most = std::min<int64_t>((tiles + sn::kAttWarps - 1) / sn::kAttWarps, sn::kAttGridMax);
-    const int grid = static_cast<int>(std::min<int64_t>(2 * sn::sm_count(), most));
+    const int64_t most = (tiles + sn::kAttWarps - 1) / sn::kAttWarps;
+    sp.slots = static_cast<int>(std::min<int64_t>(std::min(2 * sn::sm_count(), sn::kAttGridMax), most));
+    // and one for every (stream, head set) where they are short (4096 at most)
+    const int grid = static_cast<int>(std::max<int64_t>(sp.slots, std::min<int64_t>(static_cast<int64_t>(batch) * sp.sets, 4096)));
     if (head_dim == 64)
       return two ? sn::launch_decode<64, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<64, 1>(grid, st, km, vm, p, sp);
     return two ? sn::launch_decode<128, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<128, 1>(grid, st, km, vm, p, sp);
