@@ -771,19 +771,17 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
           dead = true;
         }
       };
-      constexpr uint32_t id = idesc_f16(128, 64, true, true);  // S^T += B^T (w x)
+      const uint32_t id = w.heads == 2 ? idesc_f16(128, 128, true, true) : idesc_f16(128, 64, true, true);
       for (int k = 0; k < w.chunks && !dead; ++k) {
         const int st = k % kStateStages;
         wait(ready + st, (k / kStateStages) & 1);
         if (dead) break;
         tc::fence_after_sync();
         const uint32_t at = smem_u32(smem) + st * kStateStage;
-        const uint64_t db = desc_k_rows(at, kTileBytes);
-        for (int h = 0; h < w.heads; ++h) {
-          const uint64_t dx = desc_k_rows(at + (2 + h) * kTileBytes, 16);
+        const uint64_t db = desc_k_rows(at, kTileBytes), dx = desc_k_rows(at + 2 * kTileBytes, kTileBytes);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) tc::mma_bf16(tmem + 64 * h, db + j * 128, dx + j * 128, id, k > 0 || j > 0);
-        }
+        for (int j = 0; j < 8; ++j)  // S^T += B^T (w x), of both heads
+          tc::mma_bf16(tmem, db + j * 128, dx + j * 128, id, k > 0 || j > 0);
         tc::mma_commit(empty + st);
         if (k + 1 == w.chunks) tc::mma_commit(done);
         // the stage of the chunk before this one is free once its products are done: this one's run meanwhile
@@ -804,8 +802,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
         dead = true;
       }
     };
-    // token, head and half of its 64 elements
-    const int i = tid >> 2, hh = (tid >> 1) & 1, half = tid & 1, h = w.h0 + min(hh, w.heads - 1);
+    // token, head and half of its 64 elements: eight lanes that share a phase of shared memory have eight tokens' rows
+    const int i = warp * 8 + (lane & 7), hh = lane >> 4, half = (lane >> 3) & 1, h = w.h0 + min(hh, w.heads - 1);
     const bool on = hh < w.heads;
     float a_i, a_end, dt, sx, sB;
     auto fetch = [&](int k) {
@@ -1269,7 +1267,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
       const int64_t tok = sg.start + tw;
       const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
-      const int piece = 4 * half + (lane & 3), psw = (lane >> 2) & 7;  // rows 8 apart swizzle alike
+      // 16-byte pieces are swizzled by the row's low bits reversed: eight lanes with a piece of eight rows, or with four
+      // pieces of two rows, then hit eight places
+      const int piece = 4 * half + (lane & 3), psw = __brev(lane >> 2) >> 29, osw = __brev(i & 7) >> 29;
       uint4 zv[4];
       if (p.gate) {
         const __nv_bfloat16* z = p.zx + tok * p.ld + h * 64 + 8 * piece;
@@ -1288,7 +1288,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         for (int k = 0; k < 4; ++k) sts128(stg + k * 1024 + ((piece ^ psw) << 4), zv[k].x, zv[k].y, zv[k].z, zv[k].w);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) zv[k] = lds128(xrow + (((4 * half + k) ^ sw) << 4));
+        for (int k = 0; k < 4; ++k) zv[k] = lds128(xrow + (((4 * half + k) ^ osw) << 4));
         __syncwarp();
       }
       float yv[32];
@@ -1305,7 +1305,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
           const __nv_bfloat162 b = __floats2bfloat162_rn(y.x, y.y);
           o[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
-        sts128(xrow + (((4 * half + k) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+        sts128(xrow + (((4 * half + k) ^ osw) << 4), o[0], o[1], o[2], o[3]);
       }
       __syncwarp();
       __nv_bfloat16* out = p.y + (tok * p.nh + h) * 64 + 8 * piece;
