@@ -434,12 +434,13 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
   if (on) {
     const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
     const __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
+    const __nv_bfloat16* u0 = u + static_cast<int64_t>(t0 + r0 - (W - 1)) * p.ld;
     uint4 raw[W + 7];  // inputs t0 + r0 - W + 1 .. t0 + r0 + 7
 #pragma unroll
     for (int k = 0; k < W + 7; ++k) {
       const int t = t0 + r0 + k - (W - 1);
       raw[k] = make_uint4(0, 0, 0, 0);
-      if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u + t * p.ld);
+      if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u0 + k * p.ld);
     }
     uint32_t wu[4 * W];  // [8][W] taps, 16 W bytes from a 16-byte boundary
 #pragma unroll
@@ -473,11 +474,14 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
       }
       float most = 0.f;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        o[r] = silu2(o[r]);
-        if (partial && t0 + r0 + r >= pb.len) o[r] = make_float2(0.f, 0.f);
-        most = fmaxf(fmaxf(most, fabsf(o[r].x)), fabsf(o[r].y));
+      for (int r = 0; r < 8; ++r) o[r] = silu2(o[r]);
+      if (partial) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (t0 + r0 + r >= pb.len) o[r] = make_float2(0.f, 0.f);
       }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) most = fmaxf(most, fmaxf(fabsf(o[r].x), fabsf(o[r].y)));
       top = fmaxf(top, most);
       own[c] = most == 0.f ? 0.f : pow2_floor(most);
       const float2 inv = splat(most == 0.f ? 1.f : rcp_pow2(own[c]));
