@@ -519,8 +519,10 @@ int sn_swiglu(const void *h, void *y, int batch, int d, void *stream);
  * and y_t *= SiLU(z_t) when gate.  conv_state [batch, conv_dim, d_conv] and
  * ssm_state [batch, nheads, headdim, d_state] hold each prompt's state before
  * its first token (zeros for a new stream) and are left as the state after
- * its last one, so a prompt may be taken in pieces.  A fp32 [nheads]; D and
- * dt_bias bf16 [nheads] or NULL; y [tokens, nheads, headdim].  d_conv <= 8,
+ * its last one, so a prompt may be taken in pieces.  A fp32 [nheads], negative
+ * (it is -exp(A_log)); D and dt_bias bf16 [nheads] or NULL; y [tokens, nheads,
+ * headdim].  An infinity or NaN in a prompt's rows may reach all of that
+ * prompt's outputs, up to 127 tokens back, and no other prompt's.  d_conv <= 8,
  * d_state <= 256.  workspace: sn_mamba2_prompt_workspace_size bytes, free to
  * reuse when the call's work on the stream is done.
  */

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256) prompt_conv_kernel(const PromptParams p) 
 // ---------------------------------------------------------------------------
 // Scan, token by token (any headdim, d_state <= 256): 16 lanes per (prompt,
 // head, headdim row) hold the row's state in fp32 registers, lane l the
-// elements l, l + 16, ...
+// elements l, l + 16, ...  Bounded by the chain of a token (1.7 us).
 // ---------------------------------------------------------------------------
 constexpr int kScanPerLane = 16;
 
@@ -252,12 +252,21 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 // that of the bf16 results; their range is kept by exact powers of two: every
 // 128-channel block of a chunk (x of two heads, B, C) is scaled to below 2,
 // dt to below 2 by its largest value, and the state operand by a bound of the
-// state carried along with it.  States and sums stay in fp32.
+// state carried along with it.  States and sums stay in fp32.  Causality is a
+// zero in M, so an infinity or NaN of a token reaches the earlier tokens of
+// its own chunk too (and, through the state, all later ones); other prompts
+// never share a chunk with it.  A is taken to be negative (it is -exp(A_log)),
+// so that no decay exceeds 1.
 //
 // Layout.  The convolution writes its results as the shared-memory images the
 // products read (128-byte swizzle, 128 tokens by 64 channels, 16 KB), padded
 // with zero rows to whole chunks of a prompt, so a chunk's operands come in
 // three bulk copies and no product sees another prompt's tokens.
+//
+// Measured, one prompt of 16384 tokens, 64 heads, one group (142.6 MB of rows
+// and 134.2 MB of outputs, 43 us at the copy bandwidth of 6.44 TB/s): 280 us,
+// of them 87 the convolution, 43 the states, 150 the outputs.  The tiles of x,
+// B and C (142 MB) are written by the first and read by the other two.
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 128;
 constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 64 channels of fp16
@@ -404,8 +413,12 @@ __device__ __forceinline__ uint4 state_column(const __nv_bfloat16* st, int k) {
 
 // One 128-channel block of one chunk (blockIdx.x < blocks), or 16 heads' dt
 // and decays.  Thread: 8 channels, 8 tokens.  Reads the inputs and writes the
-// tiles once: bounded by HBM (and, half as much, by the two special functions
-// of a SiLU).
+// tiles once (252 MB of HBM traffic for 16384 tokens: 39 us; measured 87, issue
+// slots 45% busy).  What it waits for is a mix: its loads, the two special
+// functions of a SiLU (32 us by themselves) and 15 warps an SM, since a
+// thread's inputs and the results that wait for the block's largest value take
+// 128 registers.  Three CTAs an SM spill (16384 tokens as fast, 1021 tokens 33 ->
+// 35 us); 4 or 2 tokens a thread read the taps and the halo more often.
 template <int W>
 __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ float s_dt[kDtHeads * 129];
@@ -690,7 +703,9 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
 // issues.  The segment's state from nothing goes to slot index + 1 of the
 // prompt; the first segment's starts from the prompt's state, which itself
 // goes to slot 0 (the last segment's CTAs of the next launch overwrite it).
-// The last segment has nothing to do.  Bounded by the reads of x.
+// The last segment has nothing to do.  Measured: 43 us for 96 segments of 32
+// chunks, 64 KB a chunk, 2400 cycles each; shared memory is busy for 1700 of them
+// (the copies in, x scaled in place, the operands of the products).
 // ---------------------------------------------------------------------------
 constexpr int kStateStages = 3;
 constexpr uint32_t kStateStage = 4 * kTileBytes;  // B, then x of two heads
@@ -891,12 +906,20 @@ constexpr int kServe = 4;  // the serving warp of a head's eight
 constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 
 // One segment of one pair of heads of a group (blockIdx.x: pair, blockIdx.y:
-// segment).  Warps 0-7 have the first head, 8-15 the second, a thread one row
+// segment): two heads, because they share B, C and C B^T and one computes while
+// the other waits for its products; shared memory, tensor memory and registers
+// are full then.  Warps 0-7 have the first head, 8-15 the second, a thread one row
 // (token i, or state n) and half of the columns of every product: 16 warps with
 // 128 registers each (a 17th for the copies would leave 96).  Of a head's warps
 // the one with the first 32 rows and the later columns has no part of M (it is
 // all above the diagonal), so it serves the others: it issues the products and
 // copies and works out the chunk's common factors.
+// Measured: 150 us for 128 segments of 32 chunks, 4.4 us (7700 cycles) a chunk
+// of two heads.  It is bounded by the chain of a chunk (S to its operand, C S,
+// M, w x, M X, outputs: each waits for the one before), with issue slots 41% busy
+// and the tensor pipe 27%.  Longer: M X into columns of its own by way of C B^T's
+// (214 us), groups of warps for the rows and for the decays (190), the outputs a
+// chunk behind (205), arrivals in place of the two barriers (165).
 __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const PromptParams p, const ChunkWork wk) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1461,7 +1484,8 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
   sn::ScanPlan plan;
   const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y) && sn::aligned16(conv_state) &&
                       sn::aligned16(conv_weight) && (!conv_bias || sn::aligned16(conv_bias));
-  // 64-element heads, 128 states, 16-byte rows: the tensor-core form
+  // 64-element heads, 128 states, 16-byte rows: the tensor-core form; anything else token by token (37 / 1021 / 16384
+  // tokens of 64 heads: 15 / 33 / 280 us, token by token 66 / 1266 / 27454)
   if (d_conv >= 2 && d_conv <= 4 && rows16 &&
       sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan) && plan.chunks <= 65535 && plan.segments <= 65535) {
     unsigned char* base = reinterpret_cast<unsigned char*>(p.xbc);
