@@ -39,8 +39,8 @@ struct PoolStrides {  // elements
 // ---------------------------------------------------------------------------
 // rotary_paged_append.  Pure data movement (a qkv row read, q / k / v
 // written, a cos / sin row per position), so it is bounded by HBM for
-// prompts (12288 tokens of 24 heads of 128: 28.6 us, 5.5 TB/s) and by the chain
-// stream - length - table - page for a decode step (48 tokens: 3.2 us).
+// prompts (12288 tokens of 24 heads of 128: 27.1 us, 5.8 TB/s) and by the chain
+// stream - length - table - page for a decode step (48 tokens: 2.8 us).
 // ---------------------------------------------------------------------------
 struct AppendParams {
   const __nv_bfloat16* qkv;  // [tokens, ld]
@@ -116,13 +116,14 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
 // The same by 16-byte chunks (head_dim and rot_dim multiples of 16, 16-byte
 // rows).  A warp takes one token: lane u + U * phase (U = head_dim / 16 units
 // a head) holds the token's 8 cos and sin values of its unit in registers and
-// takes the heads phase, phase + 32 / U, ..., six of them (blockIdx.y: the
-// next ones).  A unit is
-// the two chunks whose elements pair up (8u and rot/2 + 8u of the halves
+// takes the heads phase and phase + 32 / U (blockIdx.y: the next ones; six heads
+// a lane took 28.7 us for 27.1 and 3.5 for 2.8 below, fewer warps holding more).
+// A unit is the two chunks whose elements pair up (8u and rot/2 + 8u of the halves
 // layout) or two neighbours, so a head is read and written in whole 128-byte
 // lines.  The qkv loads wait for nothing, so they cover the look-up of the
-// stream, its length, the table row and the page.
-constexpr int kAppendHeads = 6;
+// stream, its length, the table row and the page; they are read once, so they
+// are the first to leave L2 (17.7 us for 18.7 with 48 heads of half rotation).
+constexpr int kAppendHeads = 2;
 
 template <bool kInterleaved>
 __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const AppendParams p) {
@@ -144,8 +145,8 @@ __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const Appe
   for (int i = 0; i < kAppendHeads; ++i) {
     const int h = h0 + i * phases;
     if (phase < phases && h < heads) {
-      a[i] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * p.hd + c1);
-      b[i] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * p.hd + c2);
+      a[i] = __ldcs(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * p.hd + c1));
+      b[i] = __ldcs(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * p.hd + c2));
     }
   }
   // the stream: the number of streams that end at or before t, 32 probes at a time
@@ -992,7 +993,7 @@ int sn_rotary_paged_append(const void* qkv, int64_t ld, void* q, void* k_pages, 
   auto rows16 = [](const void* base, int64_t a, int64_t b, int64_t c) {
     return sn::aligned16(base) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
   };
-  // 16-byte chunks throughout: 12288 tokens of 24 heads of 128 in 28.6 us (5.5 TB/s) against 168 us element by element
+  // 16-byte chunks throughout: 12288 tokens of 24 heads of 128 in 27.1 us (5.8 TB/s) against 168 us element by element
   if (head_dim % 16 == 0 && rot_dim % 16 == 0 && head_dim <= 512 && nheads + 2 * nheads_kv <= 65535 && rows16(qkv, ld, 0, 0) && sn::aligned16(q) &&
       rows16(k_pages, k_page_stride, k_head_stride, k_tok_stride) &&
       rows16(v_pages, v_page_stride, v_head_stride, v_tok_stride) && sn::aligned16(cos) && sn::aligned16(sin)) {
