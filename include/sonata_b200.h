@@ -558,8 +558,9 @@ int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const voi
  * and head strides, out dense; lse fp32 [batch, nheads] (log of the sum of
  * exponentials, -inf for an empty stream) or NULL.  An empty stream gives
  * zeros.  head_dim <= 256.  workspace: sn_paged_decode_workspace_size bytes,
- * 16-byte aligned, zero before the first call and left ready for the next;
- * calls that share it must not overlap.
+ * 16-byte aligned, its first 4 SN_PAGED_DECODE_COUNTERS bytes zero before the
+ * first call and left ready for the next, whatever its sizes are; calls that
+ * share it must not overlap.
  *
  * sn_copy_pages: page dst[i] = page src[i] (i < pairs, int32 on the device)
  * for each of `outer` pools outer_stride_bytes apart (layers, and k and v);
@@ -573,6 +574,7 @@ int sn_rotary_paged_append(const void *qkv, int64_t ld, void *q, void *k_pages, 
                            const int *cu_seqlens, const float *cos, const float *sin, int max_pos, int tokens,
                            int batch, int nheads, int nheads_kv, int head_dim, int rot_dim, int interleaved,
                            void *stream);
+#define SN_PAGED_DECODE_COUNTERS 2560
 size_t sn_paged_decode_workspace_size(int batch, int nheads, int head_dim);
 int sn_paged_decode_attention(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_pages,
                               int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,

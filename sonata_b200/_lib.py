@@ -29,6 +29,7 @@ SN_ACT_NONE = 1
 SN_ACT_SILU = 2
 SN_POST_NONE = 0
 SN_POST_TANH = 1
+SN_PAGED_DECODE_COUNTERS = 2560
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int

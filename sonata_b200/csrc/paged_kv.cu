@@ -364,13 +364,15 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
 constexpr int kAttWarps = 6;
 constexpr int kCutGain = 14;   // steps that a cut has to save
 constexpr int kCutSteps = 2;   // and the least a CTA takes of one
+constexpr int kJoinMost = 48;  // partial results that one CTA joins by itself
+constexpr int kJoinGroup = 8;  // and those of a group otherwise
 constexpr int kTile = 16;
 constexpr int kAttHeadsMax = 16;   // heads a CTA takes together
 constexpr int kAttGridMax = 640;   // partial results the workspace holds, two a CTA
 
 struct AttendSplit {
   float* part;       // [2 * grid][kHeadsMax][HD + 2] partial sums, maxima, outputs
-  unsigned* ticket;  // [batch * sets] arrivals, zero between calls
+  unsigned* ticket;  // [2][2 * grid] arrivals of a set's pieces or groups, of a group's pieces; zero between calls
   int group, sets;   // query heads per key/value head; head sets of a stream (hkv * sets per kv head)
   int sets_per_kv, heads_per_set;
   int slots;  // CTAs that are on the device together: no more take part in a cut
@@ -418,6 +420,108 @@ constexpr uint32_t stage_bytes() { return 2 * kTile * HD * 2; }
 template <int HD>
 constexpr uint32_t ring_bytes() { return kAttWarps * ring_stages<HD>() * stage_bytes<HD>(); }
 
+// The pieces of one (stream, head set) joined, in their order whichever CTA does it: called by each of the n CTAs that have
+// one, the mine-th, when its partial result is written.  A piece has the first of its CTA's two places, but for the first
+// piece of a set that starts inside a CTA's share (skip 1).
+template <int HD, int H>
+__device__ __forceinline__ void join_pieces(const AttendSplit& sp, unsigned char* ring, int first, int skip, int n,
+                                         int mine, int nh, __nv_bfloat16* out, float* lse) {
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kPart = H * (HD + 2);
+  // A set's tickets are those of its first piece's place, so that they do not depend on the call's sizes.  Many pieces are
+  // joined in groups, each by its last CTA to arrive and in the place of its first piece, with that place's ticket, and the groups by the last of those: about 100 pieces of 16 heads (3 streams of up to 100001 positions, one
+  // key/value head) 65 -> 51 us; with 17 to 48 pieces the second round costs more than it saves (4 streams of up to 10303
+  // positions 23.4 -> 29.3 us).
+  const int each = n > kJoinMost ? kJoinGroup : n;
+  int from = mine / each * each, step = 1, cnt = min(each, n - from);
+  bool final = each == n;
+  unsigned* arrival = sp.ticket + (final ? 0 : 2 * kAttGridMax) + 2 * (first + from) + (from == 0 ? skip : 0);
+  while (true) {
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();  // the whole CTA's partial result (the barrier above) before its arrival
+      const unsigned before = atomicAdd(arrival, 1u);
+      s_last = before == static_cast<unsigned>(cnt - 1);
+      if (s_last) *arrival = 0;  // ready for the next call
+    }
+    __syncthreads();
+    if (!s_last) break;
+    __threadfence();
+    float* const pieces = sp.part + static_cast<int64_t>(2) * (first + from) * kPart;
+    const int at0 = from == 0 ? skip * kPart : 0, stride = 2 * step * kPart;
+    auto piece = [&](int k) { return pieces + (k == 0 ? at0 : k * stride); };
+    // weights of the cnt pieces from, from + step, ...: all their maxima and sums first, then a warp a head
+    float* pm = reinterpret_cast<float*>(ring);  // [cnt][nh], the piece's factor in the end
+    float* pl = pm + cnt * nh;                   // [cnt][nh]
+    for (int e = tid; e < cnt * nh; e += kAttWarps * 32) {
+      const int k = e / nh, h = e - k * nh;
+      const float* q = piece(k);
+      pm[e] = __ldcg(q + h);
+      pl[e] = __ldcg(q + H + h);
+    }
+    __syncthreads();
+    for (int h = warp; h < nh; h += kAttWarps) {
+      float mt = -INFINITY, lt = 0.f;
+      for (int k = lane; k < cnt; k += 32) mt = fmaxf(mt, pm[k * nh + h]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+      for (int k = lane; k < cnt; k += 32) {
+        const float f = pm[k * nh + h] == -INFINITY ? 0.f : exp2_approx(pm[k * nh + h] - mt);
+        lt = fmaf(f, pl[k * nh + h], lt);
+        pm[k * nh + h] = f;
+      }
+      lt = warp_sum(lt);
+      if (final) {
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        for (int k = lane; k < cnt; k += 32) pm[k * nh + h] *= inv;
+        if (lse && lane == 0) lse[h] = (mt + log2f(lt)) * 0.6931471805599453f;
+      } else if (lane == 0) {
+        piece(0)[h] = mt;
+        piece(0)[H + h] = lt;
+      }
+    }
+    __syncthreads();
+    // four elements a thread, the pieces dealt to `deals` sets of threads
+    const int quads = nh * (HD / 4);
+    const int deals = max(1, kAttWarps * 32 / quads);
+    float4* sums = reinterpret_cast<float4*>(pm + (2 * cnt * nh + 3) / 4 * 4);  // [deals][quads]
+    for (int e = tid; e < deals * quads; e += kAttWarps * 32) {
+      const int d = e / quads, q4 = e - d * quads, h = q4 / (HD / 4);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int k = d; k < cnt; k += deals) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(piece(k) + 2 * H) + q4);
+        const float f = pm[k * nh + h];
+        v.x = fmaf(f, x.x, v.x);
+        v.y = fmaf(f, x.y, v.y);
+        v.z = fmaf(f, x.z, v.z);
+        v.w = fmaf(f, x.w, v.w);
+      }
+      sums[e] = v;
+    }
+    __syncthreads();
+    for (int e = tid; e < quads; e += kAttWarps * 32) {
+      float4 v = sums[e];
+      for (int d = 1; d < deals; ++d) {
+        const float4 x = sums[d * quads + e];
+        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+      }
+      if (final)
+        *reinterpret_cast<uint2*>(out + 4 * e) =
+            make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+      else
+        reinterpret_cast<float4*>(piece(0) + 2 * H)[e] = v;
+    }
+    if (final) break;
+    final = true;
+    from = 0;
+    step = each;
+    cnt = (n + each - 1) / each;
+    arrival = sp.ticket + 2 * first + skip;
+  }
+}
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(kAttWarps * 32, 2)
     paged_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -433,7 +537,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   __shared__ __align__(8) uint64_t full[kAttWarps][S];
   __shared__ float s_f[kAttWarps][H], s_mt[H];
   __shared__ long long s_sum[kAttWarps];
-  __shared__ int s_max[kAttWarps], s_last;
+  __shared__ int s_max[kAttWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int me = blockIdx.x;
   unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -796,82 +900,12 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       }
     }
     if (!whole) {
-      // the stream's set covers tiles [i0, i0 + nt) of the whole axis; its pieces are CTAs first .. last
+      // the stream's set covers tiles [i0, i0 + nt) of the whole axis; its pieces are CTAs first, first + 1, ...
       const long long i0 = at - lo;
-      const int first = static_cast<int>(i0 / share), last = static_cast<int>((i0 + nt - 1) / share);
-      unsigned* ticket = sp.ticket + static_cast<int64_t>(b) * sp.sets + set;
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();  // the whole CTA's partial result (the barrier above) before its arrival
-        const unsigned before = atomicAdd(ticket, 1u);
-        s_last = before == static_cast<unsigned>(last - first);
-        if (s_last) *ticket = 0;  // ready for the next call
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        // weights of the n pieces: all their maxima and sums first, then a warp a head
-        const int n = last - first + 1;
-        float* pm = reinterpret_cast<float*>(ring);  // [n][nh], the piece's factor in the end
-        float* pl = pm + n * nh;                     // [n][nh]
-        // in its CTA the piece comes first, but for a set that starts inside the first CTA's share
-        constexpr int kPart = H * (HD + 2);
-        const float* pieces = sp.part + static_cast<int64_t>(2) * first * kPart;
-        const int skip = i0 > first * share ? kPart : 0;
-        auto piece = [&](int k) { return pieces + (k == 0 ? skip : 2 * k * kPart); };
-        for (int e = tid; e < n * nh; e += kAttWarps * 32) {
-          const int k = e / nh, h = e - k * nh;
-          const float* q = piece(k);
-          pm[e] = __ldcg(q + h);
-          pl[e] = __ldcg(q + H + h);
-        }
-        __syncthreads();
-        for (int h = warp; h < nh; h += kAttWarps) {
-          float mt = -INFINITY, lt = 0.f;
-          for (int k = lane; k < n; k += 32) mt = fmaxf(mt, pm[k * nh + h]);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-          for (int k = lane; k < n; k += 32) {
-            const float f = pm[k * nh + h] == -INFINITY ? 0.f : exp2_approx(pm[k * nh + h] - mt);
-            lt = fmaf(f, pl[k * nh + h], lt);
-            pm[k * nh + h] = f;
-          }
-          lt = warp_sum(lt);
-          const float inv = lt == 0.f ? 0.f : 1.f / lt;
-          for (int k = lane; k < n; k += 32) pm[k * nh + h] *= inv;
-          if (p.lse && lane == 0)
-            p.lse[static_cast<int64_t>(b) * p.hq + h0 + h] = (mt + log2f(lt)) * 0.6931471805599453f;
-        }
-        __syncthreads();
-        // four elements a thread, the pieces dealt to `groups` sets of threads
-        const int quads = nh * (HD / 4);
-        const int groups = max(1, kAttWarps * 32 / quads);
-        float4* sums = reinterpret_cast<float4*>(pm + (2 * n * nh + 3) / 4 * 4);  // [groups][quads]
-        for (int e = tid; e < groups * quads; e += kAttWarps * 32) {
-          const int gr = e / quads, q4 = e - gr * quads, h = q4 / (HD / 4);
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int k = gr; k < n; k += groups) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(piece(k) + 2 * H) + q4);
-            const float f = pm[k * nh + h];
-            v.x = fmaf(f, x.x, v.x);
-            v.y = fmaf(f, x.y, v.y);
-            v.z = fmaf(f, x.z, v.z);
-            v.w = fmaf(f, x.w, v.w);
-          }
-          sums[e] = v;
-        }
-        __syncthreads();
-        for (int e = tid; e < quads; e += kAttWarps * 32) {
-          float4 v = sums[e];
-          for (int gr = 1; gr < groups; ++gr) {
-            const float4 x = sums[gr * quads + e];
-            v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
-          }
-          *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(b) * p.hq + h0) * HD + 4 * e) =
-              make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
-        }
-      }
+      const int first = static_cast<int>(i0 / share), n = static_cast<int>((i0 + nt - 1) / share) - first + 1;
+      const int64_t row = static_cast<int64_t>(b) * p.hq + h0;
+      join_pieces<HD, H>(sp, ring, first, i0 > first * share ? 1 : 0, n, me - first, nh,
+                         p.out + row * HD, p.lse ? p.lse + row : nullptr);
     }
     tc::fence_proxy_async_smem();
     __syncthreads();  // the rings may be filled again
@@ -1011,9 +1045,9 @@ int sn_rotary_paged_append(const void* qkv, int64_t ld, void* q, void* k_pages, 
 
 size_t sn_paged_decode_workspace_size(int batch, int nheads, int head_dim) {
   if (batch < 1 || nheads < 1 || head_dim < 1) return 0;
-  // tickets of every (stream, head set), then two partial results a CTA
-  const size_t tickets = (static_cast<size_t>(batch) * nheads * sizeof(unsigned) + 15) / 16 * 16;
-  return tickets + static_cast<size_t>(2) * sn::kAttGridMax * sn::kAttHeadsMax * (head_dim + 2) * sizeof(float);
+  // the tickets, then two partial results a CTA
+  static_assert(4 * sn::kAttGridMax == SN_PAGED_DECODE_COUNTERS);
+  return SN_PAGED_DECODE_COUNTERS * sizeof(unsigned) + static_cast<size_t>(2) * sn::kAttGridMax * sn::kAttHeadsMax * (head_dim + 2) * sizeof(float);
 }
 
 int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
@@ -1066,8 +1100,7 @@ int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_h
     sp.heads_per_set = (sp.group + sp.sets_per_kv - 1) / sp.sets_per_kv;
     sp.sets = nheads_kv * sp.sets_per_kv;
     sp.ticket = static_cast<unsigned*>(workspace);
-    const size_t tickets = (static_cast<size_t>(batch) * nheads * sizeof(unsigned) + 15) / 16 * 16;
-    sp.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + tickets);
+    sp.part = reinterpret_cast<float*>(sp.ticket + SN_PAGED_DECODE_COUNTERS);
     CUtensorMap km, vm;
     if (!sn::pool_map(&km, k_pages, p.ks, num_pages, nheads_kv, page_size, head_dim) ||
         !sn::pool_map(&vm, v_pages, p.vs, num_pages, nheads_kv, page_size, head_dim))

@@ -203,7 +203,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         ws = workspace
         if ws is None:  # only the arrival counters at its start have to be zero
             ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-            ws[:4 * batch * nheads].zero_()
+            ws[:4 * _lib.SN_PAGED_DECODE_COUNTERS].zero_()
         call("sn_paged_decode_attention", q.data_ptr(), qb, qh, *args, out.data_ptr(),
              lse.data_ptr() if return_lse else None, hd ** -0.5 if scale is None else float(scale), batch, nheads, hkv,
              hd, ws.data_ptr(), need, st)

@@ -132,6 +132,47 @@ def test_attend_unaligned_base(PK):
     assert ((got.double() - o).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("lens, hq, hkv, hd", [([20011], 16, 1, 128), ([20011], 1, 1, 64), ([13001, 0, 12345], 8, 1, 128),
+                                              ([9999, 10001], 20, 2, 64)])
+def test_attend_many_pieces(PK, lens, hq, hkv, hd):
+    """Streams cut into more pieces than one CTA joins by itself."""
+    attend_case(PK, lens, hq=hq, hkv=hkv, hd=hd, page=32, seed=7)
+
+
+def test_attend_many_pieces_repeat(PK):
+    """Joins in groups leave the workspace ready, and do not depend on who comes last."""
+    ws = PK.decode_workspace(3, 16, 128)
+    runs = []
+    for lens in ([20000, 17, 15000], [300, 200, 100], [20000, 17, 15000], [64, 30000, 1]):
+        tab, total = table(lens, 16, 9)
+        gen = torch.Generator(device="cuda").manual_seed(10)
+        kp, vp = (torch.randn(total, 1, 16, 128, device="cuda", generator=gen).to(BF16) for _ in range(2))
+        q = torch.randn(3, 16, 128, device="cuda", generator=gen).to(BF16)
+        seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        runs.append([PK.paged_decode_attention(q, kp, vp, tab, seq, workspace=ws) for _ in range(3)])
+        o, bound, _ = attend_truth(q, kp, vp, tab, lens, 16, 128 ** -0.5)
+        for got in runs[-1]:
+            assert ((got.double() - o).abs() <= bound + 1e-30).all()
+            assert torch.equal(got, runs[-1][0])
+    assert torch.equal(runs[0][0], runs[2][0])
+
+
+def test_attend_workspace_of_growing_calls(PK):
+    """One workspace for calls of more and more streams, heads and head sizes, all of them cut over CTAs."""
+    ws = PK.decode_workspace(40, 32, 128)
+    for B, hq, hkv, hd in ((1, 4, 1, 64), (2, 16, 1, 64), (2, 16, 4, 128), (5, 32, 2, 128), (40, 32, 4, 128), (1, 4, 1, 64)):
+        lens = [9000 // B + 61 * b + 1500 * (b == 0) for b in range(B)]
+        tab, total = table(lens, 16, B)
+        gen = torch.Generator(device="cuda").manual_seed(B)
+        kp, vp = (torch.randn(total, hkv, 16, hd, device="cuda", generator=gen).to(BF16) for _ in range(2))
+        q = torch.randn(B, hq, hd, device="cuda", generator=gen).to(BF16)
+        seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        o, bound, _ = attend_truth(q, kp, vp, tab, lens, 16, hd ** -0.5)
+        for _ in range(2):
+            got = PK.paged_decode_attention(q, kp, vp, tab, seq, workspace=ws)
+            assert ((got.double() - o).abs() <= bound + 1e-30).all()
+
+
 def test_attend_long_split(PK):
     """One long stream, split over many CTAs and joined; the same bits every time, one workspace for all calls."""
     lens = [50001, 20000, 3]
