@@ -411,25 +411,20 @@ __device__ __forceinline__ uint4 state_column(const __nv_bfloat16* st, int k) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// 16 bytes from global to shared memory, or 16 zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
 // One 128-channel block of one chunk (blockIdx.x < blocks), or 16 heads' dt
-// and decays.  Thread: 8 channels, 8 tokens.  Reads the inputs and writes the
-// tiles once (252 MB of HBM traffic for 16384 tokens: 39 us; measured 87, issue
-// slots 45% busy).  What it waits for is a mix: its loads, the two special
-// functions of a SiLU (32 us by themselves) and 15 warps an SM, since a
-// thread's inputs and the results that wait for the block's largest value take
-// 128 registers.  Three CTAs an SM spill (16384 tokens as fast, 1021 tokens 33 ->
-// 35 us); 4 or 2 tokens a thread read the taps and the halo more often.
+// and decays.  The inputs come through shared memory; a thread has two
+// channels of 32 tokens, a warp the 64 channels of a tile.
 template <int W>
-__global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
-  __shared__ float s_dt[kDtHeads * 129];
+__global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+  __shared__ __align__(16) unsigned char s_rows[(kChunk + W - 1) * 256];  // tokens t0 - W + 1 ..
   __shared__ float s_max[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int conv_dim = p.di + 2 * p.gds;
   const int blk = blockIdx.x;
-  const int c8 = tid & 15, r0 = (tid >> 4) * 8;
-  int d = blk * 128 + c8 * 8;  // channel of the convolution
-  if (blk >= wk.xblocks) d = p.di + (blk - wk.xblocks) * 128 + c8 * 8;
-  const bool on = blk < wk.xblocks ? d < p.di : blk < wk.blocks;
   pdl_launch_dependents();
   pdl_wait();
   const PromptBlock pb = find_block(p.prompts, kChunk, 0, blockIdx.y);
@@ -437,71 +432,82 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
   const int t0 = pb.block * kChunk;
   const int64_t chunk = blockIdx.y;
   if (blk >= wk.blocks) {
-    prompt_dt(p, wk, pb, chunk, (blk - wk.blocks) * kDtHeads, s_dt);
+    prompt_dt(p, wk, pb, chunk, (blk - wk.blocks) * kDtHeads, reinterpret_cast<float*>(s_rows));
     return;
   }
+  const int d0 = blk < wk.xblocks ? blk * 128 : p.di + (blk - wk.xblocks) * 128;  // channel of the convolution
+  const int wide = blk < wk.xblocks ? min(128, p.di - d0) : 128;                   // 64 or 128 of them
+  const int left = pb.len - t0;                                                    // tokens from here on
+  const __nv_bfloat16* u = p.zx + (static_cast<int64_t>(pb.start) + t0) * p.ld + p.di + d0;
+  // first and last inputs of the prompt: 8 channels a thread of the first chunk's first 16, which are the only ones that
+  // read or write these channels' state
+  const bool edge = t0 == 0 && tid < 16 && tid * 8 < wide;
+  __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * (p.di + 2 * p.gds) + d0 + tid * 8) * W;  // [8][W]
+  {
+    const int c = tid & 15;
+    for (int k = tid >> 4; k < kChunk + W - 1; k += 16) {
+      const int t = k - (W - 1);
+      const bool in = t < left && c * 8 < wide;
+      if (t0 + t >= 0) copy16(smem_u32(s_rows) + k * 256 + c * 16, in ? u + t * p.ld + c * 8 : u, in);
+    }
+    if (edge) {  // inputs before the prompt are the state's columns 1 .. W - 1
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k) *reinterpret_cast<uint4*>(s_rows + k * 256 + tid * 16) = state_column<W>(st, k + 1);
+    }
+  }
+  const int half = warp & 1, r0 = (warp >> 1) * 32;  // tile and tokens of the warp
+  const bool on = half * 64 < wide;
+  float2 w[W], bias = make_float2(0.f, 0.f);
+  if (on) {
+    const int d = d0 + half * 64 + 2 * lane;
+    uint32_t wu[W];  // taps of d, then of d + 1
+#pragma unroll
+    for (int k = 0; k < W; ++k) wu[k] = reinterpret_cast<const uint32_t*>(p.w + static_cast<int64_t>(d) * W)[k];
+    auto tap = [&](int e) { return e & 1 ? bf16hi(wu[e / 2]) : bf16lo(wu[e / 2]); };
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k] = make_float2(tap(k), tap(W + k));
+    if (p.bias) bias = unpack_bf16(*reinterpret_cast<const uint32_t*>(p.bias + d));
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
 
   float top = 0.f;
-  uint32_t out[4][8];  // [pair of channels][token], fp16 over the pair's own power of two
+  uint32_t out[4][8];  // [8 tokens][token], fp16 over the 8 tokens' own power of two
   float own[4];
   if (on) {
-    const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
-    const __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;  // [8][W]
-    const __nv_bfloat16* u0 = u + static_cast<int64_t>(t0 + r0 - (W - 1)) * p.ld;
-    uint4 raw[W + 7];  // inputs t0 + r0 - W + 1 .. t0 + r0 + 7
+    const unsigned char* in = s_rows + r0 * 256 + half * 128 + lane * 4;
+    float2 past[W - 1];
 #pragma unroll
-    for (int k = 0; k < W + 7; ++k) {
-      const int t = t0 + r0 + k - (W - 1);
-      raw[k] = make_uint4(0, 0, 0, 0);
-      if (t >= 0 && t < pb.len) raw[k] = *reinterpret_cast<const uint4*>(u0 + k * p.ld);
-    }
-    uint32_t wu[4 * W];  // [8][W] taps, 16 W bytes from a 16-byte boundary
+    for (int k = 0; k < W - 1; ++k) past[k] = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + k * 256));
 #pragma unroll
-    for (int k = 0; k < W; ++k)
-      *reinterpret_cast<uint4*>(wu + 4 * k) = reinterpret_cast<const uint4*>(p.w + static_cast<int64_t>(d) * W)[k];
-    uint4 bu = make_uint4(0, 0, 0, 0);
-    if (p.bias) bu = *reinterpret_cast<const uint4*>(p.bias + d);
-    if (t0 + r0 == 0) {  // the prompt's first tokens: inputs before them are the state's columns 1 .. W - 1
+    for (int g = 0; g < 4; ++g) {
+      float2 o[8];
 #pragma unroll
-      for (int k = 0; k < W - 1; ++k) raw[k] = state_column<W>(st, k + 1);
-    }
-    const bool partial = t0 + kChunk > pb.len;
+      for (int r = 0; r < 8; ++r) {
+        const float2 v = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + (W - 1 + 8 * g + r) * 256));
+        o[r] = bias;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {  // a pair of channels: few registers live at a time
-      auto tap = [&](int k) {
-        const int e0 = 2 * c * W + k, e1 = e0 + W;
-        return make_float2(e0 & 1 ? bf16hi(wu[e0 / 2]) : bf16lo(wu[e0 / 2]), e1 & 1 ? bf16hi(wu[e1 / 2]) : bf16lo(wu[e1 / 2]));
-      };
-      auto word = [&](const uint4& v) { return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w; };
-      float2 w[W], o[8];
+        for (int k = 0; k < W - 1; ++k) o[r] = fma2(past[k], w[k], o[r]);
+        o[r] = silu2(fma2(v, w[W - 1], o[r]));
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[k] = tap(k);
+        for (int k = 0; k < W - 2; ++k) past[k] = past[k + 1];
+        past[W - 2] = v;
+      }
+      if (left < kChunk) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) o[r] = unpack_bf16(word(bu));
-#pragma unroll
-      for (int k = 0; k < W + 7; ++k) {  // each input once, into the outputs it belongs to
-        const float2 v = unpack_bf16(word(raw[k]));
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-          if (k - j >= 0 && k - j < 8) o[k - j] = fma2(v, w[j], o[k - j]);
+        for (int r = 0; r < 8; ++r)
+          if (r0 + 8 * g + r >= left) o[r] = make_float2(0.f, 0.f);
       }
       float most = 0.f;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) o[r] = silu2(o[r]);
-      if (partial) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (t0 + r0 + r >= pb.len) o[r] = make_float2(0.f, 0.f);
-      }
-#pragma unroll
       for (int r = 0; r < 8; ++r) most = fmaxf(most, fmaxf(fabsf(o[r].x), fabsf(o[r].y)));
       top = fmaxf(top, most);
-      own[c] = most == 0.f ? 0.f : pow2_floor(most);
-      const float2 inv = splat(most == 0.f ? 1.f : rcp_pow2(own[c]));
+      own[g] = most == 0.f ? 0.f : pow2_floor(most);
+      const float2 inv = splat(most == 0.f ? 1.f : rcp_pow2(own[g]));
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const float2 v = mul2(o[r], inv);
-        out[c][r] = pack_f16(v.x, v.y);
+        out[g][r] = pack_f16(v.x, v.y);
       }
     }
   }
@@ -513,39 +519,34 @@ __global__ void __launch_bounds__(256, 2) prompt_conv_tile_kernel(const PromptPa
   for (int k = 0; k < 8; ++k) top = fmaxf(top, s_max[k]);
   const float sc = pow2_floor(top);
   if (tid == 0) wk.scale[chunk * wk.blocks + blk] = sc;
-  if (!on) return;
-  // tile of these channels, chunk c8 % 8 of its rows
-  unsigned char* tile;
-  if (blk < wk.xblocks) {
-    tile = wk.x + (chunk * p.nh + blk * 2 + (c8 >> 3)) * kTileBytes;
-  } else {
-    const int g = blk - wk.xblocks;
-    tile = (g < p.ng ? wk.b + (chunk * p.ng + g) * 2 * kTileBytes : wk.c + (chunk * p.ng + g - p.ng) * 2 * kTileBytes) +
-           (c8 >> 3) * kTileBytes;
-  }
-  // to the block's power of two: exact but for what falls below 2^-24 of it
-  __half2 f[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) f[c] = __float2half2_rn(own[c] * rcp_pow2(sc));
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int row = r0 + r;  // row % 8 == r
-    uint32_t o[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[c][r]), f[c]);
-      o[c] = *reinterpret_cast<const uint32_t*>(&v);
+  if (on) {
+    unsigned char* tile;
+    if (blk < wk.xblocks) {
+      tile = wk.x + (chunk * p.nh + blk * 2 + half) * kTileBytes;
+    } else {
+      const int g = blk - wk.xblocks;
+      tile = (g < p.ng ? wk.b + (chunk * p.ng + g) * 2 * kTileBytes : wk.c + (chunk * p.ng + g - p.ng) * 2 * kTileBytes) +
+             half * kTileBytes;
     }
-    *reinterpret_cast<uint4*>(tile + row * 128 + (((c8 & 7) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+    tile += r0 * 128 + (lane & 3) * 4;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      // to the block's power of two: exact but for what falls below 2^-24 of it
+      const __half2 f = __float2half2_rn(own[g] * rcp_pow2(sc));
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[g][r]), f);
+        *reinterpret_cast<uint32_t*>(tile + (8 * g + r) * 128 + (((lane >> 2) ^ r) << 4)) =
+            *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
   }
-  if (t0 + r0 == 0) {  // the state after the prompt, its last W inputs; no other thread reads or writes these channels'
-    __nv_bfloat16* st = p.conv_state + (static_cast<int64_t>(pb.seq) * conv_dim + d) * W;
-    const __nv_bfloat16* u = p.zx + static_cast<int64_t>(pb.start) * p.ld + p.di + d;
+  if (edge) {  // the state after the prompt, its last W inputs
     uint4 col[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       const int t = pb.len - W + k;  // < 0: the old state's column W + t
-      col[k] = t >= 0 ? *reinterpret_cast<const uint4*>(u + t * p.ld) : state_column<W>(st, W + t);
+      col[k] = t >= 0 ? *reinterpret_cast<const uint4*>(u + t * p.ld + tid * 8) : state_column<W>(st, W + t);
     }
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
