@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 // three bulk copies and no product sees another prompt's tokens.
 //
 // Measured, one prompt of 16384 tokens, 64 heads, one group (142.6 MB of rows
-// and 134.2 MB of outputs, 43 us at the copy bandwidth of 6.44 TB/s): 280 us,
-// of them 87 the convolution, 43 the states, 150 the outputs.  The tiles of x,
+// and 134.2 MB of outputs, 43 us at the copy bandwidth of 6.44 TB/s): 255 us,
+// of them 62 the convolution, 43 the states, 150 the outputs.  The tiles of x,
 // B and C (142 MB) are written by the first and read by the other two.
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 128;
@@ -418,9 +418,16 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
 
 // One 128-channel block of one chunk (blockIdx.x < blocks), or 16 heads' dt
 // and decays.  The inputs come through shared memory; a thread has two
-// channels of 32 tokens, a warp the 64 channels of a tile.
-template <int W>
-__global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
+// channels of 32 tokens, a warp the 64 channels of a tile.  kMany: in one run
+// of tokens and four CTAs an SM (64 registers); else in every fourth 8 tokens,
+// so that few tokens are spread over the warps, and three.
+// Inputs read and tiles written once (252 MB of HBM traffic for 16384 tokens,
+// 39 us; the special functions of a SiLU 32 us): measured 62, issue slots 66%
+// busy.  16-byte loads to registers, 8 channels of 8 tokens a thread, took 16%
+// fewer instructions but 128 registers, so 15 warps an SM where there are 30 (87
+// us).
+template <int W, bool kMany>
+__global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ __align__(16) unsigned char s_rows[(kChunk + W - 1) * 256];  // tokens t0 - W + 1 ..
   __shared__ float s_max[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -455,7 +462,8 @@ __global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptPa
       for (int k = 0; k < W - 1; ++k) *reinterpret_cast<uint4*>(s_rows + k * 256 + tid * 16) = state_column<W>(st, k + 1);
     }
   }
-  const int half = warp & 1, r0 = (warp >> 1) * 32;  // tile and tokens of the warp
+  constexpr int kNext = kMany ? 8 : 32;                             // from a thread's 8 tokens to its next
+  const int half = warp & 1, r0 = (warp >> 1) * (kMany ? 32 : 8);  // tile and first tokens of the warp
   const bool on = half * 64 < wide;
   float2 w[W], bias = make_float2(0.f, 0.f);
   if (on) {
@@ -478,13 +486,19 @@ __global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptPa
     const unsigned char* in = s_rows + r0 * 256 + half * 128 + lane * 4;
     float2 past[W - 1];
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) past[k] = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + k * 256));
-#pragma unroll
     for (int g = 0; g < 4; ++g) {
+      own[g] = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) out[g][r] = 0;
+      if (r0 + kNext * g >= left) continue;
+      if (!kMany || g == 0) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) past[k] = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + (kNext * g + k) * 256));
+      }
       float2 o[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const float2 v = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + (W - 1 + 8 * g + r) * 256));
+        const float2 v = unpack_bf16(*reinterpret_cast<const uint32_t*>(in + (W - 1 + kNext * g + r) * 256));
         o[r] = bias;
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) o[r] = fma2(past[k], w[k], o[r]);
@@ -496,7 +510,7 @@ __global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptPa
       if (left < kChunk) {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (r0 + 8 * g + r >= left) o[r] = make_float2(0.f, 0.f);
+          if (r0 + kNext * g + r >= left) o[r] = make_float2(0.f, 0.f);
       }
       float most = 0.f;
 #pragma unroll
@@ -536,7 +550,7 @@ __global__ void __launch_bounds__(256, 3) prompt_conv_tile_kernel(const PromptPa
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[g][r]), f);
-        *reinterpret_cast<uint32_t*>(tile + (8 * g + r) * 128 + (((lane >> 2) ^ r) << 4)) =
+        *reinterpret_cast<uint32_t*>(tile + (kNext * g + r) * 128 + (((lane >> 2) ^ r) << 4)) =
             *reinterpret_cast<const uint32_t*>(&v);
       }
     }
@@ -1486,7 +1500,7 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
   const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y) && sn::aligned16(conv_state) &&
                       sn::aligned16(conv_weight) && (!conv_bias || sn::aligned16(conv_bias));
   // 64-element heads, 128 states, 16-byte rows: the tensor-core form; anything else token by token (37 / 1021 / 16384
-  // tokens of 64 heads: 15 / 33 / 280 us, token by token 66 / 1266 / 27454)
+  // tokens of 64 heads: 13 / 33 / 255 us, token by token 66 / 1266 / 27454)
   if (d_conv >= 2 && d_conv <= 4 && rows16 &&
       sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan) && plan.chunks <= 65535 && plan.segments <= 65535) {
     unsigned char* base = reinterpret_cast<unsigned char*>(p.xbc);
@@ -1503,8 +1517,16 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
     wk.xblocks = plan.xblocks;
     wk.blocks = plan.blocks;
     wk.seg = plan.seg;
-    auto conv = d_conv == 4 ? sn::prompt_conv_tile_kernel<4> : d_conv == 3 ? sn::prompt_conv_tile_kernel<3> : sn::prompt_conv_tile_kernel<2>;
-    int rc = sn::launch(conv, dim3(static_cast<unsigned>(plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st, true, p, wk);
+    const int conv_blocks = plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads;
+    // more CTAs than three an SM hold at once: four (16384 tokens 255 us in all, with three 264); else three and tokens
+    // spread over the warps (37 / 1021 tokens 13.4 / 33.0 us, with four 13.9 / 34.1)
+    const bool many = plan.chunks * conv_blocks > 3 * sn::sm_count();
+    auto pick = [&](auto wide, auto narrow) { return many ? wide : narrow; };
+    auto conv = d_conv == 4   ? pick(sn::prompt_conv_tile_kernel<4, true>, sn::prompt_conv_tile_kernel<4, false>)
+                : d_conv == 3 ? pick(sn::prompt_conv_tile_kernel<3, true>, sn::prompt_conv_tile_kernel<3, false>)
+                              : pick(sn::prompt_conv_tile_kernel<2, true>, sn::prompt_conv_tile_kernel<2, false>);
+    int rc = sn::launch(conv, dim3(static_cast<unsigned>(conv_blocks), static_cast<unsigned>(plan.chunks)), dim3(256), 0, st,
+                        true, p, wk);
     if (rc != SN_OK) return rc;
     const dim3 grid(static_cast<unsigned>(plan.pairs), static_cast<unsigned>(plan.segments));
     if (!sn::smem_room<sn::prompt_scan_mma_kernel>(sn::kScanSmem)) return SN_ERR_LAUNCH;
