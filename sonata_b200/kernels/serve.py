@@ -28,7 +28,7 @@ class RaggedZonos:
         """`model`: its batch is the number of streams.  `num_pages` pages of
         `page_size` positions for all of them, `max_len` positions at most for one."""
         cfg = model.cfg
-        self.model, self.slots = model, model.batch
+        self.model, self.slots, self.max_len = model, model.batch, max_len
         self.attn = [blk for blk in model.backbone.layers if blk.is_attn]
         self.cache = PK.PagedKVCache(max(1, len(self.attn)), num_pages, cfg.num_heads_kv, cfg.head_dim, self.slots,
                                      -(-max_len // page_size), page_size)
@@ -37,6 +37,14 @@ class RaggedZonos:
         for blk in model.backbone.layers:
             if not blk.is_attn:
                 blk.mixer.alloc_state(self.slots)
+
+    def _reserve(self, counts) -> None:
+        """cache.reserve within max_len, which may end inside a page: there are no rotary angles past it."""
+        over = [s for s, c in enumerate(counts) if self.cache.lens[s] + c > self.max_len]
+        if over:
+            raise ValueError(f"stream {over[0]} would have {self.cache.lens[over[0]] + counts[over[0]]} positions of at most "
+                             f"{self.max_len}")
+        self.cache.reserve(counts)
 
     def _layers(self, h: torch.Tensor, mamba, attend) -> torch.Tensor:
         """h [rows, d_model] through the layers and the final norm."""
@@ -66,7 +74,7 @@ class RaggedZonos:
         lens = [int(n) for n in lens]
         if len(lens) != self.slots or sum(lens) != hidden.shape[0] or hidden.shape[0] == 0:
             raise ValueError(f"lens must hold {self.slots} lengths that add up to hidden's {hidden.shape[0]} rows, not 0")
-        cache.reserve(lens)
+        self._reserve(lens)
         offs = [sum(lens[:s]) for s in range(self.slots + 1)]
         cu = torch.tensor(offs, dtype=torch.int32, device=hidden.device)
 
@@ -108,7 +116,7 @@ class RaggedZonos:
         cfg, cache = self.model.cfg, self.cache
         if hidden.shape[0] != self.slots:
             raise ValueError(f"hidden must have {self.slots} rows")
-        cache.reserve([1] * self.slots)
+        self._reserve([1] * self.slots)
 
         def attend(layer, qkv):
             k, v = cache.k(layer), cache.v(layer)

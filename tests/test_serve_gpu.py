@@ -82,3 +82,27 @@ def test_refusals(cuda_lib):
     with pytest.raises(RuntimeError):
         r.prompt(x, [30, 30])  # 4 pages of 3
     assert r.cache.lens == [0, 0]
+
+
+def test_max_len_inside_a_page(cuda_lib):
+    """max_len positions and no more, whether or not it ends a page: the last one is right, the next one is refused and
+    changes nothing."""
+    from sonata_b200.kernels import decode_step as DS, serve
+    cfg = DS.ZonosBackboneConfig(n_layer=2, attn_layer_idx=[1])
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(22, cfg.d_model, device="cuda", generator=g).to(torch.bfloat16)
+    want = _dense_logits(9, cfg, x[:20])
+    m = DS.SyntheticZonos(cfg, batch=1, context=0, max_seqlen=8, seed=9)
+    r = serve.RaggedZonos(m, num_pages=10, max_len=20)  # pages of 16: two of them would hold 32
+    with pytest.raises(ValueError):
+        r.prompt(x[:21], [21])
+    assert r.cache.lens == [0] and r.cache.free_pages == 10
+    r.prompt(x[:18], [18])
+    with pytest.raises(ValueError):
+        r.prompt(x[18:21], [3])
+    for t in (18, 19):
+        _close(r.step(x[t:t + 1])[:, 0:1], want[t])
+    with pytest.raises(ValueError):
+        r.step(x[20:21])
+    assert r.cache.lens == [20]
+    assert cuda_lib.sn_device_status(1, None) == 0
