@@ -98,12 +98,17 @@ class Mamba2Mixer(torch.nn.Module):
         self.conv_ssu_supported = ds in (128, 256) and cfg.headdim % 16 == 0
         self.fused_conv_ssu = False
 
-    def alloc_state(self, batch):
+    def new_state(self, batch):
+        """(conv_state, ssm_state) of `batch` streams that have seen nothing."""
         cfg = self.cfg
         dev = self.conv_w.device
-        self.conv_state = torch.zeros(batch, self.conv_dim, cfg.d_conv, device=dev, dtype=_BF16)
-        self.ssm_state = torch.zeros(batch, cfg.nheads, cfg.headdim, cfg.d_state, device=dev, dtype=_BF16)
-        self.sync = torch.zeros(batch * cfg.ngroups, device=dev, dtype=torch.int32)  # the fused kernel's counters
+        return (torch.zeros(batch, self.conv_dim, cfg.d_conv, device=dev, dtype=_BF16),
+                torch.zeros(batch, cfg.nheads, cfg.headdim, cfg.d_state, device=dev, dtype=_BF16))
+
+    def alloc_state(self, batch):
+        self.conv_state, self.ssm_state = self.new_state(batch)
+        # the fused kernel's counters
+        self.sync = torch.zeros(batch * self.cfg.ngroups, device=self.conv_w.device, dtype=torch.int32)
 
     def step_fused_norms(self, h: torch.Tensor, residual, norm_w, norm_b):
         """The block's add + LayerNorm fused into in_proj and the gated RMSNorm
@@ -125,19 +130,24 @@ class Mamba2Mixer(torch.nn.Module):
                                    link=self.out_proj)
         return out, residual
 
-    def step(self, u: torch.Tensor, fused_glue: bool = True) -> torch.Tensor:
+    def step(self, u: torch.Tensor, fused_glue: bool = True, state=None) -> torch.Tensor:
+        """One token a stream.  `state`: a caller's own (conv_state, ssm_state),
+        updated in the place of the mixer's (with fused_glue)."""
         cfg = self.cfg
         b = u.shape[0]
         di, ds, nh = cfg.d_inner, cfg.d_state, cfg.nheads
         zxbcdt = self.in_proj(u)
         if fused_glue:
-            z, x, Bm, Cm, dt_e = MS.mamba2_split_conv(zxbcdt, self.conv_state, self.conv_w, self.conv_b, di,
+            conv_state, ssm_state = state or (self.conv_state, self.ssm_state)
+            z, x, Bm, Cm, dt_e = MS.mamba2_split_conv(zxbcdt, conv_state, self.conv_w, self.conv_b, di,
                                                       cfg.ngroups, ds, nh)
-            y = MS.selective_state_update(self.ssm_state, x, dt_e, self.A, Bm, Cm, D=self.D_e, z=None,
+            y = MS.selective_state_update(ssm_state, x, dt_e, self.A, Bm, Cm, D=self.D_e, z=None,
                                           dt_bias=self.dt_bias_e, dt_softplus=True)
             y = MS.rmsnorm_fn(y.view(b, di), self.norm_w, None, z=z, eps=cfg.norm_epsilon,
                               group_size=di // cfg.ngroups, norm_before_gate=False)
             return self.out_proj(y)
+        if state is not None:
+            raise ValueError("a caller's own state needs fused_glue")
         z = zxbcdt[:, :di].contiguous()
         xBC = zxbcdt[:, di:di + self.conv_dim].contiguous()
         dt = zxbcdt[:, di + self.conv_dim:]

@@ -25,8 +25,9 @@ from .mamba_prompt import mamba2_prompt
 
 class RaggedZonos:
     def __init__(self, model: SyntheticZonos, num_pages: int, max_len: int, page_size: int = 16):
-        """`model`: its batch is the number of streams.  `num_pages` pages of
-        `page_size` positions for all of them, `max_len` positions at most for one."""
+        """`model`: its batch is the number of streams, its weights are used and its
+        own decode state is left alone.  `num_pages` pages of `page_size`
+        positions for all streams, `max_len` positions at most for one."""
         cfg = model.cfg
         self.model, self.slots, self.max_len = model, model.batch, max_len
         self.attn = [blk for blk in model.backbone.layers if blk.is_attn]
@@ -34,9 +35,8 @@ class RaggedZonos:
                                      -(-max_len // page_size), page_size)
         self.cos, self.sin = PK.rotary_table(max_len, cfg.head_dim)
         self.workspace = PK.decode_workspace(self.slots, cfg.num_heads, cfg.head_dim)
-        for blk in model.backbone.layers:
-            if not blk.is_attn:
-                blk.mixer.alloc_state(self.slots)
+        # (conv_state, ssm_state) of each Mamba2 layer, this object's own
+        self.states = [blk.mixer.new_state(self.slots) for blk in model.backbone.layers if not blk.is_attn]
 
     def _reserve(self, counts) -> None:
         """cache.reserve within max_len, which may end inside a page: there are no rotary angles past it."""
@@ -49,7 +49,7 @@ class RaggedZonos:
     def _layers(self, h: torch.Tensor, mamba, attend) -> torch.Tensor:
         """h [rows, d_model] through the layers and the final norm."""
         cfg, residual = self.model.cfg, None
-        at = iter(range(len(self.attn)))
+        at, states = iter(range(len(self.attn))), iter(self.states)
         for blk in self.model.backbone.layers:
             h, residual = MS.layer_norm_fn(h, blk.norm_w, blk.norm_b, residual=residual, eps=cfg.norm_epsilon, prenorm=True)
             if blk.is_attn:
@@ -58,7 +58,7 @@ class RaggedZonos:
                 h, residual = MS.layer_norm_fn(h, blk.norm2_w, blk.norm2_b, residual=residual, eps=cfg.norm_epsilon, prenorm=True)
                 h = blk.mlp(h)
             else:
-                h = mamba(blk.mixer, h)
+                h = mamba(blk.mixer, next(states), h)
         bb = self.model.backbone
         return MS.layer_norm_fn(h, bb.norm_f_w, bb.norm_f_b, residual=residual, eps=cfg.norm_epsilon)
 
@@ -78,9 +78,9 @@ class RaggedZonos:
         offs = [sum(lens[:s]) for s in range(self.slots + 1)]
         cu = torch.tensor(offs, dtype=torch.int32, device=hidden.device)
 
-        def mamba(mx, h):
+        def mamba(mx, state, h):
             di, ds, nh = cfg.d_inner, cfg.d_state, cfg.nheads
-            y = mamba2_prompt(mx.in_proj(h), mx.conv_state, mx.conv_w, mx.conv_b, mx.ssm_state, mx.A_h, mx.D, mx.dt_bias,
+            y = mamba2_prompt(mx.in_proj(h), state[0], mx.conv_w, mx.conv_b, state[1], mx.A_h, mx.D, mx.dt_bias,
                               di, cfg.ngroups, ds, nh, cu_seqlens=cu, gate=True)
             y = MS.rmsnorm_fn(y.view(-1, di), mx.norm_w, None, eps=cfg.norm_epsilon, group_size=di // cfg.ngroups,
                               norm_before_gate=False)
@@ -123,23 +123,21 @@ class RaggedZonos:
             q = PK.rotary_paged_append(qkv, k, v, cache.page_table, cache.seq_lens, self.cos, self.sin, cfg.num_heads)
             return PK.paged_decode_attention(q, k, v, cache.page_table, cache.seq_lens, workspace=self.workspace).flatten(1)
 
-        return self._logits(self._layers(hidden, lambda mx, h: mx.step(h), attend))
+        return self._logits(self._layers(hidden, lambda mx, state, h: mx.step(h, state=state), attend))
 
     def fork(self, src: int, dst: int) -> None:
         """Stream `src` once more as the empty stream `dst`: its pages shared, its recurrent states copied."""
         self.cache.fork(src, dst)
-        for blk in self.model.backbone.layers:
-            if not blk.is_attn:
-                for st in (blk.mixer.conv_state, blk.mixer.ssm_state):
-                    st[dst].copy_(st[src])
+        for state in self.states:
+            for st in state:
+                st[dst].copy_(st[src])
 
     def free(self, slot: int) -> None:
         """Ends a stream: its pages are free, its recurrent states zero for the next one."""
         self.cache.free(slot)
-        for blk in self.model.backbone.layers:
-            if not blk.is_attn:
-                blk.mixer.conv_state[slot].zero_()
-                blk.mixer.ssm_state[slot].zero_()
+        for state in self.states:
+            for st in state:
+                st[slot].zero_()
 
 
 def main() -> int:

@@ -106,3 +106,32 @@ def test_max_len_inside_a_page(cuda_lib):
         r.step(x[20:21])
     assert r.cache.lens == [20]
     assert cuda_lib.sn_device_status(1, None) == 0
+
+
+def test_states_are_its_own(cuda_lib):
+    """Two of them on one model, and the model's own decode step between: none sees another's states."""
+    from sonata_b200.kernels import decode_step as DS, serve
+    cfg = DS.ZonosBackboneConfig(n_layer=2, attn_layer_idx=[1])
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(2, 12, cfg.d_model, device="cuda", generator=g).to(torch.bfloat16)
+    want = [_dense_logits(4, cfg, x[i]) for i in range(2)]
+    m = DS.SyntheticZonos(cfg, batch=1, context=0, max_seqlen=64, seed=4)
+    mixer = m.backbone.layers[0].mixer
+    own = mixer.conv_state, mixer.ssm_state
+    with torch.no_grad():
+        first = m.step(x[0, :1]).clone()
+    held = [t.clone() for t in own]
+    a = serve.RaggedZonos(m, num_pages=8, max_len=64)
+    a.prompt(x[0, :9], [9])
+    b = serve.RaggedZonos(m, num_pages=8, max_len=64)
+    b.prompt(x[1, :5], [5])
+    for t in range(9, 12):
+        _close(a.step(x[0, t:t + 1])[:, 0:1], want[0][t])
+        _close(b.step(x[1, t - 4:t - 3])[:, 0:1], want[1][t - 4])
+    # the model's states are the tensors they were, as they were
+    assert mixer.conv_state is own[0] and mixer.ssm_state is own[1]
+    assert torch.equal(own[0], held[0]) and torch.equal(own[1], held[1])
+    for t in own:
+        t.zero_()
+    with torch.no_grad():
+        assert torch.equal(m.step(x[0, :1]), first)
