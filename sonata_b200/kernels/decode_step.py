@@ -131,18 +131,24 @@ class Mamba2Mixer(torch.nn.Module):
         return out, residual
 
     def step(self, u: torch.Tensor, fused_glue: bool = True, state=None) -> torch.Tensor:
-        """One token a stream.  `state`: a caller's own (conv_state, ssm_state),
-        updated in the place of the mixer's (with fused_glue)."""
+        """One token a stream.  `state`: a caller's own (conv_state, ssm_state) pairs,
+        updated in the place of the mixer's (with fused_glue), each for as
+        many of u's rows, in order, as it has streams."""
         cfg = self.cfg
         b = u.shape[0]
         di, ds, nh = cfg.d_inner, cfg.d_state, cfg.nheads
         zxbcdt = self.in_proj(u)
         if fused_glue:
-            conv_state, ssm_state = state or (self.conv_state, self.ssm_state)
-            z, x, Bm, Cm, dt_e = MS.mamba2_split_conv(zxbcdt, conv_state, self.conv_w, self.conv_b, di,
-                                                      cfg.ngroups, ds, nh)
-            y = MS.selective_state_update(ssm_state, x, dt_e, self.A, Bm, Cm, D=self.D_e, z=None,
-                                          dt_bias=self.dt_bias_e, dt_softplus=True)
+            at, zs, ys = 0, [], []
+            for conv_state, ssm_state in state or [(self.conv_state, self.ssm_state)]:
+                rows = zxbcdt[at:at + conv_state.shape[0]]
+                z, x, Bm, Cm, dt_e = MS.mamba2_split_conv(rows, conv_state, self.conv_w, self.conv_b, di,
+                                                          cfg.ngroups, ds, nh)
+                ys.append(MS.selective_state_update(ssm_state, x, dt_e, self.A, Bm, Cm, D=self.D_e, z=None,
+                                                    dt_bias=self.dt_bias_e, dt_softplus=True))
+                zs.append(z)
+                at += rows.shape[0]
+            z, y = (v[0] if len(v) == 1 else torch.cat(v) for v in (zs, ys))
             y = MS.rmsnorm_fn(y.view(b, di), self.norm_w, None, z=z, eps=cfg.norm_epsilon,
                               group_size=di // cfg.ngroups, norm_before_gate=False)
             return self.out_proj(y)

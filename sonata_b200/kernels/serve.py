@@ -5,10 +5,11 @@ stream at its own position, over one paged cache.
 dense cache holds every stream at one common position) for streams of their
 own lengths: ``prompt`` takes any number of new tokens of any of the streams
 through the layers (``mamba2_prompt``; ``rotary_paged_append`` and attention
-over the stream's own positions), ``step`` one token of every stream
-(the decode-step ops; ``rotary_paged_append`` and ``paged_decode_attention``),
-both on the same recurrent states and pages.  ``fork`` continues a stream
-twice, ``free`` ends one.
+over the stream's own positions), ``step`` one token of every stream that
+holds any (the decode-step ops; ``rotary_paged_append`` and
+``paged_decode_attention``), both on the same recurrent states and pages.
+``fork`` continues a stream twice, ``free`` ends one: its slot is idle until
+a prompt or a fork starts another there.
 
     python -m sonata_b200.kernels.serve      # a small run on cuda:0
 """
@@ -110,20 +111,40 @@ class RaggedZonos:
         return logits
 
     @torch.no_grad()
-    def step(self, hidden: torch.Tensor) -> torch.Tensor:
-        """hidden [streams, d_model] bf16: one new token of every stream.
-        Returns logits fp32 [n_codebooks, streams, vocab]."""
+    def step(self, hidden: torch.Tensor, active=None) -> torch.Tensor:
+        """hidden [streams, d_model] bf16: one new token of every stream that
+        `active` (a truth value a stream) names, by default of those that hold
+        positions.  The other streams' rows are not read and nothing of them
+        changes.  Returns logits fp32 [n_codebooks, streams, vocab] (0 for
+        those)."""
         cfg, cache = self.model.cfg, self.cache
         if hidden.shape[0] != self.slots:
             raise ValueError(f"hidden must have {self.slots} rows")
-        self._reserve([1] * self.slots)
+        active = [n > 0 for n in cache.lens] if active is None else [bool(a) for a in active]
+        if len(active) != self.slots or not any(active):
+            raise ValueError(f"active must hold {self.slots} truth values, and at least one stream must take a token")
+        self._reserve([int(a) for a in active])
+        table, lens, runs, live = cache.page_table, cache.seq_lens, [(0, self.slots)], None
+        if not all(active):  # the active streams' rows, packed; their recurrent states stay where they are, in runs of slots
+            live = torch.tensor([s for s in range(self.slots) if active[s]], device=hidden.device)
+            hidden, table, lens = hidden[live], table[live], lens[live]
+            ends = [s for s in range(self.slots + 1) if (s < self.slots and active[s]) != (s > 0 and active[s - 1])]
+            runs = list(zip(ends[::2], ends[1::2]))
 
         def attend(layer, qkv):
             k, v = cache.k(layer), cache.v(layer)
-            q = PK.rotary_paged_append(qkv, k, v, cache.page_table, cache.seq_lens, self.cos, self.sin, cfg.num_heads)
-            return PK.paged_decode_attention(q, k, v, cache.page_table, cache.seq_lens, workspace=self.workspace).flatten(1)
+            q = PK.rotary_paged_append(qkv, k, v, table, lens, self.cos, self.sin, cfg.num_heads)
+            return PK.paged_decode_attention(q, k, v, table, lens, workspace=self.workspace).flatten(1)
 
-        return self._logits(self._layers(hidden, lambda mx, state, h: mx.step(h, state=state), attend))
+        def mamba(mx, state, h):
+            return mx.step(h, state=[(state[0][a:b], state[1][a:b]) for a, b in runs])
+
+        logits = self._logits(self._layers(hidden, mamba, attend))
+        if live is None:
+            return logits
+        out = logits.new_zeros(logits.shape[0], self.slots, logits.shape[2])
+        out[:, live] = logits
+        return out
 
     def fork(self, src: int, dst: int) -> None:
         """Stream `src` once more as the empty stream `dst`: its pages shared, its recurrent states copied."""

@@ -135,3 +135,47 @@ def test_states_are_its_own(cuda_lib):
         t.zero_()
     with torch.no_grad():
         assert torch.equal(m.step(x[0, :1]), first)
+
+
+def test_idle_streams(cuda_lib):
+    """A freed slot and one that never started stay empty through the others' steps, and a prompt or a fork into them is as
+    good as in a new one; steps of some of the streams leave the others where they are."""
+    from sonata_b200.kernels import decode_step as DS, serve
+    cfg = DS.ZonosBackboneConfig(n_layer=4, attn_layer_idx=[1, 3])
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(3, 40, cfg.d_model, device="cuda", generator=g).to(torch.bfloat16)
+    want = [_dense_logits(11, cfg, x[i]) for i in range(3)]
+    m = DS.SyntheticZonos(cfg, batch=4, context=0, max_seqlen=8, seed=11)
+    r = serve.RaggedZonos(m, num_pages=12, max_len=64)
+    junk = torch.full((cfg.d_model,), float("nan"), device="cuda", dtype=torch.bfloat16)
+    rows = lambda **k: torch.stack([k.get(f"s{s}", junk) for s in range(4)])
+    with pytest.raises(ValueError):  # no stream holds anything
+        r.step(rows())
+    r.prompt(torch.cat([x[0, :20], x[1, :9]]), [20, 9, 0, 0])
+    r.free(0)
+    for t in range(9, 12):
+        lg = r.step(rows(s1=x[1, t]))
+        _close(lg[:, 1:2], want[1][t])
+        assert not lg[:, [0, 2, 3]].any()
+    assert r.cache.lens == [0, 12, 0, 0] and r.cache.pages[0] == r.cache.pages[2] == []
+    r.prompt(x[2, :17], [17, 0, 0, 0])  # another stream in the freed slot
+    r.fork(1, 3)
+    for t in range(3):
+        lg = r.step(rows(s0=x[2, 17 + t], s1=x[1, 12 + t], s3=x[1, 12 + t]))
+        _close(lg[:, 0:1], want[2][17 + t])
+        _close(lg[:, 1:2], want[1][12 + t])
+        _close(lg[:, 3:4], want[1][12 + t])
+    # stream 0 alone, then a first token by name in the slot that never started, then all of them
+    lg = r.step(rows(s0=x[2, 20]), active=[True, False, False, False])
+    _close(lg[:, 0:1], want[2][20])
+    lg = r.step(rows(s2=x[0, 0]), active=[0, 0, 1, 0])
+    _close(lg[:, 2:3], want[0][0])
+    lg = r.step(rows(s0=x[2, 21], s1=x[1, 15], s2=x[0, 1], s3=x[1, 15]))
+    for s, i, t in ((0, 2, 21), (1, 1, 15), (2, 0, 1), (3, 1, 15)):
+        _close(lg[:, s:s + 1], want[i][t])
+    assert r.cache.lens == [22, 16, 2, 16]
+    for bad in ([True], [False] * 4):
+        with pytest.raises(ValueError):
+            r.step(rows(), active=bad)
+    assert r.cache.lens == [22, 16, 2, 16]
+    assert cuda_lib.sn_device_status(1, None) == 0
