@@ -396,6 +396,10 @@ __device__ __forceinline__ float exp2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// A warp's bounded wait for a tile: true in every lane or in none, however close to the limit it lands.
+__device__ __forceinline__ bool wait_tile(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+}
 // One tile of K or V: [head_dim / 64][16 positions][64 elements].
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int row, int head, int page, uint64_t* bar) {
   asm volatile(
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   const uint32_t k_even = og * 128 + ((t ^ og) << 4), k_odd = og * 128 + (((t + 4) ^ og) << 4);
   const uint32_t v_lo = t * 128 + ((og ^ t) << 4), v_hi = (t + 4) * 128 + ((og ^ (t + 4)) << 4);
   uint32_t parity = 0;  // of each ring slot's next wait
-  bool dead = false;    // a wait ran out: nothing more is loaded, what is in flight is still waited for
+  bool dead = false;    // a wait ran out: nothing more is loaded, what is in flight is still waited for, its tile is left out
 
   pdl_launch_dependents();
   if (tid == 0) {
@@ -725,11 +729,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       const int i = lo + warp + kAttWarps * k;
       __syncwarp();  // every lane is done with the slot of the last step
       load_next(k + S - 1, slot == 0 ? S - 1 : slot - 1);
-      const bool there = (loaded >> slot) & 1;
+      bool there = (loaded >> slot) & 1;  // the same in every lane, as everything that decides about loads and shuffles
       if (there) {
-        if (!mbar_wait_bounded(&full[warp][slot], (parity >> slot) & 1)) {
+        there = wait_tile(&full[warp][slot], (parity >> slot) & 1);
+        if (!there) {
           record_status(SN_ERR_TIMEOUT);
           dead = true;
+          wait_tile(&full[warp][slot], (parity >> slot) & 1);  // once more, as its copy may land on what the ring holds next
         }
         parity ^= 1u << slot;
       }
