@@ -549,8 +549,10 @@ int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const voi
  * them).  The first rot_dim elements of every q and k head are rotated by
  * the table row of the token's position (cos, sin fp32 [max_pos, rot_dim /
  * 2]): pairs (j, j + rot_dim / 2), or (2j, 2j + 1) when interleaved.  q goes
- * to q [tokens, nheads, head_dim], k and v to their pages.  Products and
- * sums in fp32, rounded separately, as sn_rotary_kv_append.
+ * to q [tokens, nheads, head_dim], k and v to their pages; a token whose
+ * position is out of range and a row of no stream get zeros in q and write
+ * nothing else.  Products and sums in fp32, rounded separately, as
+ * sn_rotary_kv_append.
  *
  * sn_paged_decode_attention: out[b, h] = sum_t softmax_t(scale q[b, h] .
  * k[t]) v[t] over the stream's positions t < seq_lens[b]; nheads / nheads_kv

@@ -78,15 +78,17 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
   const int t = static_cast<int>(e / (static_cast<int64_t>(h2) * heads));
   const int b = p.cu ? stream_of(p.cu, p.batch, t) : t;
   const int end = p.cu ? p.cu[b + 1] : t + 1;
-  if (p.cu && (t < p.cu[b] || t >= end)) return;  // a token of no stream
-  const int pos = p.seq_lens[b] - (end - t);
   const bool rotated = head < p.hq + p.hkv && j < p.rot / 2;
   const bool halves = rotated && !p.interleaved;
   const int i1 = halves ? j : 2 * j, i2 = halves ? j + p.rot / 2 : 2 * j + 1;
   const __nv_bfloat16* src = p.qkv + t * p.ld + static_cast<int64_t>(head) * p.hd;
   __nv_bfloat16 o1 = src[i1], o2 = src[i2];
-  if (pos < 0 || pos >= p.max_pos) {
-    record_status(SN_ERR_INVALID_ARGUMENT);
+  __nv_bfloat16* const q = p.q + (static_cast<int64_t>(t) * p.hq + head) * p.hd;  // if it is a head of q
+  const bool stray = p.cu && (t < p.cu[b] || t >= end);  // a token of no stream
+  const int pos = p.seq_lens[b] - (end - t);
+  if (stray || pos < 0 || pos >= p.max_pos) {
+    if (!stray) record_status(SN_ERR_INVALID_ARGUMENT);
+    if (head < p.hq) q[i1] = q[i2] = __float2bfloat16_rn(0.f);
     return;
   }
   if (rotated) {
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
   }
   __nv_bfloat16* dst;
   if (head < p.hq) {
-    dst = p.q + (static_cast<int64_t>(t) * p.hq + head) * p.hd;
+    dst = q;
   } else {
     const int pg = page_of(p.map, b, pos / p.map.page_size);
     if (pg < 0) {
@@ -124,6 +126,12 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
 // stream, its length, the table row and the page; they are read once, so they
 // are the first to leave L2 (17.7 us for 18.7 with 48 heads of half rotation).
 constexpr int kAppendHeads = 2;
+
+// A warp writes zeros to the n elements (a multiple of 16) of a q row.  Out of line: in the kernel it costs the others 4% of
+// their time.
+__device__ __noinline__ void zero_row(__nv_bfloat16* row, int n) {
+  for (int i = 8 * (threadIdx.x & 31); i < n; i += 256) *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+}
 
 template <bool kInterleaved>
 __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const AppendParams p) {
@@ -162,11 +170,15 @@ __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const Appe
     lo += __popc(__ballot_sync(0xffffffffu, lane < n && p.cu[min(lo + lane + 1, p.batch)] <= t));
     s = min(lo, p.batch - 1);
     end = p.cu[s + 1];
-    if (t < p.cu[s] || t >= end) return;  // a token of no stream
+    if (t < p.cu[s] || t >= end) {  // a token of no stream
+      zero_row(p.q + static_cast<int64_t>(t) * p.hq * p.hd, p.hq * p.hd);
+      return;
+    }
   }
   const int pos = p.seq_lens[s] - (end - t);
   if (pos < 0 || pos >= p.max_pos) {
     record_status(SN_ERR_INVALID_ARGUMENT);
+    zero_row(p.q + static_cast<int64_t>(t) * p.hq * p.hd, p.hq * p.hd);
     return;
   }
   const int pg = page_of(p.map, s, pos / p.map.page_size);

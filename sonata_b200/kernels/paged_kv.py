@@ -102,7 +102,7 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     elements of each q and k head are rotated by the position's row of cos /
     sin fp32 [max_pos, rot / 2]: halves (j, j + rot/2), or neighbours (2j, 2j
     + 1) when interleaved.  k and v go to their pages; returns q [tokens,
-    nheads, head_dim]."""
+    nheads, head_dim], zeros for a row of no stream or a position out of range."""
     if stream is None:
         r = fast().append(qkv, k_pages, v_pages, page_table, seq_lens, cos, sin, nheads, cu_seqlens, interleaved)
         if r is not None:

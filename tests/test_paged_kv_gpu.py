@@ -487,3 +487,34 @@ def test_refusals(PK):
             PK.rotary_table(**dict(dict(max_pos=8, rot_dim=4), **bad))
     with pytest.raises(ValueError):
         PK.decode_workspace(0, 16, 128)
+
+
+@pytest.mark.parametrize("hd,rot,inter", [(128, 128, False), (128, 64, True), (40, 24, False)])
+def test_append_refused_tokens_have_zero_q(PK, cuda_lib, hd, rot, inter):
+    """Positions past the rotary table or before the stream's start, and rows of no stream: q is zero there and the pages
+    are left alone, whatever the memory of the output held before; the other tokens are as they are in a call without them."""
+    assert cuda_lib.sn_device_status(1, None) == 0
+    g = torch.Generator(device="cuda").manual_seed(21)
+    qkv = torch.randn(14, (6 + 2 * 2) * hd, device="cuda", generator=g).to(BF16)
+    cos, sin = PK.rotary_table(20, rot)
+    tab = torch.arange(6, dtype=torch.int32, device="cuda").view(3, 2)  # two pages of 16 for each of 3 streams
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    def run(lens, cu, rows):
+        kp, vp = (torch.full((6, 2, 16, hd), 7.0, device="cuda", dtype=BF16) for _ in range(2))
+        poison = torch.full((rows.shape[0], 6, hd), float("nan"), device="cuda", dtype=BF16)
+        del poison  # the output gets this block
+        q = PK.rotary_paged_append(rows, kp, vp, tab, lens, cos, sin, 6, cu_seqlens=cu, interleaved=inter)
+        torch.cuda.synchronize()
+        return q, kp, vp
+
+    # rows 0, 1 and 12, 13 belong to no stream; stream 0: positions 18 .. 21 of a table of 20; stream 1: -2 .. 1; stream 2: 3, 4
+    q, kp, vp = run(ints(22, 2, 5), ints(2, 6, 10, 12), qkv)
+    assert cuda_lib.sn_device_status(1, None) == -1
+    kept = [2, 3, 8, 9, 10, 11]  # positions 18, 19 of stream 0; 0, 1 of stream 1; 3, 4 of stream 2
+    want = run(ints(20, 2, 5), ints(0, 2, 4, 6), qkv[kept])
+    assert cuda_lib.sn_device_status(1, None) == 0
+    assert torch.equal(q[kept], want[0]) and torch.isfinite(want[0]).all()
+    rest = [t for t in range(14) if t not in kept]
+    assert not q[rest].any()
+    assert torch.equal(kp, want[1]) and torch.equal(vp, want[2])
