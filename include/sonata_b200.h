@@ -512,7 +512,8 @@ int sn_swiglu(const void *h, void *y, int batch, int d, void *stream);
  * prompts run inside the mamba_ssm library).  zxbcdt [tokens, ld]: the
  * in_proj rows [z | x B C | dt] of all prompts, packed; prompt i holds rows
  * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32 [batch + 1] on the device;
- * NULL: one prompt of all tokens, batch 1; empty prompts are fine).
+ * NULL: one prompt of all tokens, batch 1; empty prompts are fine; rows of no
+ * prompt get zeros in y).
  *   xBC_t = SiLU(conv_bias + sum_k conv_weight[d, k] u_{t - d_conv + 1 + k}[d])
  *   dt_t  = softplus(dt + dt_bias)
  *   S_t   = exp(dt_t A) S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t + D x_t

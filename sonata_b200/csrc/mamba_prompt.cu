@@ -109,6 +109,23 @@ struct PromptParams {
   int di, gds, ds, ng, nh, hd, hpg, W, gate;
 };
 
+// Zeros in the rows of y before the first prompt and after the last (offsets clamped as above; where they fall, a row of a
+// prompt may be among them, and the scan, a later launch, writes it), shared by `count` CTAs of which this is the
+// index-th.  Out of line, since a call with such rows is the exception.
+__device__ __noinline__ void zero_rows(__nv_bfloat16* y, int n, int before, int after, int tokens, int index, int count) {
+  const int rows = before + tokens - after;
+  for (int r = index; r < rows; r += count) {
+    __nv_bfloat16* row = y + static_cast<int64_t>(r < before ? r : after + r - before) * n;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) row[i] = __float2bfloat16_rn(0.f);
+  }
+}
+__device__ __forceinline__ void zero_outside(const PromptParams& p, int index, int count) {
+  if (!p.prompts.cu) return;
+  const int tokens = p.prompts.tokens;
+  const int before = min(max(p.prompts.cu[0], 0), tokens), after = min(max(p.prompts.cu[p.prompts.batch], 0), tokens);
+  if (before > 0 || after < tokens) zero_rows(p.y, p.di, before, after, tokens, index, count);
+}
+
 // ---------------------------------------------------------------------------
 // Convolution: one thread per channel and block of kConvRows tokens.  The
 // thread of a prompt's first block also moves the channel's state on (it is
@@ -120,6 +137,7 @@ constexpr int kMaxConvWidth = 8;
 __global__ void __launch_bounds__(256) prompt_conv_kernel(const PromptParams p) {
   pdl_launch_dependents();
   pdl_wait();
+  zero_outside(p, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
   const PromptBlock pb = find_block(p.prompts, kConvRows, 1, blockIdx.y);
   if (pb.seq < 0) return;
   const int conv_dim = p.di + 2 * p.gds;
@@ -434,6 +452,9 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(co
   const int blk = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
+  // by the CTAs of dt: all of them would take 1 us of 258 longer over 16384 tokens
+  if (blk >= wk.blocks)
+    zero_outside(p, blockIdx.y * (gridDim.x - wk.blocks) + blk - wk.blocks, (gridDim.x - wk.blocks) * gridDim.y);
   const PromptBlock pb = find_block(p.prompts, kChunk, 0, blockIdx.y);
   if (pb.seq < 0) return;
   const int t0 = pb.block * kChunk;

@@ -72,7 +72,8 @@ def mamba2_prompt(zxbcdt: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     nheads, headdim, d_state] are each prompt's state before its first token
     and are updated in place; A fp32 [nheads] (negative), D / dt_bias bf16
     [nheads] or None, weight [conv_dim, W], bias [conv_dim] or None.  Returns
-    y [tokens, nheads, headdim] = S_t C_t + D x_t, times SiLU(z_t) with gate."""
+    y [tokens, nheads, headdim] = S_t C_t + D x_t, times SiLU(z_t) with gate;
+    zeros in rows of no prompt."""
     if stream is None:
         r = fast().prompt(zxbcdt, conv_state, weight, bias, ssm_state, A, D, dt_bias, d_inner, ngroups, d_state, nheads,
                           cu_seqlens, gate)

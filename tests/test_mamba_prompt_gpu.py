@@ -269,3 +269,21 @@ def test_refusals(MP):
         MP.mamba2_prompt(**make([10], W=9))
     with pytest.raises(SonataError):  # states longer than 256
         MP.mamba2_prompt(**make([10], ds=264))
+
+
+@pytest.mark.parametrize("hd,extra", [(64, 4), (64, 0), (32, 0)])  # by chunks (rows of 776 elements); token by token
+def test_rows_of_no_prompt_are_zero(MP, hd, extra):
+    """Tokens before the first and past the last prompt (a padded buffer): zeros, whatever the output's memory held; the
+    prompts are as they are without them."""
+    for front, back in ((3, 0), (0, 200), (5, 1)):
+        a, b = (make([70, 130], hd=hd, extra=extra, seed=17) for _ in range(2))
+        a["zxbcdt"] = torch.cat([a["zxbcdt"][:front], a["zxbcdt"], a["zxbcdt"][:back]])
+        a["cu_seqlens"] += front
+        poison = torch.full((front + 200 + back, 4, hd), float("nan"), device="cuda", dtype=torch.bfloat16)
+        del poison  # the output gets this block
+        ya, yb = MP.mamba2_prompt(**a), MP.mamba2_prompt(**b)
+        torch.cuda.synchronize()
+        assert torch.equal(ya[front:front + 200], yb)
+        assert not ya[:front].any() and not ya[front + 200:].any()
+        for s in ("conv_state", "ssm_state"):
+            assert torch.equal(a[s], b[s])
