@@ -198,8 +198,14 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
   const int b = static_cast<int>(row / (static_cast<int64_t>(p.nh) * p.hd));
   const int hp = static_cast<int>(row - static_cast<int64_t>(b) * p.nh * p.hd);
   const int h = hp / p.hd, g = h / p.hpg;
-  const int s0 = p.prompts.cu ? p.prompts.cu[b] : 0, e0 = p.prompts.cu ? p.prompts.cu[b + 1] : p.prompts.tokens;
-  const int start = min(max(s0, 0), p.prompts.tokens);
+  // tokens [start, end), as prompt_bounds has them: no offset below one before it
+  int start = 0;
+  const int e0 = p.prompts.cu ? p.prompts.cu[b + 1] : p.prompts.tokens;
+  if (p.prompts.cu)
+    for (int i = l16; i <= b; i += 16) start = max(start, p.prompts.cu[i]);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) start = max(start, __shfl_xor_sync(0xffffffffu, start, o));
+  start = min(start, p.prompts.tokens);
   const int end = min(max(e0, start), p.prompts.tokens);
   const int conv_dim = p.di + 2 * p.gds;
   __nv_bfloat16* st = p.ssm_state + row * p.ds;

@@ -287,3 +287,15 @@ def test_rows_of_no_prompt_are_zero(MP, hd, extra):
         assert not ya[:front].any() and not ya[front + 200:].any()
         for s in ("conv_state", "ssm_state"):
             assert torch.equal(a[s], b[s])
+
+
+@pytest.mark.parametrize("hd,extra", [(64, 4), (64, 0), (32, 0)])
+def test_falling_offsets_do_not_overlap(MP, cuda_lib, hd, extra):
+    """An offset below the one before it counts as that one, and is recorded: no token has two prompts."""
+    a, b = (make([100, 0, 20], hd=hd, extra=extra, seed=18) for _ in range(2))
+    a["cu_seqlens"][2] = 50
+    ya, yb = MP.mamba2_prompt(**a), MP.mamba2_prompt(**b)
+    assert cuda_lib.sn_device_status(1, None) == -1
+    assert torch.equal(ya, yb)
+    for s in ("conv_state", "ssm_state"):
+        assert torch.equal(a[s], b[s])
