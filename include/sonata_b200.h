@@ -526,6 +526,13 @@ int sn_swiglu(const void *h, void *y, int batch, int d, void *stream);
  * prompt's outputs, up to 127 tokens back, and no other prompt's.  d_conv <= 8,
  * d_state <= 256.  workspace: sn_mamba2_prompt_workspace_size bytes, free to
  * reuse when the call's work on the stream is done.
+ * Sums and states are fp32.  With headdim 64, d_state 128, d_conv 2 to 4, rows
+ * of whole 16 bytes and 16-byte aligned tensors the products take fp16 operands
+ * (2^-11 each, below the outputs' 2^-8), scaled by powers of two in chunks of
+ * 128 tokens.  They keep that for values of x down to 2^-27 of their head's
+ * largest in the chunk, of B and C down to 2^-27 of their group's, and for terms
+ * whose B and dt together are down to 2^-16 of the largest there (their C 2^-15
+ * besides); what is smaller has an absolute error of that size.
  */
 size_t sn_mamba2_prompt_workspace_size(int tokens, int batch, int d_inner, int ngroups, int d_state, int nheads);
 int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const void *conv_weight,

@@ -273,14 +273,24 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 //
 // Numbers.  The products are kind::f16 with fp32 accumulators.  Operands in
 // fp16 (11 significant bits) instead of bf16 (8) keep their roundings below
-// that of the bf16 results; their range is kept by exact powers of two: every
-// 128-channel block of a chunk (x of two heads, B, C) is scaled to below 2,
-// dt to below 2 by its largest value, and the state operand by a bound of the
-// state carried along with it.  States and sums stay in fp32.  Causality is a
-// zero in M, so an infinity or NaN of a token reaches the earlier tokens of
-// its own chunk too (and, through the state, all later ones); other prompts
-// never share a chunk with it.  A is taken to be negative (it is -exp(A_log)),
-// so that no decay exceeds 1.
+// that of the bf16 results.  fp16 has all of its bits from 2^-14 to 2^16 only, so
+// exact powers of two put the largest value of what shares one near the top:
+//   x      a head's 128 tokens of a chunk, to below 2^14 (its weights in the
+//          state are below 2): all bits to 2^-27 of the largest
+//   B, C   a group's 128 tokens by 128 states, likewise; then a token's row of
+//          C again, by up to 2^15, where its largest is below 1/8 of that
+//   M      (C B^T)_ij < 2^35, dt_j below 2 by the chunk's largest, 2^-21: below
+//          2^15, and about 2^5 where all are of one size.  B and dt of a score
+//          may be 2^-16 together of their largest, and C 2^-15 besides, before
+//          it loses bits
+//   S      by a bound carried along with it, to below 2^14
+// Nothing overflows; what lies further below is rounded to 2^-25 in those units
+// (the states' and rows' powers of two cost 0.4 us of 34 and 3 of 258 below).
+// States and sums stay in fp32.  Causality is a zero in M, so an
+// infinity or NaN of a token reaches the earlier tokens of its own chunk too
+// (and, through the state, all later ones); other prompts never share a chunk
+// with it.  A is taken to be negative (it is -exp(A_log)), so that no decay
+// exceeds 1.
 //
 // Layout.  The convolution writes its results as the shared-memory images the
 // products read (128-byte swizzle, 128 tokens by 64 channels, 16 KB), padded
@@ -294,16 +304,19 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 128;
 constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 64 channels of fp16
+constexpr int kRowTileBytes = 2 * kTileBytes + kChunk;  // two of them and a byte for each token
+constexpr int kTop = 14;                    // x, B and C as operands are below 2^14
+constexpr float kMScale = 1.f / (1 << 21);  // of M: 128 2^14 2^14 2 to 2^15
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ChunkWork {  // workspace arrays; chunks are counted over all prompts
   unsigned char* x;  // [chunks][nh] tiles
   unsigned char* b;  // [chunks][ng] pairs of tiles (128 states)
-  unsigned char* c;  // [chunks][ng] pairs of tiles
+  unsigned char* c;  // [chunks][ng] pairs of tiles, then the power of two of each token's row, as the exponent of a float
   float* cum;        // [chunks][nh][128] cumulative dt A / ln 2
   float* dt;         // [chunks][nh][128], 0 past the prompt's end
   float2* meta;      // [chunks][nh] largest dt; sum of dt exp(a_L - a_j)
-  float* scale;      // [chunks][blocks] power of two of each 128-channel block
+  float* scale;      // [chunks][nh + 2 ng] power of two of each head's x, each group's B and C: value / operand
   float* state;      // [slots][nh][64][128] see prompt_scan_mma_kernel
   float* total;      // [slots][nh] sum of dt A / ln 2 over a segment
   int xblocks, blocks;  // 128-channel blocks of x; of x, B and C together
@@ -453,7 +466,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
 template <int W, bool kMany>
 __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ __align__(16) unsigned char s_rows[(kChunk + W - 1) * 256];  // tokens t0 - W + 1 ..
-  __shared__ float s_max[8];
+  __shared__ float s_max[8], s_row[2][kChunk];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int blk = blockIdx.x;
   pdl_launch_dependents();
@@ -491,7 +504,7 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(co
   }
   constexpr int kNext = kMany ? 8 : 32;                             // from a thread's 8 tokens to its next
   const int half = warp & 1, r0 = (warp >> 1) * (kMany ? 32 : 8);  // tile and first tokens of the warp
-  const bool on = half * 64 < wide;
+  const bool on = half * 64 < wide, of_x = blk < wk.xblocks, of_c = blk >= wk.xblocks + p.ng;
   float2 w[W], bias = make_float2(0.f, 0.f);
   if (on) {
     const int d = d0 + half * 64 + 2 * lane;
@@ -507,7 +520,7 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(co
   __syncthreads();
 
   float top = 0.f;
-  uint32_t out[4][8];  // [8 tokens][token], fp16 over the 8 tokens' own power of two
+  uint32_t out[4][8];  // [8 tokens][token], fp16 over the 8 tokens' own power of two, below 2^13
   float own[4];
   if (on) {
     const unsigned char* in = s_rows + r0 * 256 + half * 128 + lane * 4;
@@ -539,12 +552,21 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(co
         for (int r = 0; r < 8; ++r)
           if (r0 + kNext * g + r >= left) o[r] = make_float2(0.f, 0.f);
       }
+      if (of_c) {  // the largest of each token, over the warp's states
+        unsigned mine = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(o[r].x), fabsf(o[r].y))));
+          mine = lane == r ? m : mine;
+        }
+        if (lane < 8) s_row[half][r0 + kNext * g + lane] = __uint_as_float(mine);
+      }
       float most = 0.f;
 #pragma unroll
       for (int r = 0; r < 8; ++r) most = fmaxf(most, fmaxf(fabsf(o[r].x), fabsf(o[r].y)));
       top = fmaxf(top, most);
       own[g] = most == 0.f ? 0.f : pow2_floor(most);
-      const float2 inv = splat(most == 0.f ? 1.f : rcp_pow2(own[g]));
+      const float2 inv = splat(most == 0.f ? 1.f : 4096.f * rcp_pow2(own[g]));
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const float2 v = mul2(o[r], inv);
@@ -556,27 +578,62 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(co
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s_max[warp] = top;
   __syncthreads();
+  // the largest of this head of x, or of the block of B or C
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = fmaxf(top, s_max[k]);
+  for (int k = 0; k < 8; ++k)
+    if (!of_x || (k & 1) == half) top = fmaxf(top, s_max[k]);
   const float sc = pow2_floor(top);
-  if (tid == 0) wk.scale[chunk * wk.blocks + blk] = sc;
+  // Rows of C far below the block's largest get a power of two of their own (`row`, of the token of this lane among the
+  // warp's 32); the block's is then stored negative.  Not the others, so that chunks of even tokens, the usual ones, cost
+  // the scan nothing (all rows: 262 for 258 us).
+  auto quiet = [&](int t) {
+    const float m = fmaxf(s_row[0][t], s_row[1][t]) * rcp_pow2(sc);
+    return t < left && m > 0.f && m < 1.f / 8 ? pow2_floor(m, 15) : 1.f;
+  };
+  float row = 1.f;
+  bool any = false;
+  if (of_c) {
+    const int t = r0 + kNext * (lane >> 3) + (lane & 7);
+    row = quiet(t);
+    if (half == 0) wk.c[(chunk * p.ng + blk - wk.xblocks - p.ng) * kRowTileBytes + 2 * kTileBytes + t] = __float_as_uint(row) >> 23;
+    if (warp == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) any |= quiet(lane + 32 * k) < 1.f;
+      any = __any_sync(0xffffffffu, any);
+    }
+  }
+  if (lane == 0 && on && warp < (of_x ? 2 : 1))
+    wk.scale[chunk * (p.nh + 2 * p.ng) + (of_x ? blk * 2 + half : p.nh + blk - wk.xblocks)] =
+        sc * (any ? -1.f / (1 << (kTop - 1)) : 1.f / (1 << (kTop - 1)));
   if (on) {
     unsigned char* tile;
-    if (blk < wk.xblocks) {
+    if (of_x) {
       tile = wk.x + (chunk * p.nh + blk * 2 + half) * kTileBytes;
     } else {
       const int g = blk - wk.xblocks;
-      tile = (g < p.ng ? wk.b + (chunk * p.ng + g) * 2 * kTileBytes : wk.c + (chunk * p.ng + g - p.ng) * 2 * kTileBytes) +
-             half * kTileBytes;
+      tile = of_c ? wk.c + (chunk * p.ng + g - p.ng) * kRowTileBytes : wk.b + (chunk * p.ng + g) * 2 * kTileBytes;
+      tile += half * kTileBytes;
     }
     tile += r0 * 128 + (lane & 3) * 4;
+    const float up = rcp_pow2(sc) * ((1 << (kTop - 1)) / 4096.f);
+    const bool rows = __any_sync(0xffffffffu, row < 1.f);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      // to the block's power of two: exact but for what falls below 2^-24 of it
-      const __half2 f = __float2half2_rn(own[g] * rcp_pow2(sc));
+      // to the block's power of two: exact where the result has all of its bits
+      float to = own[g] * up;
+      if (to < 1.f / (1 << 14)) {  // of fp16's own range below 2^-24: in two steps
+        to *= 1 << 12;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[g][r]), __float2half2_rn(1.f / (1 << 12)));
+          out[g][r] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      const __half2 f = __float2half2_rn(to);
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[g][r]), f);
+        __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&out[g][r]), f);
+        if (rows) v = __hmul2(v, __float2half2_rn(rcp_pow2(__shfl_sync(0xffffffffu, row, 8 * g + r))));
         *reinterpret_cast<uint32_t*>(tile + (kNext * g + r) * 128 + (((lane >> 2) ^ r) << 4)) =
             *reinterpret_cast<const uint32_t*>(&v);
       }
@@ -656,6 +713,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
   return r;
 }
+// The power of two whose exponent is the byte at a.
+__device__ __forceinline__ float lds_pow2(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+  return __uint_as_float(r << 23);
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -730,7 +793,7 @@ __device__ __forceinline__ ScanWork scan_work(const PromptParams& p, const Chunk
 }
 __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
   const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u;
-  if (pad > 512) {  // does not happen: dynamic shared memory starts on a 1024-byte boundary
+  if (pad > 384) {  // does not happen: dynamic shared memory starts on a 1024-byte boundary
     record_status(SN_ERR_MISALIGNED);
     return nullptr;
   }
@@ -752,7 +815,7 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* raw) {
 constexpr int kStateStages = 3;
 constexpr uint32_t kStateStage = 4 * kTileBytes;  // B, then x of two heads
 constexpr uint32_t kStateBytes = kStateStages * kStateStage;
-constexpr uint32_t kStateSmem = kStateBytes + 128 /* barriers */ + 512;
+constexpr uint32_t kStateSmem = kStateBytes + 128 /* barriers */ + 384;
 
 __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(const PromptParams p, const ChunkWork wk) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -800,7 +863,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
       if (k < w.chunks) {
         const int64_t chunk = last - k, th = chunk * p.nh + h;
         a = wk.cum[th * kChunk + kChunk - 1];
-        u = wk.scale[chunk * wk.blocks + h / 2] * wk.scale[chunk * wk.blocks + wk.xblocks + w.g] * pow2_floor(wk.meta[th].x);
+        const float* sc = wk.scale + chunk * (p.nh + 2 * p.ng);
+        u = sc[h] * sc[p.nh + w.g] * pow2_floor(wk.meta[th].x);
       }
       float upto = a;
 #pragma unroll
@@ -814,7 +878,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) {
-      s_unit[warp] = pow2_floor(top, 100);
+      s_unit[warp] = 2.f * pow2_floor(top, 100);  // every token's weight is below 2
       s_total[warp] = after;
     }
   }
@@ -872,8 +936,9 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
       a_i = wk.cum[th * kChunk + i];
       a_end = wk.cum[th * kChunk + kChunk - 1];
       dt = wk.dt[th * kChunk + i];
-      sx = wk.scale[chunk * wk.blocks + h / 2];
-      sB = wk.scale[chunk * wk.blocks + wk.xblocks + w.g];
+      const float* sc = wk.scale + chunk * (p.nh + 2 * p.ng);
+      sx = sc[h];
+      sB = sc[p.nh + w.g];
     };
     fetch(0);
     const float runit = rcp_pow2(s_unit[h - w.h0]);
@@ -935,14 +1000,22 @@ __global__ void __launch_bounds__(kScanThreads + 32, 1) prompt_states_kernel(con
   if (warp == 16) tc::tmem_dealloc(tmem, 128);
 }
 
-// Shared memory (from a 1024-byte boundary): two stages of B, C (32 KB each)
-// and X of two heads, the heads' state / weighted-x operands, then per head
-// the factors of the tokens.
-constexpr uint32_t kStageBytes = 6 * kTileBytes;
-constexpr uint32_t kOperandAt = 2 * kStageBytes;
-constexpr uint32_t kFactorsAt = kOperandAt + 2 * kTileBytes;
-constexpr uint32_t kScanBytes = kFactorsAt + 2 * 2 * kChunk * 4 + 256;  // and their block ends, the chunks' factors
-constexpr uint32_t kScanSmem = kScanBytes + 128 /* barriers */ + 512;
+// Shared memory (from a 1024-byte boundary): the heads' state / weighted-x
+// operands, then twice a stage of B, X of two heads, C and the exponents of C's
+// rows, with the tokens' factors and the rest behind them where the next stage's
+// boundary leaves room.
+constexpr uint32_t kOperandAt = 0;
+constexpr uint32_t kStageAt = 2 * kTileBytes;
+constexpr uint32_t kStageX = 2 * kTileBytes, kStageC = 4 * kTileBytes, kStageRows = 6 * kTileBytes;
+constexpr uint32_t kStageBytes = kStageRows + 2048;
+constexpr uint32_t kAfter0 = kStageAt + kStageRows + kChunk, kAfter1 = kAfter0 + kStageBytes;
+// factors of the tokens: [512 bytes] of head 0 (two), head 1, and the last of head 1 behind the second stage
+constexpr uint32_t kFactorsAt = kAfter0, kFactorsLast = kAfter1;
+constexpr uint32_t kEndsAt = kFactorsAt + 3 * 4 * kChunk;  // block ends of the heads, then the chunks' common factors
+constexpr uint32_t kBarsAt = kEndsAt + 256;
+static_assert(kBarsAt + 128 == kStageAt + kStageBytes);
+constexpr uint32_t kScanSmem = kFactorsLast + 4 * kChunk + 384;
+static_assert(kScanSmem <= 227 * 1024);
 // Tensor memory columns: S of two heads, C B^T, M of two heads, Y of two heads.
 constexpr int kServe = 4;  // the serving warp of a head's eight
 constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
@@ -968,7 +1041,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
   unsigned char* smem = aligned_smem(smem_raw);
   if (!smem) return;
   const uint32_t sbase = smem_u32(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScanBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarsAt);
   uint64_t *full = bars, *empty = bars + 2, *bar_g = bars + 4, *gfree = bars + 5, *bar_y2 = bars + 6, *bar_y = bars + 8,
            *bar_s = bars + 10;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 12);
@@ -980,12 +1053,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
   const int g = w.g, h0 = w.h0, heads = w.heads, c0 = w.c0, nchunks = w.chunks;
   // the copies of a chunk's operands into its stage (one thread)
   auto load = [&](int c) {
-    const uint32_t st = sbase + (c & 1) * kStageBytes;
+    const uint32_t st = sbase + kStageAt + (c & 1) * kStageBytes;
     const int64_t chunk = sg.chunk0 + c0 + c;
-    mbar_arrive_expect_tx(full + (c & 1), (4 + heads) * kTileBytes);
+    mbar_arrive_expect_tx(full + (c & 1), 2 * kTileBytes + heads * kTileBytes + kRowTileBytes);
     bulk_load(st, wk.b + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-    bulk_load(st + 2 * kTileBytes, wk.c + (chunk * p.ng + g) * 2 * kTileBytes, 2 * kTileBytes, full + (c & 1));
-    bulk_load(st + 4 * kTileBytes, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
+    bulk_load(st + kStageC, wk.c + (chunk * p.ng + g) * kRowTileBytes, kRowTileBytes, full + (c & 1));
+    bulk_load(st + kStageX, wk.x + (chunk * p.nh + h0) * kTileBytes, heads * kTileBytes, full + (c & 1));
   };
   int loaded = min(2, nchunks);  // chunks whose copies have been issued
   if (tid == kServe * 32) {
@@ -1018,12 +1091,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
   } head;
   auto fetch_head = [&](int c) {
     const int64_t th = static_cast<int64_t>(chunk0 + c) * p.nh + h;
-    const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * wk.blocks;
+    const float* sc = wk.scale + static_cast<int64_t>(chunk0 + c) * (p.nh + 2 * p.ng);
     head.a_end = wk.cum[th * kChunk + kChunk - 1];
     head.meta = wk.meta[th];
-    head.sx = sc[h / 2];
-    head.sB = sc[wk.xblocks + g];
-    head.sC = sc[wk.xblocks + p.ng + g];
+    head.sx = sc[h];
+    head.sB = sc[p.nh + g];
+    head.sC = sc[p.nh + p.ng + g];
   };
   // The first chunk's inputs and the state before the segment (row n = i of S^T, this half's 32 columns, true values):
   // all of them on their way before anything waits
@@ -1067,13 +1140,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
                    tM = tmem + kColM + wg * 64 + lanes, tY = tmem + kColY + wg * 64 + 32 * half + lanes;
     const uint32_t opnd = sbase + kOperandAt + wg * kTileBytes;
     float* fj = reinterpret_cast<float*>(smem + kFactorsAt) + wg * 2 * kChunk;  // of token j within its block, see below
-    float* ej = fj + kChunk;                                                     // exp2(a_last(block) - a_j) dt_j
-    float* cend = reinterpret_cast<float*>(smem + kFactorsAt + 2 * 2 * kChunk * 4) + wg * 16;  // [4]; first [8] maxima
+    float* ej = wg == 0 ? fj + kChunk : reinterpret_cast<float*>(smem + kFactorsLast);  // exp2(a_last(block) - a_j) dt_j
+    float* cend = reinterpret_cast<float*>(smem + kEndsAt) + wg * 16;                   // [4]; first [8] maxima
     const uint32_t row = i * 128, sw = i & 7;
     const int bar_id = 1 + wg;
     // the chunk's common factors, two buffers: 1 / sdt, a_end, S to its operand, S to the new unit and decayed;
     // C S from its operand's unit to that of M X, M X to outputs, x' to D x
-    float4* common = reinterpret_cast<float4*>(smem + kFactorsAt + 2 * 2 * kChunk * 4 + 128) + wg * 4;
+    float4* common = reinterpret_cast<float4*>(smem + kEndsAt + 128) + wg * 4;
 
     float unit = 1.f, bound = 0.f;  // S = unit * tensor memory; |S| <= bound
     {
@@ -1096,13 +1169,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       const float sb = pow2_floor(bound, 100), sS = sb * (1.f / 8192.f);  // |S / sS| < 2^14
       if (lane == 0) {
         common[2 * (c & 1)] = make_float4(rdt, head.a_end, unit * (rcp_pow2(sb) * 8192.f), dec * (unit * runit));
-        common[2 * (c & 1) + 1] = make_float4(sS * runit, head.sC * unit_new, D * head.sx, unit_new);
+        common[2 * (c & 1) + 1] = make_float4(sS * runit * kMScale, head.sC * (1.f / kMScale) * unit_new, D * head.sx, unit_new);
       }
       unit = unit_new;
-      bound = fmaf(dec, bound, unit_new * 4.f * (head.meta.y * rdt));
+      constexpr float most = static_cast<float>(1 << (2 * kTop));  // of a product of x and B
+      bound = fmaf(dec, bound, unit_new * most * (head.meta.y * rdt));
     };
     struct Factors {
-      float a_i, dtn;     // cumulative decay; dt / sdt
+      float a_i, dtn;     // cumulative decay; dt / sdt as it goes into M
       float wj;           // the token's weight in the state
       float f_op, f_dec;  // as common
       float f_y;          // exp(a_i) C S, likewise
@@ -1112,8 +1186,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     auto take = [&](int c) {
       const float4 u = common[2 * (c & 1)], w = common[2 * (c & 1) + 1];
       f.a_i = next_a;
-      f.dtn = next_dt * u.x;
-      f.wj = f.dtn * exp2_approx(u.y - next_a);
+      const float dtn = next_dt * u.x;
+      f.dtn = dtn * kMScale;
+      f.wj = dtn * exp2_approx(u.y - next_a);
       f.f_op = u.z;
       f.f_dec = u.w;
       f.f_y = exp2_approx(next_a) * w.x;
@@ -1128,7 +1203,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       if (lane == 0 && !dead) {
         tc::fence_after_sync();
         constexpr uint32_t id = idesc_f16(128, 128, false, false);
-        const uint64_t db = tc::smem_desc_sw128(smem + (c & 1) * kStageBytes), dc = db + 2 * kTileBytes / 16;
+        const uint64_t db = tc::smem_desc_sw128(smem + kStageAt + (c & 1) * kStageBytes), dc = db + kStageC / 16;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t at = ((k >> 2) * kTileBytes + (k & 3) * 32) / 16;
@@ -1150,8 +1225,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
     const uint64_t d_op = desc_k_rows(opnd, 16);
     for (int c = 0; c < nchunks; ++c) {
       const unsigned stage = c & 1, ph = (c >> 1) & 1;
-      const uint32_t sst = sbase + stage * kStageBytes;
-      const uint32_t xrow = sst + (4 + wg) * kTileBytes + row;
+      const uint32_t sst = sbase + kStageAt + stage * kStageBytes;
+      const uint32_t xrow = sst + kStageX + wg * kTileBytes + row;
       if (c > 0) {  // the last chunk's products are done: its stage, the operand buffer and S are free
         wait(bar_s + wg, (c - 1) & 1);
         tc::fence_after_sync();
@@ -1214,7 +1289,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
         if (lane == 0 && !dead) {  // Y = C S
           tc::fence_after_sync();
           constexpr uint32_t id = idesc_f16(128, 64, false, true);
-          const uint64_t dc = tc::smem_desc_sw128(smem + stage * kStageBytes + 2 * kTileBytes);
+          const uint64_t dc = tc::smem_desc_sw128(smem + kStageAt + stage * kStageBytes + kStageC);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             tc::mma_bf16(tmem + kColY + wg * 64, dc + ((k >> 2) * kTileBytes + (k & 3) * 32) / 16, d_op + k * 128, id, k > 0);
@@ -1315,7 +1390,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
           tc::fence_after_sync();
           {  // Y += M X
             constexpr uint32_t id = idesc_f16(128, 64, false, true);
-            const uint64_t dx = desc_k_rows(sst + (4 + wg) * kTileBytes, 16);
+            const uint64_t dx = desc_k_rows(sst + kStageX + wg * kTileBytes, 16);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
               mma_f16_ts(tmem + kColY + wg * 64, tmem + kColM + wg * 64 + 8 * k, dx + k * 128, id, 1);
@@ -1332,10 +1407,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) prompt_scan_mma_kernel(const 
       }
       // Outputs (and gates) go between a thread's row and whole 64-byte pieces of rows through the warp's part of the
       // chunk's X tile, which nothing reads once M X is done: lane l has 16 bytes l % 4 of rows l / 4, + 8, ...
-      const float2 fy = splat(f.fy), dx = splat(f.dx);
+      float fy_row = f.fy;
+      if (f.fy < 0.f) fy_row *= -lds_pow2(sst + kStageRows + i);  // the chunk has rows of C with powers of two of their own
+      const float2 fy = splat(fy_row), dx = splat(f.dx);
       const int tw = (c0 + c) * kChunk + q * 32 + (lane >> 2);  // the token of this lane's first piece
       const int64_t tok = sg.start + tw;
-      const uint32_t stg = sst + (4 + wg) * kTileBytes + (q * 32 + (lane >> 2)) * 128;
+      const uint32_t stg = sst + kStageX + wg * kTileBytes + (q * 32 + (lane >> 2)) * 128;
       // 16-byte pieces are swizzled by the row's low bits reversed: eight lanes with a piece of eight rows, or with four
       // pieces of two rows, then hit eight places
       const int piece = 4 * half + (lane & 3), psw = __brev(lane >> 2) >> 29, osw = __brev(i & 7) >> 29;
@@ -1455,11 +1532,11 @@ inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, i
   const size_t nch = static_cast<size_t>(r.chunks);
   r.x = take(nch * nh * kTileBytes);
   r.b = take(nch * ng * 2 * kTileBytes);
-  r.c = take(nch * ng * 2 * kTileBytes);
+  r.c = take(nch * ng * kRowTileBytes);
   r.cum = take(nch * nh * kChunk * 4);
   r.dt = take(nch * nh * kChunk * 4);
   r.meta = take(nch * nh * 8);
-  r.scale = take(nch * r.blocks * 4);
+  r.scale = take(nch * (nh + 2 * ng) * 4);
   r.state = take(static_cast<size_t>(r.slots) * nh * 64 * 128 * 4);
   r.total = take(static_cast<size_t>(r.slots) * nh * 4);
   r.bytes = at;

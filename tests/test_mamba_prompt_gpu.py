@@ -299,3 +299,167 @@ def test_falling_offsets_do_not_overlap(MP, cuda_lib, hd, extra):
     assert torch.equal(ya, yb)
     for s in ("conv_state", "ssm_state"):
         assert torch.equal(a[s], b[s])
+
+
+# ---- the form by chunks, on the tensor cores: heads of 64, 128 states, widths 2 to 4, rows of whole 16 bytes ----
+#
+# Its products' operands are rounded to fp16 (2^-11 each): x, B and C, and the masked score, or the weighted x and the state
+# operand: at most five in a term of y, three in one of the state.  Exponents: |sum dt A| < 400 in a chunk here, 577 as
+# powers of two, with about nine fp32 roundings of the sum (577 * 9 * 2^-24 ln 2 = 2e-4) and dt good to 5e-7 (2e-4): 5e-4.
+# Norm: the output's rounding (1.62e-3) and five of 2.0e-4, 1.7e-3 together, held to 2.2e-3.
+F = 2.0 ** -11
+
+
+def tile(lens, nh=4, ng=1, W=4, **k):
+    """make() with rows padded to whole 16 bytes."""
+    wide = 2 * nh * 64 + 2 * ng * 128 + nh
+    a = make(lens, nh=nh, ng=ng, W=W, extra=-wide % 8, **k)
+    assert a["zxbcdt"].stride(0) % 8 == 0
+    return a
+
+
+def check_tile(MP, a, gate=False, norm=2.2e-3, **k):
+    y0, ya, conv, ssm, sabs = truth(a, gate)
+    y = MP.mamba2_prompt(gate=gate, **a, **k)
+    torch.cuda.synchronize()
+    check(y, y0, (5 * F + 5e-4) * ya + E * y0.abs() + 1e-30, "y", norm)
+    check(a["ssm_state"], ssm, (3 * F + 5e-4) * sabs + E * ssm.abs() + 1e-30, "ssm_state", norm)
+    assert torch.equal(a["conv_state"].double(), conv)
+    return y
+
+
+@pytest.mark.parametrize("lens", [[1], [2], [3], [5], [7], [8], [31], [32], [33], [64], [127], [128], [129], [130], [256], [300],
+                                  [1000], [0, 5, 0, 130, 3, 0], [1, 1, 1, 1], [128, 128], [129, 255, 7], [1] * 70])
+@pytest.mark.parametrize("gate", [False, True])
+def test_tile_lengths(MP, lens, gate):
+    check_tile(MP, tile(lens, seed=sum(lens)), gate)
+
+
+@pytest.mark.parametrize("nh,ng,W", [(64, 1, 4), (6, 2, 4), (3, 1, 3), (8, 8, 2), (1, 1, 4), (5, 5, 4), (10, 2, 2), (48, 1, 3)])
+def test_tile_heads_and_groups(MP, nh, ng, W):
+    check_tile(MP, tile([70, 140, 9], nh=nh, ng=ng, W=W, seed=nh), gate=nh % 2 == 0)
+
+
+@pytest.mark.parametrize("off", ["bias", "D", "dt_bias", "cu_seqlens"])
+def test_tile_without_optional(MP, off):
+    a = tile([150, 31] if off != "cu_seqlens" else [333], seed=3)
+    a[off] = None
+    if off == "dt_bias":  # keep dt in its usual range
+        a["zxbcdt"][:, 2 * 256 + 256:] -= 3
+    check_tile(MP, a)
+
+
+@pytest.mark.parametrize("nh,ng,lens", [
+    (2, 1, [4000]), (2, 1, [9000]),      # many segments
+    (6, 2, [3000]), (3, 1, [1500, 900, 77]),  # three heads a group: a head alone in its pair, several prompts cut
+    (64, 1, [2048, 1, 2100, 129, 40]),   # two prompts cut once among short ones
+    (4, 1, [700] * 9), (1, 1, [5, 2000, 0, 2001, 128, 384])])
+def test_tile_segments(MP, nh, ng, lens):
+    check_tile(MP, tile(lens, nh=nh, ng=ng, seed=len(lens) + nh))
+
+
+def test_tile_strong_decay(MP):
+    """As test_strong_decay."""
+    a = tile([300, 40], seed=9, dt_shift=24.0)
+    y0, ya, conv, ssm, sabs = truth(a)
+    y = MP.mamba2_prompt(**a)
+    torch.cuda.synchronize()
+    assert torch.isfinite(y).all()
+    check(y, y0, (5 * F + 1e-2) * ya + E * y0.abs() + 1e-30, "y")
+
+
+def test_tile_pieces_equal_the_whole(MP):
+    a = tile([500], nh=8, seed=10, fresh=True)
+    y0, ya, conv, ssm, sabs = truth(a)
+    got = []
+    for s, e in ((0, 130), (130, 131), (131, 500)):
+        got.append(MP.mamba2_prompt(**dict(a, zxbcdt=a["zxbcdt"][s:e], cu_seqlens=None)))
+    torch.cuda.synchronize()
+    check(torch.cat(got), y0, (5 * F + 5e-4 + E) * ya + E * y0.abs(), "y")  # and the stored state, to bf16
+    assert torch.equal(a["conv_state"].double(), conv)
+
+
+def test_tile_prompts_do_not_touch_each_other(MP):
+    lens = [40, 200, 129, 1]
+    a, b = tile(lens, seed=12), tile(lens, seed=12)
+    b["zxbcdt"][40:240] = float("nan")
+    b["zxbcdt"][100] = float("inf")
+    ya, yb = MP.mamba2_prompt(**a), MP.mamba2_prompt(**b)
+    torch.cuda.synchronize()
+    keep = torch.ones(sum(lens), dtype=torch.bool, device="cuda")
+    keep[40:240] = False
+    assert torch.equal(ya[keep], yb[keep])
+    for s in ("conv_state", "ssm_state"):
+        assert torch.equal(a[s][[0, 2, 3]], b[s][[0, 2, 3]])
+    assert torch.isnan(yb[~keep]).any()
+
+
+def test_tile_in_a_graph_with_new_offsets(MP):
+    a = tile([100, 200], seed=14)
+    MP.mamba2_prompt(**a)  # first call outside capture
+    torch.cuda.synchronize()
+    st = [a["conv_state"].clone(), a["ssm_state"].clone()]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = MP.mamba2_prompt(**a)
+    a["cu_seqlens"].copy_(torch.tensor([0, 290, 300], dtype=torch.int32, device="cuda"))
+    a["conv_state"].copy_(st[0])
+    a["ssm_state"].copy_(st[1])
+    y0, ya, conv, ssm, sabs = truth(a)
+    g.replay()
+    torch.cuda.synchronize()
+    check(y, y0, (5 * F + 5e-4) * ya + E * y0.abs(), "y")
+    check(a["ssm_state"], ssm, (3 * F + 5e-4) * sabs + E * ssm.abs(), "ssm_state")
+
+
+# Values of unequal size: every element within the bound above, which is relative to the absolute values of its own terms.
+
+@pytest.mark.parametrize("down", [16, 22])
+@pytest.mark.parametrize("lens", [[300], [2100, 77]])  # the second with states of segments
+def test_tile_quiet_head(MP, down, lens):
+    """Every other head's x 2^-down of its neighbour's, and a quiet channel in each."""
+    a = tile(lens, nh=4, seed=30)
+    a["D"] = None
+    for h in (1, 3):
+        a["weight"][64 * h:64 * h + 64] *= 2.0 ** -down
+        a["bias"][64 * h:64 * h + 64] *= 2.0 ** -down
+    a["weight"][10:64 * 4:64] *= 2.0 ** -16
+    a["bias"][10:64 * 4:64] *= 2.0 ** -16
+    check_tile(MP, a)
+
+
+@pytest.mark.parametrize("down", [4, 8])
+def test_tile_quiet_then_loud(MP, down):
+    """The first tokens of a chunk with x, B, C and dt 2^-down of the later ones': their outputs are as good."""
+    a = tile([128, 333], nh=4, seed=31, fresh=True)
+    a["D"] = a["bias"] = None
+    di, cd = 256, 512
+    for at in (0, 128, 128 + 256):
+        a["zxbcdt"][at:at + 60, di:di + cd] *= 2.0 ** -down
+        a["zxbcdt"][at:at + 60, di + cd:di + cd + 4] -= down * 0.69
+    check_tile(MP, a)
+
+
+def test_tile_spread_over_tokens(MP):
+    """Runs of tokens whose rows are 2^0 to 2^-8 as large as others', and dt from 2^-16 to 2, in no order."""
+    a = tile([1000, 200], nh=4, seed=32)
+    a["D"] = a["bias"] = None
+    g = torch.Generator(device="cuda").manual_seed(33)
+    size = 2.0 ** -(8 * torch.rand(150, 1, device="cuda", generator=g)).repeat_interleave(8, 0)
+    di, cd = 256, 512
+    a["zxbcdt"][:, di:di + cd] *= size
+    a["zxbcdt"][:, di + cd:di + cd + 4] = torch.rand(1200, 4, device="cuda", generator=g) * 13 - 8
+    a["A"] /= 16  # dt reaches 2 here: sums of dt A as the bound has them
+    check_tile(MP, a)
+
+
+def test_tile_quiet_states(MP):
+    """B and C of every fourth state 2^-10 of the others, and an initial state of widely different elements."""
+    a = tile([260], nh=4, seed=34)
+    a["D"] = None
+    for at in (256, 384):
+        for t in ("weight", "bias"):
+            a[t][at:at + 128:4] *= 2.0 ** -10
+    g = torch.Generator(device="cuda").manual_seed(35)
+    a["ssm_state"] *= 2.0 ** -(8 * torch.rand(a["ssm_state"].shape, device="cuda", generator=g))
+    check_tile(MP, a)
