@@ -1503,7 +1503,7 @@ inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, i
   r.blocks = r.xblocks + 2 * ng;
   // Chunks a segment: the least time over the SMs' waves of both launches, from what was measured (tenths of a
   // microsecond): 43 a chunk of the outputs and 110 to start and end a CTA of them, 11 and 90 for the states.
-  const int sms = 148;
+  const int sms = sm_count();
   const int64_t nc = std::max<int64_t>(1, (tokens + kChunk - 1) / kChunk);
   const int64_t each = (nc + batch - 1) / batch;  // of a prompt, if they are alike
   int64_t best = INT64_MAX;
