@@ -1504,7 +1504,7 @@ inline bool plan_scan(int tokens, int batch, int d_inner, int ng, int d_state, i
   // Chunks a segment: the least time over the SMs' waves of both launches, from what was measured (tenths of a
   // microsecond): 43 a chunk of the outputs and 110 to start and end a CTA of them, 11 and 90 for the states.
   const int sms = sm_count();
-  const int64_t nc = std::max<int64_t>(1, (tokens + kChunk - 1) / kChunk);
+  const int64_t nc = std::max<int64_t>(1, (static_cast<int64_t>(tokens) + kChunk - 1) / kChunk);
   const int64_t each = (nc + batch - 1) / batch;  // of a prompt, if they are alike
   int64_t best = INT64_MAX;
   r.seg = static_cast<int>(each);
