@@ -6,8 +6,9 @@ Each .cu under csrc/ is compiled to an object in sonata_b200/_build/ (in
 parallel), then linked into sonata_b200/libsonata_b200.so with the CUDA
 runtime linked statically, so the library only needs the driver at run time.
 bind/fastcall.cpp, the short way from torch tensors to the C ABI, becomes
-sonata_b200/_fastcall.so against the torch of this interpreter (host code
-only; the wrappers work without it, with more host time a call).
+sonata_b200/_fastcall.*.so against the torch of this interpreter, which its
+name says (host code only; the wrappers work without it, with more host time
+a call, so a failure to build it is a warning).
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -26,7 +28,6 @@ BUILD = PKG / "_build"
 LIB = PKG / "libsonata_b200.so"
 INCLUDE = PKG.parent / "include"
 BIND_SRC = PKG / "bind" / "fastcall.cpp"
-BIND = PKG / "_fastcall.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -59,27 +60,42 @@ def _compile(src: Path) -> tuple[Path, str]:
     return obj, r.stderr
 
 
+def bind_path() -> Path:
+    """The short way's file for this interpreter and its torch: one built for others is never taken for it."""
+    import torch
+    return PKG / f"_fastcall.{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}.so"
+
+
 def build_bind(force: bool = False) -> Path:
-    if not force and BIND.exists() and BIND.stat().st_mtime >= max(
+    out = bind_path()
+    if not force and out.exists() and out.stat().st_mtime >= max(
             f.stat().st_mtime for f in (BIND_SRC, *INCLUDE.glob("*.h"))):
-        return BIND
+        return out
     import torch
     from torch.utils import cpp_extension as ext
     cuda = Path(nvcc()).resolve().parent.parent
     include = [a for d in (*ext.include_paths(), cuda / "include", sysconfig.get_path("include")) for a in ("-isystem", str(d))]
-    tmp = BIND.with_suffix(f".{os.getpid()}.tmp")
+    tmp = out.with_suffix(f".{os.getpid()}.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE), *include, str(BIND_SRC),
            "-o", str(tmp), *["-L" + d for d in ext.library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, BIND)
-    return BIND
+    os.replace(tmp, out)
+    return out
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
-    build_bind(force)
+    lib = _build_lib(force, jobs, verbose)
+    try:
+        build_bind(force)
+    except Exception as e:  # no compiler, no headers of torch or Python, ...
+        warnings.warn(f"the short way from torch tensors was not built, calls take more host time: {e}")
+    return lib
+
+
+def _build_lib(force: bool, jobs: int | None, verbose: bool) -> Path:
     if not force and LIB.exists() and LIB.stat().st_mtime >= _deps_mtime():
         return LIB
     BUILD.mkdir(exist_ok=True)

@@ -5,19 +5,19 @@ import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
+import warnings
 
 import torch
 
-from .. import _lib
+from .. import _lib, build
 
-_FAST_PATH = _lib.LIB_PATH.with_name("_fastcall.so")
 _FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_copy_pages",
                  "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size")
 
 
 class _NoFast:
-    """In the place of the short way's functions where it was not built: every
-    call is left to the wrapper."""
+    """In the place of the short way's functions where it was not built, or
+    does not load: every call is left to the wrapper."""
     attend = append = copy = prompt = staticmethod(lambda *args: None)
 
 
@@ -30,12 +30,18 @@ def fast():
     global _fast
     if _fast is None:
         lib = _lib.lib()
-        if not _FAST_PATH.exists():
+        path = build.bind_path()
+        if not path.exists():
             _fast = _NoFast
             return _fast
-        loader = importlib.machinery.ExtensionFileLoader("_fastcall", str(_FAST_PATH))
-        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fastcall", loader))
-        loader.exec_module(m)
+        loader = importlib.machinery.ExtensionFileLoader("_fastcall", str(path))
+        try:
+            m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fastcall", loader))
+            loader.exec_module(m)
+        except ImportError as e:
+            warnings.warn(f"{path.name} does not load, calls take more host time: {e}")
+            _fast = _NoFast
+            return _fast
         m.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _FAST_SYMBOLS})
         _fast = m
     return _fast
