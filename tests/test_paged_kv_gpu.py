@@ -518,3 +518,22 @@ def test_append_refused_tokens_have_zero_q(PK, cuda_lib, hd, rot, inter):
     rest = [t for t in range(14) if t not in kept]
     assert not q[rest].any()
     assert torch.equal(kp, want[1]) and torch.equal(vp, want[2])
+
+
+@pytest.mark.parametrize("lens,hq,hkv,hd", [([257], 16, 4, 128), ([1000, 0, 33], 16, 4, 64), ([700, 90], 32, 2, 128), ([500, 77], 24, 1, 64),
+                                            ([20011], 16, 1, 128), ([9000, 4097, 5], 16, 4, 128), ([300, 40], 8, 4, 96)])
+def test_attend_weights_keep_their_bits(PK, lens, hq, hkv, hd):
+    """The weights are not rounded to bf16 on the way into the product: two operands hold 16 bits of them.  |err| <= 2^-8 |o|
+    for the output, 2^-16 P for the weights and the scores' and joins' errors as above; the norm of the error that of the
+    output's rounding (1.62e-3 over evenly spread mantissas), held to 1.8e-3."""
+    g = torch.Generator(device="cuda").manual_seed(40 + hd)
+    tab, total = table(lens, 32, 40)
+    kp, vp = (torch.randn(total, hkv, 32, hd, device="cuda", generator=g).to(BF16) for _ in range(2))
+    q = (1.5 * torch.randn(len(lens), hq, hd, device="cuda", generator=g)).to(BF16)
+    o, loose, _ = attend_truth(q, kp, vp, tab, lens, 32, hd ** -0.5)
+    absv, _, _ = attend_truth(q, kp, vp.abs(), tab, lens, 32, hd ** -0.5)  # P
+    bound = loose - E * absv + 2.0 ** -16 * absv
+    got = PK.paged_decode_attention(q, kp, vp, tab, torch.tensor(lens, dtype=torch.int32, device="cuda")).double()
+    torch.cuda.synchronize()
+    assert ((got - o).abs() <= bound + 1e-30).all(), ((got - o).abs() - bound).max().item()
+    assert ((got - o).norm() / o.norm()).item() <= 1.8e-3
