@@ -567,7 +567,9 @@ int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const voi
  * query heads share a key/value head.  q [batch, nheads, head_dim] by batch
  * and head strides, out dense; lse fp32 [batch, nheads] (log of the sum of
  * exponentials, -inf for an empty stream) or NULL.  An empty stream gives
- * zeros.  head_dim <= 256.  workspace: sn_paged_decode_workspace_size bytes,
+ * zeros.  Scores, weights and sums are fp32; the products of head_dim 64 and
+ * 128 take 16 bits of the weights, in two bf16 operands, so an infinity in a v
+ * that counts may come out as a NaN.  head_dim <= 256.  workspace: sn_paged_decode_workspace_size bytes,
  * 16-byte aligned, its first 4 SN_PAGED_DECODE_COUNTERS bytes zero before the
  * first call and left ready for the next, whatever its sizes are; calls that
  * share it must not overlap.

@@ -285,12 +285,11 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 //          it loses bits
 //   S      by a bound carried along with it, to below 2^14
 // Nothing overflows; what lies further below is rounded to 2^-25 in those units
-// (the states' and rows' powers of two cost 0.4 us of 34 and 3 of 258 below).
-// States and sums stay in fp32.  Causality is a zero in M, so an
-// infinity or NaN of a token reaches the earlier tokens of its own chunk too
-// (and, through the state, all later ones); other prompts never share a chunk
-// with it.  A is taken to be negative (it is -exp(A_log)), so that no decay
-// exceeds 1.
+// (the rows' powers of two cost 5 us of 260 and 0.5 of 33 below).  States and
+// sums stay in fp32.  Causality is a zero in M, so an infinity or NaN of a token
+// reaches the earlier tokens of its own chunk too (and, through the state, all
+// later ones); other prompts never share a chunk with it.  A is taken to be
+// negative (it is -exp(A_log)), so that no decay exceeds 1.
 //
 // Layout.  The convolution writes its results as the shared-memory images the
 // products read (128-byte swizzle, 128 tokens by 64 channels, 16 KB), padded
@@ -298,8 +297,8 @@ __global__ void __launch_bounds__(256) prompt_scan_rows_kernel(const PromptParam
 // three bulk copies and no product sees another prompt's tokens.
 //
 // Measured, one prompt of 16384 tokens, 64 heads, one group (142.6 MB of rows
-// and 134.2 MB of outputs, 43 us at the copy bandwidth of 6.44 TB/s): 255 us,
-// of them 62 the convolution, 43 the states, 150 the outputs.  The tiles of x,
+// and 134.2 MB of outputs, 43 us at the copy bandwidth of 6.44 TB/s): 260 us,
+// of them 64 the convolution, 43 the states, 153 the outputs.  The tiles of x,
 // B and C (142 MB) are written by the first and read by the other two.
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 128;
@@ -459,10 +458,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
 // of tokens and four CTAs an SM (64 registers); else in every fourth 8 tokens,
 // so that few tokens are spread over the warps, and three.
 // Inputs read and tiles written once (252 MB of HBM traffic for 16384 tokens,
-// 39 us; the special functions of a SiLU 32 us): measured 62, issue slots 66%
+// 39 us; the special functions of a SiLU 32 us): measured 64, issue slots 72%
 // busy.  16-byte loads to registers, 8 channels of 8 tokens a thread, took 16%
 // fewer instructions but 128 registers, so 15 warps an SM where there are 30 (87
-// us).
+// us for 62).  What only C's rows need is in every block's code and takes 2 of
+// the 64; a copy of the code for C alone took more.
 template <int W, bool kMany>
 __global__ void __launch_bounds__(256, kMany ? 4 : 3) prompt_conv_tile_kernel(const PromptParams p, const ChunkWork wk) {
   __shared__ __align__(16) unsigned char s_rows[(kChunk + W - 1) * 256];  // tokens t0 - W + 1 ..
@@ -1029,7 +1029,7 @@ constexpr uint32_t kColS = 0, kColG = 128, kColM = 256, kColY = 384;
 // the one with the first 32 rows and the later columns has no part of M (it is
 // all above the diagonal), so it serves the others: it issues the products and
 // copies and works out the chunk's common factors.
-// Measured: 150 us for 128 segments of 32 chunks, 4.4 us (7700 cycles) a chunk
+// Measured: 153 us for 128 segments of 32 chunks, 4.5 us (7900 cycles) a chunk
 // of two heads.  It is bounded by the chain of a chunk (S to its operand, C S,
 // M, w x, M X, outputs: each waits for the one before), with issue slots 41% busy
 // and the tensor pipe 27%.  Longer: M X into columns of its own by way of C B^T's
@@ -1604,7 +1604,7 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
   const bool rows16 = sn::aligned16(zxbcdt) && ld % 8 == 0 && sn::aligned16(y) && sn::aligned16(conv_state) &&
                       sn::aligned16(conv_weight) && (!conv_bias || sn::aligned16(conv_bias));
   // 64-element heads, 128 states, 16-byte rows: the tensor-core form; anything else token by token (37 / 1021 / 16384
-  // tokens of 64 heads: 13 / 33 / 255 us, token by token 66 / 1266 / 27454)
+  // tokens of 64 heads: 14 / 33 / 260 us, token by token 66 / 1266 / 27454)
   if (d_conv >= 2 && d_conv <= 4 && rows16 &&
       sn::plan_scan(tokens, batch, d_inner, ngroups, d_state, nheads, &plan) && plan.chunks <= 65535 && plan.segments <= 65535) {
     unsigned char* base = reinterpret_cast<unsigned char*>(p.xbc);
@@ -1622,7 +1622,8 @@ int sn_mamba2_prompt(const void* zxbcdt, int64_t ld, void* conv_state, const voi
     wk.blocks = plan.blocks;
     wk.seg = plan.seg;
     const int conv_blocks = plan.blocks + (nheads + sn::kDtHeads - 1) / sn::kDtHeads;
-    // more CTAs than three an SM hold at once: four (16384 tokens 255 us in all, with three 264); else three and tokens
+    // more CTAs than three an SM hold at once: four (16384 tokens 255 us in all, with three 264, both
+    // before C's rows had powers of two); else three and tokens
     // spread over the warps (37 / 1021 tokens 13.4 / 33.0 us, with four 13.9 / 34.1)
     const bool many = plan.chunks * conv_blocks > 3 * sn::sm_count();
     auto pick = [&](auto wide, auto narrow) { return many ? wide : narrow; };

@@ -16,7 +16,7 @@
 namespace sn {
 namespace {
 
-// A page table's entry for position `pos` of stream b, or -1.
+// A page table: its entry for a block of page_size positions of stream b, or -1 where there is none.
 struct PageMap {
   const int* table;  // [batch, table_stride]
   int64_t table_stride;
@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
 //   rows of a tile; the 8 columns of heads here leave the tensor pipe idle
 //   either way).  Loads by every lane instead, into operand registers or by
 //   cp.async, took 500 instructions a tile for 280 here (3 streams of up to
-//   100001 positions: 102 and 118 us; now 84 us, 5.8 TB/s of 6.4).
+//   100001 positions: 102 and 118 us for 84; with the weights' second product
+//   86.6, 5.7 TB/s of 6.4).
 // * S^T = K q^T: the contraction index may be permuted as long as K and q
 //   agree, so lane (g = lane / 4, t = lane % 4) takes whole 16-byte chunks t,
 //   t + 4, ... of two positions, and the same chunks of q's head g.
@@ -374,9 +375,9 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
 //   warps take every sixth tile of its piece of a (stream, head) and join
 //   through shared memory; a (stream, head) cut over several CTAs is joined by
 //   the CTA that finishes last, in the order of the pieces, so the result does
-//   not depend on which one that is.  (12 warps in one CTA an SM: 84.5 and
-//   67.5 us for the long and the 64 ragged streams, 4 warps in three: 87.8 and
-//   64.3; six in two: 85.4 and 65.9.)
+//   not depend on which one that is.  (With the weights in one operand, 12 warps
+//   in one CTA an SM: 84.5 and 67.5 us for the long and the 64 ragged streams, 4
+//   warps in three: 87.8 and 64.3; six in two: 85.4 and 65.9.)
 // ---------------------------------------------------------------------------
 constexpr int kAttWarps = 6;
 constexpr int kCutGain = 14;   // steps that a cut has to save
@@ -432,7 +433,7 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 }
 __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
 
-// Tiles a warp's ring holds (24 KB for K and V together), and a CTA's shared
+// Tiles a warp's ring holds (16 KB for K and V together), and a CTA's shared
 // memory (the rings start on 1024 bytes, as the swizzle wants).
 template <int HD>
 constexpr int ring_stages() { return 2 * 128 / HD; }
@@ -451,9 +452,10 @@ __device__ __forceinline__ void join_pieces(const AttendSplit& sp, unsigned char
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kPart = H * (HD + 2);
   // A set's tickets are those of its first piece's place, so that they do not depend on the call's sizes.  Many pieces are
-  // joined in groups, each by its last CTA to arrive and in the place of its first piece, with that place's ticket, and the groups by the last of those: about 100 pieces of 16 heads (3 streams of up to 100001 positions, one
-  // key/value head) 65 -> 51 us; with 17 to 48 pieces the second round costs more than it saves (4 streams of up to 10303
-  // positions 23.4 -> 29.3 us).
+  // joined in groups, each by its last CTA to arrive and in the place of its first piece, with that place's ticket, and
+  // the groups by the last of those: about 100 pieces of 16 heads (3 streams of up to 100001 positions, one key/value
+  // head) 65 -> 51 us; with 17 to 48 pieces the second round costs more than it saves (4 streams of up to 10303 positions
+  // 23.4 -> 29.3 us).
   const int each = n > kJoinMost ? kJoinGroup : n;
   int from = mine / each * each, step = 1, cnt = min(each, n - from);
   bool final = each == n;
@@ -717,7 +719,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
         tma_load_5d(dst + (HD / 64) * BOX, &vmap, row, hk, pg, &full[warp][slot]);
       }
     };
-    // This warp's tiles are lo + warp + 4 k, k < count.  Lane l looks up the page (and the row in it) of the l-th of the
+    // This warp's tiles are lo + warp + kAttWarps k, k < count.  Lane l looks up the page (and the row in it) of the l-th of the
     // next 32, and of the 32 after those one batch ahead, so that no tile waits for the table.
     const int count = (hi - lo - warp + kAttWarps - 1) / kAttWarps;  // <= 0: none
     auto look_up = [&](int k, int& row) {
@@ -968,7 +970,7 @@ struct CopyParams {
   char* pool;
   int64_t outer_stride, page_stride, page_bytes;
   const int *src, *dst;
-  int outer, num_pages, pairs;
+  int outer, num_pages;
 };
 constexpr int kCopyBytes = 16384;  // bytes a CTA copies
 
@@ -1130,7 +1132,7 @@ int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_h
     return sn::aligned16(base) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
   };
   // whole tiles in a page and 16-byte rows: the tensor-core form (measured beside it: 64 ragged streams of up to 5000
-  // positions 2060 -> 66 us, one stream of 257 positions 56 -> 5.9 us); anything else goes row by row
+  // positions 2060 -> 67 us, one stream of 257 positions 56 -> 5.8 us); anything else goes row by row
   if ((head_dim == 64 || head_dim == 128) && page_size % sn::kTile == 0 && sn::aligned16(out) &&
       rows16(q, q_batch_stride, q_head_stride, 0) && rows16(k_pages, k_page_stride, k_head_stride, k_tok_stride) &&
       rows16(v_pages, v_page_stride, v_head_stride, v_tok_stride)) {
@@ -1177,7 +1179,6 @@ int sn_copy_pages(void* pool, int64_t outer_stride_bytes, int64_t page_stride_by
   p.dst = dst;
   p.outer = outer;
   p.num_pages = num_pages;
-  p.pairs = pairs;
   const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(outer), static_cast<unsigned>(parts));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = sn::aligned16(pool) && (outer == 1 || outer_stride_bytes % 16 == 0) &&
