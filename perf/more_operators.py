@@ -174,7 +174,8 @@ def run(s):
                                                  return_source=s["source"])
             return {"pool": s["pool"], "mass": s["mass"], **({"source": source} if s["source"] else {})}
         if s["op"] == "bounds":
-            paged_sparse.update_page_bounds(s["k_pages"], s["bounds"], s["table"], s["lens"], cu_seqlens=s["cu"])
+            # a decode step says nothing about the counts: one new token a stream
+            paged_sparse.update_page_bounds(s["k_pages"], s["bounds"], s["table"], s["lens"], cu_seqlens=None if s["new"] == "1" else s["cu"])
             return s["bounds"]
         if s["op"] == "select":
             return paged_sparse.select_blocks(s["q"], s["bounds"], s["table"], s["lens"], s["page"], s["count"], first=s["first"], last=s["last"])
