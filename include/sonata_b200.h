@@ -598,6 +598,94 @@ int sn_paged_decode_attention(const void *q, int64_t q_batch_stride, int64_t q_h
 int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_bytes, int64_t page_bytes, int outer,
                   int num_pages, const int *src, const int *dst, int pairs, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Long streams in the paged cache: positions of little weight leave it, or
+ * attention reads only some of its blocks.
+ *
+ * sn_rotary_paged_append_at: sn_rotary_paged_append with the rows of cos and
+ * sin named by positions int32 [tokens] (device): the place in the cache still
+ * is what seq_lens says, which after an eviction is no longer the position.
+ *
+ * sn_paged_decode_attention_mass: sn_paged_decode_attention, and for every
+ * key/value head hk and position t < seq_lens[b]
+ *   mass[b, hk, t] += sum over its query heads h of softmax_t(scale q[b, h] . k[t])
+ * in fp32, in the order of the heads; mass fp32 [batch, nheads_kv, at least
+ * max_pages * page_size] by strides.  A query head whose scores are all -inf
+ * adds nothing.  workspace: sn_paged_mass_workspace_size bytes for
+ * max_positions = max_pages * page_size (or more), with the same rules as the
+ * attention's.
+ *
+ * sn_evict_positions: pool bf16 [layers, 2, num_pages, nheads_kv, page_size,
+ * head_dim], dense (keys and values of all layers, one page table).  In every
+ * layer, stream b and head with n = seq_lens[b] > keep: the first `sinks` and
+ * the last `recent` positions stay, and of the others the keep - sinks -
+ * recent of the highest mass (a NaN is higher than any number; the lowest
+ * positions among equal ones).  Those kept ones that lie below keep - recent
+ * stay where they are; the places between them take the rest in ascending
+ * order; the recent ones follow in their order.  mass fp32 [layers, batch,
+ * nheads_kv, at least max_pages * page_size] by strides goes with the
+ * positions, and [keep, n) of it becomes 0.  source int32 [layers, batch,
+ * nheads_kv, keep] (or NULL) is where each place's position was, -1 past the
+ * end of a stream with n <= keep, of which nothing else changes.  seq_lens is
+ * the caller's to set to min(n, keep).  No page may be shared between streams
+ * that are cut.  recent + sinks <= keep; max_pages * page_size <= 393184.
+ *
+ * sn_update_page_bounds: bounds bf16 [num_pages, nheads_kv, 2, head_dim],
+ * dense: elementwise the least and the greatest of the keys that a page holds
+ * (NaN if one is), for the pages that hold stream b's newest cu_seqlens[b + 1]
+ * - cu_seqlens[b] positions (NULL: one a stream).
+ *
+ * sn_select_blocks: blocks int32 [batch, nheads_kv, count]: in ascending order
+ * the first `first` and the last `last` blocks (of page_size positions) of
+ * stream b, and of the others those with the highest
+ *   max over the head's query heads of sum_d max(q_d least_d, q_d greatest_d),
+ * the lowest blocks among equal ones, all of them if there are no more than
+ * count; -1 behind.  Scores are sums of exact products in 64 bits; a block with
+ * a bound that is not finite is above the others.  head_dim <= 512, max_pages
+ * <= 180216.
+ *
+ * sn_paged_sparse_attention: sn_paged_decode_attention over the positions of
+ * listed blocks only: of blocks int32 [batch, nheads_kv, count] the first
+ * min(count, ceil(seq_lens[b] / page_size)) entries are read, and those below
+ * 0 or past the stream's end left out (a block that is listed twice counts
+ * twice).  A row with no block gives zeros, lse -inf.
+ */
+int sn_rotary_paged_append_at(const void *qkv, int64_t ld, void *q, void *k_pages, int64_t k_page_stride,
+                              int64_t k_head_stride, int64_t k_tok_stride, void *v_pages, int64_t v_page_stride,
+                              int64_t v_head_stride, int64_t v_tok_stride, int num_pages, int page_size,
+                              const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens,
+                              const int *cu_seqlens, const int *positions, const float *cos, const float *sin,
+                              int max_pos, int tokens, int batch, int nheads, int nheads_kv, int head_dim, int rot_dim,
+                              int interleaved, void *stream);
+size_t sn_paged_mass_workspace_size(int batch, int nheads, int nheads_kv, int head_dim, int64_t max_positions);
+int sn_paged_decode_attention_mass(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_pages,
+                                   int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
+                                   const void *v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                                   int64_t v_tok_stride, int num_pages, int page_size, const int *page_table,
+                                   int64_t table_stride, int max_pages, const int *seq_lens, float *mass,
+                                   int64_t mass_batch_stride, int64_t mass_head_stride, void *out, float *lse,
+                                   float scale, int batch, int nheads, int nheads_kv, int head_dim, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+int sn_evict_positions(void *pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
+                       const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens, float *mass,
+                       int64_t mass_layer_stride, int64_t mass_batch_stride, int64_t mass_head_stride, int batch,
+                       int keep, int recent, int sinks, int *source, void *stream);
+int sn_update_page_bounds(const void *k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
+                          int num_pages, int page_size, const int *page_table, int64_t table_stride, int max_pages,
+                          const int *seq_lens, const int *cu_seqlens, int batch, int nheads_kv, int head_dim,
+                          void *bounds, void *stream);
+int sn_select_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *bounds, int num_pages,
+                     int page_size, const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens,
+                     int batch, int nheads, int nheads_kv, int head_dim, int count, int first, int last, int *blocks,
+                     void *stream);
+int sn_paged_sparse_attention(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_pages,
+                              int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
+                              const void *v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                              int64_t v_tok_stride, int num_pages, int page_size, const int *page_table,
+                              int64_t table_stride, int max_pages, const int *seq_lens, const int *blocks, int count,
+                              void *out, float *lse, float scale, int batch, int nheads, int nheads_kv, int head_dim,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

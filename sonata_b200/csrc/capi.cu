@@ -24,6 +24,8 @@ int tu_status_bmm(bool reset, cudaStream_t st, int* out);
 int tu_status_snake(bool reset, cudaStream_t st, int* out);
 int tu_status_paged(bool reset, cudaStream_t st, int* out);
 int tu_status_prompt(bool reset, cudaStream_t st, int* out);
+int tu_status_evict(bool reset, cudaStream_t st, int* out);
+int tu_status_sparse(bool reset, cudaStream_t st, int* out);
 }  // namespace sn
 
 extern "C" {
@@ -31,7 +33,8 @@ extern "C" {
 int sn_device_status(int reset, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int (*units[])(bool, cudaStream_t, int*) = {sn::tu_status_gemv, sn::tu_status_bmm, sn::tu_status_snake,
-                                              sn::tu_status_paged, sn::tu_status_prompt, sn::read_tu_status};
+                                              sn::tu_status_paged, sn::tu_status_prompt, sn::tu_status_evict,
+                                              sn::tu_status_sparse, sn::read_tu_status};
   int first = SN_OK;
   for (auto f : units) {
     int v = SN_OK;

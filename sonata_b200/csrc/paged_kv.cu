@@ -8,6 +8,7 @@
 // stream; seq_lens [batch] int32 is on the device, so a captured step serves
 // growing streams.  Pages and lengths out of range are never followed: the
 // kernels skip them and record SN_ERR_INVALID_ARGUMENT in the status word.
+#include "paged.cuh"
 #include "tc.cuh"
 
 #include <algorithm>
@@ -15,26 +16,6 @@
 
 namespace sn {
 namespace {
-
-// A page table: its entry for a block of page_size positions of stream b, or -1 where there is none.
-struct PageMap {
-  const int* table;  // [batch, table_stride]
-  int64_t table_stride;
-  int max_pages, num_pages, page_size;
-};
-__device__ __forceinline__ int page_of(const PageMap& m, int b, int block) {
-  if (block < 0 || block >= m.max_pages) return -1;
-  const int pg = m.table[static_cast<int64_t>(b) * m.table_stride + block];
-  return static_cast<unsigned>(pg) < static_cast<unsigned>(m.num_pages) ? pg : -1;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-struct PoolStrides {  // elements
-  int64_t page, head, tok;
-};
 
 // ---------------------------------------------------------------------------
 // rotary_paged_append.  Pure data movement (a qkv row read, q / k / v
@@ -51,19 +32,10 @@ struct AppendParams {
   PageMap map;
   const int* seq_lens;  // lengths with the new tokens
   const int* cu;        // [batch + 1] token offsets, or null: one token a stream
+  const int* positions;  // of the tokens, for their rows of cos and sin, or null: their places in the cache
   const float *cos, *sin;  // [max_pos, rot / 2]
   int tokens, batch, hq, hkv, hd, rot, max_pos, interleaved;
 };
-
-// The stream of token t: the last b with cu[b] <= t (binary search).
-__device__ __forceinline__ int stream_of(const int* cu, int batch, int t) {
-  int lo = 0, hi = batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
 
 // One thread per (token, head, element pair of the head): elements (j, j +
 // rot/2) or (2j, 2j + 1) of the rotated part, two neighbours past it.
@@ -86,13 +58,14 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
   __nv_bfloat16* const q = p.q + (static_cast<int64_t>(t) * p.hq + head) * p.hd;  // if it is a head of q
   const bool stray = p.cu && (t < p.cu[b] || t >= end);  // a token of no stream
   const int pos = p.seq_lens[b] - (end - t);
-  if (stray || pos < 0 || pos >= p.max_pos) {
+  const int turn = p.positions ? p.positions[t] : pos;
+  if (stray || pos < 0 || turn < 0 || turn >= p.max_pos) {
     if (!stray) record_status(SN_ERR_INVALID_ARGUMENT);
     if (head < p.hq) q[i1] = q[i2] = __float2bfloat16_rn(0.f);
     return;
   }
   if (rotated) {
-    const float c = p.cos[static_cast<int64_t>(pos) * (p.rot / 2) + j], s = p.sin[static_cast<int64_t>(pos) * (p.rot / 2) + j];
+    const float c = p.cos[static_cast<int64_t>(turn) * (p.rot / 2) + j], s = p.sin[static_cast<int64_t>(turn) * (p.rot / 2) + j];
     const float x1 = __bfloat162float(o1), x2 = __bfloat162float(o2);
     o1 = __float2bfloat16_rn(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
     o2 = __float2bfloat16_rn(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
@@ -176,7 +149,8 @@ __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const Appe
     }
   }
   const int pos = p.seq_lens[s] - (end - t);
-  if (pos < 0 || pos >= p.max_pos) {
+  const int angle = p.positions ? p.positions[t] : pos;
+  if (pos < 0 || angle < 0 || angle >= p.max_pos) {
     record_status(SN_ERR_INVALID_ARGUMENT);
     zero_row(p.q + static_cast<int64_t>(t) * p.hq * p.hd, p.hq * p.hd);
     return;
@@ -185,8 +159,8 @@ __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const Appe
   if (pg < 0) record_status(SN_ERR_INVALID_ARGUMENT);
   float cs[8], sn[8];
   if (turned) {
-    const float4* cr = reinterpret_cast<const float4*>(p.cos + static_cast<int64_t>(pos) * (p.rot / 2) + 8 * u);
-    const float4* sr = reinterpret_cast<const float4*>(p.sin + static_cast<int64_t>(pos) * (p.rot / 2) + 8 * u);
+    const float4* cr = reinterpret_cast<const float4*>(p.cos + static_cast<int64_t>(angle) * (p.rot / 2) + 8 * u);
+    const float4* sr = reinterpret_cast<const float4*>(p.sin + static_cast<int64_t>(angle) * (p.rot / 2) + 8 * u);
     *reinterpret_cast<float4*>(cs) = cr[0];
     *reinterpret_cast<float4*>(cs + 4) = cr[1];
     *reinterpret_cast<float4*>(sn) = sr[0];
@@ -256,19 +230,21 @@ struct AttendParams {
   float* lse;          // [batch, hq] or null
   float scale;
   int batch, hq, hkv, hd;
+  int sets_per_kv, heads_per_set;  // a key/value head's query heads in sets of at most kAttHeadsMax
+  const int* blocks;  // kListed: [batch, hkv, count] blocks of page_size positions
+  int count;
+  float* scores;  // kMass: [batch, sets, room, score_heads], times log2(e)
+  int64_t room;   // max_pages * page_size
+  int score_heads;
 };
 
-// Length of stream b, within the page table's reach.
-__device__ __forceinline__ int stream_len(const AttendParams& p, int b) {
-  const int n = p.seq_lens[b];
-  const int64_t cap = static_cast<int64_t>(p.map.max_pages) * p.map.page_size;
-  if (n < 0 || n > cap) {
-    record_status(SN_ERR_INVALID_ARGUMENT);
-    return n < 0 ? 0 : static_cast<int>(cap);
-  }
-  return n;
-}
+// What a form of the attention does besides: kMass writes the scores for the sums of weights, kListed takes listed blocks of
+// the stream's positions in the place of all of them.
+enum Kind { kPlain, kMass, kListed };
 
+__device__ __forceinline__ int stream_len(const AttendParams& p, int b) { return length_of(p.map, p.seq_lens, b); }
+
+template <Kind kKind>
 __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -285,13 +261,25 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
     o[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  for (int t = warp; t < len; t += 4) {
-    const int pg = page_of(p.map, b, t / p.map.page_size);
+  const int set = hk * p.sets_per_kv + (h - hk * (p.hq / p.hkv)) / p.heads_per_set;  // kMass: where its scores go
+  float* const scores = kKind == kMass ? p.scores + (static_cast<int64_t>(b) * p.hkv * p.sets_per_kv + set) * p.room * p.score_heads +
+                                             (h - hk * (p.hq / p.hkv)) % p.heads_per_set
+                                       : nullptr;
+  const int listed = min(p.count, (len + p.map.page_size - 1) / p.map.page_size);  // entries that are read
+  const int64_t steps = kKind == kListed ? static_cast<int64_t>(listed) * p.map.page_size : len;
+  for (int64_t i = warp; i < steps; i += 4) {
+    int blk = static_cast<int>(i / p.map.page_size);
+    const int at = static_cast<int>(i - static_cast<int64_t>(blk) * p.map.page_size);
+    if constexpr (kKind == kListed) {
+      blk = p.blocks[(static_cast<int64_t>(b) * p.hkv + hk) * p.count + blk];
+      if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + at >= len) continue;
+    }
+    const int pg = page_of(p.map, b, blk);
     if (pg < 0) {
       record_status(SN_ERR_INVALID_ARGUMENT);
+      if (kKind == kMass && lane == 0) scores[i * p.score_heads] = -INFINITY;
       continue;
     }
-    const int at = t % p.map.page_size;
     const __nv_bfloat16* kr = p.kp + pg * p.ks.page + hk * p.ks.head + at * p.ks.tok;
     const __nv_bfloat16* vr = p.vp + pg * p.vs.page + hk * p.vs.head + at * p.vs.tok;
     float s = 0.f;
@@ -301,6 +289,7 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
       if (c < p.hd) s = fmaf(qv[i], __bfloat162float(kr[c]), s);
     }
     s = warp_sum(s);
+    if (kKind == kMass && lane == 0) scores[i * p.score_heads] = s * 1.4426950408889634f;
     const float mn = fmaxf(m, s);
     const float keep = m == mn ? 1.f : expf(m - mn), w = s == -INFINITY ? 0.f : expf(s - mn);
     m = mn;
@@ -392,7 +381,6 @@ struct AttendSplit {
   float* part;       // [2 * grid][kHeadsMax][HD + 2] partial sums, maxima, outputs
   unsigned* ticket;  // [2][2 * grid] arrivals of a set's pieces or groups, of a group's pieces; zero between calls
   int group, sets;   // query heads per key/value head; head sets of a stream (hkv * sets per kv head)
-  int sets_per_kv, heads_per_set;
   int slots;  // CTAs that are on the device together: no more take part in a cut
 };
 
@@ -432,6 +420,14 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return r;
 }
 __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+// Tiles of one (stream, head set).
+template <Kind kKind>
+__device__ __forceinline__ int stream_tiles(const AttendParams& p, int len) {
+  if constexpr (kKind == kListed)
+    return min(p.count, (len + p.map.page_size - 1) / p.map.page_size) * (p.map.page_size / kTile);
+  return tiles_of(len);
+}
+constexpr int kAbsent = -2;  // a listed block that does not count, in the place of its page
 
 // Tiles a warp's ring holds (16 KB for K and V together), and a CTA's shared
 // memory (the rings start on 1024 bytes, as the swizzle wants).
@@ -545,7 +541,7 @@ __device__ __forceinline__ void join_pieces(const AttendSplit& sp, unsigned char
   }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, Kind kKind>
 __global__ void __launch_bounds__(kAttWarps * 32, 2)
     paged_decode_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                             const AttendParams p, const AttendSplit sp) {
@@ -560,6 +556,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   __shared__ __align__(8) uint64_t full[kAttWarps][S];
   __shared__ float s_f[kAttWarps][H], s_mt[H];
   __shared__ uint4 s_q[NT == 1 ? 1 : H * (HD / 8)];  // q of two 8-head tiles: as operands they would spill the loop's registers
+  __shared__ int s_base[kKind == kListed ? kAttWarps : 1][S];  // first position of the tile in each slot
   __shared__ long long s_sum[kAttWarps];
   __shared__ int s_max[kAttWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -589,7 +586,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   long long total = 0;
   int longest = 0, tiles = 0;  // up to 32 streams: tiles of stream `lane`, in every warp
   for (int b = p.batch <= 32 ? lane : tid; b < p.batch; b += kAttWarps * 32) {
-    tiles = tiles_of(stream_len(p, b));
+    tiles = stream_tiles<kKind>(p, stream_len(p, b));
     total += tiles;
     longest = max(longest, tiles);
   }
@@ -611,7 +608,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   }
   total *= sp.sets;
   for (int b = me; b < p.batch; b += gridDim.x) {
-    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : tiles_of(stream_len(p, b));
+    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : stream_tiles<kKind>(p, stream_len(p, b));
     if (n > 0) continue;  // an empty stream: zeros
     for (int c = tid; c < p.hq * HD; c += kAttWarps * 32)
       p.out[static_cast<int64_t>(b) * p.hq * HD + c] = __float2bfloat16_rn(0.f);
@@ -635,13 +632,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   if (single) {
     b = me / sp.sets;
     if (b >= p.batch) return;
-    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : tiles_of(stream_len(p, b));
+    const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : stream_tiles<kKind>(p, stream_len(p, b));
     if (n == 0) return;
     in_b = static_cast<long long>(me - b * sp.sets) * n;
   } else {
     long long before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {  // every warp for itself
-      if (p.batch > 32) tiles = b0 + lane < p.batch ? tiles_of(stream_len(p, b0 + lane)) : 0;
+      if (p.batch > 32) tiles = b0 + lane < p.batch ? stream_tiles<kKind>(p, stream_len(p, b0 + lane)) : 0;
       const long long n = static_cast<long long>(tiles) * sp.sets;
       long long upto = n;
 #pragma unroll
@@ -666,7 +663,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   bool first_piece = true;
   while (at < stop) {
     const int len = stream_len(p, b);
-    const int nt = tiles_of(len);
+    const int nt = stream_tiles<kKind>(p, len);
     if (nt == 0) {
       ++b;
       in_b = 0;
@@ -684,9 +681,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       continue;
     }
     const int hi = cut ? static_cast<int>(min(static_cast<long long>(nt), lo + (stop - at))) : nt;
-    const int hk = set / sp.sets_per_kv;
-    const int h0 = hk * sp.group + (set - hk * sp.sets_per_kv) * sp.heads_per_set;
-    const int nh = min(sp.heads_per_set, (hk + 1) * sp.group - h0);  // heads of this set
+    const int hk = set / p.sets_per_kv;
+    const int h0 = hk * sp.group + (set - hk * p.sets_per_kv) * p.heads_per_set;
+    const int nh = min(p.heads_per_set, (hk + 1) * sp.group - h0);  // heads of this set
 
     // q, in the operand layout: head g of each 8-head tile, chunks t + 4c
     uint4 qv[NT][NT == 1 ? KC : 1];
@@ -725,8 +722,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
     auto look_up = [&](int k, int& row) {
       row = 0;
       if (k >= count) return 0;
-      const int i = lo + warp + kAttWarps * k, blk = i / tpp;
+      const int i = lo + warp + kAttWarps * k;
+      int blk = i / tpp;
       row = (i - blk * tpp) * kTile;
+      if constexpr (kKind == kListed) {
+        blk = p.blocks[(static_cast<int64_t>(b) * p.hkv + hk) * p.count + blk];
+        if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + row >= len) return kAbsent;
+        row += blk * p.map.page_size;  // the position: its row in the page is what is left by whole pages
+      }
       return blk < p.map.max_pages ? p.map.table[static_cast<int64_t>(b) * p.map.table_stride + blk] : -1;
     };
     int row_now, row_then, pg_now = look_up(lane, row_now), pg_then = look_up(lane + 32, row_then);
@@ -741,17 +744,22 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       }
       const int pg = __shfl_sync(0xffffffffu, pg_now, k & 31), row = __shfl_sync(0xffffffffu, row_now, k & 31);
       if (static_cast<unsigned>(pg) >= static_cast<unsigned>(p.map.num_pages)) {
-        record_status(SN_ERR_INVALID_ARGUMENT);
+        if (kKind != kListed || pg != kAbsent) record_status(SN_ERR_INVALID_ARGUMENT);
         return;
       }
-      load_tile(row, pg, into);
+      if constexpr (kKind == kListed) {
+        if (lane == 0) s_base[warp][into] = row;
+        load_tile(row % p.map.page_size, pg, into);
+      } else {
+        load_tile(row, pg, into);
+      }
       loaded |= 1u << into;
     };
 #pragma unroll
     for (int k = 0; k < S - 1; ++k) load_next(k, k);
     int slot = 0;
     for (int k = 0; k < count; ++k) {
-      const int i = lo + warp + kAttWarps * k;
+      const int i = lo + warp + kAttWarps * k;  // the tile's place on the axis
       __syncwarp();  // every lane is done with the slot of the last step
       load_next(k + S - 1, slot == 0 ? S - 1 : slot - 1);
       bool there = (loaded >> slot) & 1;  // the same in every lane, as everything that decides about loads and shuffles
@@ -764,6 +772,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
         }
         parity ^= 1u << slot;
       }
+      const int first = kKind == kListed ? s_base[warp][slot] : i * kTile;  // its first position
       const uint32_t src = mine + slot * stage_bytes<HD>();
       slot = slot + 1 == S ? 0 : slot + 1;
       float s[NT][4], s2[NT][4];
@@ -786,8 +795,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
         }
       }
       // scores of positions og and og + 8, heads 2t and 2t + 1
-      const bool inside = there && (i + 1) * kTile <= len;  // the whole tile counts
-      const bool on0 = inside || (there && i * kTile + og < len), on1 = inside || (there && i * kTile + og + 8 < len);
+      const bool inside = there && first + kTile <= len;  // the whole tile counts
+      const bool on0 = inside || (there && first + og < len), on1 = inside || (there && first + og + 8 < len);
       bool over = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -796,6 +805,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
           s[n][k] = on0 ? (s[n][k] + s2[n][k]) * scale2 : -INFINITY;
           s[n][2 + k] = on1 ? (s[n][2 + k] + s2[n][2 + k]) * scale2 : -INFINITY;
           over |= fmaxf(s[n][k], s[n][2 + k]) > m[n][k] + 8.f;
+        }
+        if constexpr (kKind == kMass) {  // every position of the tile: -inf where it does not count
+          if (8 * n + 2 * t < nh) {
+            float* sc = p.scores + ((static_cast<int64_t>(b) * sp.sets + set) * p.room + first + og) * p.score_heads + 8 * n + 2 * t;
+            *reinterpret_cast<float2*>(sc) = make_float2(s[n][0], s[n][1]);
+            *reinterpret_cast<float2*>(sc + 8 * p.score_heads) = make_float2(s[n][2], s[n][3]);
+          }
         }
       }
       if (__any_sync(0xffffffffu, over)) {
@@ -851,7 +867,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       if (!inside) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const bool on = there && i * kTile + t + 4 * u < len;
+          const bool on = there && first + t + 4 * u < len;
 #pragma unroll
           for (int c = 0; c < VC; ++c) vr[c][u] = on ? vr[c][u] : make_uint4(0, 0, 0, 0);
         }
@@ -962,6 +978,50 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
 }
 
 // ---------------------------------------------------------------------------
+// The second launch of paged_decode_attention_mass: mass[b, hk, t] += sum over
+// the group's heads of exp(score - lse), in the order of the heads.  The final
+// maximum and sum of a row are known only at its end, so its scores (4 bytes a
+// query head, beside 4 head_dim of K and V a key/value head) wait in L2.
+// ---------------------------------------------------------------------------
+struct MassParams {
+  const float* scores;  // [batch, sets, room, score_heads]
+  const float* lse;     // [batch, hq]
+  float* mass;
+  int64_t mb, mh;  // its strides
+  PageMap map;
+  const int* seq_lens;
+  int64_t room;
+  int batch, hq, hkv, sets_per_kv, heads_per_set, score_heads;
+};
+
+__global__ void __launch_bounds__(256) add_mass_kernel(const MassParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int hk = blockIdx.y, group = p.hq / p.hkv;
+  extern __shared__ float s_lse[];  // [group], times log2(e)
+  for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
+    const int len = length_of(p.map, p.seq_lens, b);
+    __syncthreads();
+    for (int h = threadIdx.x; h < group; h += 256)
+      s_lse[h] = p.lse[static_cast<int64_t>(b) * p.hq + hk * group + h] * 1.4426950408889634f;
+    __syncthreads();
+    for (int64_t t = blockIdx.x * 256 + threadIdx.x; t < len; t += static_cast<int64_t>(gridDim.x) * 256) {
+      float sum = 0.f;
+      for (int set = 0; set < p.sets_per_kv; ++set) {
+        const float* sc = p.scores + ((static_cast<int64_t>(b) * p.hkv * p.sets_per_kv + hk * p.sets_per_kv + set) * p.room + t) * p.score_heads;
+        const int nh = min(p.heads_per_set, group - set * p.heads_per_set);
+        for (int h = 0; h < nh; ++h) {
+          const float l = s_lse[set * p.heads_per_set + h];
+          sum += l == -INFINITY ? 0.f : exp2_approx(sc[h] - l);  // no weight anywhere in this row
+        }
+      }
+      float* m = p.mass + b * p.mb + hk * p.mh + t;
+      *m += sum;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // copy_pages: pool [outer, num_pages, page_bytes] with byte strides; page
 // src[i] -> page dst[i] in every outer index.  16 KB a CTA, in one pass: bounded
 // by HBM (36000 pages of 16 KB in 178 us, 6.6 TB/s), 2.1 us for a handful.
@@ -1004,18 +1064,159 @@ inline bool pool_map(CUtensorMap* map, const void* base, const PoolStrides& st, 
   return tc::make_map_bf16_sw128(map, base, 5, dims, strides, box);
 }
 
-template <int HD, int NT>
+template <int HD, int NT, Kind kKind>
 int launch_decode(int grid, cudaStream_t st, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p,
                   const AttendSplit& sp) {
   constexpr int smem = static_cast<int>(ring_bytes<HD>()) + 1024;
-  if (!smem_room<paged_decode_mma_kernel<HD, NT>>(smem)) return SN_ERR_LAUNCH;
-  return launch(paged_decode_mma_kernel<HD, NT>, dim3(static_cast<unsigned>(grid)), dim3(kAttWarps * 32), smem, st, true, km,
+  if (!smem_room<paged_decode_mma_kernel<HD, NT, kKind>>(smem)) return SN_ERR_LAUNCH;
+  return launch(paged_decode_mma_kernel<HD, NT, kKind>, dim3(static_cast<unsigned>(grid)), dim3(kAttWarps * 32), smem, st, true, km,
                 vm, p, sp);
 }
 
-inline bool pool_ok(int64_t page, int64_t head, int64_t tok, int nheads, int page_size, int hd) {
-  // rows dense, axes in any order but not overlapping below the row
-  return tok >= hd && head >= hd && page >= hd && nheads >= 1 && page_size >= 1;
+int append(const void* qkv, int64_t ld, void* q, void* k_pages, int64_t k_page_stride,
+                           int64_t k_head_stride, int64_t k_tok_stride, void* v_pages, int64_t v_page_stride,
+                           int64_t v_head_stride, int64_t v_tok_stride, int num_pages, int page_size,
+                           const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
+                           const int* cu_seqlens, const int* positions, const float* cos, const float* sin, int max_pos, int tokens,
+                           int batch, int nheads, int nheads_kv, int head_dim, int rot_dim, int interleaved,
+                           void* stream) {
+  if (!qkv || !q || !k_pages || !v_pages || !page_table || !seq_lens || tokens < 0 || batch < 1 || nheads < 1 ||
+      nheads_kv < 1 || head_dim < 2 || head_dim % 2 != 0 || rot_dim < 0 || rot_dim % 2 != 0 || rot_dim > head_dim ||
+      num_pages < 1 || page_size < 1 || max_pages < 1 || table_stride < max_pages || max_pos < 1 ||
+      (rot_dim > 0 && (!cos || !sin)) || (!cu_seqlens && tokens != batch))
+    return SN_ERR_INVALID_ARGUMENT;
+  const int64_t width = (static_cast<int64_t>(nheads) + 2 * static_cast<int64_t>(nheads_kv)) * head_dim;
+  if (ld < width || !pool_ok(k_page_stride, k_head_stride, k_tok_stride, nheads_kv, page_size, head_dim) ||
+      !pool_ok(v_page_stride, v_head_stride, v_tok_stride, nheads_kv, page_size, head_dim))
+    return SN_ERR_INVALID_ARGUMENT;
+  if (width > INT32_MAX) return SN_ERR_UNSUPPORTED;
+  if (tokens == 0) return SN_OK;
+  AppendParams p;
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.ld = ld;
+  p.q = static_cast<__nv_bfloat16*>(q);
+  p.kp = static_cast<__nv_bfloat16*>(k_pages);
+  p.vp = static_cast<__nv_bfloat16*>(v_pages);
+  p.ks = {k_page_stride, k_head_stride, k_tok_stride};
+  p.vs = {v_page_stride, v_head_stride, v_tok_stride};
+  p.map = {page_table, table_stride, max_pages, num_pages, page_size};
+  p.seq_lens = seq_lens;
+  p.cu = cu_seqlens;
+  p.positions = positions;
+  p.cos = cos;
+  p.sin = sin;
+  p.tokens = tokens;
+  p.batch = batch;
+  p.hq = nheads;
+  p.hkv = nheads_kv;
+  p.hd = head_dim;
+  p.rot = rot_dim;
+  p.max_pos = max_pos;
+  p.interleaved = interleaved ? 1 : 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // 16-byte chunks throughout: 12288 tokens of 24 heads of 128 in 27.1 us (5.8 TB/s) against 168 us element by element
+  if (head_dim % 16 == 0 && rot_dim % 16 == 0 && head_dim <= 512 && nheads + 2 * nheads_kv <= 65535 && rows16(qkv, ld, 0, 0) && aligned16(q) &&
+      rows16(k_pages, k_page_stride, k_head_stride, k_tok_stride) &&
+      rows16(v_pages, v_page_stride, v_head_stride, v_tok_stride) && aligned16(cos) && aligned16(sin)) {
+    const int warp_heads = kAppendHeads * (32 / (head_dim / 16));
+    const dim3 grid(static_cast<unsigned>((tokens + 3) / 4),
+                    static_cast<unsigned>((nheads + 2 * nheads_kv + warp_heads - 1) / warp_heads));
+    return interleaved ? launch(rotary_paged_append_vec_kernel<true>, grid, dim3(128), 0, st, true, p)
+                       : launch(rotary_paged_append_vec_kernel<false>, grid, dim3(128), 0, st, true, p);
+  }
+  const int64_t blocks = (static_cast<int64_t>(tokens) * (width / 2) + 255) / 256;
+  if (blocks > INT32_MAX) return SN_ERR_UNSUPPORTED;
+  return launch(rotary_paged_append_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st,
+                    true, p);
+}
+
+AttendParams attend_params(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
+                           int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride, const void* v_pages,
+                           int64_t v_page_stride, int64_t v_head_stride, int64_t v_tok_stride, int num_pages,
+                           int page_size, const int* page_table, int64_t table_stride, int max_pages,
+                           const int* seq_lens, void* out, float* lse, float scale, int batch, int nheads,
+                           int nheads_kv, int head_dim) {
+  AttendParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.qb = q_batch_stride;
+  p.qh = q_head_stride;
+  p.kp = static_cast<const __nv_bfloat16*>(k_pages);
+  p.vp = static_cast<const __nv_bfloat16*>(v_pages);
+  p.ks = {k_page_stride, k_head_stride, k_tok_stride};
+  p.vs = {v_page_stride, v_head_stride, v_tok_stride};
+  p.map = {page_table, table_stride, max_pages, num_pages, page_size};
+  p.seq_lens = seq_lens;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.scale = scale;
+  p.batch = batch;
+  p.hq = nheads;
+  p.hkv = nheads_kv;
+  p.hd = head_dim;
+  return p;
+}
+
+int attend_check(const AttendParams& p, const void* workspace, size_t workspace_bytes) {
+  if (!p.q || !p.kp || !p.vp || !p.map.table || !p.seq_lens || !p.out || !workspace || p.batch < 1 || p.hq < 1 ||
+      p.hkv < 1 || p.hq % p.hkv != 0 || p.hd < 1 || p.map.num_pages < 1 || p.map.page_size < 1 ||
+      p.map.max_pages < 1 || p.map.table_stride < p.map.max_pages || p.qb < 0 || p.qh < 0)
+    return SN_ERR_INVALID_ARGUMENT;
+  if (!pool_ok(p.ks.page, p.ks.head, p.ks.tok, p.hkv, p.map.page_size, p.hd) ||
+      !pool_ok(p.vs.page, p.vs.head, p.vs.tok, p.hkv, p.map.page_size, p.hd) ||
+      workspace_bytes < sn_paged_decode_workspace_size(p.batch, p.hq, p.hd))
+    return SN_ERR_INVALID_ARGUMENT;
+  if (!aligned16(workspace)) return SN_ERR_MISALIGNED;
+  if (p.hd > 32 * kMaxHeadPerLane || static_cast<int64_t>(p.batch) * p.hq > INT32_MAX ||
+      static_cast<int64_t>(p.map.max_pages) * p.map.page_size > INT32_MAX)
+    return SN_ERR_UNSUPPORTED;
+  return SN_OK;
+}
+
+// A key/value head's query heads in sets of at most kAttHeadsMax, about equal.
+void head_sets(AttendParams& p) {
+  const int group = p.hq / p.hkv;
+  p.sets_per_kv = (group + kAttHeadsMax - 1) / kAttHeadsMax;
+  p.heads_per_set = (group + p.sets_per_kv - 1) / p.sets_per_kv;
+  p.score_heads = (p.heads_per_set + 1) / 2 * 2;  // scores are written in pairs
+}
+// Where the workspace of paged_decode_attention_mass holds the rows' lse, and the bytes of them; then the scores.
+size_t lse_at(int batch, int nheads, int head_dim) {
+  return (sn_paged_decode_workspace_size(batch, nheads, head_dim) + 15) / 16 * 16;
+}
+size_t lse_bytes(int batch, int nheads) { return (static_cast<size_t>(batch) * nheads * sizeof(float) + 15) / 16 * 16; }
+
+template <Kind kKind>
+int attend(AttendParams p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = attend_check(p, workspace, workspace_bytes);
+  if (rc != SN_OK) return rc;
+  head_sets(p);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // whole tiles in a page and 16-byte rows: the tensor-core form (measured beside it: 64 ragged streams of up to 5000
+  // positions 2060 -> 67 us, one stream of 257 positions 56 -> 5.8 us); anything else goes row by row
+  if ((p.hd == 64 || p.hd == 128) && p.map.page_size % kTile == 0 && aligned16(p.out) && rows16(p.q, p.qb, p.qh, 0) &&
+      rows16(p.kp, p.ks.page, p.ks.head, p.ks.tok) && rows16(p.vp, p.vs.page, p.vs.head, p.vs.tok)) {
+    AttendSplit sp;
+    sp.group = p.hq / p.hkv;
+    sp.sets = p.hkv * p.sets_per_kv;
+    sp.ticket = static_cast<unsigned*>(workspace);
+    sp.part = reinterpret_cast<float*>(sp.ticket + SN_PAGED_DECODE_COUNTERS);
+    CUtensorMap km, vm;
+    if (!pool_map(&km, p.kp, p.ks, p.map.num_pages, p.hkv, p.map.page_size, p.hd) ||
+        !pool_map(&vm, p.vp, p.vs, p.map.num_pages, p.hkv, p.map.page_size, p.hd))
+      return SN_ERR_LAUNCH;
+    const bool two = p.heads_per_set > 8;  // an operand takes 8 heads: two of them read a group's K and V once
+    // two CTAs an SM, and no more than the page tables (or lists) have tiles for
+    const int64_t row_pages = kKind == kListed ? std::min(p.count, p.map.max_pages) : p.map.max_pages;
+    const int64_t tiles = row_pages * (p.map.page_size / kTile) * p.batch * sp.sets;
+    const int64_t most = (tiles + kAttWarps - 1) / kAttWarps;
+    sp.slots = static_cast<int>(std::min<int64_t>(std::min(2 * sm_count(), kAttGridMax), most));
+    // and one for every (stream, head set) where they are short (4096 at most)
+    const int grid = static_cast<int>(std::max<int64_t>(sp.slots, std::min<int64_t>(static_cast<int64_t>(p.batch) * sp.sets, 4096)));
+    if (p.hd == 64)
+      return two ? launch_decode<64, 2, kKind>(grid, st, km, vm, p, sp) : launch_decode<64, 1, kKind>(grid, st, km, vm, p, sp);
+    return two ? launch_decode<128, 2, kKind>(grid, st, km, vm, p, sp) : launch_decode<128, 1, kKind>(grid, st, km, vm, p, sp);
+  }
+  return launch(paged_decode_rows_kernel<kKind>, dim3(static_cast<unsigned>(p.batch * p.hq)), dim3(128), 0, st, true, p);
 }
 
 }  // namespace
@@ -1033,56 +1234,22 @@ int sn_rotary_paged_append(const void* qkv, int64_t ld, void* q, void* k_pages, 
                            const int* cu_seqlens, const float* cos, const float* sin, int max_pos, int tokens,
                            int batch, int nheads, int nheads_kv, int head_dim, int rot_dim, int interleaved,
                            void* stream) {
-  if (!qkv || !q || !k_pages || !v_pages || !page_table || !seq_lens || tokens < 0 || batch < 1 || nheads < 1 ||
-      nheads_kv < 1 || head_dim < 2 || head_dim % 2 != 0 || rot_dim < 0 || rot_dim % 2 != 0 || rot_dim > head_dim ||
-      num_pages < 1 || page_size < 1 || max_pages < 1 || table_stride < max_pages || max_pos < 1 ||
-      (rot_dim > 0 && (!cos || !sin)) || (!cu_seqlens && tokens != batch))
-    return SN_ERR_INVALID_ARGUMENT;
-  const int64_t width = (static_cast<int64_t>(nheads) + 2 * static_cast<int64_t>(nheads_kv)) * head_dim;
-  if (ld < width || !sn::pool_ok(k_page_stride, k_head_stride, k_tok_stride, nheads_kv, page_size, head_dim) ||
-      !sn::pool_ok(v_page_stride, v_head_stride, v_tok_stride, nheads_kv, page_size, head_dim))
-    return SN_ERR_INVALID_ARGUMENT;
-  if (width > INT32_MAX) return SN_ERR_UNSUPPORTED;
-  if (tokens == 0) return SN_OK;
-  sn::AppendParams p;
-  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
-  p.ld = ld;
-  p.q = static_cast<__nv_bfloat16*>(q);
-  p.kp = static_cast<__nv_bfloat16*>(k_pages);
-  p.vp = static_cast<__nv_bfloat16*>(v_pages);
-  p.ks = {k_page_stride, k_head_stride, k_tok_stride};
-  p.vs = {v_page_stride, v_head_stride, v_tok_stride};
-  p.map = {page_table, table_stride, max_pages, num_pages, page_size};
-  p.seq_lens = seq_lens;
-  p.cu = cu_seqlens;
-  p.cos = cos;
-  p.sin = sin;
-  p.tokens = tokens;
-  p.batch = batch;
-  p.hq = nheads;
-  p.hkv = nheads_kv;
-  p.hd = head_dim;
-  p.rot = rot_dim;
-  p.max_pos = max_pos;
-  p.interleaved = interleaved ? 1 : 0;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto rows16 = [](const void* base, int64_t a, int64_t b, int64_t c) {
-    return sn::aligned16(base) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
-  };
-  // 16-byte chunks throughout: 12288 tokens of 24 heads of 128 in 27.1 us (5.8 TB/s) against 168 us element by element
-  if (head_dim % 16 == 0 && rot_dim % 16 == 0 && head_dim <= 512 && nheads + 2 * nheads_kv <= 65535 && rows16(qkv, ld, 0, 0) && sn::aligned16(q) &&
-      rows16(k_pages, k_page_stride, k_head_stride, k_tok_stride) &&
-      rows16(v_pages, v_page_stride, v_head_stride, v_tok_stride) && sn::aligned16(cos) && sn::aligned16(sin)) {
-    const int warp_heads = sn::kAppendHeads * (32 / (head_dim / 16));
-    const dim3 grid(static_cast<unsigned>((tokens + 3) / 4),
-                    static_cast<unsigned>((nheads + 2 * nheads_kv + warp_heads - 1) / warp_heads));
-    return interleaved ? sn::launch(sn::rotary_paged_append_vec_kernel<true>, grid, dim3(128), 0, st, true, p)
-                       : sn::launch(sn::rotary_paged_append_vec_kernel<false>, grid, dim3(128), 0, st, true, p);
-  }
-  const int64_t blocks = (static_cast<int64_t>(tokens) * (width / 2) + 255) / 256;
-  if (blocks > INT32_MAX) return SN_ERR_UNSUPPORTED;
-  return sn::launch(sn::rotary_paged_append_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st,
-                    true, p);
+  return sn::append(qkv, ld, q, k_pages, k_page_stride, k_head_stride, k_tok_stride, v_pages, v_page_stride, v_head_stride,
+                    v_tok_stride, num_pages, page_size, page_table, table_stride, max_pages, seq_lens, cu_seqlens, nullptr,
+                    cos, sin, max_pos, tokens, batch, nheads, nheads_kv, head_dim, rot_dim, interleaved, stream);
+}
+
+int sn_rotary_paged_append_at(const void* qkv, int64_t ld, void* q, void* k_pages, int64_t k_page_stride,
+                           int64_t k_head_stride, int64_t k_tok_stride, void* v_pages, int64_t v_page_stride,
+                           int64_t v_head_stride, int64_t v_tok_stride, int num_pages, int page_size,
+                           const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
+                           const int* cu_seqlens, const int* positions, const float* cos, const float* sin, int max_pos, int tokens,
+                           int batch, int nheads, int nheads_kv, int head_dim, int rot_dim, int interleaved,
+                           void* stream) {
+  if (!positions && tokens > 0) return SN_ERR_INVALID_ARGUMENT;
+  return sn::append(qkv, ld, q, k_pages, k_page_stride, k_head_stride, k_tok_stride, v_pages, v_page_stride, v_head_stride,
+                    v_tok_stride, num_pages, page_size, page_table, table_stride, max_pages, seq_lens, cu_seqlens, positions,
+                    cos, sin, max_pos, tokens, batch, nheads, nheads_kv, head_dim, rot_dim, interleaved, stream);
 }
 
 size_t sn_paged_decode_workspace_size(int batch, int nheads, int head_dim) {
@@ -1098,68 +1265,89 @@ int sn_paged_decode_attention(const void* q, int64_t q_batch_stride, int64_t q_h
                               int page_size, const int* page_table, int64_t table_stride, int max_pages,
                               const int* seq_lens, void* out, float* lse, float scale, int batch, int nheads,
                               int nheads_kv, int head_dim, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!q || !k_pages || !v_pages || !page_table || !seq_lens || !out || !workspace || batch < 1 || nheads < 1 ||
-      nheads_kv < 1 || nheads % nheads_kv != 0 || head_dim < 1 || num_pages < 1 || page_size < 1 || max_pages < 1 ||
-      table_stride < max_pages || q_batch_stride < 0 || q_head_stride < 0)
-    return SN_ERR_INVALID_ARGUMENT;
-  if (!sn::pool_ok(k_page_stride, k_head_stride, k_tok_stride, nheads_kv, page_size, head_dim) ||
-      !sn::pool_ok(v_page_stride, v_head_stride, v_tok_stride, nheads_kv, page_size, head_dim) ||
-      workspace_bytes < sn_paged_decode_workspace_size(batch, nheads, head_dim))
-    return SN_ERR_INVALID_ARGUMENT;
-  if (!sn::aligned16(workspace)) return SN_ERR_MISALIGNED;
-  if (head_dim > 32 * sn::kMaxHeadPerLane || static_cast<int64_t>(batch) * nheads > INT32_MAX ||
-      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
-    return SN_ERR_UNSUPPORTED;
+  return sn::attend<sn::kPlain>(
+      sn::attend_params(q, q_batch_stride, q_head_stride, k_pages, k_page_stride, k_head_stride, k_tok_stride, v_pages,
+                        v_page_stride, v_head_stride, v_tok_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, seq_lens, out, lse, scale, batch, nheads, nheads_kv, head_dim),
+      workspace, workspace_bytes, stream);
+}
+
+int sn_paged_sparse_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
+                              int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride, const void* v_pages,
+                              int64_t v_page_stride, int64_t v_head_stride, int64_t v_tok_stride, int num_pages,
+                              int page_size, const int* page_table, int64_t table_stride, int max_pages,
+                              const int* seq_lens, const int* blocks, int count, void* out, float* lse, float scale,
+                              int batch, int nheads, int nheads_kv, int head_dim, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  if (!blocks || count < 1) return SN_ERR_INVALID_ARGUMENT;
+  if (page_size > 0 && count > INT32_MAX / page_size) return SN_ERR_UNSUPPORTED;
+  sn::AttendParams p =
+      sn::attend_params(q, q_batch_stride, q_head_stride, k_pages, k_page_stride, k_head_stride, k_tok_stride, v_pages,
+                        v_page_stride, v_head_stride, v_tok_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, seq_lens, out, lse, scale, batch, nheads, nheads_kv, head_dim);
+  p.blocks = blocks;
+  p.count = count;
+  return sn::attend<sn::kListed>(p, workspace, workspace_bytes, stream);
+}
+
+size_t sn_paged_mass_workspace_size(int batch, int nheads, int nheads_kv, int head_dim, int64_t max_positions) {
+  if (batch < 1 || nheads < 1 || nheads_kv < 1 || nheads % nheads_kv != 0 || head_dim < 1 || max_positions < 1) return 0;
   sn::AttendParams p;
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.qb = q_batch_stride;
-  p.qh = q_head_stride;
-  p.kp = static_cast<const __nv_bfloat16*>(k_pages);
-  p.vp = static_cast<const __nv_bfloat16*>(v_pages);
-  p.ks = {k_page_stride, k_head_stride, k_tok_stride};
-  p.vs = {v_page_stride, v_head_stride, v_tok_stride};
-  p.map = {page_table, table_stride, max_pages, num_pages, page_size};
-  p.seq_lens = seq_lens;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.lse = lse;
-  p.scale = scale;
-  p.batch = batch;
   p.hq = nheads;
   p.hkv = nheads_kv;
-  p.hd = head_dim;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto rows16 = [](const void* base, int64_t a, int64_t b, int64_t c) {
-    return sn::aligned16(base) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
-  };
-  // whole tiles in a page and 16-byte rows: the tensor-core form (measured beside it: 64 ragged streams of up to 5000
-  // positions 2060 -> 67 us, one stream of 257 positions 56 -> 5.8 us); anything else goes row by row
-  if ((head_dim == 64 || head_dim == 128) && page_size % sn::kTile == 0 && sn::aligned16(out) &&
-      rows16(q, q_batch_stride, q_head_stride, 0) && rows16(k_pages, k_page_stride, k_head_stride, k_tok_stride) &&
-      rows16(v_pages, v_page_stride, v_head_stride, v_tok_stride)) {
-    sn::AttendSplit sp;
-    sp.group = nheads / nheads_kv;
-    sp.sets_per_kv = (sp.group + sn::kAttHeadsMax - 1) / sn::kAttHeadsMax;
-    sp.heads_per_set = (sp.group + sp.sets_per_kv - 1) / sp.sets_per_kv;
-    sp.sets = nheads_kv * sp.sets_per_kv;
-    sp.ticket = static_cast<unsigned*>(workspace);
-    sp.part = reinterpret_cast<float*>(sp.ticket + SN_PAGED_DECODE_COUNTERS);
-    CUtensorMap km, vm;
-    if (!sn::pool_map(&km, k_pages, p.ks, num_pages, nheads_kv, page_size, head_dim) ||
-        !sn::pool_map(&vm, v_pages, p.vs, num_pages, nheads_kv, page_size, head_dim))
-      return SN_ERR_LAUNCH;
-    const bool two = sp.heads_per_set > 8;  // an operand takes 8 heads: two of them read a group's K and V once
-    // two CTAs an SM, and no more than the page tables have tiles for
-    const int64_t tiles = static_cast<int64_t>(max_pages) * (page_size / sn::kTile) * batch * sp.sets;
-    const int64_t most = (tiles + sn::kAttWarps - 1) / sn::kAttWarps;
-    sp.slots = static_cast<int>(std::min<int64_t>(std::min(2 * sn::sm_count(), sn::kAttGridMax), most));
-    // and one for every (stream, head set) where they are short (4096 at most)
-    const int grid = static_cast<int>(std::max<int64_t>(sp.slots, std::min<int64_t>(static_cast<int64_t>(batch) * sp.sets, 4096)));
-    if (head_dim == 64)
-      return two ? sn::launch_decode<64, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<64, 1>(grid, st, km, vm, p, sp);
-    return two ? sn::launch_decode<128, 2>(grid, st, km, vm, p, sp) : sn::launch_decode<128, 1>(grid, st, km, vm, p, sp);
-  }
-  return sn::launch(sn::paged_decode_rows_kernel, dim3(static_cast<unsigned>(batch * nheads)), dim3(128), 0, st,
-                    true, p);
+  sn::head_sets(p);
+  return sn::lse_at(batch, nheads, head_dim) + sn::lse_bytes(batch, nheads) +
+         static_cast<size_t>(batch) * nheads_kv * p.sets_per_kv * max_positions * p.score_heads * sizeof(float);
+}
+
+int sn_paged_decode_attention_mass(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
+                                   int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
+                                   const void* v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                                   int64_t v_tok_stride, int num_pages, int page_size, const int* page_table,
+                                   int64_t table_stride, int max_pages, const int* seq_lens, float* mass,
+                                   int64_t mass_batch_stride, int64_t mass_head_stride, void* out, float* lse,
+                                   float scale, int batch, int nheads, int nheads_kv, int head_dim, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  const int64_t room = static_cast<int64_t>(max_pages) * page_size;
+  if (!mass || (nheads_kv > 1 && mass_head_stride < room) || (batch > 1 && mass_batch_stride < room))
+    return SN_ERR_INVALID_ARGUMENT;
+  sn::AttendParams p =
+      sn::attend_params(q, q_batch_stride, q_head_stride, k_pages, k_page_stride, k_head_stride, k_tok_stride, v_pages,
+                        v_page_stride, v_head_stride, v_tok_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, seq_lens, out, lse, scale, batch, nheads, nheads_kv, head_dim);
+  const int rc = sn::attend_check(p, workspace, workspace_bytes);
+  if (rc != SN_OK) return rc;
+  if (workspace_bytes < sn_paged_mass_workspace_size(batch, nheads, nheads_kv, head_dim, room))
+    return SN_ERR_INVALID_ARGUMENT;
+  const int group = nheads / nheads_kv;
+  if (nheads_kv > 65535 || group > 8192) return SN_ERR_UNSUPPORTED;  // the second launch's grid and shared memory
+  char* const ws = static_cast<char*>(workspace) + sn::lse_at(batch, nheads, head_dim);
+  if (!lse) p.lse = reinterpret_cast<float*>(ws);
+  p.scores = reinterpret_cast<float*>(ws + sn::lse_bytes(batch, nheads));
+  p.room = room;
+  const int rc2 = sn::attend<sn::kMass>(p, workspace, workspace_bytes, stream);
+  if (rc2 != SN_OK) return rc2;
+  sn::MassParams mp;
+  mp.scores = p.scores;
+  mp.lse = p.lse;
+  mp.mass = mass;
+  mp.mb = mass_batch_stride;
+  mp.mh = mass_head_stride;
+  mp.map = p.map;
+  mp.seq_lens = seq_lens;
+  mp.room = room;
+  mp.batch = batch;
+  mp.hq = nheads;
+  mp.hkv = nheads_kv;
+  sn::head_sets(p);
+  mp.sets_per_kv = p.sets_per_kv;
+  mp.heads_per_set = p.heads_per_set;
+  mp.score_heads = p.score_heads;
+  // about eight CTAs an SM, no more than the tables have positions for: the lengths are on the device
+  const int64_t rows = static_cast<int64_t>(std::min(batch, 65535)) * nheads_kv;
+  const int64_t per_row = std::min<int64_t>((room + 255) / 256, std::max<int64_t>(1, 8 * sn::sm_count() / rows));
+  return sn::launch(sn::add_mass_kernel, dim3(static_cast<unsigned>(per_row), static_cast<unsigned>(nheads_kv), static_cast<unsigned>(std::min(batch, 65535))),
+                    dim3(256), group * sizeof(float), static_cast<cudaStream_t>(stream), true, mp);
 }
 
 int sn_copy_pages(void* pool, int64_t outer_stride_bytes, int64_t page_stride_bytes, int64_t page_bytes, int outer,

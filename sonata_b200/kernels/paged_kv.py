@@ -94,7 +94,8 @@ def _pages(k_pages, v_pages, page_table, seq_lens):
 
 def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                         seq_lens: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, nheads: int,
-                        cu_seqlens: torch.Tensor | None = None, interleaved: bool = False, stream=None) -> torch.Tensor:
+                        cu_seqlens: torch.Tensor | None = None, interleaved: bool = False, stream=None,
+                        positions: torch.Tensor | None = None) -> torch.Tensor:
     """qkv [tokens, (nheads + 2 nheads_kv) head_dim] of the new tokens (row
     stride taken from the tensor): stream b's are rows cu_seqlens[b] ..
     cu_seqlens[b+1]-1 (None: one token a stream) and end at position
@@ -102,8 +103,10 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     elements of each q and k head are rotated by the position's row of cos /
     sin fp32 [max_pos, rot / 2]: halves (j, j + rot/2), or neighbours (2j, 2j
     + 1) when interleaved.  k and v go to their pages; returns q [tokens,
-    nheads, head_dim], zeros for a row of no stream or a position out of range."""
-    if stream is None:
+    nheads, head_dim], zeros for a row of no stream or a position out of range.
+    `positions` int32 [tokens] names the tokens' rows of cos / sin where their
+    places in the cache are not their positions (after evict_positions)."""
+    if stream is None and positions is None:
         r = fast().append(qkv, k_pages, v_pages, page_table, seq_lens, cos, sin, nheads, cu_seqlens, interleaved)
         if r is not None:
             return r if type(r) is not int else _lib.check("sn_rotary_paged_append", r)
@@ -126,18 +129,25 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
         for name, t in (("cos", cos), ("sin", sin)):
             require_cuda(name, t, torch.float32, 2)
         raise ValueError(f"cos and sin must be contiguous fp32 [max_pos, rot / 2], rot at most {hd}, both alike")
+    if positions is not None and not (isinstance(positions, torch.Tensor) and positions.is_cuda and positions.dtype is torch.int32
+                                      and positions.shape == (tokens,) and positions.is_contiguous()):
+        require_cuda("positions", positions, torch.int32, 1)
+        raise ValueError(f"positions must hold {tokens} contiguous numbers")
     max_pos, half = cos.shape
     dev = torch.cuda.current_device()
     if not (dev == qkv.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device() ==
-            seq_lens.get_device() == cos.get_device() == sin.get_device() == (cos if cu_seqlens is None else cu_seqlens).get_device()):
+            seq_lens.get_device() == cos.get_device() == sin.get_device() == (cos if cu_seqlens is None else cu_seqlens).get_device()
+            == (cos if positions is None else positions).get_device()):
         same_device(qkv=qkv, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, cos=cos, sin=sin,
-                    cu_seqlens=cu_seqlens)
+                    cu_seqlens=cu_seqlens, positions=positions)
+    at = () if positions is None else (positions.data_ptr(),)
 
     def launch(st):
         q = qkv.new_empty((tokens, nheads, hd))
         if tokens:
-            call("sn_rotary_paged_append", qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width, q.data_ptr(),
-                 *args, cu_seqlens.data_ptr() if cu_seqlens is not None else None, cos.data_ptr(), sin.data_ptr(),
+            call("sn_rotary_paged_append_at" if at else "sn_rotary_paged_append", qkv.data_ptr(),
+                 qkv.stride(0) if tokens > 1 else width, q.data_ptr(), *args,
+                 cu_seqlens.data_ptr() if cu_seqlens is not None else None, *at, cos.data_ptr(), sin.data_ptr(),
                  max_pos, tokens, batch, nheads, hkv, hd, 2 * half, 1 if interleaved else 0, st)
         return q
 
@@ -175,6 +185,15 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         r = fast().attend(q, k_pages, v_pages, page_table, seq_lens, scale, workspace, return_lse)
         if r is not None:
             return r if type(r) is not int else _lib.check("sn_paged_decode_attention", r)
+    return attend("sn_paged_decode_attention", q, k_pages, v_pages, page_table, seq_lens, scale, workspace, return_lse, stream,
+                  _workspace_size)
+
+
+def attend(fn: str, q, k_pages, v_pages, page_table, seq_lens, scale, workspace, return_lse, stream, size, extra=(),
+           others=None):
+    """The C entry `fn`, a form of the attention of one token a stream: `extra`
+    are its arguments after seq_lens, `others` more tensors (by name) that have
+    to be on the current device, `size` gives the bytes of its workspace."""
     if not (isinstance(q, torch.Tensor) and q.dtype is _BF16 and q.is_cuda and q.dim() == 3):
         require_cuda("q", q, _BF16, 3)
     args = _pages(k_pages, v_pages, page_table, seq_lens)
@@ -184,18 +203,18 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         raise ValueError(f"q {tuple(q.shape)} does not match {seq_lens.shape[0]} streams of {hkv} heads of {k_pages.shape[3]}")
     if qc != 1 and hd > 1:
         raise ValueError("q must be dense along its last dimension")
-    need = _workspace_size(batch, nheads, hd)
+    need = size(batch, nheads, hd)
     dev = torch.cuda.current_device()
     if not (dev == q.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device() ==
-            seq_lens.get_device()):
-        same_device(q=q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens)
+            seq_lens.get_device()) or others:
+        same_device(q=q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, **(others or {}))
     if workspace is not None and not (
             isinstance(workspace, torch.Tensor) and workspace.dtype is torch.uint8 and workspace.get_device() == dev and
             workspace.dim() == 1 and workspace.numel() >= need and workspace.is_contiguous()
             and workspace.data_ptr() % 16 == 0):
         require_cuda("workspace", workspace, torch.uint8, 1)
         same_device(workspace=workspace)
-        raise ValueError(f"workspace must hold {need} contiguous, 16-byte aligned bytes (decode_workspace)")
+        raise ValueError(f"workspace must hold {need} contiguous, 16-byte aligned bytes (decode_workspace, mass_workspace)")
 
     def launch(st):
         out = q.new_empty((batch, nheads, hd))
@@ -204,7 +223,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         if ws is None:  # only the arrival counters at its start have to be zero
             ws = torch.empty(need, device=q.device, dtype=torch.uint8)
             ws[:4 * _lib.SN_PAGED_DECODE_COUNTERS].zero_()
-        call("sn_paged_decode_attention", q.data_ptr(), qb, qh, *args, out.data_ptr(),
+        call(fn, q.data_ptr(), qb, qh, *args, *extra, out.data_ptr(),
              lse.data_ptr() if return_lse else None, hd ** -0.5 if scale is None else float(scale), batch, nheads, hkv,
              hd, ws.data_ptr(), need, st)
         return (out, lse) if return_lse else out
