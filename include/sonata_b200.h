@@ -641,8 +641,9 @@ int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_by
  *   max over the head's query heads of sum_d max(q_d least_d, q_d greatest_d),
  * the lowest blocks among equal ones, all of them if there are no more than
  * count; -1 behind.  Scores are sums of exact products in 64 bits; a block with
- * a bound that is not finite is above the others.  head_dim <= 512, max_pages
- * <= 180216.
+ * a bound that is not finite is above the others.  workspace:
+ * sn_select_blocks_workspace_size bytes, 16-byte aligned, whatever they hold.
+ * max_pages <= 262144.
  *
  * sn_paged_sparse_attention: sn_paged_decode_attention over the positions of
  * listed blocks only: of blocks int32 [batch, nheads_kv, count] the first
@@ -674,10 +675,11 @@ int sn_update_page_bounds(const void *k_pages, int64_t k_page_stride, int64_t k_
                           int num_pages, int page_size, const int *page_table, int64_t table_stride, int max_pages,
                           const int *seq_lens, const int *cu_seqlens, int batch, int nheads_kv, int head_dim,
                           void *bounds, void *stream);
+size_t sn_select_blocks_workspace_size(int batch, int nheads_kv, int max_pages);
 int sn_select_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *bounds, int num_pages,
                      int page_size, const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens,
                      int batch, int nheads, int nheads_kv, int head_dim, int count, int first, int last, int *blocks,
-                     void *stream);
+                     void *workspace, size_t workspace_bytes, void *stream);
 int sn_paged_sparse_attention(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_pages,
                               int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
                               const void *v_pages, int64_t v_page_stride, int64_t v_head_stride,

@@ -28,6 +28,13 @@ struct Abi {  // of the loaded libsonata_b200.so, set by bind()
   decltype(&sn_copy_pages) copy;
   decltype(&sn_mamba2_prompt) prompt;
   decltype(&sn_mamba2_prompt_workspace_size) prompt_size;
+  decltype(&sn_paged_decode_attention_mass) mass;
+  decltype(&sn_paged_mass_workspace_size) mass_size;
+  decltype(&sn_evict_positions) evict;
+  decltype(&sn_update_page_bounds) bounds;
+  decltype(&sn_select_blocks) select;
+  decltype(&sn_select_blocks_workspace_size) select_size;
+  decltype(&sn_paged_sparse_attention) sparse;
 } abi;
 
 using at::Tensor;
@@ -88,30 +95,184 @@ struct Pages {
 
 PyObject* status(int rc) { return PyLong_FromLong(rc); }
 
+// One token a stream: q, pages, scale and workspace as all forms of the attention take them.
+struct Attend {
+  const Tensor *q, *ws;
+  Pages p;
+  int64_t batch, heads;
+  size_t need;  // workspace bytes
+  float scale;
+  bool read(PyObject* const* a, PyObject* scale_arg, PyObject* ws_arg, int dev) {
+    q = tensor(a[0]);
+    ws = tensor(ws_arg);
+    if (!is(q, at::kBFloat16, 3, dev) || !p.read(a + 1, dev) || !is(ws, at::kByte, 1, dev) || !ws->is_contiguous() ||
+        !(scale_arg == Py_None || PyFloat_CheckExact(scale_arg)))
+      return false;
+    batch = q->size(0), heads = q->size(1);
+    if (batch != p.streams || q->size(2) != p.hd || (q->stride(2) != 1 && p.hd > 1) || heads < 1 || heads % p.heads || batch > INT32_MAX)
+      return false;
+    scale = scale_arg == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(p.hd)))
+                                 : static_cast<float>(PyFloat_AS_DOUBLE(scale_arg));
+    return true;
+  }
+  bool room(size_t n) {
+    need = n;
+    return n > 0 && static_cast<size_t>(ws->numel()) >= n && reinterpret_cast<uintptr_t>(ws->data_ptr()) % 16 == 0;
+  }
+  // f with the form's own arguments after the lengths, the output's, and the common end.
+  template <typename F, typename... Own>
+  PyObject* launch(F f, int dev, Own... own) {
+    Tensor out = at::empty({batch, heads, p.hd}, q->options());
+    const int rc = f(q->data_ptr(), q->stride(0), q->stride(1), p.k->data_ptr(), p.stride(p.k, 0), p.stride(p.k, 1),
+                     p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1), p.stride(p.v, 2),
+                     static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(), p.table_stride(),
+                     static_cast<int>(p.width), p.lens->data_ptr<int>(), own..., out.data_ptr(), nullptr, scale,
+                     static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(p.heads), static_cast<int>(p.hd),
+                     ws->data_ptr(), need, current_stream(dev));
+    return rc ? status(rc) : THPVariable_Wrap(std::move(out));
+  }
+};
+
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || a[7] != Py_False) Py_RETURN_NONE;
+  const int dev = current_device();
+  Attend t;
+  if (!t.read(a, a[5], a[6], dev) ||
+      !t.room(abi.attend_size(static_cast<int>(t.batch), static_cast<int>(t.heads), static_cast<int>(t.p.hd))))
+    Py_RETURN_NONE;
+  return t.launch(abi.attend, dev);
+  END_HANDLE_TH_ERRORS
+}
+
+// Accumulated weights [.., >= room] with a dense last axis and no overlaps.
+bool mass_ok(const Tensor* m, int64_t dim, int64_t room, int dev) {
+  if (!is(m, at::kFloat, dim, dev) || m->size(dim - 1) < room || m->stride(dim - 1) != 1) return false;
+  for (int64_t i = 0; i + 1 < dim; ++i)
+    if (m->stride(i) < (m->size(i) > 1 ? room : 0)) return false;
+  return true;
+}
+
+PyObject* mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || a[8] != Py_False) Py_RETURN_NONE;
+  const int dev = current_device();
+  const Tensor* m = tensor(a[5]);
+  Attend t;
+  if (!t.read(a, a[6], a[7], dev) || !mass_ok(m, 3, t.p.width * t.p.page, dev) || m->size(0) != t.batch || m->size(1) != t.p.heads ||
+      !t.room(abi.mass_size(static_cast<int>(t.batch), static_cast<int>(t.heads), static_cast<int>(t.p.heads),
+                            static_cast<int>(t.p.hd), t.p.width * t.p.page)))
+    Py_RETURN_NONE;
+  return t.launch(abi.mass, dev, m->data_ptr<float>(), m->stride(0), m->stride(1));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || a[8] != Py_False) Py_RETURN_NONE;
+  const int dev = current_device();
+  const Tensor* blocks = tensor(a[5]);
+  Attend t;
+  if (!is(blocks, at::kInt, 3, dev) || !blocks->is_contiguous() || !t.read(a, a[6], a[7], dev) || blocks->size(0) != t.batch ||
+      blocks->size(1) != t.p.heads || blocks->size(2) < 1 || blocks->size(2) > INT32_MAX ||
+      !t.room(abi.attend_size(static_cast<int>(t.batch), static_cast<int>(t.heads), static_cast<int>(t.p.hd))))
+    Py_RETURN_NONE;
+  return t.launch(abi.sparse, dev, blocks->data_ptr<int>(), static_cast<int>(blocks->size(2)));
+  END_HANDLE_TH_ERRORS
+}
+
+// A page table and its streams' lengths.
+struct Table {
+  const Tensor *table, *lens;
+  int64_t streams, width;
+  bool read(PyObject* const* a, int dev) {
+    table = tensor(a[0]);
+    lens = tensor(a[1]);
+    if (!is(table, at::kInt, 2, dev) || !is(lens, at::kInt, 1, dev)) return false;
+    streams = table->size(0), width = table->size(1);
+    return streams > 0 && width > 0 && streams <= INT32_MAX && width <= INT32_MAX && (table->stride(1) == 1 || width == 1) &&
+           lens->size(0) == streams && lens->is_contiguous();
+  }
+  int64_t stride() const { return streams > 1 ? table->stride(0) : width; }
+};
+
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !PyBool_Check(a[7])) Py_RETURN_NONE;
+  const int dev = current_device();
+  const Tensor *pool = tensor(a[0]), *m = tensor(a[3]);
+  Table t;
+  int keep, recent, sinks;
+  if (!is(pool, at::kBFloat16, 6, dev) || !pool->is_contiguous() || pool->numel() == 0 || pool->size(1) != 2 || !t.read(a + 1, dev) ||
+      !number(a[4], &keep) || !number(a[5], &recent) || !number(a[6], &sinks) || keep < 1 || recent < 0 || sinks < 0 ||
+      recent > keep || sinks > keep - recent)
+    Py_RETURN_NONE;
+  const int64_t layers = pool->size(0), pages = pool->size(2), heads = pool->size(3), page = pool->size(4), hd = pool->size(5);
+  if (layers > INT32_MAX || pages > INT32_MAX || heads > INT32_MAX || page > INT32_MAX || hd > INT32_MAX ||
+      !mass_ok(m, 4, t.width * page, dev) || m->size(0) != layers || m->size(1) != t.streams || m->size(2) != heads)
+    Py_RETURN_NONE;
+  Tensor source;
+  if (a[7] == Py_True) source = at::empty({layers, t.streams, heads, keep}, pool->options().dtype(at::kInt));
+  const int rc = abi.evict(pool->data_ptr(), static_cast<int>(layers), static_cast<int>(pages), static_cast<int>(page),
+                           static_cast<int>(heads), static_cast<int>(hd), t.table->data_ptr<int>(), t.stride(),
+                           static_cast<int>(t.width), t.lens->data_ptr<int>(), m->data_ptr<float>(), m->stride(0), m->stride(1),
+                           m->stride(2), static_cast<int>(t.streams), keep, recent, sinks,
+                           source.defined() ? source.data_ptr<int>() : nullptr, current_stream(dev));
+  if (rc) return status(rc);
+  if (source.defined()) return THPVariable_Wrap(std::move(source));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+bool bounds_ok(const Tensor* b, int dev) {
+  return is(b, at::kBFloat16, 4, dev) && b->is_contiguous() && b->numel() > 0 && b->size(2) == 2 && b->size(0) <= INT32_MAX;
+}
+
+PyObject* bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) Py_RETURN_NONE;
+  const int dev = current_device();
+  const Tensor *k = tensor(a[0]), *b = tensor(a[1]), *cu;
+  Table t;
+  if (!is(k, at::kBFloat16, 4, dev) || k->numel() == 0 || k->stride(3) != 1 || !bounds_ok(b, dev) || !t.read(a + 2, dev) ||
+      !dense_or_none(a[4], &cu, at::kInt, {t.streams + 1}, dev))
+    Py_RETURN_NONE;
+  const int64_t pages = k->size(0), heads = k->size(1), page = k->size(2), hd = k->size(3);
+  if (b->size(0) != pages || b->size(1) != heads || b->size(3) != hd || heads > INT32_MAX || page > INT32_MAX || hd > INT32_MAX)
+    Py_RETURN_NONE;
+  auto stride = [&](int axis) { return k->size(axis) > 1 ? k->stride(axis) : std::max(k->stride(axis), hd); };
+  const int rc = abi.bounds(k->data_ptr(), stride(0), stride(1), stride(2), static_cast<int>(pages), static_cast<int>(page),
+                            t.table->data_ptr<int>(), t.stride(), static_cast<int>(t.width), t.lens->data_ptr<int>(),
+                            cu ? cu->data_ptr<int>() : nullptr, static_cast<int>(t.streams), static_cast<int>(heads),
+                            static_cast<int>(hd), b->data_ptr(), current_stream(dev));
+  if (rc) return status(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 8) Py_RETURN_NONE;
   const int dev = current_device();
-  const Tensor *q = tensor(a[0]), *ws = tensor(a[6]);
-  Pages p;
-  if (!is(q, at::kBFloat16, 3, dev) || !p.read(a + 1, dev) || !is(ws, at::kByte, 1, dev) || !ws->is_contiguous() ||
-      !(a[5] == Py_None || PyFloat_CheckExact(a[5])) || a[7] != Py_False)
+  const Tensor *q = tensor(a[0]), *b = tensor(a[1]);
+  Table t;
+  int page, count, first, last;
+  if (!is(q, at::kBFloat16, 3, dev) || !bounds_ok(b, dev) || !t.read(a + 2, dev) || !number(a[4], &page) || !number(a[5], &count) ||
+      !number(a[6], &first) || !number(a[7], &last) || page < 1 || count < 1 || first < 0 || last < 0 || first > count ||
+      last > count - first)
     Py_RETURN_NONE;
-  const int64_t batch = q->size(0), heads = q->size(1);
-  if (batch != p.streams || q->size(2) != p.hd || q->stride(2) != 1 || heads < 1 || heads % p.heads || batch > INT32_MAX)
+  const int64_t batch = q->size(0), heads = q->size(1), hd = q->size(2), hkv = b->size(1);
+  if (batch != t.streams || hd != b->size(3) || heads < 1 || heads % hkv || heads > INT32_MAX || hd > INT32_MAX ||
+      (q->stride(2) != 1 && hd > 1))
     Py_RETURN_NONE;
-  const size_t need = abi.attend_size(static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(p.hd));
-  if (static_cast<size_t>(ws->numel()) < need || reinterpret_cast<uintptr_t>(ws->data_ptr()) % 16) Py_RETURN_NONE;
-  const float scale = a[5] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(p.hd)))
-                                      : static_cast<float>(PyFloat_AS_DOUBLE(a[5]));
-  Tensor out = at::empty({batch, heads, p.hd}, q->options());
-  const int rc = abi.attend(q->data_ptr(), q->stride(0), q->stride(1), p.k->data_ptr(), p.stride(p.k, 0), p.stride(p.k, 1),
-                            p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1), p.stride(p.v, 2),
-                            static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(), p.table_stride(),
-                            static_cast<int>(p.width), p.lens->data_ptr<int>(), out.data_ptr(), nullptr, scale,
-                            static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(p.heads),
-                            static_cast<int>(p.hd), ws->data_ptr(), need, current_stream(dev));
-  return rc ? status(rc) : THPVariable_Wrap(std::move(out));
+  Tensor blocks = at::empty({batch, hkv, count}, t.table->options());
+  const size_t need = abi.select_size(static_cast<int>(batch), static_cast<int>(hkv), static_cast<int>(t.width));
+  Tensor ws = at::empty({static_cast<int64_t>(need)}, t.table->options().dtype(at::kByte));
+  const int rc = abi.select(q->data_ptr(), q->stride(0), q->stride(1), b->data_ptr(), static_cast<int>(b->size(0)), page,
+                            t.table->data_ptr<int>(), t.stride(), static_cast<int>(t.width), t.lens->data_ptr<int>(),
+                            static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(hkv), static_cast<int>(hd), count,
+                            first, last, blocks.data_ptr<int>(), ws.data_ptr(), need, current_stream(dev));
+  return rc ? status(rc) : THPVariable_Wrap(std::move(blocks));
   END_HANDLE_TH_ERRORS
 }
 
@@ -210,13 +371,18 @@ PyObject* bind(PyObject*, PyObject* table) {
   };
   if (!get("sn_paged_decode_attention", abi.attend) || !get("sn_paged_decode_workspace_size", abi.attend_size) ||
       !get("sn_rotary_paged_append", abi.append) || !get("sn_copy_pages", abi.copy) ||
-      !get("sn_mamba2_prompt", abi.prompt) || !get("sn_mamba2_prompt_workspace_size", abi.prompt_size))
+      !get("sn_mamba2_prompt", abi.prompt) || !get("sn_mamba2_prompt_workspace_size", abi.prompt_size) ||
+      !get("sn_paged_decode_attention_mass", abi.mass) || !get("sn_paged_mass_workspace_size", abi.mass_size) ||
+      !get("sn_evict_positions", abi.evict) || !get("sn_update_page_bounds", abi.bounds) ||
+      !get("sn_select_blocks", abi.select) ||
+      !get("sn_select_blocks_workspace_size", abi.select_size) || !get("sn_paged_sparse_attention", abi.sparse))
     return nullptr;
   Py_RETURN_NONE;
 }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"attend", FAST(attend)}, {"append", FAST(append)}, {"copy", FAST(copy)}, {"prompt", FAST(prompt)},
+                         {"mass", FAST(mass)}, {"evict", FAST(evict)}, {"bounds", FAST(bounds)}, {"select", FAST(select)}, {"sparse", FAST(sparse)},
                          {"bind", bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

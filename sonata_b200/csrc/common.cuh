@@ -52,9 +52,9 @@ int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStr
   return SN_OK;
 }
 
-// Lets `Kern` have `bytes` of dynamic shared memory on the current device; asked of the runtime once a device.
-template <auto Kern>
-bool smem_room(int bytes) {
+// Sets an attribute of `Kern` on the current device; asked of the runtime once a device.
+template <auto Kern, cudaFuncAttribute attr>
+bool kernel_attribute(int value) {
   static bool done[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -62,13 +62,19 @@ bool smem_room(int bytes) {
     return false;
   }
   if (dev >= 0 && dev < 64 && done[dev]) return true;
-  if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+  if (cudaFuncSetAttribute(Kern, attr, value) != cudaSuccess) {
     cudaGetLastError();
     return false;
   }
   if (dev >= 0 && dev < 64) done[dev] = true;
   return true;
 }
+// Lets `Kern` have `bytes` of dynamic shared memory.
+template <auto Kern>
+bool smem_room(int bytes) { return kernel_attribute<Kern, cudaFuncAttributeMaxDynamicSharedMemorySize>(bytes); }
+// Lets `Kern` be launched in clusters of up to 16 CTAs.
+template <auto Kern>
+bool large_clusters() { return kernel_attribute<Kern, cudaFuncAttributeNonPortableClusterSizeAllowed>(1); }
 
 // ---------------------------------------------------------------------------
 // device helpers

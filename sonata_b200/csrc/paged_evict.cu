@@ -18,6 +18,9 @@
 namespace sn {
 namespace {
 
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictCluster = 8;  // CTAs a row at most
+
 struct EvictParams {
   char* pool;  // [layers, 2, num_pages, hkv, page_size] rows of row_bytes, dense
   int64_t layer_bytes, kv_bytes, page_bytes, head_bytes;
@@ -39,10 +42,10 @@ struct EvictParams {
 // flight.  The recent rows may overlap their places: they are read, the
 // cluster waits, they are written.
 template <typename T, int NU>  // units of T in a position's two rows, 0: 2 * row_bytes / sizeof(T)
-__global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams p) {
   constexpr int U = 8;  // units in flight a lane
   extern __shared__ uint32_t s_keys[];  // [part], then the bits [part / 32]
-  __shared__ SelectShared s_sel;
+  __shared__ SelectShared<kEvictThreads> s_sel;
   __shared__ uint32_t s_n, s_count[2];
   pdl_launch_dependents();
   pdl_wait();
@@ -59,7 +62,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
   int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
   if (n <= keep) {
     if (source)
-      for (int i = rank * kSelThreads + tid; i < keep; i += C * kSelThreads) source[i] = i < n ? i : -1;
+      for (int i = rank * kEvictThreads + tid; i < keep; i += C * kEvictThreads) source[i] = i < n ? i : -1;
     cluster_bar(C);  // nobody leaves while its n may be read
     return;
   }
@@ -72,12 +75,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
   const int i0 = min(rank * each, c), i1 = min(i0 + each, c), len = i1 - i0;
   uint32_t nholes = 0, nmovers = 0;  // in this CTA
   if (m > 0) {
-    for (int i = tid; i < len; i += kSelThreads) s_keys[i] = order_key(mass[sinks + i0 + i]);
+    for (int i = tid; i < len; i += kEvictThreads) s_keys[i] = order_key(mass[sinks + i0 + i]);
     __syncthreads();
     const Cutoff<uint32_t> cut = find_cutoff(s_keys, len, static_cast<uint32_t>(m), s_sel, C, rank);
     choose(s_keys, len, cut, s_bits, s_sel);
     __syncthreads();  // the keys are done with: the lists go over them, holes from the front, movers from the back
-    const int words = (len + 31) / 32, per = (words + kSelWarps - 1) / kSelWarps;
+    const int words = (len + 31) / 32, per = (words + kEvictWarps - 1) / kEvictWarps;
     const int w0 = min(warp * per, words), w1 = min(w0 + per, words);
     auto split = [&](int w, uint32_t& hole, uint32_t& mover) {  // of word w's candidates
       const int at = sinks + i0 + 32 * w, there = min(32, len - 32 * w);
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
     }
     __syncthreads();
     uint32_t ah = 0, am = 0;
-    for (int v = 0; v < kSelWarps; ++v) {
+    for (int v = 0; v < kEvictWarps; ++v) {
       if (v == warp) {
         ah = nholes;
         am = nmovers;
@@ -121,7 +124,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
     }
   }
   if (source)
-    for (int i = rank * kSelThreads + tid; i < sinks; i += C * kSelThreads) source[i] = i;
+    for (int i = rank * kEvictThreads + tid; i < sinks; i += C * kEvictThreads) source[i] = i;
   if (tid == 0) {
     s_count[0] = nholes;
     s_count[1] = nmovers;
@@ -139,17 +142,17 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
     }
     return pg * p.page_bytes + static_cast<int64_t>(at - blk * p.map.page_size) * p.row_bytes;
   };
-  const int wid = warp * C + rank, warps = kSelWarps * C;
+  const int wid = warp * C + rank, warps = kEvictWarps * C;
 
   // ---- movers into holes ----
-  int hole_at[kClusterMost + 1], mover_at[kClusterMost + 1];  // the CTAs' first places in the lists
+  int hole_at[kEvictCluster + 1], mover_at[kEvictCluster + 1];  // the CTAs' first places in the lists
   hole_at[0] = mover_at[0] = 0;
 #pragma unroll
-  for (int r = 0; r < kClusterMost; ++r) {
+  for (int r = 0; r < kEvictCluster; ++r) {
     hole_at[r + 1] = hole_at[r] + (r < C ? static_cast<int>(peer_u32(&s_count[0], r)) : 0);
     mover_at[r + 1] = mover_at[r] + (r < C ? static_cast<int>(peer_u32(&s_count[1], r)) : 0);
   }
-  const int pairs = min(hole_at[kClusterMost], mover_at[kClusterMost]);  // they are equal
+  const int pairs = min(hole_at[kEvictCluster], mover_at[kEvictCluster]);  // they are equal
   const int batch = min(32, (pairs + warps - 1) / warps);
   for (int first = wid * batch; first < pairs; first += warps * batch) {
     const int cnt = min(batch, pairs - first);
@@ -158,7 +161,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
       const int i = first + lane;
       int rh = 0, rm = 0, oh = 0, om = 0;
 #pragma unroll
-      for (int r = 1; r < kClusterMost; ++r) {
+      for (int r = 1; r < kEvictCluster; ++r) {
         if (i >= hole_at[r]) rh = r, oh = hole_at[r];
         if (i >= mover_at[r]) rm = r, om = mover_at[r];
       }
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_kernel(const EvictParams p)
     }
   }
   cluster_bar(C);
-  for (int i = keep + rank * kSelThreads + tid; i < n; i += C * kSelThreads) mass[i] = 0.f;
+  for (int i = keep + rank * kEvictThreads + tid; i < n; i += C * kEvictThreads) mass[i] = 0.f;
 }
 
 constexpr int kPartMost = 49152;  // candidates a CTA holds (200 KB)
@@ -244,7 +247,7 @@ int launch_evict(int rows, int C, cudaStream_t st, const EvictParams& p) {
   if (!smem_room<evict_kernel<T, NU>>((kPartMost + kPartMost / 32) * 4)) return SN_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * C);
-  cfg.blockDim = dim3(kSelThreads);
+  cfg.blockDim = dim3(kEvictThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -283,8 +286,8 @@ extern "C" int sn_evict_positions(void* pool, int layers, int num_pages, int pag
       (layers > 1 && mass_layer_stride < room))
     return SN_ERR_INVALID_ARGUMENT;
   const int64_t rows = static_cast<int64_t>(layers) * batch * nheads_kv;
-  if (rows > INT32_MAX / sn::kClusterMost || head_dim > 8192 ||
-      room > static_cast<int64_t>(sn::kClusterMost) * (sn::kPartMost - 4))
+  if (rows > INT32_MAX / sn::kEvictCluster || head_dim > 8192 ||
+      room > static_cast<int64_t>(sn::kEvictCluster) * (sn::kPartMost - 4))
     return SN_ERR_UNSUPPORTED;
   sn::EvictParams p;
   p.pool = static_cast<char*>(pool);
@@ -307,7 +310,7 @@ extern "C" int sn_evict_positions(void* pool, int layers, int num_pages, int pag
   p.sinks = sinks;
   // CTAs a row: as many as the shared memory asks for, and more where there are few long rows
   int C = 1;
-  while (C < sn::kClusterMost && (room > static_cast<int64_t>(C) * (sn::kPartMost - 4) ||
+  while (C < sn::kEvictCluster && (room > static_cast<int64_t>(C) * (sn::kPartMost - 4) ||
                                   (rows * C < 2 * sn::sm_count() && room > 1024 * C)))
     C *= 2;
   p.part = static_cast<int>((room + C - 1) / C + 4);

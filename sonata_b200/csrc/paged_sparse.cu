@@ -148,21 +148,37 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 
 // ---------------------------------------------------------------------------
 // select_blocks.  For each (stream, key/value head) the score of a block is
-// the greatest over the head's query heads of sum_d max(q_d least_d, q_d
-// greatest_d); the first `first` and last `last` blocks and the highest
-// scores of the others are listed in ascending order, -1 behind.  The products
-// of two bf16 values are exact, and they are added up in 64 bits, so the choice
-// does not depend on the order of the sum.  One cluster a (stream, head), the
-// scores' keys in its shared memory.
+// the greatest over the head's query heads of
+//   sum_d max(q_d least_d, q_d greatest_d) = sum_d min(q_d, 0) least_d + max(q_d, 0) greatest_d;
+// the first `first` and last `last` blocks and the highest scores of the others
+// are listed in ascending order, -1 behind.  The products of two bf16 values are
+// exact, and scores are compared as their sums in 64 bits, so the choice does
+// not depend on the order of a sum; a block with a bound that is not finite
+// ranks above all.
 //
-// Four lanes take a block: lane t the 16-byte pieces t, t + 4, ... of both rows.
-// max(q l, q g) = q (q < 0 ? l : g), one 64-bit multiply-add.  A bf16 value's
-// bits, moved into the upper word of a double, are that value times 2^-896,
-// zeros and subnormals too; q is multiplied by 2^800 for it, which leaves the
-// order as it is.  A block with a bound that is not finite ranks above all.
+// Sums of all blocks in 64 bits would be bound by the conversions and by shared
+// memory (3 streams of up to 100001 positions, pages of 16: 66 us where reading
+// the bounds takes 5), and all but a few of the blocks do not need them:
+// * The tensor cores give every sum in 32 bits, s, and the sum of its terms'
+//   absolute values, at most S over a row's blocks.  |s - score| < E = 2^-13 S +
+//   2^-110: 256 terms at most go in by 16, each such sum of 17 is off by less
+//   than 17 units in the 22nd bit of its largest term, 272 2^-22 S in all; and
+//   products under 2^-126 may count as 0.
+// * One histogram of s over their range finds the bin of the last one that would
+//   be chosen.  Blocks whose s is more than 2 E above that bin are chosen, more
+//   than 2 E below it are not: their scores lie on the same side of the last
+//   chosen one's.  The few between get their sums in 64 bits and are ranked, by
+//   comparing all of them.
+// Two launches: scores, spread evenly over the device and bound by reading the
+// bounds, and choices, a CTA a row, bound by the chain of its steps.  In one
+// launch, a cluster of 8 CTAs a row with the scores in shared memory, exchanges
+// of a few kilobytes between the CTAs took 2 to 3 us each (22 us for the three
+// streams).
 // ---------------------------------------------------------------------------
-constexpr int kSelHeads = 4;      // query heads at a time
-constexpr int kSelMost = 22528;   // blocks a CTA's shared memory holds the keys of (180 KB)
+constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
+constexpr int kChooseHeld = 16;     // keys a thread holds
+constexpr int kFewExact = 64;        // blocks that are ranked by comparing all of them
+constexpr int kChooseMost = 262144;  // blocks of a stream: three bits each in shared memory
 
 struct SelectParams {
   const __nv_bfloat16* q;
@@ -170,163 +186,352 @@ struct SelectParams {
   const __nv_bfloat16* bounds;
   PageMap map;
   const int* seq_lens;
-  int* blocks;  // [batch, hkv, count]
+  int* blocks;      // [batch, hkv, count]
+  uint2* scores;    // [batch, hkv, max_pages]: key of s, sum of absolute values; of the blocks that are not first or last
+  uint64_t* exact;  // the same blocks' keys of sums in 64 bits, where they are needed
   int batch, hq, hkv, hd, count, first, last;
-  int part;  // keys a CTA holds
 };
 
-// kVec: pieces of 8 elements are 16-byte loads (head_dim a multiple of 8).
-template <bool kVec>
-__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) unsigned char s_raw[];
-  uint64_t* const s_keys = reinterpret_cast<uint64_t*>(s_raw);                   // [part]
-  uint32_t* const s_bits = reinterpret_cast<uint32_t*>(s_keys + p.part);         // [part / 32], even
-  __shared__ SelectShared s_sel;
-  __shared__ uint32_t s_n, s_count;
-  const int pieces = (p.hd + 7) / 8;
-  double* const s_q = reinterpret_cast<double*>(s_bits + (p.part / 32 + 3) / 2 * 2);  // [kSelHeads][8 pieces]
+// Blocks of a stream, and those that are compared: first .. first + compared - 1.
+__device__ __forceinline__ int stream_blocks(const SelectParams& p, int b, int& compared) {
+  const int64_t n = length_of(p.map, p.seq_lens, b);
+  const int nb = static_cast<int>((n + p.map.page_size - 1) / p.map.page_size);
+  compared = nb <= p.count || p.first + p.last == p.count ? 0 : nb - p.first - p.last;
+  return nb;
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Scores in 32 bits.  A warp takes 16 blocks at a time, their bounds straight from memory as operands: the contraction index
+// may be permuted as long as both sides agree, so lane (g, t) takes the 16-byte chunks t, t + 4, ... of blocks g and g + 8,
+// and of query head g.  blockIdx.y is the row, blockIdx.x takes groups of 64 blocks, gridDim.x of them apart.
+template <int HD>
+__global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams p) {
+  constexpr int KC = HD / 32;  // chunks a lane takes of a row
   pdl_launch_dependents();
   pdl_wait();
-  uint32_t nranks;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nranks));
-  const int C = static_cast<int>(nranks), rank = static_cast<int>(ctarank());
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  for (int row = blockIdx.y; row < p.batch * p.hkv; row += gridDim.y) {
+    const int b = row / p.hkv, hk = row - b * p.hkv, group = p.hq / p.hkv;
+    uint2* const out = p.scores + static_cast<int64_t>(row) * p.map.max_pages;
+    const int start = blockIdx.x * 64 + (threadIdx.x >> 5) * 16, stride = gridDim.x * 64;
+    auto page = [&](int i) { return page_of(p.map, b, p.first + i); };  // of the table's entries past the stream's end, too
+    for (int h0 = 0; h0 < group; h0 += 8) {
+      int i = start;
+      int pg0 = page(i + g), pg1 = page(i + g + 8);
+      int len;
+      stream_blocks(p, b, len);
+      uint4 qn[KC], qp[KC];  // the negative and the positive part of head g
+      const __nv_bfloat16* q = p.q + b * p.qb + static_cast<int64_t>(hk * group + h0 + g) * p.qh;
+#pragma unroll
+      for (int k = 0; k < KC; ++k) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (h0 + g < group) {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(q + 8 * (t + 4 * k));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = e[2 * j] | static_cast<uint32_t>(e[2 * j + 1]) << 16;
+        }
+        qn[k] = make_uint4(min2(w[0], 0), min2(w[1], 0), min2(w[2], 0), min2(w[3], 0));
+        qp[k] = make_uint4(max2(w[0], 0), max2(w[1], 0), max2(w[2], 0), max2(w[3], 0));
+      }
+      for (; i < len; i += stride) {
+        const __nv_bfloat16* r0 = p.bounds + (static_cast<int64_t>(max(pg0, 0)) * p.hkv + hk) * 2 * HD + 8 * t;
+        const __nv_bfloat16* r1 = p.bounds + (static_cast<int64_t>(max(pg1, 0)) * p.hkv + hk) * 2 * HD + 8 * t;
+        uint4 a0[2 * KC], a1[2 * KC];  // chunks of the least and of the greatest keys
+#pragma unroll
+        for (int k = 0; k < 2 * KC; ++k) {
+          a0[k] = *reinterpret_cast<const uint4*>(r0 + 32 * k);
+          a1[k] = *reinterpret_cast<const uint4*>(r1 + 32 * k);
+        }
+        const bool ok0 = pg0 >= 0, ok1 = pg1 >= 0;
+        if ((i + g < len && !ok0) || (i + g + 8 < len && !ok1)) record_status(SN_ERR_INVALID_ARGUMENT);
+        pg0 = page(i + stride + g);
+        pg1 = page(i + stride + g + 8);
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+        constexpr uint32_t kAbs = 0x7fff7fffu;
+#pragma unroll
+        for (int k = 0; k < 2 * KC; ++k) {
+          const uint4 q4 = k < KC ? qn[k % KC] : qp[k % KC], x = a0[k], y = a1[k];
+          mma_bf16(s, x.x, y.x, x.y, y.y, q4.x, q4.y);
+          mma_bf16(s, x.z, y.z, x.w, y.w, q4.z, q4.w);
+          mma_bf16(m, x.x & kAbs, y.x & kAbs, x.y & kAbs, y.y & kAbs, q4.x & kAbs, q4.y & kAbs);
+          mma_bf16(m, x.z & kAbs, y.z & kAbs, x.w & kAbs, y.w & kAbs, q4.z & kAbs, q4.w & kAbs);
+        }
+        // heads 2t and 2t + 1 of blocks g and g + 8; an absolute sum that is not finite is infinite
+        const bool two = h0 + 2 * t + 1 < group, one = h0 + 2 * t < group;
+        auto wide = [](float x) { return x < INFINITY ? x : INFINITY; };
+        float v0 = one ? s[0] : -INFINITY, v1 = one ? s[2] : -INFINITY;
+        float m0 = fmaxf(wide(m[0]), wide(m[1])), m1 = fmaxf(wide(m[2]), wide(m[3]));
+        if (two) v0 = fmaxf(v0, s[1]), v1 = fmaxf(v1, s[3]);
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+          v0 = fmaxf(v0, __shfl_xor_sync(0xffffffffu, v0, o));
+          v1 = fmaxf(v1, __shfl_xor_sync(0xffffffffu, v1, o));
+          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        }
+        const int at = i + g + 8 * t;
+        if (t < 2 && at < len) {
+          uint2 v = (t ? ok1 : ok0) ? make_uint2(order_key(t ? v1 : v0), __float_as_uint(t ? m1 : m0)) : make_uint2(0, 0);
+          if (h0 > 0) {
+            const uint2 before = out[at];  // this lane's own
+            v = make_uint2(max(v.x, before.x), max(v.y, before.y));
+          }
+          out[at] = v;
+        }
+      }
+    }
+  }
+}
+
+// The key of one block's score in 64 bits; a warp.
+__device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, int hk, int block) {
+  const int lane = threadIdx.x & 31, group = p.hq / p.hkv;
+  const int pg = page_of(p.map, b, block);
+  if (pg < 0) return 0;
+  const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(pg) * p.hkv + hk) * 2 * p.hd;
+  const __nv_bfloat16* q = p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh;
+  uint64_t best = 0;
+  bool odd = false;
+  for (int h0 = 0; h0 < group; h0 += 4) {  // four heads at a time: a chain of loads and shuffles each
+    double sum[4] = {0., 0., 0., 0.};
+#pragma unroll 4
+    for (int d = lane; d < p.hd; d += 32) {
+      const float l = __bfloat162float(lo[d]), g = __bfloat162float(lo[p.hd + d]);
+      odd |= !(fabsf(l) < INFINITY) || !(fabsf(g) < INFINITY);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float v = __bfloat162float(q[min(h0 + h, group - 1) * p.qh + d]);
+        sum[h] = fma(static_cast<double>(v), static_cast<double>(v < 0.f ? l : g), sum[h]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) best = max(best, order_key(sum[h]));
+  }
+  return __any_sync(0xffffffffu, odd) ? ~0ull : best;
+}
+
+// Scores in 64 bits of all blocks, a warp a block: any head_dim and alignment.
+__global__ void __launch_bounds__(128) exact_scores_kernel(const SelectParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int row = blockIdx.y; row < p.batch * p.hkv; row += gridDim.y) {
+    const int b = row / p.hkv, hk = row - b * p.hkv;
+    int len;
+    stream_blocks(p, b, len);
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 5); i < len; i += gridDim.x * 4) {
+      const uint64_t key = exact_score(p, b, hk, p.first + i);
+      if ((threadIdx.x & 31) == 0) {
+        p.exact[static_cast<int64_t>(row) * p.map.max_pages + i] = key;
+        if (page_of(p.map, b, p.first + i) < 0) record_status(SN_ERR_INVALID_ARGUMENT);
+      }
+    }
+  }
+}
+
+// One CTA a row; kScored: block_scores_kernel has run, else exact_scores_kernel.
+template <bool kScored>
+__global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const SelectParams p) {
+  extern __shared__ uint32_t s_bits[];
+  __shared__ SelectShared<kChooseThreads> s_sel;
+  __shared__ uint32_t s_range[3];  // least and greatest key, S
+  __shared__ uint64_t s_few[kFewExact];
+  __shared__ int s_few_at[kFewExact];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / C, b = row / p.hkv, hk = row % p.hkv;
-  if (tid == 0) s_n = length_of(p.map, p.seq_lens, b);
-  cluster_bar(C);
-  const int n = static_cast<int>(peer_u32(&s_n, 0));
-  const int nb = static_cast<int>((static_cast<int64_t>(n) + p.map.page_size - 1) / p.map.page_size);
+  const uint32_t below = (1u << lane) - 1;
+  const int row = blockIdx.x, b = row / p.hkv, hk = row - b * p.hkv;
+  if (tid < 3) s_range[tid] = tid == 0 ? 0xffffffffu : 0;
+  constexpr int Q = SelectShared<kChooseThreads>::kQuads;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) s_sel.hist[0][Q * tid + q] = make_uint4(0, 0, 0, 0);
+  pdl_launch_dependents();
+  pdl_wait();
   int* const out = p.blocks + static_cast<int64_t>(row) * p.count;
-  if (nb <= p.count) {
-    for (int i = rank * kSelThreads + tid; i < p.count; i += C * kSelThreads) out[i] = i < nb ? i : -1;
-    cluster_bar(C);
+  int len;
+  const int nb = stream_blocks(p, b, len), need = p.count - p.first - p.last;
+  if (len == 0) {  // all of a short stream's blocks, or none but the first and the last
+    for (int i = tid; i < p.count; i += kChooseThreads) out[i] = nb <= p.count ? (i < nb ? i : -1) : i < p.first ? i : nb - p.count + i;
     return;
   }
-  for (int i = rank * kSelThreads + tid; i < p.first + p.last; i += C * kSelThreads) {
+  for (int i = tid; i < p.first + p.last; i += kChooseThreads) {
     if (i < p.first) out[i] = i;
     else out[p.count - p.last + i - p.first] = nb - p.last + i - p.first;
   }
-  const int need = p.count - p.first - p.last, c = nb - p.first - p.last;
-  if (need == 0) {
-    cluster_bar(C);
-    return;
-  }
-  const int each = (c + C - 1) / C;
-  const int i0 = min(rank * each, c), len = min(i0 + each, c) - i0;  // blocks first + i0 ..
-
-  // ---- scores ----
-  const int group = p.hq / p.hkv, t = lane & 3;
-  for (int g0 = 0; g0 < group; g0 += kSelHeads) {
-    const int nh = min(kSelHeads, group - g0);
+  const uint2* const scores = p.scores + static_cast<int64_t>(row) * p.map.max_pages;
+  uint64_t* const exact = p.exact + static_cast<int64_t>(row) * p.map.max_pages;
+  const int words = (len + 31) / 32;
+  uint32_t* const s_in = s_bits;            // [words] chosen
+  uint32_t* const s_open = s_in + words;    // [words] to be compared in 64 bits
+  uint32_t* const s_won = s_open + words;   // [words] which of those are chosen, in their order
+  const int per = ((words + kChooseWarps - 1) / kChooseWarps + 31) / 32 * 32;
+  const int w0 = min(warp * per, words), w1 = min(w0 + per, words);  // the words a warp counts and lists, a lane a word
+  // exclusive sums over the lanes, and all of it
+  auto scan = [&](uint32_t v, uint32_t& all) {
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    all = __shfl_sync(0xffffffffu, upto, 31);
+    return upto - v;
+  };
+  if constexpr (kScored) {
+    // the keys of words warp, warp + 16, ...: the first 16 of a warp stay in registers, the rest are read again
+    uint32_t held[kChooseHeld];
+    uint32_t least = 0xffffffffu, most = 0, S = 0;
+    auto range = [&](uint2 v) {
+      least = min(least, v.x);
+      most = max(most, v.x);
+      S = max(S, v.y);  // non-negative floats
+    };
+#pragma unroll
+    for (int j = 0; j < kChooseHeld; ++j) {
+      const int i = tid + j * kChooseThreads;
+      held[j] = 0;
+      if (i < len) {
+        const uint2 v = scores[i];
+        held[j] = v.x;
+        range(v);
+      }
+    }
+#pragma unroll 4
+    for (int i = tid + kChooseHeld * kChooseThreads; i < len; i += kChooseThreads) range(scores[i]);
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    S = __reduce_max_sync(0xffffffffu, S);
     __syncthreads();
-    for (int e = tid; e < kSelHeads * 8 * pieces; e += kSelThreads) {
-      const int h = e / (8 * pieces), d = e - h * 8 * pieces;
-      double v = 0.;
-      if (h < nh && d < p.hd) v = static_cast<double>(__bfloat162float(p.q[b * p.qb + (hk * group + g0 + h) * p.qh + d])) * 0x1p800;
-      s_q[e] = v;
+    if (lane == 0) {
+      atomicMin(&s_range[0], least);
+      atomicMax(&s_range[1], most);
+      atomicMax(&s_range[2], S);
     }
     __syncthreads();
-    for (int i = warp * 8 + (lane >> 2); i < (len + 7) / 8 * 8; i += kSelWarps * 8) {
-      const bool there = i < len;
-      int pg = -1;
-      if (there) {
-        pg = page_of(p.map, b, p.first + i0 + i);
-        if (pg < 0) record_status(SN_ERR_INVALID_ARGUMENT);
+    least = s_range[0];
+    const int shift = max(0, 32 - __clz(s_range[1] - least) - kDigitBits);
+    uint32_t* const bins = reinterpret_cast<uint32_t*>(s_sel.hist[0]);
+#pragma unroll
+    for (int j = 0; j < kChooseHeld; ++j)
+      if (tid + j * kChooseThreads < len) atomicAdd(bins + min((held[j] - least) >> shift, kBins - 1u), 1u);
+#pragma unroll 4
+    for (int i = tid + kChooseHeld * kChooseThreads; i < len; i += kChooseThreads)
+      atomicAdd(bins + min((scores[i].x - least) >> shift, kBins - 1u), 1u);
+    __syncthreads();
+    find_bin<Q>(s_sel.hist[0], static_cast<uint32_t>(need), s_sel, 1, 0);
+    const uint32_t first_key = least + (s_sel.digit << shift);
+    const float E2 = fmaf(__uint_as_float(s_range[2]), 0x1p-12f, 0x1p-109f);  // 2 E
+    const float lo = order_value(first_key) - E2, hi = order_value(first_key + ((1u << shift) - 1)) + E2;
+    const bool sure = fabsf(lo) < INFINITY && fabsf(hi) < INFINITY;
+    uint32_t nin = 0, nopen = 0;
+    auto sort_word = [&](int i, uint32_t key) {  // of the warp's lanes' blocks i
+      if (i - lane >= len) return;
+      const float v = order_value(key);
+      const uint32_t in = __ballot_sync(0xffffffffu, sure && i < len && key != 0 && v > hi);
+      const uint32_t open = __ballot_sync(0xffffffffu, i < len && (!sure || (key != 0 && v >= lo && v <= hi)));
+      if (lane == 0) {
+        s_in[i / 32] = in;
+        s_open[i / 32] = open;
       }
-      const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(max(pg, 0)) * p.hkv + hk) * 2 * p.hd;
-      double acc[kSelHeads] = {0., 0., 0., 0.};
-      bool odd = false;  // a bound that is not finite
-      for (int k = t; k < pieces; k += 4) {
-        uint32_t l[4], g[4];
-        if constexpr (kVec) {
-          *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(lo + 8 * k);
-          *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(lo + p.hd + 8 * k);
-        } else {
-          const uint16_t* e = reinterpret_cast<const uint16_t*>(lo) + 8 * k;
+      nin += __popc(in);
+      nopen += __popc(open);
+    };
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int d = 8 * k + 2 * j;
-            l[j] = (d < p.hd ? e[2 * j] : 0u) | (d + 1 < p.hd ? static_cast<uint32_t>(e[2 * j + 1]) << 16 : 0u);
-            g[j] = (d < p.hd ? e[p.hd + 2 * j] : 0u) | (d + 1 < p.hd ? static_cast<uint32_t>(e[p.hd + 2 * j + 1]) << 16 : 0u);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t wl = j & 1 ? l[j / 2] >> 16 : l[j / 2] & 0xffffu, wg = j & 1 ? g[j / 2] >> 16 : g[j / 2] & 0xffffu;
-          odd |= (wl & 0x7f80u) == 0x7f80u || (wg & 0x7f80u) == 0x7f80u;
-          const int dl = static_cast<int>((wl & 0x8000u) << 16 | (wl & 0x7fffu) << 13);
-          const int dg = static_cast<int>((wg & 0x8000u) << 16 | (wg & 0x7fffu) << 13);
-#pragma unroll
-          for (int h = 0; h < kSelHeads; ++h) {
-            const double q = s_q[h * 8 * pieces + 8 * k + j];
-            acc[h] = fma(q, __hiloint2double(q < 0. ? dl : dg, 0), acc[h]);
-          }
-        }
-      }
-      uint64_t best = 0;
-#pragma unroll
-      for (int h = 0; h < kSelHeads; ++h) {
-        acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 1);
-        acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 2);
-        if (h < nh) best = max(best, order_key(acc[h]));
-      }
-      odd = __ballot_sync(0xffffffffu, odd) >> (lane & 28) & 15;
-      if (odd) best = ~0ull;
-      if (pg < 0) best = 0;
-      if (there && t == 0) s_keys[i] = g0 == 0 ? best : max(best, s_keys[i]);
+    for (int j = 0; j < kChooseHeld; ++j) sort_word(tid + j * kChooseThreads, held[j]);
+    for (int i = tid + kChooseHeld * kChooseThreads; i - lane < len; i += kChooseThreads) sort_word(i, i < len ? scores[i].x : 0);
+    if (lane == 0) {  // (s_sel.warp of find_bin has been read: that was before its last barrier)
+      s_sel.warp[warp] = nin;
+      s_sel.warp2[warp] = nopen;
     }
+    __syncthreads();
+    uint32_t all_in = 0, all_open = 0;
+#pragma unroll
+    for (int v = 0; v < kChooseWarps; ++v) {
+      all_in += s_sel.warp[v];
+      all_open += s_sel.warp2[v];
+    }
+    const uint32_t wanted = static_cast<uint32_t>(need) - all_in;
+    if (all_open != wanted) {
+      // the open blocks in their order, those before this warp's words first
+      __syncthreads();  // s_sel.warp2 has been read
+      uint32_t mine = 0;
+      for (int w = w0 + lane; w < w1; w += 32) mine += __popc(s_open[w]);
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if (lane == 0) s_sel.warp2[warp] = mine;
+      __syncthreads();
+      uint32_t open_at = 0;
+#pragma unroll
+      for (int v = 0; v < kChooseWarps; ++v) open_at += v < warp ? s_sel.warp2[v] : 0;
+      if (all_open <= kFewExact) {
+        uint32_t k = open_at;
+        for (int w = w0; w < w1; w += 32) {  // to a list, a lane a word, so that every warp takes as many of them
+          uint32_t left = w + lane < w1 ? s_open[w + lane] : 0, all;
+          for (uint32_t at = k + scan(__popc(left), all); left; left &= left - 1, ++at) s_few_at[at] = 32 * (w + lane) + __ffs(left) - 1;
+          k += all;
+        }
+        __syncthreads();
+        for (uint32_t i = warp; i < all_open; i += kChooseWarps) {
+          const uint64_t key = exact_score(p, b, hk, p.first + s_few_at[i]);
+          if (lane == 0) s_few[i] = key;
+        }
+        __syncthreads();
+        if (tid < all_open) {
+          const uint64_t key = s_few[tid];
+          uint32_t better = 0;
+          for (uint32_t j = 0; j < all_open; ++j) better += s_few[j] > key || (s_few[j] == key && j < tid);
+          if (better >= wanted) atomicAnd(&s_open[s_few_at[tid] / 32], ~(1u << (s_few_at[tid] & 31)));
+        }
+      } else {
+        uint32_t k = open_at;
+        for (int w = w0; w < w1; ++w)
+          for (uint32_t left = s_open[w]; left; left &= left - 1, ++k) {
+            const uint64_t key = exact_score(p, b, hk, p.first + 32 * w + __ffs(left) - 1);
+            if (lane == 0) exact[k] = key;
+          }
+        __syncthreads();
+        const Cutoff<uint64_t> cut = find_cutoff(exact, static_cast<int>(all_open), wanted, s_sel, 1, 0);
+        choose(exact, static_cast<int>(all_open), cut, s_won, s_sel);
+        __syncthreads();
+        k = open_at;
+        for (int w = w0; w < w1; ++w) {  // back to their blocks
+          const uint32_t open = s_open[w], i = k + __popc(open & below);
+          const uint32_t word = __ballot_sync(0xffffffffu, (open >> lane & 1) && (s_won[i / 32] >> (i % 32) & 1));
+          __syncwarp();
+          if (lane == 0) s_open[w] = word;
+          k += __popc(open);
+        }
+      }
+      __syncthreads();
+    }
+  } else {
+    const Cutoff<uint64_t> cut = find_cutoff(exact, len, static_cast<uint32_t>(need), s_sel, 1, 0);
+    choose(exact, len, cut, s_in, s_sel);
+    for (int w = tid; w < words; w += kChooseThreads) s_open[w] = 0;
+    __syncthreads();
   }
+  // ---- the list, in ascending order ----
+  uint32_t mine = 0;
+  for (int w = w0 + lane; w < w1; w += 32) mine += __popc(s_in[w] | s_open[w]);
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  __syncthreads();  // s_sel.warp has been read
+  if (lane == 0) s_sel.warp[warp] = mine;
   __syncthreads();
-
-  // ---- the choice, in ascending order ----
-  const Cutoff<uint64_t> cut = find_cutoff(s_keys, len, static_cast<uint32_t>(need), s_sel, C, rank);
-  choose(s_keys, len, cut, s_bits, s_sel);
-  __syncthreads();
-  const int words = (len + 31) / 32, per = (words + kSelWarps - 1) / kSelWarps;
-  const int w0 = min(warp * per, words), w1 = min(w0 + per, words);
-  uint32_t cnt = 0;
-  for (int w = w0 + lane; w < w1; w += 32) cnt += __popc(s_bits[w]);
-  cnt = __reduce_add_sync(0xffffffffu, cnt);
-  if (lane == 0) s_sel.warp[warp] = cnt;
-  __syncthreads();
-  uint32_t at = 0, all = 0;
-  for (int v = 0; v < kSelWarps; ++v) {
-    if (v == warp) at = all;
-    all += s_sel.warp[v];
+  uint32_t at = p.first;
+#pragma unroll
+  for (int v = 0; v < kChooseWarps; ++v) at += v < warp ? s_sel.warp[v] : 0;
+  for (int w = w0; w < w1; w += 32) {
+    uint32_t left = w + lane < w1 ? s_in[w + lane] | s_open[w + lane] : 0, all;
+    for (uint32_t k = at + scan(__popc(left), all); left; left &= left - 1, ++k) out[k] = p.first + 32 * (w + lane) + __ffs(left) - 1;
+    at += all;
   }
-  if (tid == 0) s_count = all;
-  cluster_bar(C);
-  for (int r = 0; r < rank; ++r) at += peer_u32(&s_count, r);
-  for (int w = w0; w < w1; ++w) {
-    const uint32_t word = s_bits[w];
-    if ((word >> lane) & 1) out[p.first + at + __popc(word & ((1u << lane) - 1))] = p.first + i0 + 32 * w + lane;
-    at += __popc(word);
-  }
-  cluster_bar(C);  // nobody leaves while its count may be read
-}
-
-template <bool kVec>
-int launch_select(int rows, int C, size_t smem, cudaStream_t st, const SelectParams& p) {
-  if (!smem_room<select_blocks_kernel<kVec>>(210 * 1024)) return SN_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows) * C);
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(C);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, select_blocks_kernel<kVec>, p) != cudaSuccess) {
-    cudaGetLastError();
-    return SN_ERR_LAUNCH;
-  }
-  return SN_OK;
 }
 
 }  // namespace
@@ -366,18 +571,23 @@ int sn_update_page_bounds(const void* k_pages, int64_t k_page_stride, int64_t k_
   return sn::launch(sn::page_bounds_rows_kernel, grid, dim3(128), 0, st, true, p);
 }
 
+size_t sn_select_blocks_workspace_size(int batch, int nheads_kv, int max_pages) {
+  if (batch < 1 || nheads_kv < 1 || max_pages < 1) return 0;
+  return static_cast<size_t>(batch) * nheads_kv * max_pages * (sizeof(uint64_t) + sizeof(uint2));
+}
+
 int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* bounds, int num_pages,
                      int page_size, const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
                      int batch, int nheads, int nheads_kv, int head_dim, int count, int first, int last, int* blocks,
-                     void* stream) {
-  if (!q || !bounds || !page_table || !seq_lens || !blocks || num_pages < 1 || page_size < 1 || max_pages < 1 ||
-      table_stride < max_pages || batch < 1 || nheads < 1 || nheads_kv < 1 || nheads % nheads_kv != 0 || head_dim < 1 ||
-      q_batch_stride < 0 || q_head_stride < 0 || count < 1 || first < 0 || last < 0 || first > count ||
-      last > count - first)
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !bounds || !page_table || !seq_lens || !blocks || !workspace || num_pages < 1 || page_size < 1 ||
+      max_pages < 1 || table_stride < max_pages || batch < 1 || nheads < 1 || nheads_kv < 1 || nheads % nheads_kv != 0 ||
+      head_dim < 1 || q_batch_stride < 0 || q_head_stride < 0 || count < 1 || first < 0 || last < 0 || first > count ||
+      last > count - first || workspace_bytes < sn_select_blocks_workspace_size(batch, nheads_kv, max_pages))
     return SN_ERR_INVALID_ARGUMENT;
+  if (!sn::aligned16(workspace)) return SN_ERR_MISALIGNED;
   const int64_t rows = static_cast<int64_t>(batch) * nheads_kv;
-  if (head_dim > 512 || rows > INT32_MAX / sn::kClusterMost || max_pages > sn::kClusterMost * (sn::kSelMost - 1) ||
-      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+  if (rows > INT32_MAX || max_pages > sn::kChooseMost || static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
     return SN_ERR_UNSUPPORTED;
   sn::SelectParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -387,6 +597,8 @@ int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_strid
   p.map = {page_table, table_stride, max_pages, num_pages, page_size};
   p.seq_lens = seq_lens;
   p.blocks = blocks;
+  p.exact = static_cast<uint64_t*>(workspace);
+  p.scores = reinterpret_cast<uint2*>(p.exact + rows * max_pages);
   p.batch = batch;
   p.hq = nheads;
   p.hkv = nheads_kv;
@@ -394,17 +606,26 @@ int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_strid
   p.count = count;
   p.first = first;
   p.last = last;
-  // CTAs a row: as many as the shared memory asks for, and more where there are few long rows
-  int C = 1;
-  while (C < sn::kClusterMost && (max_pages > C * (sn::kSelMost - 1) || (rows * C < 2 * sn::sm_count() && max_pages > 128 * C)))
-    C *= 2;
-  p.part = (max_pages + C - 1) / C + 1;
-  const size_t smem = static_cast<size_t>(p.part) * 8 + (p.part / 32 + 3) / 2 * 2 * 4 +
-                      static_cast<size_t>(sn::kSelHeads) * ((head_dim + 7) / 8 * 8) * 8;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int r = static_cast<int>(rows);
-  return head_dim % 8 == 0 && sn::aligned16(bounds) ? sn::launch_select<true>(r, C, smem, st, p)
-                                                    : sn::launch_select<false>(r, C, smem, st, p);
+  const bool scored = sn::aligned16(bounds) && (head_dim == 64 || head_dim == 128);
+  const size_t smem = static_cast<size_t>((max_pages + 31) / 32) * 3 * sizeof(uint32_t);
+  constexpr int kRoom = sn::kChooseMost / 32 * 3 * sizeof(uint32_t);
+  if (!(scored ? sn::smem_room<sn::choose_blocks_kernel<true>>(kRoom) : sn::smem_room<sn::choose_blocks_kernel<false>>(kRoom)))
+    return SN_ERR_LAUNCH;
+  if (max_pages > count) {  // there may be something to compare
+    // as many CTAs a row as the table has blocks for, and over all rows no more than a few for each place on the device:
+    // the lengths are on the device
+    const int64_t y = std::min<int64_t>(rows, 65535), per_cta = scored ? 64 : 4;
+    const int64_t x = std::min<int64_t>((max_pages + per_cta - 1) / per_cta, std::max<int64_t>(1, (scored ? 4 : 16) * sn::sm_count() / y));
+    const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y));
+    const int rc = !scored         ? sn::launch(sn::exact_scores_kernel, grid, dim3(128), 0, st, true, p)
+                   : head_dim == 64 ? sn::launch(sn::block_scores_kernel<64>, grid, dim3(128), 0, st, true, p)
+                                    : sn::launch(sn::block_scores_kernel<128>, grid, dim3(128), 0, st, true, p);
+    if (rc != SN_OK) return rc;
+  }
+  const dim3 grid(static_cast<unsigned>(rows));
+  return scored ? sn::launch(sn::choose_blocks_kernel<true>, grid, dim3(sn::kChooseThreads), smem, st, true, p)
+                : sn::launch(sn::choose_blocks_kernel<false>, grid, dim3(sn::kChooseThreads), smem, st, true, p);
 }
 
 }  // extern "C"

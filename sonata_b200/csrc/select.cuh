@@ -14,11 +14,7 @@
 namespace sn {
 namespace {
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;
-constexpr int kClusterMost = 8;
-static_assert(kBins == 4 * kSelThreads, "four bins a thread");
 
 __device__ __forceinline__ uint32_t ctarank() {
   uint32_t r;
@@ -40,6 +36,18 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t* local, int rank) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+// The address of `local`'s place in the shared memory of CTA `rank`.
+__device__ __forceinline__ uint32_t peer_at(const void* local, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void put_u32(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void put_u64(uint32_t at, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
 __device__ __forceinline__ uint4 peer_u128(const uint4* local, int rank) {
   uint32_t a;
   uint4 v;
@@ -60,9 +68,14 @@ __device__ __forceinline__ uint64_t order_key(double v) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
+__device__ __forceinline__ float order_value(uint32_t key) { return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key); }
+
+template <int T>  // threads of a CTA
 struct SelectShared {
+  static constexpr int kWarps = T / 32, kQuads = kBins / (4 * T);  // each thread has kQuads times four neighbouring bins
+  static_assert(kQuads * 4 * T == kBins);
   uint4 hist[2][kBins / 4];
-  uint32_t warp[kSelWarps], warp2[kSelWarps];
+  uint32_t warp[kWarps], warp2[kWarps];
   uint32_t digit, above, here;
 };
 
@@ -75,54 +88,99 @@ struct Cutoff {
   uint32_t need, before;
 };
 
-// The `need` highest (at least 1, at most all) of the cluster's keys; `len` of them are this CTA's.  All threads of all CTAs
-// call it.  `top`: bits from here up are the same in all keys.
-template <typename K>
-__device__ Cutoff<K> find_cutoff(const K* keys, int len, uint32_t need, SelectShared& s, int C, int rank, int top = 8 * sizeof(K),
-                                 K prefix = 0) {
+// The bin of 4 Q T in which the need-th highest of all the cluster's keys lies: to s.digit, with the number of keys in higher
+// bins to s.above and that in it to s.here.  After a cluster barrier, which makes the histograms visible; all threads of all
+// CTAs.  A load from a peer takes most of a microsecond, so eight peers' are in flight at once.
+template <int Q, int T>
+__device__ void find_bin(const uint4* hist, uint32_t need, SelectShared<T>& s, int C, int rank) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  s.hist[0][tid] = make_uint4(0, 0, 0, 0);
+  uint4 t[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) t[q] = hist[Q * tid + q];
+  for (int r0 = 1; r0 < C; r0 += 8) {
+    uint4 o[8][Q];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r0 + r < C) {
+        const int peer = rank + r0 + r < C ? rank + r0 + r : rank + r0 + r - C;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) o[r][q] = peer_u128(hist + Q * tid + q, peer);
+      }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r0 + r < C) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          t[q].x += o[r][q].x;
+          t[q].y += o[r][q].y;
+          t[q].z += o[r][q].z;
+          t[q].w += o[r][q].w;
+        }
+      }
+  }
+  uint32_t mine = 0;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) mine += t[q].x + t[q].y + t[q].z + t[q].w;
+  uint32_t upto = mine;  // keys in this thread's bins and those of the threads after it
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_down_sync(0xffffffffu, upto, o);
+    if (lane + o < 32) upto += v;
+  }
+  if (lane == 0) s.warp[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 1; w < SelectShared<T>::kWarps; ++w)
+    if (w > warp) upto += s.warp[w];
+  if (upto >= need && upto - mine < need) {  // one thread
+    uint32_t above = upto - mine, here = 0;
+    int bin = -1;
+#pragma unroll
+    for (int q = Q - 1; q >= 0; --q) {
+      const uint32_t c[4] = {t[q].w, t[q].z, t[q].y, t[q].x};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (bin >= 0) continue;
+        if (above + c[j] >= need) {
+          bin = 4 * (Q * tid + q) + 3 - j;
+          here = c[j];
+        } else {
+          above += c[j];
+        }
+      }
+    }
+    s.digit = bin;
+    s.above = above;
+    s.here = here;
+  }
+  __syncthreads();
+}
+
+// The `need` highest (at least 1, at most all) of the cluster's keys; `len` of them are this CTA's.  All threads of all CTAs
+// call it.
+template <int T, typename K>
+__device__ Cutoff<K> find_cutoff(const K* keys, int len, uint32_t need, SelectShared<T>& s, int C, int rank) {
+  constexpr int Q = SelectShared<T>::kQuads;
+  const int tid = threadIdx.x;
+  int top = 8 * sizeof(K);
+  K prefix = 0;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) s.hist[0][Q * tid + q] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   for (int pass = 0;; ++pass) {
     uint4* const hist = s.hist[pass & 1];
     uint32_t* const bins = reinterpret_cast<uint32_t*>(hist);
     const int low = top > kDigitBits ? top - kDigitBits : 0, width = top - low;
     const uint32_t mask = (1u << width) - 1;
-    for (int i = tid; i < len; i += kSelThreads) {
+    for (int i = tid; i < len; i += T) {
       const K k = keys[i];
       if (top == 8 * sizeof(K) || (k >> top) == prefix) atomicAdd(bins + (static_cast<uint32_t>(k >> low) & mask), 1u);
     }
     cluster_bar(C);
-    s.hist[(pass + 1) & 1][tid] = make_uint4(0, 0, 0, 0);  // everyone has read it: that was before this pass's barrier
-    uint4 t = hist[tid];
-    for (int r = 1; r < C; ++r) {
-      const uint4 o = peer_u128(hist + tid, (rank + r) % C);
-      t.x += o.x;
-      t.y += o.y;
-      t.z += o.z;
-      t.w += o.w;
-    }
-    // keys in this thread's bins and those of the threads after it
-    uint32_t upto = t.x + t.y + t.z + t.w;
-    const uint32_t mine = upto;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_down_sync(0xffffffffu, upto, o);
-      if (lane + o < 32) upto += v;
-    }
-    if (lane == 0) s.warp[warp] = upto;
-    __syncthreads();
-    for (int w = warp + 1; w < kSelWarps; ++w) upto += s.warp[w];
-    if (upto >= need && upto - mine < need) {  // one thread
-      uint32_t above = upto - mine;
-      const uint32_t c[4] = {t.w, t.z, t.y, t.x};
-      int j = 0;
-      while (j < 3 && above + c[j] < need) above += c[j++];
-      s.digit = 4 * tid + 3 - j;
-      s.above = above;
-      s.here = c[j];
-    }
-    __syncthreads();
+    for (int q = 0; q < Q; ++q)  // everyone has read it: that was before this pass's barrier
+      s.hist[(pass + 1) & 1][Q * tid + q] = make_uint4(0, 0, 0, 0);
+    find_bin<Q>(hist, need, s, C, rank);
     const uint32_t digit = s.digit, here = s.here;
     need -= s.above;
     prefix = static_cast<K>(top == 8 * sizeof(K) ? 0 : prefix << width) | digit;
@@ -133,16 +191,17 @@ __device__ Cutoff<K> find_cutoff(const K* keys, int len, uint32_t need, SelectSh
         for (int r = 0; r < rank; ++r) cut.before += peer_u32(bins + digit, r);
       return cut;
     }
-    // the next pass writes s.warp and s.digit after its barrier, which every thread of this CTA reaches from here
+    // the next pass writes s after its barrier, which every thread of this CTA reaches from here
   }
 }
 
 // One bit a key, chosen or not, in bits[0 .. (len + 31) / 32): a warp takes consecutive words.  All threads call it, with a
 // barrier after it before the bits are read.
-template <typename K>
-__device__ void choose(const K* keys, int len, const Cutoff<K>& cut, uint32_t* bits, SelectShared& s) {
+template <int T, typename K>
+__device__ void choose(const K* keys, int len, const Cutoff<K>& cut, uint32_t* bits, SelectShared<T>& s) {
+  constexpr int kWarps = SelectShared<T>::kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int words = (len + 31) / 32, per = (words + kSelWarps - 1) / kSelWarps;
+  const int words = (len + 31) / 32, per = (words + kWarps - 1) / kWarps;
   const int w0 = min(warp * per, words), w1 = min(w0 + per, words);
   auto equal = [&](int w) {
     const int i = 32 * w + lane;

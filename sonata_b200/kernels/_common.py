@@ -12,13 +12,16 @@ import torch
 from .. import _lib, build
 
 _FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_copy_pages",
-                 "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size")
+                 "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size", "sn_paged_decode_attention_mass",
+                 "sn_paged_mass_workspace_size", "sn_evict_positions", "sn_update_page_bounds", "sn_select_blocks",
+                 "sn_select_blocks_workspace_size",
+                 "sn_paged_sparse_attention")
 
 
 class _NoFast:
     """In the place of the short way's functions where it was not built, or
     does not load: every call is left to the wrapper."""
-    attend = append = copy = prompt = staticmethod(lambda *args: None)
+    attend = append = copy = prompt = mass = evict = bounds = select = sparse = staticmethod(lambda *args: None)
 
 
 _fast = None

@@ -17,7 +17,7 @@ import torch
 
 from .. import _lib
 from . import paged_kv as PK
-from ._common import call, current_handle, on_stream, require_cuda, same_device
+from ._common import call, current_handle, fast, on_stream, require_cuda, same_device
 
 
 @functools.lru_cache(maxsize=256)
@@ -51,6 +51,10 @@ def paged_decode_attention_mass(q: torch.Tensor, k_pages: torch.Tensor, v_pages:
     [batch, nheads_kv, at least max_pages * page_size] (batch and head strides
     taken from the tensor); places past a stream's end are not touched.
     `workspace`: mass_workspace."""
+    if stream is None:
+        r = fast().mass(q, k_pages, v_pages, page_table, seq_lens, mass, scale, workspace, return_lse)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_paged_decode_attention_mass", r)
     if not (isinstance(page_table, torch.Tensor) and page_table.dim() == 2 and isinstance(k_pages, torch.Tensor) and k_pages.dim() == 4):
         PK._pages(k_pages, v_pages, page_table, seq_lens)
     (batch, width), (_, hkv, page, _) = page_table.shape, k_pages.shape
@@ -77,6 +81,10 @@ def evict_positions(pool: torch.Tensor, page_table: torch.Tensor, seq_lens: torc
     streams share must not be cut in either.  With return_source: int32
     [n_layers, batch, nheads_kv, keep], where each place's position was (-1 past
     the end of a stream that was left alone)."""
+    if stream is None:
+        r = fast().evict(pool, page_table, seq_lens, mass, keep, recent, sinks, return_source)
+        if r is not None:
+            return _lib.check("sn_evict_positions", r) if type(r) is int else None if r is True else r
     require_cuda("pool", pool, torch.bfloat16, 6)
     if not pool.is_contiguous() or min(pool.shape) < 1 or pool.shape[1] != 2:
         raise ValueError("pool must be a contiguous, non-empty [n_layers, 2, num_pages, nheads_kv, page_size, head_dim] tensor")

@@ -12,8 +12,9 @@ from __future__ import annotations
 
 import torch
 
+from .. import _lib
 from . import paged_kv as PK
-from ._common import call, current_handle, on_stream, require_cuda, same_device
+from ._common import call, current_handle, fast, on_stream, require_cuda, same_device
 
 _BF16 = torch.bfloat16
 
@@ -52,6 +53,10 @@ def update_page_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: 
     the last cu_seqlens[b+1] - cu_seqlens[b] of the seq_lens[b] (None: one a
     stream).  k_pages [num_pages, nheads_kv, page_size, head_dim] by its
     strides."""
+    if stream is None:
+        r = fast().bounds(k_pages, bounds, page_table, seq_lens, cu_seqlens)
+        if r is not None:
+            return None if r is True else _lib.check("sn_update_page_bounds", r)
     PK._pool("k_pages", k_pages)
     n, hkv, page, hd = k_pages.shape
     _check_bounds(bounds, hkv, hd, n)
@@ -78,6 +83,10 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tenso
     A block's score is the greatest over the key/value head's query heads of
     sum_d max(q_d least_d, q_d greatest_d), no less than any q . k in it.
     q [batch, nheads, head_dim] by batch and head strides."""
+    if stream is None:
+        r = fast().select(q, bounds, page_table, seq_lens, page_size, count, first, last)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_select_blocks", r)
     require_cuda("q", q, _BF16, 3)
     _check_bounds(bounds)
     _check_table(page_table, seq_lens)
@@ -95,9 +104,11 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tenso
 
     def launch(st):
         blocks = torch.empty((batch, hkv, count), device=q.device, dtype=torch.int32)
+        need = _lib.lib().sn_select_blocks_workspace_size(batch, hkv, width)
+        ws = torch.empty(need, device=q.device, dtype=torch.uint8)
         call("sn_select_blocks", q.data_ptr(), q.stride(0), q.stride(1), bounds.data_ptr(), pages, page_size, page_table.data_ptr(),
              page_table.stride(0) if batch > 1 else width, width, seq_lens.data_ptr(), batch, nheads, hkv, hd, count, first, last,
-             blocks.data_ptr(), st)
+             blocks.data_ptr(), ws.data_ptr(), need, st)
         return blocks
 
     return _on(stream, launch)
@@ -111,6 +122,10 @@ def paged_sparse_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     first min(count, ceil(seq_lens[b] / page_size)) are read.  Entries below 0 or
     past the stream's end are left out; a block listed twice counts twice.
     `workspace`: decode_workspace."""
+    if stream is None:
+        r = fast().sparse(q, k_pages, v_pages, page_table, seq_lens, blocks, scale, workspace, return_lse)
+        if r is not None:
+            return r if type(r) is not int else _lib.check("sn_paged_sparse_attention", r)
     if not (isinstance(page_table, torch.Tensor) and page_table.dim() == 2 and isinstance(k_pages, torch.Tensor) and k_pages.dim() == 4):
         PK._pages(k_pages, v_pages, page_table, seq_lens)
     require_cuda("blocks", blocks, torch.int32, 3)

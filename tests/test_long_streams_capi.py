@@ -74,7 +74,7 @@ def test_update_page_bounds(L, change, rc):
 
 def select(L, **k):
     a = dict(q=p, qb=2048, qh=128, bounds=p, np=8, page=16, tab=p, ts=4, mp=4, lens=p, batch=2, hq=16, hkv=4, hd=128, count=3, first=1, last=1, blocks=p,
-             stream=None)
+             ws=p, wsb=BIG, stream=None)
     a.update(k)
     return L.sn_select_blocks(*a.values())
 
@@ -82,9 +82,16 @@ def select(L, **k):
 @pytest.mark.parametrize("change,rc", [
     (dict(q=None), -1), (dict(bounds=None), -1), (dict(tab=None), -1), (dict(lens=None), -1), (dict(blocks=None), -1), (dict(hq=15), -1), (dict(count=0), -1),
     (dict(first=-1), -1), (dict(last=-1), -1), (dict(first=2, last=2), -1), (dict(first=4), -1), (dict(qb=-1), -1), (dict(page=0), -1), (dict(ts=3), -1),
-    (dict(hd=513), -3), (dict(mp=180217, ts=180217), -3), (dict(batch=1 << 28), -3)])
+    (dict(ws=None), -1), (dict(wsb=2 * 4 * 4 * 16 - 1), -1), (dict(ws=ctypes.c_void_p(264)), -2), (dict(mp=262145, ts=262145), -3)])
 def test_select_blocks(L, change, rc):
     assert select(L, **change) == rc
+
+
+def test_select_workspace(L):
+    f = L.sn_select_blocks_workspace_size
+    assert f(0, 4, 10) == f(1, 0, 10) == f(1, 4, 0) == 0
+    assert 0 < f(1, 4, 10) < f(2, 4, 10) < f(2, 4, 1000)
+    assert f(3000, 8, 200000) > 1 << 36
 
 
 def sparse(L, **k):

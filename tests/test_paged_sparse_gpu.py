@@ -403,3 +403,29 @@ def test_refusals(PS):
                 dict(workspace=torch.zeros(64, device="cuda", dtype=torch.uint8))):
         with pytest.raises((TypeError, ValueError)):
             PS.paged_sparse_attention(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["subnormal bounds", "subnormal queries", "cancelling", "border"])
+def test_select_where_32_bits_are_not_enough(PS, hd, kind):
+    """Bounds or queries below 2^-126 that the sums still depend on, sums whose large terms cancel, and a border at which many
+    blocks differ in bits that only 64 hold (more of them than are ranked by comparing all)."""
+    def make(q, bounds, tab):
+        if kind == "subnormal bounds":
+            bounds.copy_((bounds.float() * 1e-39).to(BF16))
+            q.copy_((q.float() * 1e37).to(BF16))
+        if kind == "subnormal queries":
+            bounds.copy_((bounds.float() * 1e37).to(BF16))
+            q.copy_((q.float() * 1e-39).to(BF16))
+        if kind == "cancelling":
+            q[..., 0], q[..., 1] = 1.0, 1.0
+            bounds[..., 0] = 2.0 ** 40
+            bounds[..., 1] = -2.0 ** 40
+        if kind == "border":
+            q.fill_(1.0)
+            bounds.fill_(1.0)
+            n = torch.arange(len(bounds), device="cuda")
+            bounds[..., 5] = (2.0 ** -20 * (1 + n % 64))[:, None, None].to(BF16)
+            bounds[..., 6] = (2.0 ** -40 * (1 + n * 37 % 101))[:, None, None].to(BF16)
+    select_case(PS, [16 * 900, 16 * 130], 90, 1, 2, hq=8, hkv=2, hd=hd, make=make, seed=11)
+    select_case(PS, [16 * 6000], 400, 1, 2, hq=4, hkv=1, hd=hd, make=make, seed=12)
