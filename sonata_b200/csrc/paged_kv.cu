@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace sn {
 namespace {
@@ -414,6 +415,15 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
       : "memory");
 }
+// The same, and the first to leave L2.
+__device__ __forceinline__ void tma_load_5d_first(void* dst, const CUtensorMap* map, int row, int head, int page, uint64_t* bar,
+                                                  uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7], %8;" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
@@ -700,6 +710,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       __syncthreads();
     }
     const uint32_t q_at = smem_u32(s_q) + g * (HD * 2) + t * 16;  // chunks of odd heads swapped in fours: no two in a bank
+    float* const scores =
+        kKind == kMass ? p.scores + ((static_cast<int64_t>(b) * sp.sets + set) * p.room + og) * p.score_heads + 2 * t : nullptr;
     float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -712,8 +724,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
       if (lane == 0) {
         unsigned char* dst = ring + warp * (S * stage_bytes<HD>()) + slot * stage_bytes<HD>();
         mbar_arrive_expect_tx(&full[warp][slot], stage_bytes<HD>());
-        tma_load_5d(dst, &kmap, row, hk, pg, &full[warp][slot]);
-        tma_load_5d(dst + (HD / 64) * BOX, &vmap, row, hk, pg, &full[warp][slot]);
+        if constexpr (kKind == kMass) {  // the scores wait in L2, so keys and values pass through
+          const uint64_t policy = l2_policy_evict_first();
+          tma_load_5d_first(dst, &kmap, row, hk, pg, &full[warp][slot], policy);
+          tma_load_5d_first(dst + (HD / 64) * BOX, &vmap, row, hk, pg, &full[warp][slot], policy);
+        } else {
+          tma_load_5d(dst, &kmap, row, hk, pg, &full[warp][slot]);
+          tma_load_5d(dst + (HD / 64) * BOX, &vmap, row, hk, pg, &full[warp][slot]);
+        }
       }
     };
     // This warp's tiles are lo + warp + kAttWarps k, k < count.  Lane l looks up the page (and the row in it) of the l-th of the
@@ -808,7 +826,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
         }
         if constexpr (kKind == kMass) {  // every position of the tile: -inf where it does not count
           if (8 * n + 2 * t < nh) {
-            float* sc = p.scores + ((static_cast<int64_t>(b) * sp.sets + set) * p.room + first + og) * p.score_heads + 8 * n + 2 * t;
+            float* sc = scores + static_cast<int64_t>(first) * p.score_heads + 8 * n;
             *reinterpret_cast<float2*>(sc) = make_float2(s[n][0], s[n][1]);
             *reinterpret_cast<float2*>(sc + 8 * p.score_heads) = make_float2(s[n][2], s[n][3]);
           }
@@ -994,29 +1012,54 @@ struct MassParams {
   int batch, hq, hkv, sets_per_kv, heads_per_set, score_heads;
 };
 
+// V: scores loaded at once (4 where the heads of a set are stored in fours, else 2).  Four positions a thread, all of their
+// loads in flight.
+constexpr int kMassSteps = 4;
+template <int V>
 __global__ void __launch_bounds__(256) add_mass_kernel(const MassParams p) {
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
   pdl_launch_dependents();
   pdl_wait();
-  const int hk = blockIdx.y, group = p.hq / p.hkv;
-  extern __shared__ float s_lse[];  // [group], times log2(e)
+  const int hk = blockIdx.y, group = p.hq / p.hkv, tid = threadIdx.x;
+  extern __shared__ float s_lse[];  // [group], times log2(e); infinite for a row without weights
   for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
     const int len = length_of(p.map, p.seq_lens, b);
+    if (static_cast<int64_t>(blockIdx.x) * 256 * kMassSteps >= len) continue;
     __syncthreads();
-    for (int h = threadIdx.x; h < group; h += 256)
-      s_lse[h] = p.lse[static_cast<int64_t>(b) * p.hq + hk * group + h] * 1.4426950408889634f;
+    for (int h = tid; h < group; h += 256) {
+      const float l = p.lse[static_cast<int64_t>(b) * p.hq + hk * group + h] * 1.4426950408889634f;
+      s_lse[h] = l == -INFINITY ? INFINITY : l;
+    }
     __syncthreads();
-    for (int64_t t = blockIdx.x * 256 + threadIdx.x; t < len; t += static_cast<int64_t>(gridDim.x) * 256) {
-      float sum = 0.f;
+    float* const mass = p.mass + b * p.mb + hk * p.mh;
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * 256 * kMassSteps + tid; t0 < len; t0 += static_cast<int64_t>(gridDim.x) * 256 * kMassSteps) {
+      float sum[kMassSteps], old[kMassSteps];
+#pragma unroll
+      for (int k = 0; k < kMassSteps; ++k) {
+        sum[k] = 0.f;
+        old[k] = t0 + 256 * k < len ? mass[t0 + 256 * k] : 0.f;
+      }
       for (int set = 0; set < p.sets_per_kv; ++set) {
-        const float* sc = p.scores + ((static_cast<int64_t>(b) * p.hkv * p.sets_per_kv + hk * p.sets_per_kv + set) * p.room + t) * p.score_heads;
+        const float* sc = p.scores + ((static_cast<int64_t>(b) * p.hkv + hk) * p.sets_per_kv + set) * p.room * p.score_heads;
+        const float* lse = s_lse + set * p.heads_per_set;
         const int nh = min(p.heads_per_set, group - set * p.heads_per_set);
-        for (int h = 0; h < nh; ++h) {
-          const float l = s_lse[set * p.heads_per_set + h];
-          sum += l == -INFINITY ? 0.f : exp2_approx(sc[h] - l);  // no weight anywhere in this row
+        for (int h = 0; h < nh; h += V) {
+          Vec v[kMassSteps];
+#pragma unroll
+          for (int k = 0; k < kMassSteps; ++k)  // past the end: the last position's, not counted
+            v[k] = __ldcs(reinterpret_cast<const Vec*>(sc + min(t0 + 256 * k, static_cast<int64_t>(len - 1)) * p.score_heads + h));
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (h + j >= nh) continue;
+            const float l = lse[h + j];
+#pragma unroll
+            for (int k = 0; k < kMassSteps; ++k) sum[k] += exp2_approx(reinterpret_cast<const float*>(&v[k])[j] - l);
+          }
         }
       }
-      float* m = p.mass + b * p.mb + hk * p.mh + t;
-      *m += sum;
+#pragma unroll
+      for (int k = 0; k < kMassSteps; ++k)
+        if (t0 + 256 * k < len) mass[t0 + 256 * k] = old[k] + sum[k];
     }
   }
 }
@@ -1344,10 +1387,13 @@ int sn_paged_decode_attention_mass(const void* q, int64_t q_batch_stride, int64_
   mp.heads_per_set = p.heads_per_set;
   mp.score_heads = p.score_heads;
   // about eight CTAs an SM, no more than the tables have positions for: the lengths are on the device
-  const int64_t rows = static_cast<int64_t>(std::min(batch, 65535)) * nheads_kv;
-  const int64_t per_row = std::min<int64_t>((room + 255) / 256, std::max<int64_t>(1, 8 * sn::sm_count() / rows));
-  return sn::launch(sn::add_mass_kernel, dim3(static_cast<unsigned>(per_row), static_cast<unsigned>(nheads_kv), static_cast<unsigned>(std::min(batch, 65535))),
-                    dim3(256), group * sizeof(float), static_cast<cudaStream_t>(stream), true, mp);
+  const int z = std::min(batch, 65535);
+  const int64_t span = 256 * sn::kMassSteps, rows = static_cast<int64_t>(z) * nheads_kv;
+  const int64_t x = std::min<int64_t>((room + span - 1) / span, std::max<int64_t>(1, 8 * sn::sm_count() / rows));
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(nheads_kv), static_cast<unsigned>(z));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return p.score_heads % 4 == 0 ? sn::launch(sn::add_mass_kernel<4>, grid, dim3(256), group * sizeof(float), st, true, mp)
+                                : sn::launch(sn::add_mass_kernel<2>, grid, dim3(256), group * sizeof(float), st, true, mp);
 }
 
 int sn_copy_pages(void* pool, int64_t outer_stride_bytes, int64_t page_stride_bytes, int64_t page_bytes, int outer,
