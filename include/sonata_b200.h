@@ -628,7 +628,9 @@ int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_by
  * nheads_kv, keep] (or NULL) is where each place's position was, -1 past the
  * end of a stream with n <= keep, of which nothing else changes.  seq_lens is
  * the caller's to set to min(n, keep).  No page may be shared between streams
- * that are cut.  recent + sinks <= keep; max_pages * page_size <= 393184.
+ * that are cut.  recent + sinks <= keep; max_pages * page_size <= 2^19.
+ * workspace: sn_evict_workspace_size bytes for max_positions = max_pages *
+ * page_size, 16-byte aligned, whatever they hold.
  *
  * sn_update_page_bounds: bounds bf16 [num_pages, nheads_kv, 2, head_dim],
  * dense: elementwise the least and the greatest of the keys that a page holds
@@ -667,10 +669,12 @@ int sn_paged_decode_attention_mass(const void *q, int64_t q_batch_stride, int64_
                                    int64_t mass_batch_stride, int64_t mass_head_stride, void *out, float *lse,
                                    float scale, int batch, int nheads, int nheads_kv, int head_dim, void *workspace,
                                    size_t workspace_bytes, void *stream);
+size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions);
 int sn_evict_positions(void *pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
                        const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens, float *mass,
                        int64_t mass_layer_stride, int64_t mass_batch_stride, int64_t mass_head_stride, int batch,
-                       int keep, int recent, int sinks, int *source, void *stream);
+                       int keep, int recent, int sinks, int *source, void *workspace, size_t workspace_bytes,
+                       void *stream);
 int sn_update_page_bounds(const void *k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_tok_stride,
                           int num_pages, int page_size, const int *page_table, int64_t table_stride, int max_pages,
                           const int *seq_lens, const int *cu_seqlens, int batch, int nheads_kv, int head_dim,

@@ -31,6 +31,7 @@ struct Abi {  // of the loaded libsonata_b200.so, set by bind()
   decltype(&sn_paged_decode_attention_mass) mass;
   decltype(&sn_paged_mass_workspace_size) mass_size;
   decltype(&sn_evict_positions) evict;
+  decltype(&sn_evict_workspace_size) evict_size;
   decltype(&sn_update_page_bounds) bounds;
   decltype(&sn_select_blocks) select;
   decltype(&sn_select_blocks_workspace_size) select_size;
@@ -211,13 +212,14 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (layers > INT32_MAX || pages > INT32_MAX || heads > INT32_MAX || page > INT32_MAX || hd > INT32_MAX ||
       !mass_ok(m, 4, t.width * page, dev) || m->size(0) != layers || m->size(1) != t.streams || m->size(2) != heads)
     Py_RETURN_NONE;
-  Tensor source;
+  const size_t need = abi.evict_size(static_cast<int>(layers), static_cast<int>(t.streams), static_cast<int>(heads), t.width * page);
+  Tensor ws = at::empty({static_cast<int64_t>(need)}, pool->options().dtype(at::kByte)), source;
   if (a[7] == Py_True) source = at::empty({layers, t.streams, heads, keep}, pool->options().dtype(at::kInt));
   const int rc = abi.evict(pool->data_ptr(), static_cast<int>(layers), static_cast<int>(pages), static_cast<int>(page),
                            static_cast<int>(heads), static_cast<int>(hd), t.table->data_ptr<int>(), t.stride(),
                            static_cast<int>(t.width), t.lens->data_ptr<int>(), m->data_ptr<float>(), m->stride(0), m->stride(1),
                            m->stride(2), static_cast<int>(t.streams), keep, recent, sinks,
-                           source.defined() ? source.data_ptr<int>() : nullptr, current_stream(dev));
+                           source.defined() ? source.data_ptr<int>() : nullptr, ws.data_ptr(), need, current_stream(dev));
   if (rc) return status(rc);
   if (source.defined()) return THPVariable_Wrap(std::move(source));
   Py_RETURN_TRUE;
@@ -373,7 +375,8 @@ PyObject* bind(PyObject*, PyObject* table) {
       !get("sn_rotary_paged_append", abi.append) || !get("sn_copy_pages", abi.copy) ||
       !get("sn_mamba2_prompt", abi.prompt) || !get("sn_mamba2_prompt_workspace_size", abi.prompt_size) ||
       !get("sn_paged_decode_attention_mass", abi.mass) || !get("sn_paged_mass_workspace_size", abi.mass_size) ||
-      !get("sn_evict_positions", abi.evict) || !get("sn_update_page_bounds", abi.bounds) ||
+      !get("sn_evict_positions", abi.evict) || !get("sn_evict_workspace_size", abi.evict_size) ||
+       !get("sn_update_page_bounds", abi.bounds) ||
       !get("sn_select_blocks", abi.select) ||
       !get("sn_select_blocks_workspace_size", abi.select_size) || !get("sn_paged_sparse_attention", abi.sparse))
     return nullptr;

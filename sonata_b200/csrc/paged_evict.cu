@@ -18,8 +18,16 @@
 namespace sn {
 namespace {
 
-constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictCluster = 8;  // CTAs a row at most
+// Two launches: the plan of each row (a CTA each: what stays, the lists of holes and movers, mass), bound by the chain of
+// its steps, and the moves, bound by HBM.  In one launch, a cluster a row, either the choice is shared out, its histograms
+// exchanged through distributed shared memory (12 layers of a stream of 2112 positions 27 us, of 30011 59), or the other
+// CTAs of the cluster wait for the one that makes it (30 and 95 us).
+constexpr int kEvictMost = 1 << 19;   // candidates of a stream: two bits each in shared memory
+constexpr int kEvictWords = 52992;    // of shared memory for those bits and for keys
+constexpr int kEvictCopy = 1024;      // 16-byte pieces of one copy to shared memory
+constexpr int kEvictRanked = 256;     // keys that are ranked by comparing all of them
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
+constexpr int kMoveCluster = 8;       // CTAs a row at most
 
 struct EvictParams {
   char* pool;  // [layers, 2, num_pages, hkv, page_size] rows of row_bytes, dense
@@ -27,110 +35,323 @@ struct EvictParams {
   int row_bytes;
   PageMap map;
   const int* seq_lens;
-  float* mass;  // [layers, batch, hkv, >= capacity] by strides
+  float* mass;  // [layers, batch, hkv, >= room] by strides
   int64_t ml, mb, mh;
   int* source;  // [layers, batch, hkv, keep] or null
+  int2* head;   // [layers, batch, hkv]: n, pairs of a hole and a mover
+  int* plan;    // [layers, batch, hkv] of plan_ints: holes from the front and movers from the back, then keys
+  int room;     // max_pages * page_size
   int batch, hkv, keep, recent, sinks;
-  int part;  // candidates a CTA's shared memory holds
+  int held;     // keys in shared memory: all candidates' or none (then they are in the plan)
 };
 
-// One cluster a (layer, stream, head).  The candidates' keys lie in the
-// cluster's shared memory, consecutive parts in its CTAs, so that the choice
-// (select.cuh) reads mass once; then the same memory holds the lists of holes
-// and movers, and all warps of the cluster take pairs of them.  A warp's lanes
-// look up 32 pairs at once and copy K and V rows by 16 bytes, eight loads in
-// flight.  The recent rows may overlap their places: they are read, the
-// cluster waits, they are written.
+__host__ __device__ constexpr int64_t keys_at(int64_t room) { return (room + 3) / 4 * 4; }
+__host__ __device__ constexpr int64_t plan_ints(int64_t room) { return 2 * keys_at(room) + 4; }
+
+// The plan of a row.  A histogram of the keys over their range finds the bin of the last one that stays, its key is found
+// among that bin's by comparing all of them (by further histograms where they are many and not all equal), and what stays is
+// what is above it, and the first ones that equal it.  Passes over the keys are bound by issue slots (30000 of them: 940
+// warp steps), so each makes words of 32 bits, and the rest is done on those, a lane a word.
+template <int T>
+__global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const EvictParams p) {
+  constexpr int kWarps = T / 32;
+  extern __shared__ __align__(16) uint32_t s_dyn[];
+  __shared__ SelectShared<T> s_sel;
+  __shared__ uint32_t s_range[4], s_found, s_cut[2], s_rank[kEvictRanked];
+  __shared__ __align__(8) uint64_t s_copied;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x, h = row % p.hkv, b = row / p.hkv % p.batch, layer = row / p.hkv / p.batch;
+  const int keep = p.keep, recent = p.recent, sinks = p.sinks, edge = keep - recent;  // places below: sinks, then candidates that stay
+  if (tid < 4) s_range[tid] = tid & 1 ? 0 : 0xffffffffu;
+  if (tid == 0) {
+    s_found = 0;
+    mbar_init(&s_copied, 1);
+    fence_barrier_init();
+  }
+  s_sel.clear();
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+  int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
+  int* const plan = p.plan + row * plan_ints(p.room);
+  float* const mass = p.mass + layer * p.ml + b * p.mb + h * p.mh;
+  const int n = length_of(p.map, p.seq_lens, b);
+  if (n <= keep) {
+    if (tid == 0) p.head[row] = make_int2(n, 0);
+    if (source)
+      for (int i = tid; i < keep; i += T) source[i] = i < n ? i : -1;
+    return;
+  }
+  const int c = n - recent - sinks, m = edge - sinks, words = (c + 31) / 32;  // candidates, and those that stay
+  int* const holes = plan;
+  int* const movers = plan + p.room - 1;  // backwards
+  uint32_t pairs = 0;
+  const int* list = nullptr;  // holes and then movers in shared memory, where they fit
+  if (m > 0) {
+    uint32_t* const s_in = s_dyn;            // a bit a candidate: stays
+    uint32_t* const s_equal = s_in + words;  // equals the last one that stays
+    const float* const value = mass + sinks;
+    // whole 16 bytes, and what lies before and behind them
+    const int head = min(c, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(value) & 15)) / 4 & 3)), quads = (c - head) / 4;
+    const bool held = c <= p.held;
+    uint32_t* const keys = (held ? s_dyn + (2 * words + 3) / 4 * 4 : reinterpret_cast<uint32_t*>(plan + keys_at(p.room))) +
+                           (4 - head) % 4;
+    uint32_t least = 0xffffffffu, most = 0;
+    auto take = [&](float v) {
+      const uint32_t k = order_key(v);
+      least = min(least, k);
+      most = max(most, k);
+      return k;
+    };
+    const int rest = c - head - 4 * quads;
+    if (tid < head) keys[tid] = take(value[tid]);
+    if (tid < rest) keys[c - rest + tid] = take(value[c - rest + tid]);
+    const float4* const value4 = reinterpret_cast<const float4*>(value + head);
+    uint4* const keys4 = reinterpret_cast<uint4*>(keys + head);
+    if (held) {  // copied past L1, of which so much shared memory leaves little: loads by the threads took 7 us for 5.5 of 30000
+      if (tid == 0)
+        for (int i = 0; i < quads; i += kEvictCopy) {
+          const uint32_t bytes = 16 * min(kEvictCopy, quads - i);
+          mbar_expect_tx(&s_copied, bytes);
+          bulk_g2s(keys4 + i, value4 + i, bytes, &s_copied, l2_policy_evict_normal());
+        }
+      if (tid == 0) mbar_arrive(&s_copied);
+      if (!mbar_wait_bounded(&s_copied, 0)) {
+        record_status(SN_ERR_TIMEOUT);
+        mbar_wait_bounded(&s_copied, 0);  // once more, as the copies land in this CTA's memory
+      }
+    }
+#pragma unroll 4
+    for (int i = tid; i < quads; i += T) {
+      const float4 v = held ? *reinterpret_cast<const float4*>(keys4 + i) : value4[i];
+      keys4[i] = make_uint4(take(v.x), take(v.y), take(v.z), take(v.w));
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(&s_range[0], least);
+      atomicMax(&s_range[1], most);
+    }
+    __syncthreads();
+    least = s_range[0];
+    const int shift = max(0, 32 - __clz(s_range[1] - least) - SelectShared<T>::kBits);
+    // keys in the lowest bin are counted apart: it is where positions without any weight lie
+    uint32_t low = 0;
+#pragma unroll 4
+    for (int i = tid; i < c; i += T) {
+      const uint32_t d = (keys[i] - least) >> shift;
+      if (d == 0) ++low;
+      else atomicAdd(s_sel.bins() + d, 1u);
+    }
+    low = __reduce_add_sync(0xffffffffu, low);
+    if (lane == 0 && low) atomicAdd(s_sel.bins(), low);
+    __syncthreads();
+    find_bin(static_cast<uint32_t>(m), s_sel);
+    const uint32_t digit = s_sel.digit, here = s_sel.here;
+    uint32_t need = m - s_sel.above;  // of those that equal the last one
+    uint32_t from = least + (digit << shift), upto = from + ((1u << shift) - 1);  // keys that equal it, for all that matters
+    if (here != need) {
+      uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll 4
+      for (int i = tid; i < c; i += T) {
+        const uint32_t k = keys[i];
+        if (k - from > upto - from) continue;
+        lo = min(lo, k);
+        hi = max(hi, k);
+        if (here <= kEvictRanked) s_rank[atomicAdd(&s_found, 1u)] = k;
+      }
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      if (lane == 0) {
+        atomicMin(&s_range[2], lo);
+        atomicMax(&s_range[3], hi);
+      }
+      __syncthreads();
+      if (s_range[2] == s_range[3]) {
+        from = upto = s_range[2];
+      } else if (here <= kEvictRanked) {
+        for (uint32_t k = warp; k < here; k += kWarps) {
+          const uint32_t mine = s_rank[k];
+          uint32_t above = 0, same = 0;
+          for (uint32_t j = lane; j < here; j += 32) {
+            above += s_rank[j] > mine;
+            same += s_rank[j] == mine;
+          }
+          above = __reduce_add_sync(0xffffffffu, above);
+          same = __reduce_add_sync(0xffffffffu, same);
+          if (lane == 0 && above < need && above + same >= need) {  // it, and those equal to it, which write the same
+            s_cut[0] = mine;
+            s_cut[1] = need - above;
+          }
+        }
+        __syncthreads();
+        from = upto = s_cut[0];
+        need = s_cut[1];
+      } else {
+        const Cutoff<uint32_t> cut = find_cutoff<uint32_t>([&](int i) { return keys[i]; }, c, static_cast<uint32_t>(m), s_sel);
+        from = cut.prefix << cut.shift;
+        upto = from + ((1u << cut.shift) - 1);
+        need = cut.need;
+      }
+    }
+#pragma unroll 2
+    for (int w = warp; w < words; w += kWarps) {
+      const int i = 32 * w + lane;
+      const uint32_t k = i < c ? keys[i] : 0;
+      const uint32_t in = __ballot_sync(0xffffffffu, i < c && k > upto), equal = __ballot_sync(0xffffffffu, i < c && k - from <= upto - from);
+      if (lane == 0) {
+        s_in[w] = in;
+        s_equal[w] = equal;
+      }
+    }
+    // ---- words: a warp has consecutive ones ----
+    const int per = (words + kWarps - 1) / kWarps, w0 = min(warp * per, words), w1 = min(w0 + per, words);
+    auto scan = [&](uint32_t v, uint32_t& all) {  // exclusive sums over the lanes, and all of it
+      uint32_t sum = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      all = __shfl_sync(0xffffffffu, sum, 31);
+      return sum - v;
+    };
+    auto before = [&](const uint32_t* counts, uint32_t& all) {  // the sum over the warps before this one, and over all
+      uint32_t v = lane < kWarps ? counts[lane] : 0;
+      const uint32_t sum = scan(v, all);
+      return __shfl_sync(0xffffffffu, sum, warp);
+    };
+    __syncthreads();
+    // the first `need` of the equal ones stay
+    uint32_t mine = 0, all;
+    for (int w = w0 + lane; w < w1; w += 32) mine += __popc(s_equal[w]);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) s_sel.warp[warp] = mine;
+    __syncthreads();
+    uint32_t at = before(s_sel.warp, all);
+    // ... and what does not stay below the edge is a hole, what stays above it moves
+    auto front = [&](int w) {  // the word's candidates below the edge
+      const int k = min(max(edge - (sinks + 32 * w), 0), 32);
+      return k < 32 ? (1u << k) - 1 : 0xffffffffu;
+    };
+    auto valid = [&](int w) { return c - 32 * w < 32 ? (1u << (c - 32 * w)) - 1 : 0xffffffffu; };
+    mine = 0;
+    uint32_t mine_holes = 0;
+    for (int w = w0; w < w1; w += 32) {
+      const int k = w + lane;
+      uint32_t equal = k < w1 ? s_equal[k] : 0;
+      const uint32_t rank = at + scan(__popc(equal), all);
+      at += all;
+      if (k >= w1) continue;
+      const uint32_t left = rank < need ? need - rank : 0;  // of this word's
+      while (static_cast<uint32_t>(__popc(equal)) > left) equal ^= 0x80000000u >> __clz(equal);
+      const uint32_t in = s_in[k] | equal, low_ones = front(k), hole = ~in & low_ones & valid(k), mover = in & ~low_ones;
+      s_in[k] = in;
+      s_equal[k] = hole | mover;
+      mine += __popc(hole | mover);
+      mine_holes += __popc(hole);
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    mine_holes = __reduce_add_sync(0xffffffffu, mine_holes);
+    __syncthreads();  // s_sel.warp has been read
+    if (lane == 0) {
+      s_sel.warp[warp] = mine;
+      s_sel.warp2[warp] = mine_holes;
+    }
+    __syncthreads();
+    at = before(s_sel.warp, all);
+    before(s_sel.warp2, pairs);
+    // the lists: holes come before movers, so that one running count serves both
+    if (held) list = reinterpret_cast<const int*>(keys);  // (the keys are done with)
+    for (int w = w0; w < w1; w += 32) {
+      uint32_t word = w + lane < w1 ? s_equal[w + lane] : 0;
+      const int place = sinks + 32 * (w + lane) - 1;
+      for (uint32_t k = at + scan(__popc(word), all); word; word &= word - 1, ++k) {
+        const int v = place + __ffs(word);
+        *(k < pairs ? holes + k : movers - (k - pairs)) = v;
+        if (held) keys[k] = v;
+      }
+      at += all;
+    }
+  }
+  if (source)  // of what stays where it is, and for now of the holes
+    for (int i = tid; i < edge; i += T) source[i] = i;
+  __syncthreads();
+  if (tid == 0) p.head[row] = make_int2(n, static_cast<int>(pairs));
+  // mass, as the rows will go: movers into holes, then the recent ones, which may overlap their places, then zeros
+  float w[4];
+  auto read_recent = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j * T + tid;
+      if (k < recent) w[j] = mass[n - recent + k];
+    }
+  };
+  read_recent(0);
+#pragma unroll 4
+  for (uint32_t i = tid; i < pairs; i += T) {
+    const int hole = list ? list[i] : holes[i], mover = list ? list[pairs + i] : *(movers - i);
+    mass[hole] = mass[mover];
+    if (source) source[hole] = mover;
+  }
+  __syncthreads();
+  for (int k0 = 0; k0 < recent; k0 += 4 * T) {
+    if (k0 > 0) {
+      read_recent(k0);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j * T + tid;
+      if (k >= recent) continue;
+      mass[edge + k] = w[j];
+      if (source) source[edge + k] = n - recent + k;
+    }
+  }
+  {
+    float* const tail = mass + keep;
+    const int len = n - keep, head = min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tail) & 15)) / 4 & 3)), quads = (len - head) / 4;
+    if (tid < head) tail[tid] = 0.f;
+    if (tid < len - head - 4 * quads) tail[head + 4 * quads + tid] = 0.f;
+    for (int i = tid; i < quads; i += T) reinterpret_cast<float4*>(tail + head)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
+__device__ __forceinline__ uint32_t ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Barrier over the cluster of C CTAs, for what they read and write in global memory.
+__device__ __forceinline__ void cluster_bar(int C) {
+  if (C == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+// One cluster a (layer, stream, head).  All its warps take pairs of holes and movers; when those have left, the recent rows go
+// to their places, which movers may have lain in, and which recent rows may overlap: what the cluster holds at once is read
+// before the barrier, further ones are read and written round by round.  A warp's lanes look up 32 positions at once and copy
+// K and V rows by 16 bytes, eight loads in flight a lane.
 template <typename T, int NU>  // units of T in a position's two rows, 0: 2 * row_bytes / sizeof(T)
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const EvictParams p) {
   constexpr int U = 8;  // units in flight a lane
-  extern __shared__ uint32_t s_keys[];  // [part], then the bits [part / 32]
-  __shared__ SelectShared<kEvictThreads> s_sel;
-  __shared__ uint32_t s_n, s_count[2];
   pdl_launch_dependents();
   pdl_wait();
   uint32_t nranks;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nranks));
   const int C = static_cast<int>(nranks), rank = static_cast<int>(ctarank());
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / C;
-  const int h = row % p.hkv, b = row / p.hkv % p.batch, layer = row / p.hkv / p.batch;
-  if (tid == 0) s_n = length_of(p.map, p.seq_lens, b);
-  cluster_bar(C);
-  const int n = static_cast<int>(peer_u32(&s_n, 0));  // one reading for all of the cluster
-  const int keep = p.keep, recent = p.recent, sinks = p.sinks;
-  int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
-  if (n <= keep) {
-    if (source)
-      for (int i = rank * kEvictThreads + tid; i < keep; i += C * kEvictThreads) source[i] = i < n ? i : -1;
-    cluster_bar(C);  // nobody leaves while its n may be read
-    return;
-  }
-  float* const mass = p.mass + layer * p.ml + b * p.mb + h * p.mh;
-  const int edge = keep - recent;               // places below: sinks, then chosen candidates
-  const int c = n - recent - sinks, m = edge - sinks;  // candidates, and those that stay
-  uint32_t* const s_bits = s_keys + p.part;
-  // this CTA's candidates: positions sinks + i0 .. sinks + i1 - 1
-  const int each = ((c + C - 1) / C + 3) / 4 * 4;
-  const int i0 = min(rank * each, c), i1 = min(i0 + each, c), len = i1 - i0;
-  uint32_t nholes = 0, nmovers = 0;  // in this CTA
-  if (m > 0) {
-    for (int i = tid; i < len; i += kEvictThreads) s_keys[i] = order_key(mass[sinks + i0 + i]);
-    __syncthreads();
-    const Cutoff<uint32_t> cut = find_cutoff(s_keys, len, static_cast<uint32_t>(m), s_sel, C, rank);
-    choose(s_keys, len, cut, s_bits, s_sel);
-    __syncthreads();  // the keys are done with: the lists go over them, holes from the front, movers from the back
-    const int words = (len + 31) / 32, per = (words + kEvictWarps - 1) / kEvictWarps;
-    const int w0 = min(warp * per, words), w1 = min(w0 + per, words);
-    auto split = [&](int w, uint32_t& hole, uint32_t& mover) {  // of word w's candidates
-      const int at = sinks + i0 + 32 * w, there = min(32, len - 32 * w);
-      const uint32_t valid = there < 32 ? (1u << there) - 1 : 0xffffffffu;
-      const int front = min(max(edge - at, 0), 32);  // that many lie below the edge
-      const uint32_t low = front < 32 ? (1u << front) - 1 : 0xffffffffu;
-      hole = ~s_bits[w] & low & valid;
-      mover = s_bits[w] & ~low & valid;
-    };
-    uint32_t nh = 0, nm = 0, hole, mover;
-    for (int w = w0 + lane; w < w1; w += 32) {
-      split(w, hole, mover);
-      nh += __popc(hole);
-      nm += __popc(mover);
-    }
-    nh = __reduce_add_sync(0xffffffffu, nh);
-    nm = __reduce_add_sync(0xffffffffu, nm);
-    if (lane == 0) {
-      s_sel.warp[warp] = nh;
-      s_sel.warp2[warp] = nm;
-    }
-    __syncthreads();
-    uint32_t ah = 0, am = 0;
-    for (int v = 0; v < kEvictWarps; ++v) {
-      if (v == warp) {
-        ah = nholes;
-        am = nmovers;
-      }
-      nholes += s_sel.warp[v];
-      nmovers += s_sel.warp2[v];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    for (int w = w0; w < w1; ++w) {
-      split(w, hole, mover);
-      const int at = sinks + i0 + 32 * w + lane;
-      if ((hole >> lane) & 1) s_keys[ah + __popc(hole & below)] = at;
-      if ((mover >> lane) & 1) s_keys[p.part - 1 - (am + __popc(mover & below))] = at;
-      if (source && at < edge && 32 * w + lane < len && !((hole >> lane) & 1)) source[at] = at;
-      ah += __popc(hole);
-      am += __popc(mover);
-    }
-  }
-  if (source)
-    for (int i = rank * kEvictThreads + tid; i < sinks; i += C * kEvictThreads) source[i] = i;
-  if (tid == 0) {
-    s_count[0] = nholes;
-    s_count[1] = nmovers;
-  }
-  cluster_bar(C);  // the lists and their lengths are there
-
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int keep = p.keep, recent = p.recent, edge = keep - recent;
+  const int64_t row = blockIdx.x / C;
+  const int h = static_cast<int>(row % p.hkv), b = static_cast<int>(row / p.hkv % p.batch), layer = static_cast<int>(row / p.hkv / p.batch);
+  const int* const plan = p.plan + row * plan_ints(p.room);
+  const int2 head = p.head[row];
+  const int n = head.x, pairs = head.y;
+  if (n <= keep) return;
   const int nu = NU ? NU : static_cast<int>(2 * p.row_bytes / sizeof(T));
   char* const base = p.pool + layer * p.layer_bytes + h * p.head_bytes;
   // where a position's K row is, or -1
@@ -142,113 +363,86 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams 
     }
     return pg * p.page_bytes + static_cast<int64_t>(at - blk * p.map.page_size) * p.row_bytes;
   };
-  const int wid = warp * C + rank, warps = kEvictWarps * C;
-
-  // ---- movers into holes ----
-  int hole_at[kEvictCluster + 1], mover_at[kEvictCluster + 1];  // the CTAs' first places in the lists
-  hole_at[0] = mover_at[0] = 0;
+  // Unit u0 + 32 j + this lane of the cnt positions that the lanes have looked up: which of them, and its offset in it.
+  auto unit = [&](int u0, int j, int cnt, int& at) {
+    int e;
+    if constexpr (NU > 0) {  // u0 is a multiple of 32
+      at = u0 / NU + j * (32 / NU) + lane / NU;
+      e = lane % NU;
+    } else {
+      const int u = u0 + 32 * j + lane;
+      at = u / nu;
+      e = u - at * nu;
+    }
+    const bool in = at < cnt;
+    at &= 31;
+    constexpr int64_t size = sizeof(T);
+    return in ? (e >= nu / 2 ? p.kv_bytes - nu / 2 * size : 0) + e * size : int64_t{-1};
+  };
+  auto load = [&](int64_t from, int64_t to, int cnt, int u0, T (&v)[U]) {
 #pragma unroll
-  for (int r = 0; r < kEvictCluster; ++r) {
-    hole_at[r + 1] = hole_at[r] + (r < C ? static_cast<int>(peer_u32(&s_count[0], r)) : 0);
-    mover_at[r + 1] = mover_at[r] + (r < C ? static_cast<int>(peer_u32(&s_count[1], r)) : 0);
-  }
-  const int pairs = min(hole_at[kEvictCluster], mover_at[kEvictCluster]);  // they are equal
+    for (int j = 0; j < U; ++j) {
+      int at;
+      const int64_t off = unit(u0, j, cnt, at), f = __shfl_sync(0xffffffffu, from, at), t = __shfl_sync(0xffffffffu, to, at);
+      if (off >= 0 && f >= 0 && t >= 0) v[j] = *reinterpret_cast<const T*>(base + f + off);
+    }
+  };
+  auto store = [&](int64_t from, int64_t to, int cnt, int u0, const T (&v)[U]) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      int at;
+      const int64_t off = unit(u0, j, cnt, at), f = __shfl_sync(0xffffffffu, from, at), t = __shfl_sync(0xffffffffu, to, at);
+      if (off >= 0 && f >= 0 && t >= 0) *reinterpret_cast<T*>(base + t + off) = v[j];
+    }
+  };
+  const int warps = kMoveWarps * C, wid = warp * C + rank;
+
+  // rows of the recent positions that a warp holds at once, and where this lane's first one is and goes
+  const int per = min(32, max(1, 32 * U / nu)), round = per * warps;
+  int64_t recent_from = -1, recent_to = -1;
+  auto look_up_recent = [&](int k) {
+    recent_from = recent_to = -1;
+    if (lane >= per || k >= recent) return;
+    recent_from = place(n - recent + k);
+    recent_to = place(edge + k);
+  };
+  look_up_recent(wid * per + lane);
+  // ---- movers into holes ----
   const int batch = min(32, (pairs + warps - 1) / warps);
   for (int first = wid * batch; first < pairs; first += warps * batch) {
-    const int cnt = min(batch, pairs - first);
+    const int cnt = min(batch, pairs - first), units = cnt * nu;
     int64_t from = -1, to = -1;
     if (lane < cnt) {
-      const int i = first + lane;
-      int rh = 0, rm = 0, oh = 0, om = 0;
-#pragma unroll
-      for (int r = 1; r < kEvictCluster; ++r) {
-        if (i >= hole_at[r]) rh = r, oh = hole_at[r];
-        if (i >= mover_at[r]) rm = r, om = mover_at[r];
-      }
-      const int hole = static_cast<int>(peer_u32(s_keys + (i - oh), rh));
-      const int mover = static_cast<int>(peer_u32(s_keys + (p.part - 1 - (i - om)), rm));
-      from = place(mover);
-      to = place(hole);
-      mass[hole] = mass[mover];
-      if (source) source[hole] = mover;
-      if (from < 0) to = -1;
+      to = place(plan[first + lane]);
+      from = place(plan[p.room - 1 - (first + lane)]);
     }
-    const int units = cnt * nu;
     for (int u0 = 0; u0 < units; u0 += 32 * U) {
       T v[U];
-      int64_t dst[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = u0 + 32 * j + lane, at = min(u / nu, cnt - 1), e = u - at * nu;
-        const int64_t off = (e >= nu / 2 ? p.kv_bytes - static_cast<int64_t>(nu / 2) * sizeof(T) : 0) + static_cast<int64_t>(e) * sizeof(T);
-        const int64_t f = __shfl_sync(0xffffffffu, from, at);
-        dst[j] = __shfl_sync(0xffffffffu, to, at);
-        if (u >= units) dst[j] = -1;
-        if (dst[j] >= 0) {
-          v[j] = *reinterpret_cast<const T*>(base + f + off);
-          dst[j] += off;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (dst[j] >= 0) *reinterpret_cast<T*>(base + dst[j]) = v[j];
+      load(from, to, cnt, u0, v);
+      store(from, to, cnt, u0, v);
     }
   }
-  cluster_bar(C);  // the movers have left, the lists are done with
-
-  // ---- the recent positions, one after another: n - recent + k -> edge + k ----
+  // ---- the recent positions, n - recent + k -> edge + k ----
   const bool overlap = n - keep < recent;
-  const int per = min(32, max(1, 32 * U / nu)), round = per * warps;  // rows a warp (one a lane to look up), and all, take at once
+  bool moved = false;  // the movers have left
   for (int u0 = 0; u0 < nu; u0 += 32 * U) {  // (a part of the row, where a warp cannot hold a whole one)
     for (int k0 = 0; k0 < recent; k0 += round) {
-      const int mine = k0 + wid * per, cnt = min(max(recent - mine, 0), per), k = mine + lane;
-      int64_t from = -1, to = -1;
-      float w = 0.f;
-      if (lane < cnt) {
-        from = place(n - recent + k);
-        to = place(edge + k);
-        w = mass[n - recent + k];
-        if (from < 0) to = -1;
-      }
-      const int units = min(cnt * nu, u0 + 32 * U);
+      const int mine = k0 + wid * per, cnt = min(max(recent - mine, 0), per);
+      if (moved) look_up_recent(mine + lane);
       T v[U];
-      int64_t dst[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = u0 + 32 * j + lane, at = min(u / nu, max(cnt - 1, 0)), e = u - at * nu;
-        const int64_t off = (e >= nu / 2 ? p.kv_bytes - static_cast<int64_t>(nu / 2) * sizeof(T) : 0) + static_cast<int64_t>(e) * sizeof(T);
-        const int64_t f = __shfl_sync(0xffffffffu, from, at);
-        dst[j] = __shfl_sync(0xffffffffu, to, at);
-        if (u >= units) dst[j] = -1;
-        if (dst[j] >= 0) {
-          v[j] = *reinterpret_cast<const T*>(base + f + off);
-          dst[j] += off;
-        }
-      }
-      if (overlap) cluster_bar(C);
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (dst[j] >= 0) *reinterpret_cast<T*>(base + dst[j]) = v[j];
-      if (lane < cnt && u0 == 0) {
-        mass[edge + k] = w;
-        if (source) source[edge + k] = n - recent + k;
-      }
+      load(recent_from, recent_to, cnt, u0, v);
+      if (!moved || overlap) cluster_bar(C);
+      moved = true;
+      store(recent_from, recent_to, cnt, u0, v);
     }
   }
-  cluster_bar(C);
-  for (int i = keep + rank * kEvictThreads + tid; i < n; i += C * kEvictThreads) mass[i] = 0.f;
 }
 
-constexpr int kPartMost = 49152;  // candidates a CTA holds (200 KB)
-
 template <typename T, int NU>
-int launch_evict(int rows, int C, cudaStream_t st, const EvictParams& p) {
-  const size_t smem = (static_cast<size_t>(p.part) + (p.part + 31) / 32) * sizeof(uint32_t);
-  if (!smem_room<evict_kernel<T, NU>>((kPartMost + kPartMost / 32) * 4)) return SN_ERR_LAUNCH;
+int launch_move(int rows, int C, cudaStream_t st, const EvictParams& p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * C);
-  cfg.blockDim = dim3(kEvictThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(kMoveThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -259,11 +453,17 @@ int launch_evict(int rows, int C, cudaStream_t st, const EvictParams& p) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, evict_kernel<T, NU>, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, evict_move_kernel<T, NU>, p) != cudaSuccess) {
     cudaGetLastError();
     return SN_ERR_LAUNCH;
   }
   return SN_OK;
+}
+
+template <int T>
+int launch_plan(int rows, size_t smem, cudaStream_t st, const EvictParams& p) {
+  if (!smem_room<evict_plan_kernel<T>>(kEvictWords * 4)) return SN_ERR_LAUNCH;
+  return launch(evict_plan_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(T), smem, st, true, p);
 }
 
 }  // namespace
@@ -272,23 +472,30 @@ int tu_status_evict(bool reset, cudaStream_t st, int* out) { return read_tu_stat
 
 }  // namespace sn
 
-extern "C" int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
-                                  const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
-                                  float* mass, int64_t mass_layer_stride, int64_t mass_batch_stride,
-                                  int64_t mass_head_stride, int batch, int keep, int recent, int sinks, int* source,
-                                  void* stream) {
-  if (!pool || !page_table || !seq_lens || !mass || layers < 1 || num_pages < 1 || page_size < 1 || nheads_kv < 1 ||
-      head_dim < 1 || max_pages < 1 || table_stride < max_pages || batch < 1 || keep < 1 || recent < 0 || sinks < 0 ||
-      recent > keep || sinks > keep - recent)
+extern "C" {
+
+size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions) {
+  if (layers < 1 || batch < 1 || nheads_kv < 1 || max_positions < 1) return 0;
+  return static_cast<size_t>(layers) * batch * nheads_kv * (sizeof(int2) + sn::plan_ints(max_positions) * sizeof(int)) + 16;
+}
+
+int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
+                       const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens, float* mass,
+                       int64_t mass_layer_stride, int64_t mass_batch_stride, int64_t mass_head_stride, int batch,
+                       int keep, int recent, int sinks, int* source, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  if (!pool || !page_table || !seq_lens || !mass || !workspace || layers < 1 || num_pages < 1 || page_size < 1 ||
+      nheads_kv < 1 || head_dim < 1 || max_pages < 1 || table_stride < max_pages || batch < 1 || keep < 1 || recent < 0 ||
+      sinks < 0 || recent > keep || sinks > keep - recent)
     return SN_ERR_INVALID_ARGUMENT;
   const int64_t room = static_cast<int64_t>(max_pages) * page_size;
   if ((nheads_kv > 1 && mass_head_stride < room) || (batch > 1 && mass_batch_stride < room) ||
-      (layers > 1 && mass_layer_stride < room))
+      (layers > 1 && mass_layer_stride < room) ||
+      workspace_bytes < sn_evict_workspace_size(layers, batch, nheads_kv, room))
     return SN_ERR_INVALID_ARGUMENT;
+  if (!sn::aligned16(workspace)) return SN_ERR_MISALIGNED;
   const int64_t rows = static_cast<int64_t>(layers) * batch * nheads_kv;
-  if (rows > INT32_MAX / sn::kEvictCluster || head_dim > 8192 ||
-      room > static_cast<int64_t>(sn::kEvictCluster) * (sn::kPartMost - 4))
-    return SN_ERR_UNSUPPORTED;
+  if (rows > INT32_MAX / sn::kMoveCluster || head_dim > 8192 || room > sn::kEvictMost) return SN_ERR_UNSUPPORTED;
   sn::EvictParams p;
   p.pool = static_cast<char*>(pool);
   p.row_bytes = 2 * head_dim;
@@ -303,23 +510,29 @@ extern "C" int sn_evict_positions(void* pool, int layers, int num_pages, int pag
   p.mb = mass_batch_stride;
   p.mh = mass_head_stride;
   p.source = source;
+  p.head = static_cast<int2*>(workspace);
+  p.plan = reinterpret_cast<int*>(p.head + (rows + 1) / 2 * 2);
+  p.room = static_cast<int>(room);
   p.batch = batch;
   p.hkv = nheads_kv;
   p.keep = keep;
   p.recent = recent;
   p.sinks = sinks;
-  // CTAs a row: as many as the shared memory asks for, and more where there are few long rows
-  int C = 1;
-  while (C < sn::kEvictCluster && (room > static_cast<int64_t>(C) * (sn::kPartMost - 4) ||
-                                  (rows * C < 2 * sn::sm_count() && room > 1024 * C)))
-    C *= 2;
-  p.part = static_cast<int>((room + C - 1) / C + 4);
+  const int bits = static_cast<int>((room + 31) / 32 * 2 + 8);  // two a candidate, and room to align the keys
+  p.held = room <= sn::kEvictWords - bits ? static_cast<int>(room) : 0;
+  const size_t smem = static_cast<size_t>(bits + p.held) * sizeof(uint32_t);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int r = static_cast<int>(rows);
+  const int rc = rows <= sn::sm_count() ? sn::launch_plan<1024>(r, smem, st, p) : sn::launch_plan<512>(r, smem, st, p);
+  if (rc != SN_OK) return rc;
+  // three CTAs fit on an SM; two a row at least, as not all of the streams may be cut
+  const int C = static_cast<int>(std::clamp<int64_t>(3 * sn::sm_count() / rows, 2, sn::kMoveCluster));
   if (sn::aligned16(pool) && p.row_bytes % 16 == 0) {
-    if (head_dim == 128) return sn::launch_evict<uint4, 32>(r, C, st, p);
-    if (head_dim == 64) return sn::launch_evict<uint4, 16>(r, C, st, p);
-    return sn::launch_evict<uint4, 0>(r, C, st, p);
+    if (head_dim == 128) return sn::launch_move<uint4, 32>(r, C, st, p);
+    if (head_dim == 64) return sn::launch_move<uint4, 16>(r, C, st, p);
+    return sn::launch_move<uint4, 0>(r, C, st, p);
   }
-  return sn::launch_evict<uint16_t, 0>(r, C, st, p);
+  return sn::launch_move<uint16_t, 0>(r, C, st, p);
 }
+
+}  // extern "C"

@@ -350,9 +350,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const 
   const uint32_t below = (1u << lane) - 1;
   const int row = blockIdx.x, b = row / p.hkv, hk = row - b * p.hkv;
   if (tid < 3) s_range[tid] = tid == 0 ? 0xffffffffu : 0;
-  constexpr int Q = SelectShared<kChooseThreads>::kQuads;
-#pragma unroll
-  for (int q = 0; q < Q; ++q) s_sel.hist[0][Q * tid + q] = make_uint4(0, 0, 0, 0);
+  s_sel.clear();
   pdl_launch_dependents();
   pdl_wait();
   int* const out = p.blocks + static_cast<int64_t>(row) * p.count;
@@ -417,16 +415,15 @@ __global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const 
     }
     __syncthreads();
     least = s_range[0];
-    const int shift = max(0, 32 - __clz(s_range[1] - least) - kDigitBits);
-    uint32_t* const bins = reinterpret_cast<uint32_t*>(s_sel.hist[0]);
+    const int shift = max(0, 32 - __clz(s_range[1] - least) - SelectShared<kChooseThreads>::kBits);
 #pragma unroll
     for (int j = 0; j < kChooseHeld; ++j)
-      if (tid + j * kChooseThreads < len) atomicAdd(bins + min((held[j] - least) >> shift, kBins - 1u), 1u);
+      if (tid + j * kChooseThreads < len) atomicAdd(s_sel.bins() + min((held[j] - least) >> shift, SelectShared<kChooseThreads>::kBins - 1u), 1u);
 #pragma unroll 4
     for (int i = tid + kChooseHeld * kChooseThreads; i < len; i += kChooseThreads)
-      atomicAdd(bins + min((scores[i].x - least) >> shift, kBins - 1u), 1u);
+      atomicAdd(s_sel.bins() + min((scores[i].x - least) >> shift, SelectShared<kChooseThreads>::kBins - 1u), 1u);
     __syncthreads();
-    find_bin<Q>(s_sel.hist[0], static_cast<uint32_t>(need), s_sel, 1, 0);
+    find_bin(static_cast<uint32_t>(need), s_sel);
     const uint32_t first_key = least + (s_sel.digit << shift);
     const float E2 = fmaf(__uint_as_float(s_range[2]), 0x1p-12f, 0x1p-109f);  // 2 E
     const float lo = order_value(first_key) - E2, hi = order_value(first_key + ((1u << shift) - 1)) + E2;
@@ -497,8 +494,9 @@ __global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const 
             if (lane == 0) exact[k] = key;
           }
         __syncthreads();
-        const Cutoff<uint64_t> cut = find_cutoff(exact, static_cast<int>(all_open), wanted, s_sel, 1, 0);
-        choose(exact, static_cast<int>(all_open), cut, s_won, s_sel);
+        auto key = [&](int i) { return exact[i]; };
+        const Cutoff<uint64_t> cut = find_cutoff<uint64_t>(key, static_cast<int>(all_open), wanted, s_sel);
+        choose(key, static_cast<int>(all_open), cut, s_won, s_sel);
         __syncthreads();
         k = open_at;
         for (int w = w0; w < w1; ++w) {  // back to their blocks
@@ -512,8 +510,9 @@ __global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const 
       __syncthreads();
     }
   } else {
-    const Cutoff<uint64_t> cut = find_cutoff(exact, len, static_cast<uint32_t>(need), s_sel, 1, 0);
-    choose(exact, len, cut, s_in, s_sel);
+    auto key = [&](int i) { return exact[i]; };
+    const Cutoff<uint64_t> cut = find_cutoff<uint64_t>(key, len, static_cast<uint32_t>(need), s_sel);
+    choose(key, len, cut, s_in, s_sel);
     for (int w = tid; w < words; w += kChooseThreads) s_open[w] = 0;
     __syncthreads();
   }

@@ -13,7 +13,7 @@ from .. import _lib, build
 
 _FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_copy_pages",
                  "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size", "sn_paged_decode_attention_mass",
-                 "sn_paged_mass_workspace_size", "sn_evict_positions", "sn_update_page_bounds", "sn_select_blocks",
+                 "sn_paged_mass_workspace_size", "sn_evict_positions", "sn_evict_workspace_size", "sn_update_page_bounds", "sn_select_blocks",
                  "sn_select_blocks_workspace_size",
                  "sn_paged_sparse_attention")
 
