@@ -277,8 +277,14 @@ class PagedKVCache:
     and one copy_pages call moves a page everywhere.  `page_table` int32
     [slots, max_pages] and `seq_lens` int32 [slots] are device tensors that
     reserve / fork / free / compact update in place, so a captured decode step
-    goes on using them.  Full pages may be shared between forked streams (they
-    are never written again); a stream's last, partly filled page never is."""
+    goes on using them.  Full pages may be shared between forked streams (only
+    evict writes to them, in copies of its own); a stream's last, partly filled
+    page never is.
+
+    track_mass and track_bounds add what paged_evict and paged_sparse keep
+    beside the pages, which then follows them: `mass` fp32 [n_layers, slots,
+    nheads_kv, max_pages * page_size], `bounds` bf16 [n_layers, num_pages,
+    nheads_kv, 2, head_dim]."""
 
     def __init__(self, n_layers: int, num_pages: int, nheads_kv: int, head_dim: int, slots: int, max_pages: int,
                  page_size: int = 16, device="cuda"):
@@ -292,12 +298,29 @@ class PagedKVCache:
         self.lens = [0] * slots
         self._users = [0] * num_pages
         self._free = list(range(num_pages))  # a heap: the lowest free page first
+        self.mass = self.bounds = None
 
     def k(self, layer: int) -> torch.Tensor:
         return self.pool[layer, 0]
 
     def v(self, layer: int) -> torch.Tensor:
         return self.pool[layer, 1]
+
+    def track_mass(self) -> torch.Tensor:
+        """The weights that paged_decode_attention_mass adds up, zeros so far:
+        mass[layer] is its argument."""
+        if self.mass is None:
+            layers, _, _, heads = self.pool.shape[:4]
+            self.mass = torch.zeros(layers, len(self.lens), heads, self.max_pages * self.page_size, device=self.pool.device)
+        return self.mass
+
+    def track_bounds(self) -> torch.Tensor:
+        """Room for the bounds of the keys' pages: bounds[layer] is the argument of
+        update_page_bounds, to be called for the new tokens, and select_blocks."""
+        if self.bounds is None:
+            from .paged_sparse import page_bounds
+            self.bounds = page_bounds(self.pool[:, 0])
+        return self.bounds
 
     @property
     def free_pages(self) -> int:
@@ -352,6 +375,8 @@ class PagedKVCache:
             self.pages[dst].append(self._take())
             self._copy([self.pages[src][full]], [self.pages[dst][full]])
         self.lens[dst] = self.lens[src]
+        if self.mass is not None:
+            self.mass[:, dst].copy_(self.mass[:, src])
         self._upload([dst])
 
     def free(self, slot: int) -> None:
@@ -359,7 +384,54 @@ class PagedKVCache:
         for p in self.pages[slot]:
             self._drop(p)
         self.pages[slot], self.lens[slot] = [], 0
+        if self.mass is not None:
+            self.mass[:, slot].zero_()
         self._upload([slot])
+
+    def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> list[int]:
+        """Cuts every stream with more than `keep` positions down to `keep`, by the
+        weights of track_mass (paged_evict.evict_positions); returns the slots that
+        were cut.  Pages that another stream shares are copied first; nothing is
+        changed if there are not enough free ones for that."""
+        if self.mass is None:
+            raise RuntimeError("eviction goes by the positions' weights: track_mass() before the first token")
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"keep must be positive and cover recent and sinks, which must not be negative: got {keep}, {recent}, {sinks}")
+        cut = [s for s, n in enumerate(self.lens) if n > keep]
+        if not cut:
+            return []
+        stay = -(-keep // self.page_size)  # pages of a cut stream, all of which may be written
+        users, own = list(self._users), []  # (slot, place) of the pages that become copies
+        for s in cut:
+            for i, p in enumerate(self.pages[s][:stay]):
+                if users[p] > 1:
+                    users[p] -= 1
+                    own.append((s, i))
+        if len(own) > len(self._free):
+            raise RuntimeError(f"out of pages: {len(own)} needed, {len(self._free)} free")
+        src = [self.pages[s][i] for s, i in own]
+        dst = [self._take() for _ in own]
+        if own:
+            self._copy(src, dst)
+            for (s, i), p in zip(own, dst):
+                self._drop(self.pages[s][i])
+                self.pages[s][i] = p
+            self._upload({s for s, _ in own})
+        from . import paged_evict
+        paged_evict.evict_positions(self.pool, self.page_table, self.seq_lens, self.mass, keep, recent=recent, sinks=sinks)
+        for s in cut:
+            for p in self.pages[s][stay:]:
+                self._drop(p)
+            del self.pages[s][stay:]
+            self.lens[s] = keep
+        self._upload(cut)
+        if self.bounds is not None:
+            from . import paged_sparse
+            new = [keep if s in cut else 0 for s in range(len(self.lens))]
+            cu = torch.tensor([sum(new[:s]) for s in range(len(new) + 1)], dtype=torch.int32, device=self.pool.device)
+            for layer in range(self.pool.shape[0]):
+                paged_sparse.update_page_bounds(self.k(layer), self.bounds[layer], self.page_table, self.seq_lens, cu_seqlens=cu)
+        return cut
 
     def compact(self) -> int:
         """Moves used pages to the lowest numbers; returns how many moved.  (The
@@ -379,5 +451,7 @@ class PagedKVCache:
         return len(src)
 
     def _copy(self, src, dst) -> None:
-        dev = self.pool.device
-        copy_pages(self.pool, torch.tensor(src, dtype=torch.int32, device=dev), torch.tensor(dst, dtype=torch.int32, device=dev))
+        src, dst = (torch.tensor(v, dtype=torch.int32, device=self.pool.device) for v in (src, dst))
+        copy_pages(self.pool, src, dst)
+        if self.bounds is not None:
+            copy_pages(self.bounds, src, dst)
