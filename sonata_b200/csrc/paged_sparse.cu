@@ -40,7 +40,7 @@ __device__ __forceinline__ int64_t first_slot(const BoundsParams& p, int b) {
 // Work items: (touched page, head).
 __device__ __forceinline__ int64_t bounds_items(const BoundsParams& p) { return (p.cu ? first_slot(p, p.batch) : p.batch) * p.hkv; }
 
-// The page of work item `slot` and the keys that count in it, or -1.
+// The page of work item `slot` and the keys that count in it, or -1; a warp.
 __device__ __forceinline__ int touched(const BoundsParams& p, int64_t slot, int& rows) {
   int b, block;
   if (!p.cu) {
@@ -50,12 +50,15 @@ __device__ __forceinline__ int touched(const BoundsParams& p, int64_t slot, int&
     block = (n - 1) / p.map.page_size;
     rows = n - block * p.map.page_size;
   } else {
-    int lo = 0, hi = p.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first_slot(p, mid) <= slot) lo = mid; else hi = mid - 1;
+    // the last stream that begins at or before the slot, 32 of them looked at at a time
+    const int lane = threadIdx.x & 31;
+    b = -1;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int some = __popc(__ballot_sync(0xffffffffu, b0 + lane < p.batch && first_slot(p, min(b0 + lane, p.batch - 1)) <= slot));
+      b += some;
+      if (some < 32) break;
     }
-    b = lo;
+    if (b < 0) return -1;
     const int n = length_of(p.map, p.seq_lens, b), fresh = min(p.cu[b + 1] - p.cu[b], n);
     if (fresh < 1) return -1;
     const int64_t at = (n - fresh) / p.map.page_size + (slot - first_slot(p, b));
@@ -99,11 +102,15 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsParams p) 
     lo.x = lo.y = lo.z = lo.w = 0x7f807f80u;  // infinities
     hi.x = hi.y = hi.z = hi.w = 0xff80ff80u;
     if (c < pieces) {
-#pragma unroll 8
-      for (int r = group; r < rows; r += groups) {
-        const uint4 k = *reinterpret_cast<const uint4*>(src + r * p.ks.tok);
-        lo.x = min2(lo.x, k.x), lo.y = min2(lo.y, k.y), lo.z = min2(lo.z, k.z), lo.w = min2(lo.w, k.w);
-        hi.x = max2(hi.x, k.x), hi.y = max2(hi.y, k.y), hi.z = max2(hi.z, k.z), hi.w = max2(hi.w, k.w);
+      for (int r0 = group; r0 < rows; r0 += 8 * groups) {  // eight loads in flight, the last row's again past the end
+        uint4 k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const uint4*>(src + min(r0 + j * groups, rows - 1) * p.ks.tok);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          lo.x = min2(lo.x, k[j].x), lo.y = min2(lo.y, k[j].y), lo.z = min2(lo.z, k[j].z), lo.w = min2(lo.w, k[j].w);
+          hi.x = max2(hi.x, k[j].x), hi.y = max2(hi.y, k[j].y), hi.z = max2(hi.z, k[j].z), hi.w = max2(hi.w, k[j].w);
+        }
       }
     }
     for (int o = L; o < 32; o *= 2) {
