@@ -182,8 +182,6 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 // of a few kilobytes between the CTAs took 2 to 3 us each (22 us for the three
 // streams).
 // ---------------------------------------------------------------------------
-constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
-constexpr int kChooseHeld = 16;     // keys a thread holds
 constexpr int kFewExact = 64;        // blocks that are ranked by comparing all of them
 constexpr int kChooseMost = 262144;  // blocks of a stream: three bits each in shared memory
 
@@ -215,7 +213,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 
 // Scores in 32 bits.  A warp takes 16 blocks at a time, their bounds straight from memory as operands: the contraction index
 // may be permuted as long as both sides agree, so lane (g, t) takes the 16-byte chunks t, t + 4, ... of blocks g and g + 8,
-// and of query head g.  blockIdx.y is the row, blockIdx.x takes groups of 64 blocks, gridDim.x of them apart.
+// and of query head g.  (Brought to a ring in shared memory by bulk copies, two tiles in flight: 48 ragged streams 16.5 us for
+// 14.5, the three long ones 17.7 for 16.4.)  blockIdx.y is the row, blockIdx.x takes groups of 64 blocks, gridDim.x of them apart.
 template <int HD>
 __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams p) {
   constexpr int KC = HD / 32;  // chunks a lane takes of a row
@@ -346,8 +345,9 @@ __global__ void __launch_bounds__(128) exact_scores_kernel(const SelectParams p)
 }
 
 // One CTA a row; kScored: block_scores_kernel has run, else exact_scores_kernel.
-template <bool kScored>
-__global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const SelectParams p) {
+template <bool kScored, int kChooseThreads>
+__global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) choose_blocks_kernel(const SelectParams p) {
+  constexpr int kChooseWarps = kChooseThreads / 32, kChooseHeld = kChooseThreads > 512 ? 8 : 16;  // keys a thread holds
   extern __shared__ uint32_t s_bits[];
   __shared__ SelectShared<kChooseThreads> s_sel;
   __shared__ uint32_t s_range[3];  // least and greatest key, S
@@ -540,6 +540,12 @@ __global__ void __launch_bounds__(kChooseThreads, 2) choose_blocks_kernel(const 
   }
 }
 
+template <bool kScored, int T>
+int launch_choose(int rows, size_t smem, cudaStream_t st, const SelectParams& p) {
+  if (!smem_room<choose_blocks_kernel<kScored, T>>(kChooseMost / 32 * 3 * sizeof(uint32_t))) return SN_ERR_LAUNCH;
+  return launch(choose_blocks_kernel<kScored, T>, dim3(static_cast<unsigned>(rows)), dim3(T), smem, st, true, p);
+}
+
 }  // namespace
 
 int tu_status_sparse(bool reset, cudaStream_t st, int* out) { return read_tu_status(reset, st, out); }
@@ -615,9 +621,6 @@ int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_strid
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool scored = sn::aligned16(bounds) && (head_dim == 64 || head_dim == 128);
   const size_t smem = static_cast<size_t>((max_pages + 31) / 32) * 3 * sizeof(uint32_t);
-  constexpr int kRoom = sn::kChooseMost / 32 * 3 * sizeof(uint32_t);
-  if (!(scored ? sn::smem_room<sn::choose_blocks_kernel<true>>(kRoom) : sn::smem_room<sn::choose_blocks_kernel<false>>(kRoom)))
-    return SN_ERR_LAUNCH;
   if (max_pages > count) {  // there may be something to compare
     // as many CTAs a row as the table has blocks for, and over all rows no more than a few for each place on the device:
     // the lengths are on the device
@@ -629,9 +632,11 @@ int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_strid
                                     : sn::launch(sn::block_scores_kernel<128>, grid, dim3(128), 0, st, true, p);
     if (rc != SN_OK) return rc;
   }
-  const dim3 grid(static_cast<unsigned>(rows));
-  return scored ? sn::launch(sn::choose_blocks_kernel<true>, grid, dim3(sn::kChooseThreads), smem, st, true, p)
-                : sn::launch(sn::choose_blocks_kernel<false>, grid, dim3(sn::kChooseThreads), smem, st, true, p);
+  // the choice is a chain of steps: more threads a row where there are few rows (3 streams of up to 100001 positions, 12 rows:
+  // 256 threads 18.9 us, 512 16.4, 1024 18.7), two CTAs an SM where there are many
+  const int r = static_cast<int>(rows);
+  if (!scored) return sn::launch_choose<false, 256>(r, smem, st, p);
+  return rows <= sn::sm_count() ? sn::launch_choose<true, 512>(r, smem, st, p) : sn::launch_choose<true, 256>(r, smem, st, p);
 }
 
 }  // extern "C"
