@@ -669,7 +669,7 @@ int sn_paged_decode_attention_mass(const void *q, int64_t q_batch_stride, int64_
                                    int64_t mass_batch_stride, int64_t mass_head_stride, void *out, float *lse,
                                    float scale, int batch, int nheads, int nheads_kv, int head_dim, void *workspace,
                                    size_t workspace_bytes, void *stream);
-size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions);
+size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions, int keep);
 int sn_evict_positions(void *pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
                        const int *page_table, int64_t table_stride, int max_pages, const int *seq_lens, float *mass,
                        int64_t mass_layer_stride, int64_t mass_batch_stride, int64_t mass_head_stride, int batch,

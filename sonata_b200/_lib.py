@@ -87,7 +87,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                                        _I64, _P, _P, ctypes.c_float, _I, _I, _I, _I, _P, ctypes.c_size_t, _P], _I),
     "sn_evict_positions": ([_P, _I, _I, _I, _I, _I, _P, _I64, _I, _P, _P, _I64, _I64, _I64, _I, _I, _I, _I, _P, _P, ctypes.c_size_t, _P],
                            _I),
-    "sn_evict_workspace_size": ([_I, _I, _I, _I64], ctypes.c_size_t),
+    "sn_evict_workspace_size": ([_I, _I, _I, _I64, _I], ctypes.c_size_t),
     "sn_update_page_bounds": ([_P, _I64, _I64, _I64, _I, _I, _P, _I64, _I, _P, _P, _I, _I, _I, _P, _P], _I),
     "sn_select_blocks_workspace_size": ([_I, _I, _I], ctypes.c_size_t),
     "sn_select_blocks": ([_P, _I64, _I64, _P, _I, _I, _P, _I64, _I, _P] + [_I] * 7 + [_P, _P, ctypes.c_size_t, _P], _I),

@@ -25,6 +25,7 @@ struct Abi {  // of the loaded libsonata_b200.so, set by bind()
   decltype(&sn_paged_decode_attention) attend;
   decltype(&sn_paged_decode_workspace_size) attend_size;
   decltype(&sn_rotary_paged_append) append;
+  decltype(&sn_rotary_paged_append_at) append_at;
   decltype(&sn_copy_pages) copy;
   decltype(&sn_mamba2_prompt) prompt;
   decltype(&sn_mamba2_prompt_workspace_size) prompt_size;
@@ -212,7 +213,7 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (layers > INT32_MAX || pages > INT32_MAX || heads > INT32_MAX || page > INT32_MAX || hd > INT32_MAX ||
       !mass_ok(m, 4, t.width * page, dev) || m->size(0) != layers || m->size(1) != t.streams || m->size(2) != heads)
     Py_RETURN_NONE;
-  const size_t need = abi.evict_size(static_cast<int>(layers), static_cast<int>(t.streams), static_cast<int>(heads), t.width * page);
+  const size_t need = abi.evict_size(static_cast<int>(layers), static_cast<int>(t.streams), static_cast<int>(heads), t.width * page, keep);
   Tensor ws = at::empty({static_cast<int64_t>(need)}, pool->options().dtype(at::kByte)), source;
   if (a[7] == Py_True) source = at::empty({layers, t.streams, heads, keep}, pool->options().dtype(at::kInt));
   const int rc = abi.evict(pool->data_ptr(), static_cast<int>(layers), static_cast<int>(pages), static_cast<int>(page),
@@ -280,9 +281,9 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 10) Py_RETURN_NONE;
+  if (n != 10 && n != 11) Py_RETURN_NONE;
   const int dev = current_device();
-  const Tensor *qkv = tensor(a[0]), *cos = tensor(a[5]), *sin = tensor(a[6]), *cu;
+  const Tensor *qkv = tensor(a[0]), *cos = tensor(a[5]), *sin = tensor(a[6]), *cu, *angle = nullptr;
   Pages p;
   int heads;
   if (!is(qkv, at::kBFloat16, 2, dev) || !p.read(a + 1, dev) || !is(cos, at::kFloat, 2, dev) ||
@@ -291,17 +292,20 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t tokens = qkv->size(0), width = (heads + 2 * p.heads) * p.hd;
   if (tokens < 1 || tokens > INT32_MAX || qkv->size(1) != width || qkv->stride(1) != 1 || cos->size(0) < 1 ||
-      cos->size(0) > INT32_MAX || 2 * cos->size(1) > p.hd || (!cu && tokens != p.streams) || p.streams > INT32_MAX)
+      cos->size(0) > INT32_MAX || 2 * cos->size(1) > p.hd || (!cu && tokens != p.streams) || p.streams > INT32_MAX ||
+      (n == 11 && !dense_or_none(a[10], &angle, at::kInt, {tokens}, dev)))
     Py_RETURN_NONE;
   Tensor q = at::empty({tokens, heads, p.hd}, qkv->options());
-  const int rc = abi.append(qkv->data_ptr(), tokens > 1 ? qkv->stride(0) : width, q.data_ptr(), p.k->data_ptr(),
-                            p.stride(p.k, 0), p.stride(p.k, 1), p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1),
-                            p.stride(p.v, 2), static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(),
-                            p.table_stride(), static_cast<int>(p.width), p.lens->data_ptr<int>(),
-                            cu ? cu->data_ptr<int>() : nullptr, cos->data_ptr<float>(), sin->data_ptr<float>(),
-                            static_cast<int>(cos->size(0)), static_cast<int>(tokens), static_cast<int>(p.streams), heads,
-                            static_cast<int>(p.heads), static_cast<int>(p.hd), static_cast<int>(2 * cos->size(1)),
-                            a[9] == Py_True, current_stream(dev));
+  auto launch = [&](auto f, auto... positions) {
+    return f(qkv->data_ptr(), tokens > 1 ? qkv->stride(0) : width, q.data_ptr(), p.k->data_ptr(), p.stride(p.k, 0),
+             p.stride(p.k, 1), p.stride(p.k, 2), p.v->data_ptr(), p.stride(p.v, 0), p.stride(p.v, 1), p.stride(p.v, 2),
+             static_cast<int>(p.n), static_cast<int>(p.page), p.table->data_ptr<int>(), p.table_stride(),
+             static_cast<int>(p.width), p.lens->data_ptr<int>(), cu ? cu->data_ptr<int>() : nullptr, positions...,
+             cos->data_ptr<float>(), sin->data_ptr<float>(), static_cast<int>(cos->size(0)), static_cast<int>(tokens),
+             static_cast<int>(p.streams), heads, static_cast<int>(p.heads), static_cast<int>(p.hd),
+             static_cast<int>(2 * cos->size(1)), static_cast<int>(a[9] == Py_True), current_stream(dev));
+  };
+  const int rc = angle ? launch(abi.append_at, static_cast<const int*>(angle->data_ptr<int>())) : launch(abi.append);
   return rc ? status(rc) : THPVariable_Wrap(std::move(q));
   END_HANDLE_TH_ERRORS
 }
@@ -372,7 +376,7 @@ PyObject* bind(PyObject*, PyObject* table) {
     return true;
   };
   if (!get("sn_paged_decode_attention", abi.attend) || !get("sn_paged_decode_workspace_size", abi.attend_size) ||
-      !get("sn_rotary_paged_append", abi.append) || !get("sn_copy_pages", abi.copy) ||
+      !get("sn_rotary_paged_append", abi.append) || !get("sn_rotary_paged_append_at", abi.append_at) || !get("sn_copy_pages", abi.copy) ||
       !get("sn_mamba2_prompt", abi.prompt) || !get("sn_mamba2_prompt_workspace_size", abi.prompt_size) ||
       !get("sn_paged_decode_attention_mass", abi.mass) || !get("sn_paged_mass_workspace_size", abi.mass_size) ||
       !get("sn_evict_positions", abi.evict) || !get("sn_evict_workspace_size", abi.evict_size) ||

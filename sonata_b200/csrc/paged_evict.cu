@@ -39,14 +39,19 @@ struct EvictParams {
   int64_t ml, mb, mh;
   int* source;  // [layers, batch, hkv, keep] or null
   int2* head;   // [layers, batch, hkv]: n, pairs of a hole and a mover
-  int* plan;    // [layers, batch, hkv] of plan_ints: holes from the front and movers from the back, then keys
-  int room;     // max_pages * page_size
+  int* plan;    // [layers, batch, hkv] of plan_ints: holes, movers, and the keys where shared memory does not hold them
+  int64_t plan_ints;
+  int most;     // pairs of a row at most, a multiple of 4
   int batch, hkv, keep, recent, sinks;
   int held;     // keys in shared memory: all candidates' or none (then they are in the plan)
 };
 
-__host__ __device__ constexpr int64_t keys_at(int64_t room) { return (room + 3) / 4 * 4; }
-__host__ __device__ constexpr int64_t plan_ints(int64_t room) { return 2 * keys_at(room) + 4; }
+// Of max_pages * page_size = room positions: the words of shared memory for two bits each, and room to align the keys;
+// whether it holds their keys as well; pairs of a hole and a mover at most, and the integers of a row's plan.
+int64_t bit_words(int64_t room) { return (room + 31) / 32 * 2 + 8; }
+bool keys_held(int64_t room) { return bit_words(room) + room <= kEvictWords; }
+int64_t most_pairs(int64_t room, int64_t keep) { return (std::min(room / 2, keep) + 3) / 4 * 4; }
+int64_t plan_size(int64_t room, int64_t keep) { return 2 * most_pairs(room, keep) + (keys_held(room) ? 0 : (room + 3) / 4 * 4 + 4); }
 
 // The plan of a row.  A histogram of the keys over their range finds the bin of the last one that stays, its key is found
 // among that bin's by comparing all of them (by further histograms where they are many and not all equal), and what stays is
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
   pdl_launch_dependents();
   pdl_wait();
   int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
-  int* const plan = p.plan + row * plan_ints(p.room);
+  int* const plan = p.plan + row * p.plan_ints;
   float* const mass = p.mass + layer * p.ml + b * p.mb + h * p.mh;
   const int n = length_of(p.map, p.seq_lens, b);
   if (n <= keep) {
@@ -83,8 +88,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     return;
   }
   const int c = n - recent - sinks, m = edge - sinks, words = (c + 31) / 32;  // candidates, and those that stay
-  int* const holes = plan;
-  int* const movers = plan + p.room - 1;  // backwards
+  int *const holes = plan, *const movers = plan + p.most;
   uint32_t pairs = 0;
   const int* list = nullptr;  // holes and then movers in shared memory, where they fit
   if (m > 0) {
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     // whole 16 bytes, and what lies before and behind them
     const int head = min(c, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(value) & 15)) / 4 & 3)), quads = (c - head) / 4;
     const bool held = c <= p.held;
-    uint32_t* const keys = (held ? s_dyn + (2 * words + 3) / 4 * 4 : reinterpret_cast<uint32_t*>(plan + keys_at(p.room))) +
+    uint32_t* const keys = (held ? s_dyn + (2 * words + 3) / 4 * 4 : reinterpret_cast<uint32_t*>(plan + 2 * p.most)) +
                            (4 - head) % 4;
     uint32_t least = 0xffffffffu, most = 0;
     auto take = [&](float v) {
@@ -269,7 +273,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
       const int place = sinks + 32 * (w + lane) - 1;
       for (uint32_t k = at + scan(__popc(word), all); word; word &= word - 1, ++k) {
         const int v = place + __ffs(word);
-        *(k < pairs ? holes + k : movers - (k - pairs)) = v;
+        *(k < pairs ? holes + k : movers + (k - pairs)) = v;
         if (held) keys[k] = v;
       }
       at += all;
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
   read_recent(0);
 #pragma unroll 4
   for (uint32_t i = tid; i < pairs; i += T) {
-    const int hole = list ? list[i] : holes[i], mover = list ? list[pairs + i] : *(movers - i);
+    const int hole = list ? list[i] : holes[i], mover = list ? list[pairs + i] : movers[i];
     mass[hole] = mass[mover];
     if (source) source[hole] = mover;
   }
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   const int keep = p.keep, recent = p.recent, edge = keep - recent;
   const int64_t row = blockIdx.x / C;
   const int h = static_cast<int>(row % p.hkv), b = static_cast<int>(row / p.hkv % p.batch), layer = static_cast<int>(row / p.hkv / p.batch);
-  const int* const plan = p.plan + row * plan_ints(p.room);
+  const int* const plan = p.plan + row * p.plan_ints;
   const int2 head = p.head[row];
   const int n = head.x, pairs = head.y;
   if (n <= keep) return;
@@ -414,7 +418,7 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
     int64_t from = -1, to = -1;
     if (lane < cnt) {
       to = place(plan[first + lane]);
-      from = place(plan[p.room - 1 - (first + lane)]);
+      from = place(plan[p.most + first + lane]);
     }
     for (int u0 = 0; u0 < units; u0 += 32 * U) {
       T v[U];
@@ -474,9 +478,9 @@ int tu_status_evict(bool reset, cudaStream_t st, int* out) { return read_tu_stat
 
 extern "C" {
 
-size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions) {
-  if (layers < 1 || batch < 1 || nheads_kv < 1 || max_positions < 1) return 0;
-  return static_cast<size_t>(layers) * batch * nheads_kv * (sizeof(int2) + sn::plan_ints(max_positions) * sizeof(int)) + 16;
+size_t sn_evict_workspace_size(int layers, int batch, int nheads_kv, int64_t max_positions, int keep) {
+  if (layers < 1 || batch < 1 || nheads_kv < 1 || max_positions < 1 || keep < 1) return 0;
+  return static_cast<size_t>(layers) * batch * nheads_kv * (sizeof(int2) + sn::plan_size(max_positions, keep) * sizeof(int)) + 16;
 }
 
 int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int nheads_kv, int head_dim,
@@ -491,7 +495,7 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   const int64_t room = static_cast<int64_t>(max_pages) * page_size;
   if ((nheads_kv > 1 && mass_head_stride < room) || (batch > 1 && mass_batch_stride < room) ||
       (layers > 1 && mass_layer_stride < room) ||
-      workspace_bytes < sn_evict_workspace_size(layers, batch, nheads_kv, room))
+      workspace_bytes < sn_evict_workspace_size(layers, batch, nheads_kv, room, keep))
     return SN_ERR_INVALID_ARGUMENT;
   if (!sn::aligned16(workspace)) return SN_ERR_MISALIGNED;
   const int64_t rows = static_cast<int64_t>(layers) * batch * nheads_kv;
@@ -512,15 +516,15 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   p.source = source;
   p.head = static_cast<int2*>(workspace);
   p.plan = reinterpret_cast<int*>(p.head + (rows + 1) / 2 * 2);
-  p.room = static_cast<int>(room);
+  p.plan_ints = sn::plan_size(room, keep);
+  p.most = static_cast<int>(sn::most_pairs(room, keep));
   p.batch = batch;
   p.hkv = nheads_kv;
   p.keep = keep;
   p.recent = recent;
   p.sinks = sinks;
-  const int bits = static_cast<int>((room + 31) / 32 * 2 + 8);  // two a candidate, and room to align the keys
-  p.held = room <= sn::kEvictWords - bits ? static_cast<int>(room) : 0;
-  const size_t smem = static_cast<size_t>(bits + p.held) * sizeof(uint32_t);
+  p.held = sn::keys_held(room) ? static_cast<int>(room) : 0;
+  const size_t smem = static_cast<size_t>(sn::bit_words(room) + p.held) * sizeof(uint32_t);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int r = static_cast<int>(rows);
   const int rc = rows <= sn::sm_count() ? sn::launch_plan<1024>(r, smem, st, p) : sn::launch_plan<512>(r, smem, st, p);

@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib, build
 
-_FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_copy_pages",
+_FAST_SYMBOLS = ("sn_paged_decode_attention", "sn_paged_decode_workspace_size", "sn_rotary_paged_append", "sn_rotary_paged_append_at", "sn_copy_pages",
                  "sn_mamba2_prompt", "sn_mamba2_prompt_workspace_size", "sn_paged_decode_attention_mass",
                  "sn_paged_mass_workspace_size", "sn_evict_positions", "sn_evict_workspace_size", "sn_update_page_bounds", "sn_select_blocks",
                  "sn_select_blocks_workspace_size",

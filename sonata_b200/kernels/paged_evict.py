@@ -102,7 +102,7 @@ def evict_positions(pool: torch.Tensor, page_table: torch.Tensor, seq_lens: torc
 
     def launch(st):
         source = torch.empty((layers, batch, hkv, keep), device=pool.device, dtype=torch.int32) if return_source else None
-        need = _lib.lib().sn_evict_workspace_size(layers, batch, hkv, width * page)
+        need = _lib.lib().sn_evict_workspace_size(layers, batch, hkv, width * page, keep)
         ws = torch.empty(need, device=pool.device, dtype=torch.uint8)
         call("sn_evict_positions", pool.data_ptr(), layers, pages, page, hkv, hd, page_table.data_ptr(),
              page_table.stride(0) if batch > 1 else width, width, seq_lens.data_ptr(), mass.data_ptr(), mass.stride(0), mass.stride(1),

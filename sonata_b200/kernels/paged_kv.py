@@ -106,8 +106,9 @@ def rotary_paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
     nheads, head_dim], zeros for a row of no stream or a position out of range.
     `positions` int32 [tokens] names the tokens' rows of cos / sin where their
     places in the cache are not their positions (after evict_positions)."""
-    if stream is None and positions is None:
-        r = fast().append(qkv, k_pages, v_pages, page_table, seq_lens, cos, sin, nheads, cu_seqlens, interleaved)
+    if stream is None:
+        args = (qkv, k_pages, v_pages, page_table, seq_lens, cos, sin, nheads, cu_seqlens, interleaved)
+        r = fast().append(*args) if positions is None else fast().append(*args, positions)
         if r is not None:
             return r if type(r) is not int else _lib.check("sn_rotary_paged_append", r)
     if not (isinstance(qkv, torch.Tensor) and qkv.dtype is _BF16 and qkv.is_cuda and qkv.dim() == 2):

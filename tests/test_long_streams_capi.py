@@ -54,7 +54,7 @@ def evict(L, **k):
     (dict(pool=None), -1), (dict(tab=None), -1), (dict(lens=None), -1), (dict(mass=None), -1), (dict(layers=0), -1), (dict(np=0), -1), (dict(page=0), -1),
     (dict(hkv=0), -1), (dict(hd=0), -1), (dict(mp=0), -1), (dict(ts=3), -1), (dict(batch=0), -1), (dict(keep=0), -1), (dict(recent=-1), -1),
     (dict(sinks=-1), -1), (dict(recent=32), -1), (dict(recent=31, sinks=2), -1), (dict(mh=63), -1), (dict(mb=63), -1), (dict(ml=63), -1),
-    (dict(ws=None), -1), (dict(wsb=2 * 2 * 4 * 132 * 4), -1), (dict(ws=ctypes.c_void_p(264)), -2),
+    (dict(ws=None), -1), (dict(wsb=2 * 2 * 4 * (64 * 4 + 8)), -1), (dict(wsb=2 * 2 * 4 * (64 * 4 + 8) + 16, batch=0), -1), (dict(ws=ctypes.c_void_p(264)), -2),
     (dict(mp=32769, ts=32769, ml=BIG, mb=BIG, mh=BIG), -3), (dict(hd=8193), -3), (dict(batch=1 << 28, wsb=1 << 50), -3)])
 def test_evict(L, change, rc):
     assert evict(L, **change) == rc
@@ -62,9 +62,10 @@ def test_evict(L, change, rc):
 
 def test_evict_workspace(L):
     f = L.sn_evict_workspace_size
-    assert f(0, 1, 1, 1) == f(1, 0, 1, 1) == f(1, 1, 0, 1) == f(1, 1, 1, 0) == 0
-    assert 0 < f(1, 2, 4, 100) < f(2, 2, 4, 100) < f(2, 2, 4, 1000)
-    assert f(12, 300, 8, 1 << 20) > 1 << 37
+    assert f(0, 1, 1, 1, 1) == f(1, 0, 1, 1, 1) == f(1, 1, 0, 1, 1) == f(1, 1, 1, 0, 1) == f(1, 1, 1, 1, 0) == 0
+    assert 0 < f(1, 2, 4, 100, 9) < f(2, 2, 4, 100, 9) < f(2, 2, 4, 100, 50) == f(2, 2, 4, 100, 90) < f(2, 2, 4, 1000, 90)
+    assert f(12, 48, 4, 30000, 2048) < 40 << 20  # lists of at most keep pairs
+    assert f(12, 300, 8, 1 << 19, 1 << 18) > 1 << 36
 
 
 def bounds(L, **k):

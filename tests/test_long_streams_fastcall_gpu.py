@@ -23,7 +23,7 @@ def _both(common, monkeypatch, run):
 
     class Spy:
         pass
-    for name in ("mass", "evict", "bounds", "select", "sparse"):
+    for name in ("append", "mass", "evict", "bounds", "select", "sparse"):
         f = getattr(common.fast(), name)
         setattr(Spy, name, staticmethod(lambda *a, f=f: taken.append(f(*a)) or taken[-1]))
     with monkeypatch.context() as m:
@@ -76,6 +76,25 @@ def test_same_bits(ways, monkeypatch):
     _both(common, monkeypatch, lambda: (PS.select_blocks(q, bounds, tab, lens, 16, 3, first=1, last=1),))
     blocks = PS.select_blocks(q, bounds, tab, lens, 16, 3)
     _both(common, monkeypatch, lambda: (PS.paged_sparse_attention(q, kp, vp, tab, lens, blocks, workspace=ws),))
+
+
+def test_append_with_positions(ways, monkeypatch):
+    common, PK, *_ = ways
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF16)
+    tab = torch.arange(12, device="cuda", dtype=torch.int32).view(2, 6)
+    lens, cu = (torch.tensor(v, device="cuda", dtype=torch.int32) for v in ([90, 33], [0, 5, 7]))
+    cos, sin = PK.rotary_table(300, 64)
+    for qkv, c, at in ((r(7, 24 * 128), cu, range(200, 207)), (r(2, 24 * 128), None, (299, 3))):
+        at = torch.tensor(list(at), device="cuda", dtype=torch.int32)
+
+        def run():
+            kp, vp = torch.zeros(12, 4, 16, 128, device="cuda", dtype=BF16), torch.zeros(12, 4, 16, 128, device="cuda", dtype=BF16)
+            return PK.rotary_paged_append(qkv, kp, vp, tab, lens, cos, sin, 16, cu_seqlens=c, positions=at), kp, vp
+        _both(common, monkeypatch, run)
+        f = common.fast().append
+        plain = (qkv, *(torch.zeros(12, 4, 16, 128, device="cuda", dtype=BF16) for _ in range(2)), tab, lens, cos, sin, 16, c, False)
+        assert f(*plain, at.long()) is None and f(*plain, at[:-1]) is None and f(*plain, at, at) is None
 
 
 def test_leaves_the_rest_alone(ways):
