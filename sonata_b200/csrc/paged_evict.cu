@@ -25,7 +25,6 @@ namespace {
 constexpr int kEvictMost = 1 << 19;   // candidates of a stream: two bits each in shared memory
 constexpr int kEvictWords = 52992;    // of shared memory for those bits and for keys
 constexpr int kEvictCopy = 1024;      // 16-byte pieces of one copy to shared memory
-constexpr int kEvictRanked = 256;     // keys that are ranked by comparing all of them
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
 constexpr int kMoveCluster = 8;       // CTAs a row at most
 
@@ -53,23 +52,22 @@ bool keys_held(int64_t room) { return bit_words(room) + room <= kEvictWords; }
 int64_t most_pairs(int64_t room, int64_t keep) { return (std::min(room / 2, keep) + 3) / 4 * 4; }
 int64_t plan_size(int64_t room, int64_t keep) { return 2 * most_pairs(room, keep) + (keys_held(room) ? 0 : (room + 3) / 4 * 4 + 4); }
 
-// The plan of a row.  A histogram of the keys over their range finds the bin of the last one that stays, its key is found
-// among that bin's by comparing all of them (by further histograms where they are many and not all equal), and what stays is
-// what is above it, and the first ones that equal it.  Passes over the keys are bound by issue slots (30000 of them: 940
-// warp steps), so each makes words of 32 bits, and the rest is done on those, a lane a word.
+// The plan of a row.  A histogram of the keys' upper bits (of the masses' exponents and first bits) finds the bin of the last
+// one that stays.  One more pass makes two bits of each key, above that bin and in it, and everything after that is done on
+// those, a lane a word of 32: histograms of what is in the bin, over its own range, until all of it stays or all of it is equal
+// (then the first ones stay); the holes and movers; their lists.  A pass over the keys is bound by issue slots (30000 of them:
+// 940 warp steps, 3 us), so there are two.
 template <int T>
 __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const EvictParams p) {
   constexpr int kWarps = T / 32;
   extern __shared__ __align__(16) uint32_t s_dyn[];
   __shared__ SelectShared<T> s_sel;
-  __shared__ uint32_t s_range[4], s_found, s_cut[2], s_rank[kEvictRanked];
+  __shared__ uint32_t s_range[2];
   __shared__ __align__(8) uint64_t s_copied;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x, h = row % p.hkv, b = row / p.hkv % p.batch, layer = row / p.hkv / p.batch;
   const int keep = p.keep, recent = p.recent, sinks = p.sinks, edge = keep - recent;  // places below: sinks, then candidates that stay
-  if (tid < 4) s_range[tid] = tid & 1 ? 0 : 0xffffffffu;
   if (tid == 0) {
-    s_found = 0;
     mbar_init(&s_copied, 1);
     fence_barrier_init();
   }
@@ -100,11 +98,15 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     const bool held = c <= p.held;
     uint32_t* const keys = (held ? s_dyn + (2 * words + 3) / 4 * 4 : reinterpret_cast<uint32_t*>(plan + 2 * p.most)) +
                            (4 - head) % 4;
-    uint32_t least = 0xffffffffu, most = 0;
+    // a key's bin: its bits under the sign's, or 0 for negative ones.  Keys in the lowest bin are counted apart: it is where
+    // positions without any weight lie
+    constexpr int kBits = SelectShared<T>::kBits, kShift = 31 - kBits;
+    auto bin = [](uint32_t k) { return k >> 31 ? k >> kShift & (SelectShared<T>::kBins - 1) : 0u; };
+    uint32_t low = 0;
     auto take = [&](float v) {
-      const uint32_t k = order_key(v);
-      least = min(least, k);
-      most = max(most, k);
+      const uint32_t k = order_key(v), d = bin(k);
+      if (d == 0) ++low;
+      else atomicAdd(s_sel.bins() + d, 1u);
       return k;
     };
     const int rest = c - head - 4 * quads;
@@ -130,83 +132,25 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
       const float4 v = held ? *reinterpret_cast<const float4*>(keys4 + i) : value4[i];
       keys4[i] = make_uint4(take(v.x), take(v.y), take(v.z), take(v.w));
     }
-    least = __reduce_min_sync(0xffffffffu, least);
-    most = __reduce_max_sync(0xffffffffu, most);
-    __syncthreads();
-    if (lane == 0) {
-      atomicMin(&s_range[0], least);
-      atomicMax(&s_range[1], most);
-    }
-    __syncthreads();
-    least = s_range[0];
-    const int shift = max(0, 32 - __clz(s_range[1] - least) - SelectShared<T>::kBits);
-    // keys in the lowest bin are counted apart: it is where positions without any weight lie
-    uint32_t low = 0;
-#pragma unroll 4
-    for (int i = tid; i < c; i += T) {
-      const uint32_t d = (keys[i] - least) >> shift;
-      if (d == 0) ++low;
-      else atomicAdd(s_sel.bins() + d, 1u);
-    }
-    low = __reduce_add_sync(0xffffffffu, low);
-    if (lane == 0 && low) atomicAdd(s_sel.bins(), low);
-    __syncthreads();
-    find_bin(static_cast<uint32_t>(m), s_sel);
-    const uint32_t digit = s_sel.digit, here = s_sel.here;
-    uint32_t need = m - s_sel.above;  // of those that equal the last one
-    uint32_t from = least + (digit << shift), upto = from + ((1u << shift) - 1);  // keys that equal it, for all that matters
-    if (here != need) {
-      uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll 4
-      for (int i = tid; i < c; i += T) {
-        const uint32_t k = keys[i];
-        if (k - from > upto - from) continue;
-        lo = min(lo, k);
-        hi = max(hi, k);
-        if (here <= kEvictRanked) s_rank[atomicAdd(&s_found, 1u)] = k;
-      }
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      if (lane == 0) {
-        atomicMin(&s_range[2], lo);
-        atomicMax(&s_range[3], hi);
-      }
+    auto count_low = [&] {
+      low = __reduce_add_sync(0xffffffffu, low);
+      if (lane == 0 && low) atomicAdd(s_sel.bins(), low);
       __syncthreads();
-      if (s_range[2] == s_range[3]) {
-        from = upto = s_range[2];
-      } else if (here <= kEvictRanked) {
-        for (uint32_t k = warp; k < here; k += kWarps) {
-          const uint32_t mine = s_rank[k];
-          uint32_t above = 0, same = 0;
-          for (uint32_t j = lane; j < here; j += 32) {
-            above += s_rank[j] > mine;
-            same += s_rank[j] == mine;
-          }
-          above = __reduce_add_sync(0xffffffffu, above);
-          same = __reduce_add_sync(0xffffffffu, same);
-          if (lane == 0 && above < need && above + same >= need) {  // it, and those equal to it, which write the same
-            s_cut[0] = mine;
-            s_cut[1] = need - above;
-          }
-        }
-        __syncthreads();
-        from = upto = s_cut[0];
-        need = s_cut[1];
-      } else {
-        const Cutoff<uint32_t> cut = find_cutoff<uint32_t>([&](int i) { return keys[i]; }, c, static_cast<uint32_t>(m), s_sel);
-        from = cut.prefix << cut.shift;
-        upto = from + ((1u << cut.shift) - 1);
-        need = cut.need;
-      }
-    }
+    };
+    count_low();
+    find_bin(static_cast<uint32_t>(m), s_sel);
+    uint32_t here = s_sel.here, need = m - s_sel.above;  // in the bin, and of those that stay
+    {
+      const uint32_t digit = s_sel.digit;
 #pragma unroll 2
-    for (int w = warp; w < words; w += kWarps) {
-      const int i = 32 * w + lane;
-      const uint32_t k = i < c ? keys[i] : 0;
-      const uint32_t in = __ballot_sync(0xffffffffu, i < c && k > upto), equal = __ballot_sync(0xffffffffu, i < c && k - from <= upto - from);
-      if (lane == 0) {
-        s_in[w] = in;
-        s_equal[w] = equal;
+      for (int w = warp; w < words; w += kWarps) {
+        const int i = 32 * w + lane;
+        const uint32_t d = i < c ? bin(keys[i]) : 0;
+        const uint32_t in = __ballot_sync(0xffffffffu, i < c && d > digit), equal = __ballot_sync(0xffffffffu, i < c && d == digit);
+        if (lane == 0) {
+          s_in[w] = in;
+          s_equal[w] = equal;
+        }
       }
     }
     // ---- words: a warp has consecutive ones ----
@@ -221,11 +165,53 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
       all = __shfl_sync(0xffffffffu, sum, 31);
       return sum - v;
     };
+    __syncthreads();
     auto before = [&](const uint32_t* counts, uint32_t& all) {  // the sum over the warps before this one, and over all
       uint32_t v = lane < kWarps ? counts[lane] : 0;
       const uint32_t sum = scan(v, all);
       return __shfl_sync(0xffffffffu, sum, warp);
     };
+    // the bin's keys, until all or none of them differ in whether they stay
+    while (here != need) {
+      if (tid < 2) s_range[tid] = tid == 0 ? 0xffffffffu : 0;
+      s_sel.clear();
+      __syncthreads();
+      auto each = [&](auto f) {  // f(word, bit, key) of this lane's
+        for (int w = w0 + lane; w < w1; w += 32)
+          for (uint32_t left = s_equal[w]; left; left &= left - 1) f(w, left & (0u - left), keys[32 * w + __ffs(left) - 1]);
+      };
+      uint32_t lo = 0xffffffffu, hi = 0;
+      each([&](int, uint32_t, uint32_t k) {
+        lo = min(lo, k);
+        hi = max(hi, k);
+      });
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      if (lane == 0) {
+        atomicMin(&s_range[0], lo);
+        atomicMax(&s_range[1], hi);
+      }
+      __syncthreads();
+      lo = s_range[0];
+      hi = s_range[1];
+      if (lo == hi) break;  // equal: the first ones stay
+      const int shift = max(0, 32 - __clz(hi - lo) - kBits);
+      low = 0;
+      each([&](int, uint32_t, uint32_t k) {
+        if ((k - lo) >> shift == 0) ++low;
+        else atomicAdd(s_sel.bins() + ((k - lo) >> shift), 1u);
+      });
+      count_low();
+      find_bin(need, s_sel);
+      const uint32_t digit = s_sel.digit;
+      here = s_sel.here;
+      need -= s_sel.above;
+      each([&](int w, uint32_t bit, uint32_t k) {
+        const uint32_t d = (k - lo) >> shift;
+        if (d > digit) s_in[w] |= bit;
+        if (d != digit) s_equal[w] &= ~bit;
+      });
+    }
     __syncthreads();
     // the first `need` of the equal ones stay
     uint32_t mine = 0, all;
