@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     // a key's bin: its bits under the sign's, or 0 for negative ones.  Keys in the lowest bin are counted apart: it is where
     // positions without any weight lie
     constexpr int kBits = SelectShared<T>::kBits, kShift = 31 - kBits;
-    auto bin = [](uint32_t k) { return k >> 31 ? k >> kShift & (SelectShared<T>::kBins - 1) : 0u; };
+    constexpr uint32_t kZero = 0x80000000u;
+    auto bin = [](uint32_t k) { return (max(k, kZero) - kZero) >> kShift; };
     uint32_t low = 0;
     auto take = [&](float v) {
       const uint32_t k = order_key(v), d = bin(k);
@@ -141,17 +142,19 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     find_bin(static_cast<uint32_t>(m), s_sel);
     uint32_t here = s_sel.here, need = m - s_sel.above;  // in the bin, and of those that stay
     {
-      const uint32_t digit = s_sel.digit;
-#pragma unroll 2
-      for (int w = warp; w < words; w += kWarps) {
-        const int i = 32 * w + lane;
-        const uint32_t d = i < c ? bin(keys[i]) : 0;
-        const uint32_t in = __ballot_sync(0xffffffffu, i < c && d > digit), equal = __ballot_sync(0xffffffffu, i < c && d == digit);
+      const uint32_t digit = s_sel.digit, from = digit == 0 ? 0 : kZero + (digit << kShift);
+      const uint32_t upto = kZero + (digit << kShift) + ((1u << kShift) - 1), span = upto - from;
+      auto mark = [&](int w, uint32_t k, bool in) {
+        const uint32_t above = __ballot_sync(0xffffffffu, in && k > upto), equal = __ballot_sync(0xffffffffu, in && k - from <= span);
         if (lane == 0) {
-          s_in[w] = in;
+          s_in[w] = above;
           s_equal[w] = equal;
         }
-      }
+      };
+      const int whole = c / 32;
+#pragma unroll 4
+      for (int w = warp; w < whole; w += kWarps) mark(w, keys[32 * w + lane], true);
+      if (whole < words && warp == whole % kWarps) mark(whole, 32 * whole + lane < c ? keys[32 * whole + lane] : 0, 32 * whole + lane < c);
     }
     // ---- words: a warp has consecutive ones ----
     const int per = (words + kWarps - 1) / kWarps, w0 = min(warp * per, words), w1 = min(w0 + per, words);
@@ -252,24 +255,33 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
     __syncthreads();
     at = before(s_sel.warp, all);
     before(s_sel.warp2, pairs);
-    // the lists: holes come before movers, so that one running count serves both
-    if (held) list = reinterpret_cast<const int*>(keys);  // (the keys are done with)
-    for (int w = w0; w < w1; w += 32) {
-      uint32_t word = w + lane < w1 ? s_equal[w + lane] : 0;
-      const int place = sinks + 32 * (w + lane) - 1;
-      for (uint32_t k = at + scan(__popc(word), all); word; word &= word - 1, ++k) {
-        const int v = place + __ffs(word);
-        *(k < pairs ? holes + k : movers + (k - pairs)) = v;
-        if (held) keys[k] = v;
+    // the lists: holes come before movers, so that one running count serves both.  In shared memory over the keys, which are
+    // done with, as single stores to global memory would bind (30000 candidates: 3.5 us)
+    if (held) list = reinterpret_cast<const int*>(keys);
+    auto put = [&](uint32_t k, int v) {
+      if (held) keys[k] = v;
+      else *(k < pairs ? holes + k : movers + (k - pairs)) = v;
+    };
+    if (per <= 8) {  // few words a warp: one after another, a lane a candidate
+      for (int w = w0; w < w1; ++w) {
+        const uint32_t word = s_equal[w];
+        if (word >> lane & 1) put(at + __popc(word & ((1u << lane) - 1)), sinks + 32 * w + lane);
+        at += __popc(word);
       }
-      at += all;
+    } else {
+      for (int w = w0; w < w1; w += 32) {
+        uint32_t word = w + lane < w1 ? s_equal[w + lane] : 0;
+        for (uint32_t k = at + scan(__popc(word), all); word; word &= word - 1, ++k) put(k, sinks + 32 * (w + lane) - 1 + __ffs(word));
+        at += all;
+      }
     }
   }
   if (source)  // of what stays where it is, and for now of the holes
     for (int i = tid; i < edge; i += T) source[i] = i;
   __syncthreads();
   if (tid == 0) p.head[row] = make_int2(n, static_cast<int>(pairs));
-  // mass, as the rows will go: movers into holes, then the recent ones, which may overlap their places, then zeros
+  // mass, as the rows will go: movers into holes, then the recent ones, which may overlap their places (zeros behind are left
+  // to the other launch, which has more threads)
   float w[4];
   auto read_recent = [&](int k0) {
 #pragma unroll
@@ -282,6 +294,10 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
 #pragma unroll 4
   for (uint32_t i = tid; i < pairs; i += T) {
     const int hole = list ? list[i] : holes[i], mover = list ? list[pairs + i] : movers[i];
+    if (list) {
+      holes[i] = hole;
+      movers[i] = mover;
+    }
     mass[hole] = mass[mover];
     if (source) source[hole] = mover;
   }
@@ -298,13 +314,6 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const Ev
       mass[edge + k] = w[j];
       if (source) source[edge + k] = n - recent + k;
     }
-  }
-  {
-    float* const tail = mass + keep;
-    const int len = n - keep, head = min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tail) & 15)) / 4 & 3)), quads = (len - head) / 4;
-    if (tid < head) tail[tid] = 0.f;
-    if (tid < len - head - 4 * quads) tail[head + 4 * quads + tid] = 0.f;
-    for (int i = tid; i < quads; i += T) reinterpret_cast<float4*>(tail + head)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -342,6 +351,14 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   const int2 head = p.head[row];
   const int n = head.x, pairs = head.y;
   if (n <= keep) return;
+  {  // mass behind what is kept: whole 16 bytes, and what lies before and behind them
+    const int threads = kMoveThreads * C, me = rank * kMoveThreads + static_cast<int>(threadIdx.x);
+    float* const tail = p.mass + layer * p.ml + b * p.mb + h * p.mh + keep;
+    const int len = n - keep, before = min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tail) & 15)) / 4 & 3)), quads = (len - before) / 4;
+    if (me < before) tail[me] = 0.f;
+    if (me < len - before - 4 * quads) tail[before + 4 * quads + me] = 0.f;
+    for (int i = me; i < quads; i += threads) reinterpret_cast<float4*>(tail + before)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   const int nu = NU ? NU : static_cast<int>(2 * p.row_bytes / sizeof(T));
   char* const base = p.pool + layer * p.layer_bytes + h * p.head_bytes;
   // where a position's K row is, or -1

@@ -9,9 +9,9 @@ namespace {
 
 // Keys whose order as unsigned numbers is that of the values: NaN above all, both zeros alike.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(v), size = u & 0x7fffffffu;
+  const uint32_t key = static_cast<int>(u) < 0 && size != 0 ? ~u : size | 0x80000000u;
+  return size > 0x7f800000u ? 0xffffffffu : key;
 }
 __device__ __forceinline__ uint64_t order_key(double v) {
   if (v != v) return ~0ull;
@@ -57,9 +57,8 @@ __device__ void find_bin(uint32_t need, SelectShared<T>& s) {
   }
   if (lane == 0) s.warp[warp] = upto;
   __syncthreads();
-#pragma unroll
-  for (int w = 1; w < SelectShared<T>::kWarps; ++w)
-    if (w > warp) upto += s.warp[w];
+  uint32_t after = lane < SelectShared<T>::kWarps && lane > warp ? s.warp[lane] : 0;
+  upto += __reduce_add_sync(0xffffffffu, after);
   if (upto >= need && upto - mine < need) {  // one thread
     uint32_t above = upto - mine, here = 0;
     int bin = -1;
