@@ -253,9 +253,29 @@ def test_evict_over_a_cluster(PE, n, keep):
     evict_case(PE, [n], keep, 100, 5, hkv=1, hd=8, page=64, seed=n)
 
 
-def test_evict_wide_table(PE):
-    """A table with room for far more positions than there are."""
-    evict_case(PE, [500, 100], 300, 10, 1, width=4000, hd=8, seed=3)
+@pytest.mark.parametrize("n,keep", [(49650, 30000), (49700, 1000), (60001, 50000), (200003, 100000), (70000, 69999)])
+def test_evict_where_shared_memory_ends(PE, n, keep):
+    """Keys that just fit into shared memory, and ever more that do not."""
+    evict_case(PE, [n], keep, 130, 3, hkv=1, hd=2, page=64, seed=n)
+
+
+@pytest.mark.parametrize("streams", [2, 40])
+def test_evict_wide_table(PE, streams):
+    """A table with room for far more positions than there are (and than shared memory holds keys of)."""
+    evict_case(PE, [500, 100] * (streams // 2), 300, 10, 1, width=4000, hkv=4, hd=8, seed=3)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_evict_narrow_and_wide_masses(PE, seed):
+    """Masses in the last bits of one exponent, and over all exponents: one bin of the first histogram and all of them."""
+    def mass(layers, B, hkv, room, g):
+        u = torch.rand(layers, B, hkv, room, device="cuda", generator=g)
+        if seed == 0:
+            return 1 + (u * 64).round() * 2.0 ** -23
+        if seed == 1:
+            return 1 + (u * 2.0 ** 16).round() * 2.0 ** -23
+        return torch.exp2(u * 250 - 125) * (1 if seed == 2 else -1)
+    evict_case(PE, [200, 3000, 9000], 150, 20, 3, mass=mass, hd=8, seed=seed)
 
 
 def test_evict_many_rows(PE):
