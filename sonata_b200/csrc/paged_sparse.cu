@@ -178,11 +178,14 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 //   than 2 E below it are not: their scores lie on the same side of the last
 //   chosen one's.  The few between get their sums in 64 bits and are ranked, by
 //   comparing all of them.
+// * A block whose absolute sum is not finite has no s to go by: such blocks are
+//   always among those between, and the bin above which blocks are chosen for
+//   certain is the one that would be if they all were.
 // Two launches: scores, spread evenly over the device and bound by reading the
 // bounds, and choices, a CTA a row, bound by the chain of its steps.  In one
 // launch, a cluster of 8 CTAs a row with the scores in shared memory, exchanges
 // of a few kilobytes between the CTAs took 2 to 3 us each (22 us for the three
-// streams; now 15.9, about 7 of them the scores of 38 MB of bounds, and 14.6 for
+// streams; now 16.4, about 7 of them the scores of 31 MB of bounds, and 14.9 for
 // 48 streams of up to 8000 positions).
 // ---------------------------------------------------------------------------
 constexpr int kFewExact = 64;        // blocks that are ranked by comparing all of them
@@ -195,10 +198,13 @@ struct SelectParams {
   PageMap map;
   const int* seq_lens;
   int* blocks;      // [batch, hkv, count]
-  uint2* scores;    // [batch, hkv, max_pages]: key of s, sum of absolute values; of the blocks that are not first or last
+  uint2* scores;    // [batch, hkv, max_pages]: key of s (kOddKey: none; 0: no page), sum of absolute values; of the blocks that
+                    // are not first or last
   uint64_t* exact;  // the same blocks' keys of sums in 64 bits, where they are needed
   int batch, hq, hkv, hd, count, first, last;
 };
+
+constexpr uint32_t kOddKey = 0xffffffffu;
 
 // Blocks of a stream, and those that are compared: first .. first + compared - 1.
 __device__ __forceinline__ int stream_blocks(const SelectParams& p, int b, int& compared) {
@@ -270,7 +276,7 @@ __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams
           mma_bf16(m, x.x & kAbs, y.x & kAbs, x.y & kAbs, y.y & kAbs, q4.x & kAbs, q4.y & kAbs);
           mma_bf16(m, x.z & kAbs, y.z & kAbs, x.w & kAbs, y.w & kAbs, q4.z & kAbs, q4.w & kAbs);
         }
-        // heads 2t and 2t + 1 of blocks g and g + 8; an absolute sum that is not finite is infinite
+        // heads 2t and 2t + 1 of blocks g and g + 8; an absolute sum that is not a number is infinite
         const bool two = h0 + 2 * t + 1 < group, one = h0 + 2 * t < group;
         auto wide = [](float x) { return x < INFINITY ? x : INFINITY; };
         float v0 = one ? s[0] : -INFINITY, v1 = one ? s[2] : -INFINITY;
@@ -285,7 +291,11 @@ __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams
         }
         const int at = i + g + 8 * t;
         if (t < 2 && at < len) {
-          uint2 v = (t ? ok1 : ok0) ? make_uint2(order_key(t ? v1 : v0), __float_as_uint(t ? m1 : m0)) : make_uint2(0, 0);
+          uint2 v = make_uint2(0, 0);
+          if (t ? ok1 : ok0) {
+            const float wide_sum = t ? m1 : m0;
+            v = wide_sum < INFINITY ? make_uint2(order_key(t ? v1 : v0), __float_as_uint(wide_sum)) : make_uint2(kOddKey, 0);
+          }
           if (h0 > 0) {
             const uint2 before = out[at];  // this lane's own
             v = make_uint2(max(v.x, before.x), max(v.y, before.y));
@@ -329,6 +339,48 @@ __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, in
   return __any_sync(0xffffffffu, odd) ? ~0ull : best;
 }
 
+// The keys of eight blocks' scores in 64 bits, four lanes a block (block < 0: none); a warp, head_dim a multiple of 32, bounds
+// on 16 bytes.  For many of them: a bf16 value's bits moved into the upper word of a double are that value times 2^-896,
+// subnormal ones too, so that no conversions (16 a cycle and SM) bind; with q times 2^1023 more, which leaves the order as it is,
+// products and sums, multiples of 2^-266 times 2^-769, are held exactly.  Out of line, as are the few other steps that most
+// calls do not take: what is taken runs once a CTA, and waits for its instructions (16 -> 19 us with all of it inline).
+__device__ __noinline__ uint64_t exact_scores(const SelectParams& p, int b, int hk, int block) {
+  const int t = threadIdx.x & 3, group = p.hq / p.hkv;
+  const int pg = block < 0 ? -1 : page_of(p.map, b, block);
+  const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(max(pg, 0)) * p.hkv + hk) * 2 * p.hd;
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh);
+  auto widen = [](uint32_t u) { return __hiloint2double(static_cast<int>((u & 0x8000u) << 16 | (u & 0x7fffu) << 13), 0); };
+  uint64_t best = 0;
+  bool odd = false;
+  for (int h0 = 0; h0 < group; h0 += 4) {
+    double sum[4] = {0., 0., 0., 0.};
+    for (int k = t; k < p.hd / 8; k += 4) {
+      uint32_t l[4], g[4];
+      *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(lo + 8 * k);
+      *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(lo + p.hd + 8 * k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t wl = j & 1 ? l[j / 2] >> 16 : l[j / 2] & 0xffffu, wg = j & 1 ? g[j / 2] >> 16 : g[j / 2] & 0xffffu;
+        odd |= (wl & 0x7f80u) == 0x7f80u || (wg & 0x7f80u) == 0x7f80u;
+        const double least = widen(wl), greatest = widen(wg);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t v = q[min(h0 + h, group - 1) * p.qh + 8 * k + j];
+          sum[h] = fma(widen(v) * 0x1p1023, v >> 15 ? least : greatest, sum[h]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      best = max(best, order_key(sum[h]));
+    }
+  }
+  odd = __ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 28) & 15;
+  return pg < 0 ? 0 : odd ? ~0ull : best;
+}
+
 // Scores in 64 bits of all blocks, a warp a block: any head_dim and alignment.
 __global__ void __launch_bounds__(128) exact_scores_kernel(const SelectParams p) {
   pdl_launch_dependents();
@@ -347,19 +399,53 @@ __global__ void __launch_bounds__(128) exact_scores_kernel(const SelectParams p)
   }
 }
 
+// The range and number of the scores of a row in which some blocks have none, and the number of those that have a page.
+__device__ __noinline__ void regular_range(const uint2* scores, int len, uint32_t* s_range, uint32_t& least, uint32_t& most, uint32_t& scored,
+                                           uint32_t& odd) {
+  least = 0xffffffffu;
+  most = scored = odd = 0;
+  for (int i = threadIdx.x; i < len; i += blockDim.x) {
+    const uint32_t key = scores[i].x;
+    if (key == kOddKey) ++odd;
+    if (key == 0 || key == kOddKey) continue;
+    ++scored;
+    least = min(least, key);
+    most = max(most, key);
+  }
+  __syncthreads();  // s_range has been read
+  if (threadIdx.x < 2) s_range[threadIdx.x] = threadIdx.x == 0 ? 0xffffffffu : 0;
+  __syncthreads();
+  atomicMin(&s_range[0], least);
+  atomicMax(&s_range[1], most);
+  atomicAdd(&s_range[3], scored);
+  atomicAdd(&s_range[4], odd);
+  __syncthreads();
+  least = s_range[0];
+  most = s_range[1];
+  scored = s_range[3];
+  odd = s_range[4];
+}
+
+// Bits of the `need` highest of `len` keys.
+template <int T>
+__device__ __noinline__ void choose_exact(const uint64_t* keys, int len, uint32_t need, uint32_t* bits, SelectShared<T>& s) {
+  auto key = [&](int i) { return keys[i]; };
+  const Cutoff<uint64_t> cut = find_cutoff<uint64_t>(key, len, need, s);
+  choose(key, len, cut, bits, s);
+}
+
 // One CTA a row; kScored: block_scores_kernel has run, else exact_scores_kernel.
 template <bool kScored, int kChooseThreads>
-__global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) choose_blocks_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) choose_blocks_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kChooseWarps = kChooseThreads / 32, kChooseHeld = kChooseThreads > 512 ? 8 : 16;  // keys a thread holds
   extern __shared__ uint32_t s_bits[];
   __shared__ SelectShared<kChooseThreads> s_sel;
-  __shared__ uint32_t s_range[3];  // least and greatest key, S
+  __shared__ uint32_t s_range[5];  // least and greatest key, S, and for regular_range
   __shared__ uint64_t s_few[kFewExact];
   __shared__ int s_few_at[kFewExact];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t below = (1u << lane) - 1;
   const int row = blockIdx.x, b = row / p.hkv, hk = row - b * p.hkv;
-  if (tid < 3) s_range[tid] = tid == 0 ? 0xffffffffu : 0;
+  if (tid < 5) s_range[tid] = tid == 0 ? 0xffffffffu : 0;
   s_sel.clear();
   pdl_launch_dependents();
   pdl_wait();
@@ -374,7 +460,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
     if (i < p.first) out[i] = i;
     else out[p.count - p.last + i - p.first] = nb - p.last + i - p.first;
   }
-  const uint2* const scores = p.scores + static_cast<int64_t>(row) * p.map.max_pages;
+  uint2* const scores = p.scores + static_cast<int64_t>(row) * p.map.max_pages;
   uint64_t* const exact = p.exact + static_cast<int64_t>(row) * p.map.max_pages;
   const int words = (len + 31) / 32;
   uint32_t* const s_in = s_bits;            // [words] chosen
@@ -425,25 +511,36 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
     }
     __syncthreads();
     least = s_range[0];
-    const int shift = max(0, 32 - __clz(s_range[1] - least) - SelectShared<kChooseThreads>::kBits);
+    most = s_range[1];
+    uint32_t scored = len, odd = 0;  // blocks that have a score, and that have none
+    if (least == 0 || most == kOddKey) regular_range(scores, len, s_range, least, most, scored, odd);
+    const bool sure = static_cast<uint32_t>(need) <= scored;  // else all blocks with a score may be needed
+    const uint32_t span = most - least;
+    const int shift = max(0, 32 - __clz(span) - SelectShared<kChooseThreads>::kBits);
+    auto count = [&](uint32_t key) {
+      if (key - least <= span) atomicAdd(s_sel.bins() + ((key - least) >> shift), 1u);  // one with a score
+    };
 #pragma unroll
-    for (int j = 0; j < kChooseHeld; ++j)
-      if (tid + j * kChooseThreads < len) atomicAdd(s_sel.bins() + min((held[j] - least) >> shift, SelectShared<kChooseThreads>::kBins - 1u), 1u);
+    for (int j = 0; j < kChooseHeld; ++j) count(held[j]);
 #pragma unroll 4
-    for (int i = tid + kChooseHeld * kChooseThreads; i < len; i += kChooseThreads)
-      atomicAdd(s_sel.bins() + min((scores[i].x - least) >> shift, SelectShared<kChooseThreads>::kBins - 1u), 1u);
+    for (int i = tid + kChooseHeld * kChooseThreads; i < len; i += kChooseThreads) count(scores[i].x);
     __syncthreads();
-    find_bin(static_cast<uint32_t>(need), s_sel);
-    const uint32_t first_key = least + (s_sel.digit << shift);
     const float E2 = fmaf(__uint_as_float(s_range[2]), 0x1p-12f, 0x1p-109f);  // 2 E
-    const float lo = order_value(first_key) - E2, hi = order_value(first_key + ((1u << shift) - 1)) + E2;
-    const bool sure = fabsf(lo) < INFINITY && fabsf(hi) < INFINITY;
+    float lo = 0.f, hi = INFINITY;
+    for (uint32_t want = sure ? need : 0; want > 0;) {
+      find_bin(want, s_sel);
+      const uint32_t first_key = least + (s_sel.digit << shift);
+      if (want == static_cast<uint32_t>(need)) lo = order_value(first_key) - E2;
+      if (want + odd == static_cast<uint32_t>(need)) hi = order_value(min(first_key + ((1u << shift) - 1), most)) + E2;
+      want = want == static_cast<uint32_t>(need) && odd > 0 && want > odd ? want - odd : 0;
+      if (want > 0) __syncthreads();  // the digit has been read
+    }
     uint32_t nin = 0, nopen = 0;
     auto sort_word = [&](int i, uint32_t key) {  // of the warp's lanes' blocks i
       if (i - lane >= len) return;
-      const float v = order_value(key);
-      const uint32_t in = __ballot_sync(0xffffffffu, sure && i < len && key != 0 && v > hi);
-      const uint32_t open = __ballot_sync(0xffffffffu, i < len && (!sure || (key != 0 && v >= lo && v <= hi)));
+      const float v = order_value(key);  // without a score, a NaN
+      const uint32_t in = __ballot_sync(0xffffffffu, sure && v > hi);
+      const uint32_t open = __ballot_sync(0xffffffffu, (v >= lo && v <= hi) || key == kOddKey || (!sure && i < len));
       if (lane == 0) {
         s_in[i / 32] = in;
         s_open[i / 32] = open;
@@ -477,16 +574,18 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
       uint32_t open_at = 0;
 #pragma unroll
       for (int v = 0; v < kChooseWarps; ++v) open_at += v < warp ? s_sel.warp2[v] : 0;
-      if (all_open <= kFewExact) {
-        uint32_t k = open_at;
-        for (int w = w0; w < w1; w += 32) {  // to a list, a lane a word, so that every warp takes as many of them
-          uint32_t left = w + lane < w1 ? s_open[w + lane] : 0, all;
-          for (uint32_t at = k + scan(__popc(left), all); left; left &= left - 1, ++at) s_few_at[at] = 32 * (w + lane) + __ffs(left) - 1;
-          k += all;
-        }
-        __syncthreads();
+      // a list of them, a lane a word, so that every warp takes as many of them; a long one over the scores, which are done with
+      const bool few = all_open <= kFewExact;
+      int* const at = few ? s_few_at : reinterpret_cast<int*>(scores);
+      for (int w = w0; w < w1; w += 32) {
+        uint32_t left = w + lane < w1 ? s_open[w + lane] : 0, all;
+        for (uint32_t k = open_at + scan(__popc(left), all); left; left &= left - 1, ++k) at[k] = 32 * (w + lane) + __ffs(left) - 1;
+        open_at += all;
+      }
+      __syncthreads();
+      if (few) {
         for (uint32_t i = warp; i < all_open; i += kChooseWarps) {
-          const uint64_t key = exact_score(p, b, hk, p.first + s_few_at[i]);
+          const uint64_t key = exact_score(p, b, hk, p.first + at[i]);
           if (lane == 0) s_few[i] = key;
         }
         __syncthreads();
@@ -494,35 +593,24 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
           const uint64_t key = s_few[tid];
           uint32_t better = 0;
           for (uint32_t j = 0; j < all_open; ++j) better += s_few[j] > key || (s_few[j] == key && j < tid);
-          if (better >= wanted) atomicAnd(&s_open[s_few_at[tid] / 32], ~(1u << (s_few_at[tid] & 31)));
+          if (better >= wanted) atomicAnd(&s_open[at[tid] / 32], ~(1u << (at[tid] & 31)));
         }
       } else {
-        uint32_t k = open_at;
-        for (int w = w0; w < w1; ++w)
-          for (uint32_t left = s_open[w]; left; left &= left - 1, ++k) {
-            const uint64_t key = exact_score(p, b, hk, p.first + 32 * w + __ffs(left) - 1);
-            if (lane == 0) exact[k] = key;
-          }
-        __syncthreads();
-        auto key = [&](int i) { return exact[i]; };
-        const Cutoff<uint64_t> cut = find_cutoff<uint64_t>(key, static_cast<int>(all_open), wanted, s_sel);
-        choose(key, static_cast<int>(all_open), cut, s_won, s_sel);
-        __syncthreads();
-        k = open_at;
-        for (int w = w0; w < w1; ++w) {  // back to their blocks
-          const uint32_t open = s_open[w], i = k + __popc(open & below);
-          const uint32_t word = __ballot_sync(0xffffffffu, (open >> lane & 1) && (s_won[i / 32] >> (i % 32) & 1));
-          __syncwarp();
-          if (lane == 0) s_open[w] = word;
-          k += __popc(open);
+        for (uint32_t i = 8 * warp; i < all_open; i += 8 * kChooseWarps) {
+          const uint32_t k = i + lane / 4;
+          const uint64_t key = exact_scores(p, b, hk, k < all_open ? p.first + at[k] : -1);
+          if (k < all_open && (lane & 3) == 0) exact[k] = key;
         }
+        __syncthreads();
+        choose_exact(exact, static_cast<int>(all_open), wanted, s_won, s_sel);
+        __syncthreads();
+        for (uint32_t i = tid; i < all_open; i += kChooseThreads)
+          if (!(s_won[i / 32] >> (i % 32) & 1)) atomicAnd(&s_open[at[i] / 32], ~(1u << (at[i] & 31)));
       }
       __syncthreads();
     }
   } else {
-    auto key = [&](int i) { return exact[i]; };
-    const Cutoff<uint64_t> cut = find_cutoff<uint64_t>(key, len, static_cast<uint32_t>(need), s_sel);
-    choose(key, len, cut, s_in, s_sel);
+    choose_exact(exact, len, static_cast<uint32_t>(need), s_in, s_sel);
     for (int w = tid; w < words; w += kChooseThreads) s_open[w] = 0;
     __syncthreads();
   }

@@ -429,3 +429,19 @@ def test_select_where_32_bits_are_not_enough(PS, hd, kind):
             bounds[..., 6] = (2.0 ** -40 * (1 + n * 37 % 101))[:, None, None].to(BF16)
     select_case(PS, [16 * 900, 16 * 130], 90, 1, 2, hq=8, hkv=2, hd=hd, make=make, seed=11)
     select_case(PS, [16 * 6000], 400, 1, 2, hq=4, hkv=1, hd=hd, make=make, seed=12)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 40])
+@pytest.mark.parametrize("odd", [1, 7, 30, 60, 300])
+def test_select_with_blocks_that_have_no_score(PS, hd, odd):
+    """Blocks with an infinity or a NaN in their bounds, and blocks whose sums overflow 32 bits (on either side), among others:
+    fewer and more of them than are wanted."""
+    def make(q, bounds, tab):
+        g = torch.Generator(device="cuda").manual_seed(odd)
+        at = torch.randperm(len(bounds), device="cuda", generator=g)[:odd]
+        for i, pg in enumerate(at.tolist()):
+            if i % 3 == 0:
+                bounds[pg, 0, i % 2, i % hd] = [float("inf"), float("nan"), -float("inf")][i // 3 % 3]
+            else:  # finite, but not in 32 bits
+                bounds[pg, i % 2, :, :] = (bounds[pg, i % 2].float().sign() * 3e38).to(BF16)
+    select_case(PS, [16 * 400, 16 * 90], 40, 1, 2, hq=8, hkv=2, hd=hd, make=make, seed=odd)
