@@ -533,7 +533,9 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   const size_t smem = static_cast<size_t>(sn::bit_words(room) + p.held) * sizeof(uint32_t);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int r = static_cast<int>(rows);
-  const int rc = rows <= sn::sm_count() ? sn::launch_plan<1024>(r, smem, st, p) : sn::launch_plan<512>(r, smem, st, p);
+  // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
+  // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512
+  const int rc = rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p) : sn::launch_plan<512>(r, smem, st, p);
   if (rc != SN_OK) return rc;
   // three CTAs fit on an SM; two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM
   // of its own (4 rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)
