@@ -40,6 +40,7 @@ struct AppendParams {
 
 // One thread per (token, head, element pair of the head): elements (j, j +
 // rot/2) or (2j, 2j + 1) of the rotated part, two neighbours past it.
+template <bool kAt>  // positions are given
 __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -59,8 +60,8 @@ __global__ void __launch_bounds__(256) rotary_paged_append_kernel(const AppendPa
   __nv_bfloat16* const q = p.q + (static_cast<int64_t>(t) * p.hq + head) * p.hd;  // if it is a head of q
   const bool stray = p.cu && (t < p.cu[b] || t >= end);  // a token of no stream
   const int pos = p.seq_lens[b] - (end - t);
-  const int turn = p.positions ? p.positions[t] : pos;
-  if (stray || pos < 0 || turn < 0 || turn >= p.max_pos) {
+  const int turn = kAt ? p.positions[t] : pos;
+  if (stray || pos < 0 || (kAt && turn < 0) || turn >= p.max_pos) {
     if (!stray) record_status(SN_ERR_INVALID_ARGUMENT);
     if (head < p.hq) q[i1] = q[i2] = __float2bfloat16_rn(0.f);
     return;
@@ -107,7 +108,7 @@ __device__ __noinline__ void zero_row(__nv_bfloat16* row, int n) {
   for (int i = 8 * (threadIdx.x & 31); i < n; i += 256) *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
 }
 
-template <bool kInterleaved>
+template <bool kInterleaved, bool kAt>
 __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const AppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(128) rotary_paged_append_vec_kernel(const Appe
     }
   }
   const int pos = p.seq_lens[s] - (end - t);
-  const int angle = p.positions ? p.positions[t] : pos;
-  if (pos < 0 || angle < 0 || angle >= p.max_pos) {
+  const int angle = kAt ? p.positions[t] : pos;
+  if (pos < 0 || (kAt && angle < 0) || angle >= p.max_pos) {
     record_status(SN_ERR_INVALID_ARGUMENT);
     zero_row(p.q + static_cast<int64_t>(t) * p.hq * p.hd, p.hq * p.hd);
     return;
@@ -266,21 +267,21 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
   float* const scores = kKind == kMass ? p.scores + (static_cast<int64_t>(b) * p.hkv * p.sets_per_kv + set) * p.room * p.score_heads +
                                              (h - hk * (p.hq / p.hkv)) % p.heads_per_set
                                        : nullptr;
-  const int listed = min(p.count, (len + p.map.page_size - 1) / p.map.page_size);  // entries that are read
-  const int64_t steps = kKind == kListed ? static_cast<int64_t>(listed) * p.map.page_size : len;
-  for (int64_t i = warp; i < steps; i += 4) {
-    int blk = static_cast<int>(i / p.map.page_size);
-    const int at = static_cast<int>(i - static_cast<int64_t>(blk) * p.map.page_size);
+  // entries of the list that are read; the host has checked that count pages fit
+  const int steps = kKind == kListed ? min(p.count, (len + p.map.page_size - 1) / p.map.page_size) * p.map.page_size : len;
+  for (int t = warp; t < steps; t += 4) {
+    int blk = t / p.map.page_size;
     if constexpr (kKind == kListed) {
       blk = p.blocks[(static_cast<int64_t>(b) * p.hkv + hk) * p.count + blk];
-      if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + at >= len) continue;
+      if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + t % p.map.page_size >= len) continue;
     }
     const int pg = page_of(p.map, b, blk);
     if (pg < 0) {
       record_status(SN_ERR_INVALID_ARGUMENT);
-      if (kKind == kMass && lane == 0) scores[i * p.score_heads] = -INFINITY;
+      if (kKind == kMass && lane == 0) scores[static_cast<int64_t>(t) * p.score_heads] = -INFINITY;
       continue;
     }
+    const int at = t % p.map.page_size;
     const __nv_bfloat16* kr = p.kp + pg * p.ks.page + hk * p.ks.head + at * p.ks.tok;
     const __nv_bfloat16* vr = p.vp + pg * p.vs.page + hk * p.vs.head + at * p.vs.tok;
     float s = 0.f;
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
       if (c < p.hd) s = fmaf(qv[i], __bfloat162float(kr[c]), s);
     }
     s = warp_sum(s);
-    if (kKind == kMass && lane == 0) scores[i * p.score_heads] = s * 1.4426950408889634f;
+    if (kKind == kMass && lane == 0) scores[static_cast<int64_t>(t) * p.score_heads] = s * 1.4426950408889634f;
     const float mn = fmaxf(m, s);
     const float keep = m == mn ? 1.f : expf(m - mn), w = s == -INFINITY ? 0.f : expf(s - mn);
     m = mn;
@@ -1169,13 +1170,14 @@ int append(const void* qkv, int64_t ld, void* q, void* k_pages, int64_t k_page_s
     const int warp_heads = kAppendHeads * (32 / (head_dim / 16));
     const dim3 grid(static_cast<unsigned>((tokens + 3) / 4),
                     static_cast<unsigned>((nheads + 2 * nheads_kv + warp_heads - 1) / warp_heads));
-    return interleaved ? launch(rotary_paged_append_vec_kernel<true>, grid, dim3(128), 0, st, true, p)
-                       : launch(rotary_paged_append_vec_kernel<false>, grid, dim3(128), 0, st, true, p);
+    auto kernel = interleaved ? (positions ? rotary_paged_append_vec_kernel<true, true> : rotary_paged_append_vec_kernel<true, false>)
+                              : (positions ? rotary_paged_append_vec_kernel<false, true> : rotary_paged_append_vec_kernel<false, false>);
+    return launch(kernel, grid, dim3(128), 0, st, true, p);
   }
   const int64_t blocks = (static_cast<int64_t>(tokens) * (width / 2) + 255) / 256;
   if (blocks > INT32_MAX) return SN_ERR_UNSUPPORTED;
-  return launch(rotary_paged_append_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st,
-                    true, p);
+  return launch(positions ? rotary_paged_append_kernel<true> : rotary_paged_append_kernel<false>, dim3(static_cast<unsigned>(blocks)),
+                dim3(256), 0, st, true, p);
 }
 
 AttendParams attend_params(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* k_pages,
