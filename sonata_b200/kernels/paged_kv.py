@@ -316,12 +316,22 @@ class PagedKVCache:
         return self.mass
 
     def track_bounds(self) -> torch.Tensor:
-        """Room for the bounds of the keys' pages: bounds[layer] is the argument of
-        update_page_bounds, to be called for the new tokens, and select_blocks."""
+        """The bounds of the keys' pages, those of the positions so far: bounds[layer]
+        is the argument of update_page_bounds, to be called for the new tokens, and of
+        select_blocks."""
         if self.bounds is None:
             from .paged_sparse import page_bounds
             self.bounds = page_bounds(self.pool[:, 0])
+            if any(self.lens):
+                self._bound(self.lens)
         return self.bounds
+
+    def _bound(self, counts) -> None:
+        """The bounds of the pages of each slot's last counts[s] positions, in all layers."""
+        from . import paged_sparse
+        cu = torch.tensor([sum(counts[:s]) for s in range(len(counts) + 1)], dtype=torch.int32, device=self.pool.device)
+        for layer in range(self.pool.shape[0]):
+            paged_sparse.update_page_bounds(self.k(layer), self.bounds[layer], self.page_table, self.seq_lens, cu_seqlens=cu)
 
     @property
     def free_pages(self) -> int:
@@ -427,11 +437,7 @@ class PagedKVCache:
             self.lens[s] = keep
         self._upload(cut)
         if self.bounds is not None:
-            from . import paged_sparse
-            new = [keep if s in cut else 0 for s in range(len(self.lens))]
-            cu = torch.tensor([sum(new[:s]) for s in range(len(new) + 1)], dtype=torch.int32, device=self.pool.device)
-            for layer in range(self.pool.shape[0]):
-                paged_sparse.update_page_bounds(self.k(layer), self.bounds[layer], self.page_table, self.seq_lens, cu_seqlens=cu)
+            self._bound([keep if s in cut else 0 for s in range(len(self.lens))])
         return cut
 
     def compact(self) -> int:

@@ -161,6 +161,18 @@ def test_forked_streams_are_cut_apart(cpu):
     consistent(c)
 
 
+def test_bounds_of_what_is_there(cpu):
+    """track_bounds after the first tokens: their pages' bounds, too."""
+    c = make()
+    write(c, 0, [float(i * 7 % 31) for i in range(30)])
+    write(c, 2, [5.0])
+    c.fork(0, 1)
+    assert c.track_bounds() is c.track_bounds() is c.bounds
+    consistent(c)
+    c.evict(9, 3)
+    consistent(c)
+
+
 def test_limits(cpu):
     c = make(pages=9)
     write(c, 0, [1.0] * 29)
