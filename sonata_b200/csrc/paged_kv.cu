@@ -372,6 +372,8 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
 // ---------------------------------------------------------------------------
 constexpr int kAttWarps = 6;
 constexpr int kCutGain = 14;   // steps that a cut has to save
+constexpr int kCutGainListed = 8;  // the same of listed blocks, whose pieces have a CTA each (3 streams of 64 blocks of 16: cut 11.6, not 14.3 us;
+                                   // 48 of up to 64 blocks, which 3 would cut: 28.1, 23.6)
 constexpr int kCutSteps = 2;   // and the least a CTA takes of one
 constexpr int kJoinMost = 48;  // partial results that one CTA joins by itself
 constexpr int kJoinGroup = 8;  // and those of a group otherwise
@@ -383,7 +385,7 @@ struct AttendSplit {
   float* part;       // [2 * grid][kHeadsMax][HD + 2] partial sums, maxima, outputs
   unsigned* ticket;  // [2][2 * grid] arrivals of a set's pieces or groups, of a group's pieces; zero between calls
   int group, sets;   // query heads per key/value head; head sets of a stream (hkv * sets per kv head)
-  int slots;  // CTAs that are on the device together: no more take part in a cut
+  int slots;  // CTAs that are on the device together: no more take part in a cut into even shares
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -632,15 +634,59 @@ __global__ void __launch_bounds__(kAttWarps * 32, 2)
   // its share of the tiles.  Measured, cut / not: 4 streams of 2000 positions 13.5 / 20.5 us, 2 of 1500 13.9 / 14.3, 50 of
   // 931 to 1863 31.5 / 28.9, 86 of up to 906 with one key/value head 34.8 / 19.3.
   const int grid = min(static_cast<int>(gridDim.x), sp.slots);  // CTAs with a share
-  const bool cut = longest - total / grid > kCutGain * kAttWarps;
+  const bool cut = longest - total / grid > (kKind == kListed ? kCutGainListed : kCutGain) * kAttWarps;
   const bool single = !cut && static_cast<long long>(p.batch) * sp.sets <= gridDim.x;
-  const long long share = max((total + grid - 1) / grid, cut ? static_cast<long long>(kCutSteps) * kAttWarps : 1LL);
+  long long share = max((total + grid - 1) / grid, cut ? static_cast<long long>(kCutSteps) * kAttWarps : 1LL);
   long long at = me * share;
-  const long long stop = single ? at + 1 : me < grid ? min(at + share, total) : 0;
-  if (at >= stop) return;
+  long long stop = single ? at + 1 : me < grid ? min(at + share, total) : 0;
   int b = 0;
   long long in_b = 0;  // place of `at` within the stream's tiles, head set by head set
-  if (single) {
+  // Listed blocks are few tiles a (stream, head set), so a CTA whose share ended one and began the next would take nearly twice
+  // the time of the others: where there are CTAs enough, each (stream, head set) begins with a share of its own (128 blocks of 16
+  // of 3 streams 15.7 -> 12.2 us, of 8 19.6 -> 16.4).  The axis then has unused places behind each.
+  bool even = false;
+  if constexpr (kKind == kListed) {
+    for (int more = 0; cut && more <= 4; ++more) {  // with somewhat larger shares, if need be
+      const long long mine = share + share * more / 4, place = me * mine;
+      long long before = 0;
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {  // every warp for itself
+        if (p.batch > 32) tiles = b0 + lane < p.batch ? stream_tiles<kKind>(p, stream_len(p, b0 + lane)) : 0;
+        const long long own = (tiles + mine - 1) / mine, n = own * sp.sets;
+        long long upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, me >= before + upto - n && me < before + upto);
+        if (here) {
+          const int l = __ffs(here) - 1;
+          b = b0 + l;
+          const long long pieces = __shfl_sync(0xffffffffu, own, l), k = me - before - __shfl_sync(0xffffffffu, upto - n, l);
+          const int nt = __shfl_sync(0xffffffffu, tiles, l);
+          const long long from = k % pieces * mine;
+          in_b = k / pieces * nt + from;
+          stop = place + min(mine, nt - from);
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      if (before <= min(static_cast<int>(gridDim.x), kAttGridMax)) {
+        if (me >= before) return;
+        even = true;
+        share = mine;
+        at = place;
+        break;
+      }
+    }
+    if (cut && !even) {  // not enough CTAs
+      b = 0;
+      in_b = 0;
+      stop = me < grid ? min(at + share, total) : 0;
+    }
+  }
+  if (at >= stop) return;
+  if (even) {  // b, in_b and stop are set
+  } else if (single) {
     b = me / sp.sets;
     if (b >= p.batch) return;
     const int n = p.batch <= 32 ? __shfl_sync(0xffffffffu, tiles, b) : stream_tiles<kKind>(p, stream_len(p, b));

@@ -314,7 +314,10 @@ def test_sparse_all_blocks_is_attention(PS):
     lens = [700, 33, 0, 1000]
     blocks = torch.arange(63, device="cuda", dtype=torch.int32).expand(4, 4, 63).contiguous()
     got, q, kp, vp, tab = sparse_case(PS, lens, 63, blocks=blocks)
-    assert torch.equal(got, PK.paged_decode_attention(q, kp, vp, tab, ints(lens)))
+    _, bound, _ = sparse_truth(q, kp, vp, tab, lens, blocks, 128 ** -0.5)
+    # both are within the bound of the same sums, whatever pieces they are cut into: within twice the bound of one another
+    d = (got.double() - PK.paged_decode_attention(q, kp, vp, tab, ints(lens)).double()).abs()
+    assert (d <= 2 * bound).all()
 
 
 def test_sparse_bad_pages(PS, cuda_lib):
