@@ -19,6 +19,8 @@ from .. import _lib
 from . import paged_kv as PK
 from ._common import call, current_handle, fast, on_stream, require_cuda, same_device
 
+EVICT_MOST = 1 << 19  # max_pages * page_size that evict_positions takes
+
 
 @functools.lru_cache(maxsize=256)
 def _mass_size(batch: int, nheads: int, nheads_kv: int, head_dim: int, max_positions: int) -> int:
@@ -78,9 +80,9 @@ def evict_positions(pool: torch.Tensor, page_table: torch.Tensor, seq_lens: torc
     ones follow in order; mass goes with it and is zero behind.  Streams with no
     more than `keep` positions are left alone.  seq_lens is not changed: the
     caller sets it to min(n, keep) (PagedKVCache.evict does).  A page that two
-    streams share must not be cut in either.  With return_source: int32
-    [n_layers, batch, nheads_kv, keep], where each place's position was (-1 past
-    the end of a stream that was left alone)."""
+    streams share must not be cut in either; max_pages * page_size is EVICT_MOST
+    at most.  With return_source: int32 [n_layers, batch, nheads_kv, keep], where
+    each place's position was (-1 past the end of a stream that was left alone)."""
     if stream is None:
         r = fast().evict(pool, page_table, seq_lens, mass, keep, recent, sinks, return_source)
         if r is not None:

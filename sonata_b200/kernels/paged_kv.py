@@ -269,6 +269,10 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, stream=
             call("sn_copy_pages", *args, st)
 
 
+class OutOfPages(RuntimeError):
+    """A PagedKVCache has too few free pages for what was asked; nothing was changed."""
+
+
 class PagedKVCache:
     """The pages of all layers' keys and values, and the host's book-keeping of
     who owns them: `slots` streams, each a list of pages and a length.
@@ -363,7 +367,7 @@ class PagedKVCache:
             raise ValueError(f"a stream would need {max(want)} pages of at most {self.max_pages}")
         need = sum(w - len(p) for w, p in zip(want, self.pages))
         if need > len(self._free):
-            raise RuntimeError(f"out of pages: {need} needed, {len(self._free)} free")
+            raise OutOfPages(f"out of pages: {need} needed, {len(self._free)} free")
         grown = [s for s, w in enumerate(want) if w > len(self.pages[s])]
         for s in grown:
             self.pages[s] += [self._take() for _ in range(want[s] - len(self.pages[s]))]
@@ -378,7 +382,7 @@ class PagedKVCache:
         full = self.lens[src] // self.page_size
         partial = self.lens[src] % self.page_size > 0
         if partial and not self._free:
-            raise RuntimeError("out of pages: 1 needed, 0 free")
+            raise OutOfPages("out of pages: 1 needed, 0 free")
         self.pages[dst] = self.pages[src][:full]
         for p in self.pages[dst]:
             self._users[p] += 1
@@ -419,7 +423,7 @@ class PagedKVCache:
                     users[p] -= 1
                     own.append((s, i))
         if len(own) > len(self._free):
-            raise RuntimeError(f"out of pages: {len(own)} needed, {len(self._free)} free")
+            raise OutOfPages(f"out of pages: {len(own)} needed, {len(self._free)} free")
         src = [self.pages[s][i] for s, i in own]
         dst = [self._take() for _ in own]
         if own:

@@ -45,8 +45,10 @@ class RaggedZonos:
         `recent` among them; it is cut when it has four pages more.  `attend_blocks`:
         blocks of page_size positions that a step attends to in each key/value head,
         the first and the last two among them."""
-        if budget is not None and (attend_blocks is not None or not recent + sinks <= budget):
-            raise ValueError("budget must cover recent and sinks, and goes without attend_blocks")
+        if budget is not None and (attend_blocks is not None or budget < 1 or min(recent, sinks) < 0 or recent + sinks > budget):
+            raise ValueError("budget must be positive and cover recent and sinks, and goes without attend_blocks")
+        if budget is not None and -(-max_len // page_size) * page_size > PE.EVICT_MOST:
+            raise ValueError(f"a budget goes with at most {PE.EVICT_MOST} positions of a stream")
         if attend_blocks is not None and attend_blocks < 3:
             raise ValueError("attend_blocks must be at least 3")
         cfg = model.cfg
@@ -86,7 +88,7 @@ class RaggedZonos:
         if self.budget is not None and max(self.cache.lens) >= self.budget + 4 * self.cache.page_size:
             try:
                 self.cache.evict(self.budget, recent=self.recent, sinks=self.sinks)
-            except RuntimeError:  # no free pages to take shared ones apart: nothing was cut, the next step tries again
+            except PK.OutOfPages:  # no free pages to take shared ones apart: nothing was cut, the next step tries again
                 pass
 
     def _weigh(self, layer: int, slot: int, q: torch.Tensor) -> None:

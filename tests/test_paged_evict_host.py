@@ -189,3 +189,34 @@ def test_limits(cpu):
     assert c.evict(29) == []
     with pytest.raises(RuntimeError):
         PK.PagedKVCache(1, 1, 1, 1, 1, 1, device="cpu").evict(1)
+
+
+def test_budget_passes_errors_on(cpu):
+    """A budget's cut waits for free pages, and for nothing else."""
+    from sonata_b200.kernels import serve
+    r = object.__new__(serve.RaggedZonos)
+    r.budget, r.recent, r.sinks, r.cache = 8, 4, 1, make(pages=9)
+    write(r.cache, 0, [1.0] * 29)
+    r.cache.fork(0, 1)
+    r._cut()  # two pages for the first of them, none free
+    assert r.cache.lens == [29, 29, 0, 0]
+    r.cache.free(1)
+
+    def fail(*args, **kwargs):
+        raise RuntimeError("of the device")
+
+    right, PE.evict_positions = PE.evict_positions, fail  # the fixture puts the operator back
+    with pytest.raises(RuntimeError, match="of the device"):
+        r._cut()
+    assert r.cache.lens == [29, 0, 0, 0]
+    PE.evict_positions = right
+    r._cut()
+    assert r.cache.lens == [8, 0, 0, 0]
+
+
+def test_budget_refusals():
+    from sonata_b200.kernels import serve
+    for bad in (dict(budget=0, recent=0, sinks=0), dict(budget=8, recent=-1, sinks=1), dict(budget=8, recent=1, sinks=-1),
+                dict(budget=8, recent=4, sinks=5), dict(budget=80, attend_blocks=8), dict(budget=80, max_len=PE.EVICT_MOST + 1)):
+        with pytest.raises(ValueError):
+            serve.RaggedZonos(None, num_pages=9, **{"max_len": 100, **bad})
