@@ -320,6 +320,21 @@ def test_sparse_all_blocks_is_attention(PS):
     assert (d <= 2 * bound).all()
 
 
+@pytest.mark.parametrize("lens,hkv,count", [
+    ([16] * 45 + [20000, 300, 20000], 2, 1000),  # over 32 streams, with somewhat larger shares
+    ([3000] + [9] * 142 + [2500], 4, 150),            # more pieces than CTAs
+    ([40] * 300 + [6400, 0, 6400], 4, 400),      # more (stream, head)s than partial results have places for
+])
+def test_sparse_cuts(PS, lens, hkv, count):
+    from sonata_b200 import _lib
+    from sonata_b200.kernels import paged_kv as PK
+    ws = PK.decode_workspace(len(lens), 2 * hkv, 64)
+    runs = [sparse_case(PS, lens, count, hq=2 * hkv, hkv=hkv, hd=64, workspace=ws, seed=count)[0] for _ in range(2)]
+    assert torch.equal(*runs)
+    counters = ws[:4 * _lib.SN_PAGED_DECODE_COUNTERS].view(torch.int32)
+    assert not counters.any()  # ready for the next call
+
+
 def test_sparse_bad_pages(PS, cuda_lib):
     g = torch.Generator(device="cuda").manual_seed(0)
     kp, vp = (torch.randn(4, 1, 16, 64, device="cuda", generator=g).to(BF16) for _ in range(2))
