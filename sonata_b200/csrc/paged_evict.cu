@@ -60,7 +60,7 @@ int64_t plan_size(int64_t room, int64_t keep) { return 2 * most_pairs(room, keep
 // (then the first ones stay); the holes and movers; their lists.  A pass over the keys is bound by issue slots (30000 of them:
 // 940 warp steps, 3 us), so there are two.
 template <int T>
-__global__ void __launch_bounds__(T, T > 512 ? 1 : 2) evict_plan_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_kernel(const EvictParams p) {
   constexpr int kWarps = T / 32;
   extern __shared__ __align__(16) uint32_t s_dyn[];
   __shared__ SelectShared<T> s_sel;
@@ -534,8 +534,11 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int r = static_cast<int>(rows);
   // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
-  // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512
-  const int rc = rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p) : sn::launch_plan<512>(r, smem, st, p);
+  // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512,
+  // and where there are more than two an SM, 256, six CTAs an SM (4096 rows of 2112: 225 -> 201, 480 of 9000 125 -> 127)
+  const int rc = rows > 2 * sn::sm_count()                   ? sn::launch_plan<256>(r, smem, st, p)
+                 : rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p)
+                                                         : sn::launch_plan<512>(r, smem, st, p);
   if (rc != SN_OK) return rc;
   // three CTAs fit on an SM; two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM
   // of its own (4 rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)

@@ -36,7 +36,7 @@ struct BoundsParams {
 
 // Stream b's touched blocks have slots cu[b] / page + 2 b and following: n new tokens touch n / page + 2 blocks at most.
 __device__ __forceinline__ int64_t first_slot(const BoundsParams& p, int b) {
-  return static_cast<int64_t>(max(p.cu[b], 0)) / p.map.page_size + 2 * static_cast<int64_t>(b);
+  return max(p.cu[b], 0) / p.map.page_size + 2 * static_cast<int64_t>(b);
 }
 
 // Work items: (touched page, head).
@@ -434,10 +434,10 @@ __device__ __noinline__ void choose_exact(const uint64_t* keys, int len, uint32_
   choose(key, len, cut, bits, s);
 }
 
-// One CTA a row; kScored: block_scores_kernel has run, else exact_scores_kernel.
-template <bool kScored, int kChooseThreads>
-__global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) choose_blocks_kernel(const __grid_constant__ SelectParams p) {
-  constexpr int kChooseWarps = kChooseThreads / 32, kChooseHeld = kChooseThreads > 512 ? 8 : 16;  // keys a thread holds
+// One CTA a row, kPerSM of them an SM; kScored: block_scores_kernel has run, else exact_scores_kernel.
+template <bool kScored, int kChooseThreads, int kPerSM>
+__global__ void __launch_bounds__(kChooseThreads, kPerSM) choose_blocks_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kChooseWarps = kChooseThreads / 32, kChooseHeld = kPerSM > 2 ? 4 : 16;  // keys a thread holds
   extern __shared__ uint32_t s_bits[];
   __shared__ SelectShared<kChooseThreads> s_sel;
   __shared__ uint32_t s_range[5];  // least and greatest key, S, and for regular_range
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
     return upto - v;
   };
   if constexpr (kScored) {
-    // the keys of words warp, warp + 16, ...: the first 16 of a warp stay in registers, the rest are read again
+    // the keys of words warp, warp + 16, ...: the first of a warp stay in registers, the rest are read again
     uint32_t held[kChooseHeld];
     uint32_t least = 0xffffffffu, most = 0, S = 0;
     auto range = [&](uint2 v) {
@@ -631,10 +631,10 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseThreads > 256 ? 1 : 2) 
   }
 }
 
-template <bool kScored, int T>
+template <bool kScored, int T, int kPerSM>
 int launch_choose(int rows, size_t smem, cudaStream_t st, const SelectParams& p) {
-  if (!smem_room<choose_blocks_kernel<kScored, T>>(kChooseMost / 32 * 3 * sizeof(uint32_t))) return SN_ERR_LAUNCH;
-  return launch(choose_blocks_kernel<kScored, T>, dim3(static_cast<unsigned>(rows)), dim3(T), smem, st, true, p);
+  if (!smem_room<choose_blocks_kernel<kScored, T, kPerSM>>(kChooseMost / 32 * 3 * sizeof(uint32_t))) return SN_ERR_LAUNCH;
+  return launch(choose_blocks_kernel<kScored, T, kPerSM>, dim3(static_cast<unsigned>(rows)), dim3(T), smem, st, true, p);
 }
 
 }  // namespace
@@ -724,10 +724,13 @@ int sn_select_blocks(const void* q, int64_t q_batch_stride, int64_t q_head_strid
     if (rc != SN_OK) return rc;
   }
   // the choice is a chain of steps: more threads a row where there are few rows (3 streams of up to 100001 positions, 12 rows:
-  // 256 threads 18.9 us, 512 16.4, 1024 18.7), two CTAs an SM where there are many
+  // 256 threads 18.9 us, 512 16.4, 1024 18.7), two CTAs an SM where there are more, and four, with fewer keys in registers,
+  // where there are more than two an SM (2048 rows of 500 blocks 136 -> 120, of 125 68 -> 53; 192 rows of 500 18.4 -> 20.5)
   const int r = static_cast<int>(rows);
-  if (!scored) return sn::launch_choose<false, 256>(r, smem, st, p);
-  return rows <= sn::sm_count() ? sn::launch_choose<true, 512>(r, smem, st, p) : sn::launch_choose<true, 256>(r, smem, st, p);
+  if (!scored) return sn::launch_choose<false, 256, 2>(r, smem, st, p);
+  return rows <= sn::sm_count()       ? sn::launch_choose<true, 512, 1>(r, smem, st, p)
+         : rows <= 2 * sn::sm_count() ? sn::launch_choose<true, 256, 2>(r, smem, st, p)
+                                      : sn::launch_choose<true, 256, 4>(r, smem, st, p);
 }
 
 }  // extern "C"
