@@ -39,12 +39,13 @@ struct EvictParams {
   float* mass;  // [layers, batch, hkv, >= room] by strides
   int64_t ml, mb, mh;
   int* source;  // [layers, batch, hkv, keep] or null
-  int2* head;   // [layers, batch, hkv]: n, pairs of a hole and a mover
+  int2* head;   // [layers, batch, hkv]: n, pairs of a hole and a mover (-1: the rows are moved)
   int* plan;    // [layers, batch, hkv] of plan_ints: holes, movers, and the keys where shared memory does not hold them
   int64_t plan_ints;
   int most;     // pairs of a row at most, a multiple of 4
   int batch, hkv, keep, recent, sinks;
   int held;     // keys in shared memory: all candidates' or none (then they are in the plan)
+  int units;    // 16-byte pieces of a position's two rows, 0: rows are not such
 };
 
 // Of max_pages * page_size = room positions: the words of shared memory for two bits each, and room to align the keys;
@@ -53,6 +54,55 @@ int64_t bit_words(int64_t room) { return (room + 31) / 32 * 2 + 8; }
 bool keys_held(int64_t room) { return bit_words(room) + room <= kEvictWords; }
 int64_t most_pairs(int64_t room, int64_t keep) { return (std::min(room / 2, keep) + 3) / 4 * 4; }
 int64_t plan_size(int64_t room, int64_t keep) { return 2 * most_pairs(room, keep) + (keys_held(room) ? 0 : (room + 3) / 4 * 4 + 4); }
+
+// Where a position's K row is in its layer and head, or -1.
+__device__ __forceinline__ int64_t place(const EvictParams& p, int b, int at) {
+  const int blk = at / p.map.page_size, pg = page_of(p.map, b, blk);
+  if (pg < 0) {
+    record_status(SN_ERR_INVALID_ARGUMENT);
+    return -1;
+  }
+  return pg * p.page_bytes + static_cast<int64_t>(at - blk * p.map.page_size) * p.row_bytes;
+}
+
+// Few rows are moved by the CTA that has planned them, its lists in shared memory, while the other launch finds nothing to do:
+// kFewUnits pieces of 16 bytes a thread at once.  A stream's 64 positions over its budget, 64 recent ones (48 rows, masses that
+// the calls before have not put in order) 17.0 -> 13.4 us, 152 over it 17.5 -> 16.5; 256, which have more than kFewPieces,
+// would take 18.4 where they now take 16.6.
+constexpr int kFewMoves = 512, kFewPieces = 8192, kFewUnits = 8;
+struct Move { int64_t from, to; };
+template <int T>
+__device__ __forceinline__ void move_few(const EvictParams& p, int layer, int b, int h, int n, int pairs, const int* list, Move* moves) {
+  const int tid = threadIdx.x, recent = p.recent, edge = p.keep - recent, total = pairs + recent, nu = p.units;
+  char* const base = p.pool + layer * p.layer_bytes + h * p.head_bytes;
+  for (int i = tid; i < total; i += T) {
+    const int from = i < pairs ? list[pairs + i] : n - recent + (i - pairs), to = i < pairs ? list[i] : edge + (i - pairs);
+    moves[i] = {place(p, b, from), place(p, b, to)};
+  }
+  __syncthreads();
+  // movers by as many as fit at once, the recent ones all in the last round, as their places may be those of movers and of one another
+  for (int u0 = 0, end; u0 < total * nu; u0 = end) {
+    end = total * nu - u0 <= kFewUnits * T ? total * nu : min(u0 + kFewUnits * T, pairs * nu);
+    uint4 v[kFewUnits];
+    // piece u0 + j T + this thread of the rows' ones: its offset in a row, and whether it is to be moved
+    auto piece = [&](int j, Move& move, int64_t& off) {
+      const int u = u0 + j * T + tid, i = u / nu, e = u - i * nu;
+      if (u >= end) return false;
+      move = moves[i];
+      off = (e >= nu / 2 ? p.kv_bytes - nu / 2 * 16 : 0) + e * 16;
+      return move.from >= 0 && move.to >= 0;
+    };
+    Move move;
+    int64_t off;
+#pragma unroll
+    for (int j = 0; j < kFewUnits; ++j)
+      if (piece(j, move, off)) v[j] = *reinterpret_cast<const uint4*>(base + move.from + off);
+    if (end == total * nu) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kFewUnits; ++j)
+      if (piece(j, move, off)) *reinterpret_cast<uint4*>(base + move.to + off) = v[j];
+  }
+}
 
 // The plan of a row.  A histogram of the keys' upper bits (of the masses' exponents and first bits) finds the bin of the last
 // one that stays.  One more pass makes two bits of each key, above that bin and in it, and everything after that is done on
@@ -75,7 +125,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
   }
   s_sel.clear();
   __syncthreads();
-  pdl_launch_dependents();
+  if constexpr (T <= 256) pdl_launch_dependents();  // (else later: CTAs of the other launch would only wait, and it may have nothing to do)
   pdl_wait();
   int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
   int* const plan = p.plan + row * p.plan_ints;
@@ -281,9 +331,17 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
   if (source)  // of what stays where it is, and for now of the holes
     for (int i = tid; i < edge; i += T) source[i] = i;
   __syncthreads();
-  if (tid == 0) p.head[row] = make_int2(n, static_cast<int>(pairs));
-  // mass, as the rows will go: movers into holes, then the recent ones, which may overlap their places (zeros behind are left
-  // to the other launch, which has more threads)
+  if constexpr (T > 256) pdl_launch_dependents();
+  // (the histogram, which is done with, holds where the rows come from and go)
+  const bool few = T > 256 && p.units > 0 && n - keep <= T && pairs + recent <= kFewMoves &&
+                   static_cast<int>(pairs + recent) * p.units <= kFewPieces && recent * p.units <= kFewUnits * T && (list || pairs == 0);
+  if (tid == 0) p.head[row] = make_int2(n, few ? -1 : static_cast<int>(pairs));
+  if constexpr (T > 256) {
+    static_assert(sizeof(s_sel.hist) >= kFewMoves * sizeof(Move));
+    if (few) move_few<T>(p, layer, b, h, n, static_cast<int>(pairs), list, reinterpret_cast<Move*>(s_sel.hist));
+  }
+  // mass, as the rows go: movers into holes, then the recent ones, which may overlap their places (zeros behind are left to the
+  // other launch, which has more threads, if there is something for it to do)
   float w[4];
   auto read_recent = [&](int k0) {
 #pragma unroll
@@ -296,7 +354,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
 #pragma unroll 4
   for (uint32_t i = tid; i < pairs; i += T) {
     const int hole = list ? list[i] : holes[i], mover = list ? list[pairs + i] : movers[i];
-    if (list) {
+    if (list && !few) {
       holes[i] = hole;
       movers[i] = mover;
     }
@@ -304,6 +362,7 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
     if (source) source[hole] = mover;
   }
   __syncthreads();
+  if (few && keep + tid < n) mass[keep + tid] = 0.f;
   for (int k0 = 0; k0 < recent; k0 += 4 * T) {
     if (k0 > 0) {
       read_recent(k0);
@@ -352,7 +411,7 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   const int* const plan = p.plan + row * p.plan_ints;
   const int2 head = p.head[row];
   const int n = head.x, pairs = head.y;
-  if (n <= keep) return;
+  if (n <= keep || pairs < 0) return;  // nothing to do, or done
   {  // mass behind what is kept: whole 16 bytes, and what lies before and behind them
     const int threads = kMoveThreads * C, me = rank * kMoveThreads + static_cast<int>(threadIdx.x);
     float* const tail = p.mass + layer * p.ml + b * p.mb + h * p.mh + keep;
@@ -363,15 +422,6 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   }
   const int nu = NU ? NU : static_cast<int>(2 * p.row_bytes / sizeof(T));
   char* const base = p.pool + layer * p.layer_bytes + h * p.head_bytes;
-  // where a position's K row is, or -1
-  auto place = [&](int at) -> int64_t {
-    const int blk = at / p.map.page_size, pg = page_of(p.map, b, blk);
-    if (pg < 0) {
-      record_status(SN_ERR_INVALID_ARGUMENT);
-      return -1;
-    }
-    return pg * p.page_bytes + static_cast<int64_t>(at - blk * p.map.page_size) * p.row_bytes;
-  };
   // Unit u0 + 32 j + this lane of the cnt positions that the lanes have looked up: which of them, and its offset in it.
   auto unit = [&](int u0, int j, int cnt, int& at) {
     int e;
@@ -412,8 +462,8 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   auto look_up_recent = [&](int k) {
     recent_from = recent_to = -1;
     if (lane >= per || k >= recent) return;
-    recent_from = place(n - recent + k);
-    recent_to = place(edge + k);
+    recent_from = place(p, b, n - recent + k);
+    recent_to = place(p, b, edge + k);
   };
   look_up_recent(wid * per + lane);
   // ---- movers into holes ----
@@ -422,8 +472,8 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
     const int cnt = min(batch, pairs - first), units = cnt * nu;
     int64_t from = -1, to = -1;
     if (lane < cnt) {
-      to = place(plan[first + lane]);
-      from = place(plan[p.most + first + lane]);
+      to = place(p, b, plan[first + lane]);
+      from = place(p, b, plan[p.most + first + lane]);
     }
     for (int u0 = 0; u0 < units; u0 += 32 * U) {
       T v[U];
@@ -529,6 +579,7 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   p.keep = keep;
   p.recent = recent;
   p.sinks = sinks;
+  p.units = sn::aligned16(pool) && p.row_bytes % 16 == 0 ? 2 * p.row_bytes / 16 : 0;
   p.held = sn::keys_held(room) ? static_cast<int>(room) : 0;
   const size_t smem = static_cast<size_t>(sn::bit_words(room) + p.held) * sizeof(uint32_t);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -540,11 +591,12 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
                  : rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p)
                                                          : sn::launch_plan<512>(r, smem, st, p);
   if (rc != SN_OK) return rc;
-  // three CTAs fit on an SM; two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM
-  // of its own (4 rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)
+  // three CTAs fit on an SM, one beside a plan: all of them start at once (48 rows, 320 moved rows each, 8 CTAs a row 18.3, 7
+  // 16.6); two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM of its own (4
+  // rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)
   const int C = rows * sn::kMoveCluster <= sn::sm_count() ? sn::kMoveCluster
-                                                          : static_cast<int>(std::clamp<int64_t>(3 * sn::sm_count() / rows, 2, 8));
-  if (sn::aligned16(pool) && p.row_bytes % 16 == 0) {
+                                                          : static_cast<int>(std::clamp<int64_t>((3 * sn::sm_count() - 2 * rows) / rows, 2, 8));
+  if (p.units) {
     if (head_dim == 128) return sn::launch_move<uint4, 32>(r, C, st, p);
     if (head_dim == 64) return sn::launch_move<uint4, 16>(r, C, st, p);
     return sn::launch_move<uint4, 0>(r, C, st, p);
