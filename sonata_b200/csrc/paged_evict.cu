@@ -20,10 +20,10 @@ namespace {
 
 // Two launches: the plan of each row (a CTA each: what stays, the lists of holes and movers, mass), bound by the chain of
 // its steps (7 us for 2044 candidates, 21 for 29739, of which 4 the load of their masses), and the moves, bound by HBM where
-// there are many (172 MB in 33 us, 5.2 TB/s) and by the chain list - table - row - barrier where there are few.  12 layers of
-// a stream of 2112 positions cut by 64: 14.7 us (18.9 with nothing in L2), of 30011 cut to 4096: 58 us.  In one launch, a
-// cluster a row, either the choice is shared out, its histograms exchanged through distributed shared memory (27 us for the
-// former), or the other CTAs of the cluster wait for the one that makes it (30 us).
+// there are many (172 MB in 33 us, 5.2 TB/s); few are moved with the plan.  12 layers of a stream of 2112 positions cut by 64:
+// 13.1 us (15.5 with nothing in L2), of 30011 cut to 4096: 58 us.  In one launch, a cluster a row, either the choice is shared
+// out, its histograms exchanged through distributed shared memory (27 us for the former), or the other CTAs of the cluster
+// wait for the one that makes it (30 us).
 constexpr int kEvictMost = 1 << 19;   // candidates of a stream: two bits each in shared memory
 constexpr int kEvictWords = 52992;    // of shared memory for those bits and for keys
 constexpr int kEvictCopy = 1024;      // 16-byte pieces of one copy to shared memory
@@ -110,7 +110,7 @@ __device__ __forceinline__ void move_few(const EvictParams& p, int layer, int b,
 // (then the first ones stay); the holes and movers; their lists.  A pass over the keys is bound by issue slots (30000 of them:
 // 940 warp steps, 3 us), so there are two.
 template <int T>
-__global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(T, 1024 / T) evict_plan_kernel(const EvictParams p) {
   constexpr int kWarps = T / 32;
   extern __shared__ __align__(16) uint32_t s_dyn[];
   __shared__ SelectShared<T> s_sel;
@@ -125,7 +125,6 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
   }
   s_sel.clear();
   __syncthreads();
-  if constexpr (T <= 256) pdl_launch_dependents();  // (else later: CTAs of the other launch would only wait, and it may have nothing to do)
   pdl_wait();
   int* const source = p.source ? p.source + static_cast<int64_t>(row) * keep : nullptr;
   int* const plan = p.plan + row * p.plan_ints;
@@ -331,15 +330,13 @@ __global__ void __launch_bounds__(T, T > 512 ? 1 : T > 256 ? 2 : 6) evict_plan_k
   if (source)  // of what stays where it is, and for now of the holes
     for (int i = tid; i < edge; i += T) source[i] = i;
   __syncthreads();
-  if constexpr (T > 256) pdl_launch_dependents();
+  pdl_launch_dependents();  // not before: CTAs of the other launch would only wait, and it may have nothing to do
   // (the histogram, which is done with, holds where the rows come from and go)
-  const bool few = T > 256 && p.units > 0 && n - keep <= T && pairs + recent <= kFewMoves &&
+  const bool few = p.units > 0 && n - keep <= T && pairs + recent <= kFewMoves &&
                    static_cast<int>(pairs + recent) * p.units <= kFewPieces && recent * p.units <= kFewUnits * T && (list || pairs == 0);
   if (tid == 0) p.head[row] = make_int2(n, few ? -1 : static_cast<int>(pairs));
-  if constexpr (T > 256) {
-    static_assert(sizeof(s_sel.hist) >= kFewMoves * sizeof(Move));
-    if (few) move_few<T>(p, layer, b, h, n, static_cast<int>(pairs), list, reinterpret_cast<Move*>(s_sel.hist));
-  }
+  static_assert(sizeof(s_sel.hist) >= kFewMoves * sizeof(Move));
+  if (few) move_few<T>(p, layer, b, h, n, static_cast<int>(pairs), list, reinterpret_cast<Move*>(s_sel.hist));
   // mass, as the rows go: movers into holes, then the recent ones, which may overlap their places (zeros behind are left to the
   // other launch, which has more threads, if there is something for it to do)
   float w[4];
@@ -586,7 +583,8 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   const int r = static_cast<int>(rows);
   // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
   // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512,
-  // and where there are more than two an SM, 256, six CTAs an SM (4096 rows of 2112: 225 -> 201, 480 of 9000 125 -> 127)
+  // and where there are more than two an SM, 256, four CTAs an SM, whose moves fill the waits of one another's plans (4096 rows
+  // of 2112: 191 -> 144, 768 rows 41 -> 35, 144 of them with work 18.4 -> 19.8, 480 of 9000 129 -> 125)
   const int rc = rows > 2 * sn::sm_count()                   ? sn::launch_plan<256>(r, smem, st, p)
                  : rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p)
                                                          : sn::launch_plan<512>(r, smem, st, p);

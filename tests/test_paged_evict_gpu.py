@@ -299,6 +299,13 @@ def test_evict_ties_and_odd_values(PE, kind):
     evict_case(PE, [200, 3000], 150, 20, 3, mass=mass, hd=8, seed=6)
 
 
+@pytest.mark.parametrize("recent,sinks", [(0, 0), (64, 4), (65, 0), (128, 4), (129, 0), (256, 0)])
+@pytest.mark.parametrize("layers,hkv", [(1, 1), (5, 8)])
+def test_evict_few_and_many_moves(PE, layers, hkv, recent, sinks):
+    """Streams over their budget by a few positions and by more than one CTA moves, of few rows and of many."""
+    evict_case(PE, [601, 664, 640, 728, 800, 855, 856, 857, 1111, 1113, 1300, 600], 600, recent, sinks, layers=layers, hkv=hkv, hd=128, seed=recent)
+
+
 def test_evict_strides_and_what_lies_behind(PE):
     """A mass with room behind the table's reach, by strides; places past a stream's end and other streams' pages as they were."""
     g = torch.Generator(device="cuda").manual_seed(7)
@@ -328,6 +335,23 @@ def test_evict_bad_pages_and_lengths(PE, cuda_lib):
         PE.evict_positions(pool, ints([[0, 1, 2, 3]]), ints([n]), mass, 32, recent=4)
         torch.cuda.synchronize()
         assert cuda_lib.sn_device_status(1, None) == -1
+
+
+def test_evict_bad_pages_of_many_moves(PE, cuda_lib):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    tab, total = table([1600], 16, g)
+    pool = torch.randn(1, 2, total, 1, 16, 64, device="cuda", generator=g).to(BF16)
+    mass = torch.rand(1, 1, 1, 1600, device="cuda", generator=g)
+    want = evict_truth(pool, tab, [1600], mass, 512, 64, 0)
+    hidden, seen = tab[0, 0].item(), tab[0, 31].item()  # a page that stays, the page of the newest places
+    tab[0, 0] = total + 5
+    before = pool.clone()
+    assert cuda_lib.sn_device_status(1, None) == 0
+    PE.evict_positions(pool, tab, ints([1600]), mass, 512, recent=64)
+    torch.cuda.synchronize()
+    assert cuda_lib.sn_device_status(1, None) == -1
+    assert torch.equal(pool[:, :, hidden], before[:, :, hidden])
+    assert torch.equal(pool[:, :, seen], want[0][:, :, seen])
 
 
 def test_evict_twice_keeps_the_newest(PE):
