@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 // bounds, and choices, a CTA a row, bound by the chain of its steps.  In one
 // launch, a cluster of 8 CTAs a row with the scores in shared memory, exchanges
 // of a few kilobytes between the CTAs took 2 to 3 us each (22 us for the three
-// streams; now 16.4, about 7 of them the scores of 31 MB of bounds, and 14.9 for
+// streams; now 15.4, about 7 of them the scores of 31 MB of bounds, and 14.6 for
 // 48 streams of up to 8000 positions).
 // ---------------------------------------------------------------------------
 constexpr int kFewExact = 64;        // blocks that are ranked by comparing all of them
@@ -227,7 +227,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 template <int HD>
 __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams p) {
   constexpr int KC = HD / 32;  // chunks a lane takes of a row
-  pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   for (int row = blockIdx.y; row < p.batch * p.hkv; row += gridDim.y) {
@@ -305,6 +304,7 @@ __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams
       }
     }
   }
+  pdl_launch_dependents();  // not before: a CTA of the choice takes half an SM or all of it (3 long streams 17.4 -> 17.1 us)
 }
 
 // The key of one block's score in 64 bits; a warp.
