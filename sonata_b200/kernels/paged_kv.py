@@ -406,24 +406,40 @@ class PagedKVCache:
     def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> list[int]:
         """Cuts every stream with more than `keep` positions down to `keep`, by the
         weights of track_mass (paged_evict.evict_positions); returns the slots that
-        were cut.  Pages that another stream shares are copied first; nothing is
-        changed if there are not enough free ones for that."""
+        were cut.  Pages that another stream shares are copied first.  Where too few
+        are free for all copies, the streams that need the fewest are cut first and
+        the pages that they leave serve the others; streams for which that is not
+        enough stay as they are (OutOfPages if those are all: nothing was changed)."""
         if self.mass is None:
             raise RuntimeError("eviction goes by the positions' weights: track_mass() before the first token")
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"keep must be positive and cover recent and sinks, which must not be negative: got {keep}, {recent}, {sinks}")
-        cut = [s for s, n in enumerate(self.lens) if n > keep]
-        if not cut:
-            return []
+        left = [s for s, n in enumerate(self.lens) if n > keep]
         stay = -(-keep // self.page_size)  # pages of a cut stream, all of which may be written
-        users, own = list(self._users), []  # (slot, place) of the pages that become copies
-        for s in cut:
-            for i, p in enumerate(self.pages[s][:stay]):
-                if users[p] > 1:
-                    users[p] -= 1
+        cut, need = [], 0
+        while left:
+            now, own, users = [], [], list(self._users)  # streams that can be cut at once, (slot, place) of their pages that become copies
+            shared = lambda s: [i for i, p in enumerate(self.pages[s][:stay]) if users[p] > 1]
+            for s in sorted(left, key=lambda s: len(shared(s))):
+                mine = shared(s)
+                if len(own) + len(mine) > len(self._free):
+                    need = need or len(own) + len(mine)
+                    continue
+                for i in mine:
+                    users[self.pages[s][i]] -= 1
                     own.append((s, i))
-        if len(own) > len(self._free):
-            raise OutOfPages(f"out of pages: {len(own)} needed, {len(self._free)} free")
+                now.append(s)
+            if not now:
+                break
+            left = [s for s in left if s not in now]
+            self._evict(now, own, left, keep, recent, sinks)
+            cut += now
+        if left and not cut:
+            raise OutOfPages(f"out of pages: {need} needed, {len(self._free)} free")
+        return sorted(cut)
+
+    def _evict(self, cut, own, left, keep: int, recent: int, sinks: int) -> None:
+        """Cuts the streams `cut`, whose pages `own` (slot, place) become copies; those of `left` are over `keep`, too, and stay."""
         src = [self.pages[s][i] for s, i in own]
         dst = [self._take() for _ in own]
         if own:
@@ -432,8 +448,11 @@ class PagedKVCache:
                 self._drop(self.pages[s][i])
                 self.pages[s][i] = p
             self._upload({s for s, _ in own})
+        lens = self.seq_lens if not left else torch.tensor([0 if s in left else n for s, n in enumerate(self.lens)], dtype=torch.int32,
+                                                           device=self.pool.device)
         from . import paged_evict
-        paged_evict.evict_positions(self.pool, self.page_table, self.seq_lens, self.mass, keep, recent=recent, sinks=sinks)
+        paged_evict.evict_positions(self.pool, self.page_table, lens, self.mass, keep, recent=recent, sinks=sinks)
+        stay = -(-keep // self.page_size)
         for s in cut:
             for p in self.pages[s][stay:]:
                 self._drop(p)
@@ -442,7 +461,6 @@ class PagedKVCache:
         self._upload(cut)
         if self.bounds is not None:
             self._bound([keep if s in cut else 0 for s in range(len(self.lens))])
-        return cut
 
     def compact(self) -> int:
         """Moves used pages to the lowest numbers; returns how many moved.  (The

@@ -59,7 +59,9 @@ class RaggedZonos:
         self.cos, self.sin = PK.rotary_table(max_len, cfg.head_dim)
         self.workspace = PK.decode_workspace(self.slots, cfg.num_heads, cfg.head_dim)
         self.budget, self.recent, self.sinks, self.attend_blocks = budget, recent, sinks, attend_blocks
-        self.seen = [0] * self.slots  # positions of each stream; no more than the budget and four pages of them are cached
+        # positions of each stream; with a budget, no more than that and four pages of them are cached, unless streams share
+        # pages and there are none free to take them apart
+        self.seen = [0] * self.slots
         if budget is not None:
             self.cache.track_mass()
             self.workspace = PE.mass_workspace(max(self.slots, self.OBSERVE), cfg.num_heads, cfg.num_heads_kv, cfg.head_dim,
@@ -88,7 +90,7 @@ class RaggedZonos:
         if self.budget is not None and max(self.cache.lens) >= self.budget + 4 * self.cache.page_size:
             try:
                 self.cache.evict(self.budget, recent=self.recent, sinks=self.sinks)
-            except PK.OutOfPages:  # no free pages to take shared ones apart: nothing was cut, the next step tries again
+            except PK.OutOfPages:  # no free pages to take shared ones apart: what is left uncut is tried again by the next step
                 pass
 
     def _weigh(self, layer: int, slot: int, q: torch.Tensor) -> None:

@@ -220,3 +220,59 @@ def test_budget_refusals():
                 dict(budget=8, recent=4, sinks=5), dict(budget=80, attend_blocks=8), dict(budget=80, max_len=PE.EVICT_MOST + 1)):
         with pytest.raises(ValueError):
             serve.RaggedZonos(None, num_pages=9, **{"max_len": 100, **bad})
+
+
+def kept(old, keep, recent):
+    """The values of a stream cut to `keep`, by the weights that write() gives layer 1 (in any order)."""
+    free = sorted(old[:len(old) - recent], key=lambda v: -(v * 53 % 103))
+    return sorted(free[:keep - recent] + old[len(old) - recent:])
+
+
+@pytest.mark.parametrize("bounds", [False, True])
+def test_a_cut_that_needs_no_pages_goes_first(cpu, bounds):
+    """No free page, two streams that share all of theirs and one that shares none: its pages serve the others' copies."""
+    c, update = make(pages=15, bounds=bounds), cpu if bounds else None
+    write(c, 1, [float(i + 1) for i in range(28)], update)
+    c.fork(1, 0)
+    write(c, 2, [float(i + 40) for i in range(29)], update)
+    assert c.free_pages == 0
+    before = [read(c, s) for s in range(3)]
+    assert c.evict(8, 4) == [0, 1, 2] and c.lens == [8, 8, 8, 0] and c.free_pages == 15 - 6
+    consistent(c)
+    for s in range(3):
+        assert sorted(read(c, s)) == kept(before[s], 8, 4) and read(c, s)[4:] == before[s][-4:]
+
+
+def test_streams_without_pages_for_their_copies_are_left(cpu):
+    c = make(pages=15)
+    write(c, 1, [float(i + 1) for i in range(28)])
+    c.fork(1, 0)
+    write(c, 2, [float(i + 40) for i in range(29)])
+    before, mass = [read(c, s) for s in range(3)], c.mass.clone()
+    assert c.evict(24, 4) == [2] and c.lens == [28, 28, 24, 0] and c.free_pages == 2  # six copies for either of the others
+    consistent(c)
+    assert [read(c, 0), read(c, 1)] == before[:2] and torch.equal(c.mass[:, :2], mass[:, :2])
+    assert sorted(read(c, 2)) == kept(before[2], 24, 4)
+    with pytest.raises(PK.OutOfPages):  # nothing that can be cut
+        c.evict(24, 4)
+    consistent(c)
+    assert c.lens == [28, 28, 24, 0]
+    c.free(2)
+    assert c.evict(24, 4) == [0, 1] and c.lens == [24, 24, 0, 0]
+    consistent(c)
+    for s in range(2):
+        assert sorted(read(c, s)) == kept(before[s], 24, 4)
+
+
+def test_budget_of_a_stream_beside_shared_ones(cpu):
+    """RaggedZonos: a stream of pages of its own is cut although others, which share theirs, would need free ones."""
+    from sonata_b200.kernels import serve
+    r = object.__new__(serve.RaggedZonos)
+    r.budget, r.recent, r.sinks, r.cache = 20, 4, 1, make(pages=24)
+    write(r.cache, 0, [1.0] * 40)
+    r.cache.fork(0, 1)
+    write(r.cache, 2, [2.0] * 56)
+    assert r.cache.free_pages == 0
+    r._cut()
+    assert r.cache.lens == [20, 20, 20, 0]
+    r.cache.reserve([1, 1, 1, 0])
