@@ -643,7 +643,8 @@ int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_by
  *   max over the head's query heads of sum_d max(q_d least_d, q_d greatest_d),
  * the lowest blocks among equal ones, all of them if there are no more than
  * count; -1 behind.  Scores are sums of exact products in 64 bits; a block with
- * a bound that is not finite is above the others.  workspace:
+ * a bound that is not finite is above the others, and all blocks rank alike where
+ * an element of one of the head's queries is not finite.  workspace:
  * sn_select_blocks_workspace_size bytes, 16-byte aligned, whatever they hold.
  * max_pages <= 262144.
  *

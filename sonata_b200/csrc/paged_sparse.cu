@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 // are listed in ascending order, -1 behind.  The products of two bf16 values are
 // exact, and scores are compared as their sums in 64 bits, so the choice does
 // not depend on the order of a sum; a block with a bound that is not finite
-// ranks above all.
+// ranks above all, and so do all blocks for a head with a query that is not.
 //
 // Sums of all blocks in 64 bits would be bound by the conversions and by shared
 // memory (3 streams of up to 100001 positions, pages of 16: 66 us where reading
@@ -334,24 +334,36 @@ __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, in
       for (int h = 0; h < 4; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
     }
 #pragma unroll
-    for (int h = 0; h < 4; ++h) best = max(best, order_key(sum[h]));
+    for (int h = 0; h < 4; ++h) {
+      best = max(best, order_key(sum[h]));
+      odd |= !(fabs(sum[h]) < INFINITY);  // of finite values none comes near
+    }
   }
   return __any_sync(0xffffffffu, odd) ? ~0ull : best;
 }
 
-// The keys of eight blocks' scores in 64 bits, four lanes a block (block < 0: none); a warp, head_dim a multiple of 32, bounds
+// Whether an element of the queries of a key/value head is not finite; all threads, the same in all of them.
+__device__ __noinline__ bool odd_query(const SelectParams& p, int b, int hk) {
+  const int group = p.hq / p.hkv;
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh);
+  bool odd = false;
+  for (int h = 0; h < group; ++h)
+    for (int d = threadIdx.x; d < p.hd; d += blockDim.x) odd |= (q[h * p.qh + d] & 0x7f80u) == 0x7f80u;
+  return __syncthreads_or(odd);
+}
+
+// The keys of eight blocks' scores in 64 bits, four lanes a block (block < 0: none), all the highest if `odd`; a warp, head_dim a multiple of 32, bounds
 // on 16 bytes.  For many of them: a bf16 value's bits moved into the upper word of a double are that value times 2^-896,
 // subnormal ones too, so that no conversions (16 a cycle and SM) bind; with q times 2^1023 more, which leaves the order as it is,
 // products and sums, multiples of 2^-266 times 2^-769, are held exactly.  Out of line, as are the few other steps that most
 // calls do not take: what is taken runs once a CTA, and waits for its instructions (16 -> 19 us with all of it inline).
-__device__ __noinline__ uint64_t exact_scores(const SelectParams& p, int b, int hk, int block) {
+__device__ __noinline__ uint64_t exact_scores(const SelectParams& p, int b, int hk, int block, bool odd) {
   const int t = threadIdx.x & 3, group = p.hq / p.hkv;
   const int pg = block < 0 ? -1 : page_of(p.map, b, block);
   const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(max(pg, 0)) * p.hkv + hk) * 2 * p.hd;
   const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh);
   auto widen = [](uint32_t u) { return __hiloint2double(static_cast<int>((u & 0x8000u) << 16 | (u & 0x7fffu) << 13), 0); };
   uint64_t best = 0;
-  bool odd = false;
   for (int h0 = 0; h0 < group; h0 += 4) {
     double sum[4] = {0., 0., 0., 0.};
     for (int k = t; k < p.hd / 8; k += 4) {
@@ -596,9 +608,10 @@ __global__ void __launch_bounds__(kChooseThreads, kPerSM) choose_blocks_kernel(c
           if (better >= wanted) atomicAnd(&s_open[at[tid] / 32], ~(1u << (at[tid] & 31)));
         }
       } else {
+        const bool odd = odd_query(p, b, hk);  // its widened bits would pass for numbers
         for (uint32_t i = 8 * warp; i < all_open; i += 8 * kChooseWarps) {
           const uint32_t k = i + lane / 4;
-          const uint64_t key = exact_scores(p, b, hk, k < all_open ? p.first + at[k] : -1);
+          const uint64_t key = exact_scores(p, b, hk, k < all_open ? p.first + at[k] : -1, odd);
           if (k < all_open && (lane & 3) == 0) exact[k] = key;
         }
         __syncthreads();

@@ -81,7 +81,9 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tenso
     and last `last` blocks, and of the others those with the highest score, the
     lowest among equal ones (all of them where there are no more than `count`).
     A block's score is the greatest over the key/value head's query heads of
-    sum_d max(q_d least_d, q_d greatest_d), no less than any q . k in it.
+    sum_d max(q_d least_d, q_d greatest_d), no less than any q . k in it; one
+    with a bound that is not finite is above all, and with a query that is not
+    finite all of the head's blocks are alike.
     q [batch, nheads, head_dim] by batch and head strides."""
     if stream is None:
         r = fast().select(q, bounds, page_table, seq_lens, page_size, count, first, last)

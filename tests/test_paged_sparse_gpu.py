@@ -463,3 +463,26 @@ def test_select_with_blocks_that_have_no_score(PS, hd, odd):
             else:  # finite, but not in 32 bits
                 bounds[pg, i % 2, :, :] = (bounds[pg, i % 2].float().sign() * 3e38).to(BF16)
     select_case(PS, [16 * 400, 16 * 90], 40, 1, 2, hq=8, hkv=2, hd=hd, make=make, seed=odd)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96, 40])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("hq,nb", [(2, 40), (8, 40), (10, 40), (8, 500), (24, 500)])
+def test_select_with_a_query_that_is_not_finite(PS, hd, value, hq, nb):
+    """All blocks of its key/value head rank alike, whatever number of them is compared: the lowest ones are listed."""
+    def make(q, bounds, tab):
+        q[0, hq // 2 - 1, hd // 2] = value
+        bounds[::5, 0, :, hd // 2] = 0.0
+
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    tab, total = table([16 * nb, 16 * nb - 3], 16, g)
+    a, c = (torch.randn(total, 2, hd, device="cuda", generator=g) for _ in range(2))
+    bounds = torch.stack([torch.minimum(a, c), torch.maximum(a, c)], 2).to(BF16)
+    q = torch.randn(2, hq, hd, device="cuda", generator=g).to(BF16)
+    make(q, bounds, tab)
+    lens = [16 * nb, 16 * nb - 3]
+    got = PS.select_blocks(q, bounds, tab, ints(lens), 16, 12, first=1, last=2)
+    want = select_truth(q, bounds, tab, lens, 16, 12, 1, 2)
+    want[0, 0] = ints([*range(10), nb - 2, nb - 1])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
