@@ -642,9 +642,10 @@ int sn_copy_pages(void *pool, int64_t outer_stride_bytes, int64_t page_stride_by
  * stream b, and of the others those with the highest
  *   max over the head's query heads of sum_d max(q_d least_d, q_d greatest_d),
  * the lowest blocks among equal ones, all of them if there are no more than
- * count; -1 behind.  Scores are sums of exact products in 64 bits; a block with
- * a bound that is not finite is above the others, and all blocks rank alike where
- * an element of one of the head's queries is not finite.  workspace:
+ * count; -1 behind.  Scores are sums of exact products in 64 bits, added in one
+ * order; a block with a bound that is not finite is above the others, and all
+ * blocks rank alike where an element of one of the head's queries is not finite.
+ * workspace:
  * sn_select_blocks_workspace_size bytes, 16-byte aligned, whatever they hold.
  * max_pages <= 262144.
  *

@@ -161,8 +161,10 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 //   sum_d max(q_d least_d, q_d greatest_d) = sum_d min(q_d, 0) least_d + max(q_d, 0) greatest_d;
 // the first `first` and last `last` blocks and the highest scores of the others
 // are listed in ascending order, -1 behind.  The products of two bf16 values are
-// exact, and scores are compared as their sums in 64 bits, so the choice does
-// not depend on the order of a sum; a block with a bound that is not finite
+// exact, and scores are compared as their sums in 64 bits, which are added in
+// one order wherever it is done (elements d mod 32 by rising d, then these 32 in
+// pairs of neighbours): where terms span more than 53 bits and a sum rounds, the
+// choice is the same all the same.  A block with a bound that is not finite
 // ranks above all, and so do all blocks for a head with a query that is not.
 //
 // Sums of all blocks in 64 bits would be bound by the conversions and by shared
@@ -177,7 +179,8 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 //   be chosen.  Blocks whose s is more than 2 E above that bin are chosen, more
 //   than 2 E below it are not: their scores lie on the same side of the last
 //   chosen one's.  The few between get their sums in 64 bits and are ranked, by
-//   comparing all of them.
+//   comparing all of them.  (A sum's rounding in 64 bits, 2^-46 S at most, is
+//   far within what is left of E.)
 // * A block whose absolute sum is not finite has no s to go by: such blocks are
 //   always among those between, and the bin above which blocks are chosen for
 //   certain is the one that would be if they all were.
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(128, 4) block_scores_kernel(const SelectParams
   pdl_launch_dependents();  // not before: a CTA of the choice takes half an SM or all of it (3 long streams 17.4 -> 17.1 us)
 }
 
-// The key of one block's score in 64 bits; a warp.
+// The key of one block's score in 64 bits; a warp, lane l the elements l mod 32.
 __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, int hk, int block) {
   const int lane = threadIdx.x & 31, group = p.hq / p.hkv;
   const int pg = page_of(p.map, b, block);
@@ -329,7 +332,7 @@ __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, in
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 1; o < 32; o <<= 1) {
 #pragma unroll
       for (int h = 0; h < 4; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
     }
@@ -342,55 +345,68 @@ __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, in
   return __any_sync(0xffffffffu, odd) ? ~0ull : best;
 }
 
-// Whether an element of the queries of a key/value head is not finite; all threads, the same in all of them.
-__device__ __noinline__ bool odd_query(const SelectParams& p, int b, int hk) {
-  const int group = p.hq / p.hkv;
+// The keys of scores in 64 bits of blocks first + at[k], k < many, to keys[k]: for many of them, a warp eight blocks, four lanes a
+// block, kHeads query heads at a time; head_dim 64 or 128, bounds on 16 bytes, all threads.  A bf16 value's bits moved into the
+// upper word of a double are that value times 2^-896, subnormal ones too, so that no conversions (16 a cycle and SM) bind; with q
+// times 2^1023 more, which leaves the order as it is, the products, multiples of 2^-266 times 2^-769, are held exactly, and
+// no sum of them needs a bit below what a double has.  Added in exact_score's order: lane t has the elements 8 t .. 8 t + 7 mod 32.
+// Out of line, as are the few other steps that most calls do not take: what is taken runs once a CTA, and waits for its
+// instructions (16 -> 19 us with all of it inline).
+// 6251 blocks of a row that are all equal: 303 us; 512 rows of 500: 100.
+template <int T, int kHeads>
+__device__ __noinline__ void exact_scores(const SelectParams& p, int b, int hk, const int* at, uint32_t many, uint64_t* keys,
+                                          SelectShared<T>& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, group = p.hq / p.hkv;
   const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh);
-  bool odd = false;
-  for (int h = 0; h < group; ++h)
-    for (int d = threadIdx.x; d < p.hd; d += blockDim.x) odd |= (q[h * p.qh + d] & 0x7f80u) == 0x7f80u;
-  return __syncthreads_or(odd);
-}
-
-// The keys of eight blocks' scores in 64 bits, four lanes a block (block < 0: none), all the highest if `odd`; a warp, head_dim a multiple of 32, bounds
-// on 16 bytes.  For many of them: a bf16 value's bits moved into the upper word of a double are that value times 2^-896,
-// subnormal ones too, so that no conversions (16 a cycle and SM) bind; with q times 2^1023 more, which leaves the order as it is,
-// products and sums, multiples of 2^-266 times 2^-769, are held exactly.  Out of line, as are the few other steps that most
-// calls do not take: what is taken runs once a CTA, and waits for its instructions (16 -> 19 us with all of it inline).
-__device__ __noinline__ uint64_t exact_scores(const SelectParams& p, int b, int hk, int block, bool odd) {
-  const int t = threadIdx.x & 3, group = p.hq / p.hkv;
-  const int pg = block < 0 ? -1 : page_of(p.map, b, block);
-  const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(max(pg, 0)) * p.hkv + hk) * 2 * p.hd;
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q + b * p.qb + static_cast<int64_t>(hk) * group * p.qh);
+  double* const s_q = reinterpret_cast<double*>(s.hist);  // [kHeads][hd], over the histogram, which is done with
+  static_assert(sizeof(s.hist) >= kHeads * 128 * sizeof(double));
   auto widen = [](uint32_t u) { return __hiloint2double(static_cast<int>((u & 0x8000u) << 16 | (u & 0x7fffu) << 13), 0); };
-  uint64_t best = 0;
-  for (int h0 = 0; h0 < group; h0 += 4) {
-    double sum[4] = {0., 0., 0., 0.};
-    for (int k = t; k < p.hd / 8; k += 4) {
-      uint32_t l[4], g[4];
-      *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(lo + 8 * k);
-      *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(lo + p.hd + 8 * k);
+  auto odd_bits = [](uint32_t u) { return (u & 0x7f80u) == 0x7f80u; };
+  for (int h0 = 0; h0 < group; h0 += kHeads) {
+    bool odd_query = false;  // its widened bits would pass for numbers
+    __syncthreads();         // the histogram, or the last heads' queries, have been read
+    for (int i = threadIdx.x; i < kHeads * p.hd; i += T) {
+      const uint32_t v = q[min(h0 + i / p.hd, group - 1) * p.qh + i % p.hd];
+      s_q[i] = widen(v) * 0x1p1023;
+      odd_query |= odd_bits(v);
+    }
+    odd_query = __syncthreads_or(odd_query);
+    for (uint32_t i = 8 * warp; i < many; i += 8 * (T / 32)) {
+      const uint32_t k = i + lane / 4;
+      const int pg = k < many ? page_of(p.map, b, p.first + at[k]) : -1;
+      const __nv_bfloat16* lo = p.bounds + (static_cast<int64_t>(max(pg, 0)) * p.hkv + hk) * 2 * p.hd;
+      double sum[kHeads][8] = {};
+      bool odd = odd_query;
+      for (int c = 8 * t; c < p.hd; c += 32) {
+        uint32_t l[4], g[4];
+        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(lo + c);
+        *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(lo + p.hd + c);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t wl = j & 1 ? l[j / 2] >> 16 : l[j / 2] & 0xffffu, wg = j & 1 ? g[j / 2] >> 16 : g[j / 2] & 0xffffu;
-        odd |= (wl & 0x7f80u) == 0x7f80u || (wg & 0x7f80u) == 0x7f80u;
-        const double least = widen(wl), greatest = widen(wg);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t wl = j & 1 ? l[j / 2] >> 16 : l[j / 2] & 0xffffu, wg = j & 1 ? g[j / 2] >> 16 : g[j / 2] & 0xffffu;
+          odd |= odd_bits(wl) || odd_bits(wg);
+          const double least = widen(wl), greatest = widen(wg);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const uint32_t v = q[min(h0 + h, group - 1) * p.qh + 8 * k + j];
-          sum[h] = fma(widen(v) * 0x1p1023, v >> 15 ? least : greatest, sum[h]);
+          for (int h = 0; h < kHeads; ++h) {
+            const double v = s_q[h * p.hd + c + j];
+            sum[h][j] = fma(v, __double2hiint(v) < 0 ? least : greatest, sum[h][j]);
+          }
         }
       }
-    }
+      uint64_t best = 0;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-      best = max(best, order_key(sum[h]));
+      for (int h = 0; h < kHeads; ++h) {
+        const double* x = sum[h];
+        double all = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        all += __shfl_xor_sync(0xffffffffu, all, 1);
+        all += __shfl_xor_sync(0xffffffffu, all, 2);
+        best = max(best, order_key(all));
+      }
+      if (__ballot_sync(0xffffffffu, odd) >> (lane & 28) & 15) best = ~0ull;
+      if (pg < 0) best = 0;
+      if (t == 0 && k < many) keys[k] = h0 > 0 ? max(best, keys[k]) : best;
     }
   }
-  odd = __ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 28) & 15;
-  return pg < 0 ? 0 : odd ? ~0ull : best;
 }
 
 // Scores in 64 bits of all blocks, a warp a block: any head_dim and alignment.
@@ -608,12 +624,7 @@ __global__ void __launch_bounds__(kChooseThreads, kPerSM) choose_blocks_kernel(c
           if (better >= wanted) atomicAnd(&s_open[at[tid] / 32], ~(1u << (at[tid] & 31)));
         }
       } else {
-        const bool odd = odd_query(p, b, hk);  // its widened bits would pass for numbers
-        for (uint32_t i = 8 * warp; i < all_open; i += 8 * kChooseWarps) {
-          const uint32_t k = i + lane / 4;
-          const uint64_t key = exact_scores(p, b, hk, k < all_open ? p.first + at[k] : -1, odd);
-          if (k < all_open && (lane & 3) == 0) exact[k] = key;
-        }
+        exact_scores<kChooseThreads, (kPerSM > 2 ? 2 : 4)>(p, b, hk, at, all_open, exact, s_sel);
         __syncthreads();
         choose_exact(exact, static_cast<int>(all_open), wanted, s_won, s_sel);
         __syncthreads();

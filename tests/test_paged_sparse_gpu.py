@@ -486,3 +486,30 @@ def test_select_with_a_query_that_is_not_finite(PS, hd, value, hq, nb):
     want[0, 0] = ints([*range(10), nb - 2, nb - 1])
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96, 40])
+@pytest.mark.parametrize("nb,count", [(50, 20), (300, 100), (1500, 700)])
+def test_select_where_64_bits_round(PS, hd, nb, count):
+    """Sums whose terms span more than 53 bits: each block has the same terms at other places, so that only the rounding of the
+    sums tells them apart, and it is that of one order whatever number of blocks is compared: elements d mod 32, then those sums
+    in pairs of neighbours."""
+    g = torch.Generator(device="cuda").manual_seed(nb + hd)
+    terms = torch.randn(hd, device="cuda", generator=g) * 2.0 ** torch.randint(0, 70, (hd,), device="cuda", generator=g)
+    place = torch.rand(nb, 2, hd, device="cuda", generator=g).argsort(-1)
+    bounds = terms.to(BF16)[place][:, :, None].expand(-1, -1, 2, -1).contiguous()
+    q = torch.tensor([1.0, -2.0, 0.5, -1.0], device="cuda").to(BF16).view(1, 4, 1).expand(1, 4, hd).contiguous()
+    x = bounds[:, :, 0].double()[:, :, None] * q.view(2, 2, hd).double()  # [nb, hkv, group, hd]
+    x = torch.nn.functional.pad(x, (0, -hd % 32)).unflatten(-1, (-1, 32))
+    s = torch.zeros_like(x[..., 0, :])
+    for i in range(x.shape[-2]):
+        s = s + x[..., i, :]
+    for _ in range(5):
+        s = s[..., ::2] + s[..., 1::2]
+    score = s[..., 0].amax(-1)
+    assert score[:, 0].unique().numel() > 2  # the order does matter
+    tab = torch.arange(nb, device="cuda", dtype=torch.int32)[None]
+    got = PS.select_blocks(q, bounds, tab, ints([16 * nb]), 16, count, first=0, last=0)
+    for h in range(2):
+        v = score[:, h].tolist()
+        assert got[0, h].tolist() == sorted(sorted(range(nb), key=lambda i: (-v[i], i))[:count])
