@@ -494,23 +494,51 @@ __global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const Evict
   }
 }
 
+// The launch of the moves, in clusters of C.
+struct MoveLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  MoveLaunch(int rows, int C, cudaStream_t st) {
+    cfg.gridDim = dim3(static_cast<unsigned>(rows) * C);
+    cfg.blockDim = dim3(kMoveThreads);
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(C);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+  MoveLaunch(const MoveLaunch&) = delete;
+};
+
+// Whether the current device takes clusters of kMoveCluster: it need not (above 8 they are not portable), and has to be asked
+// before the plan is launched, which has moved the masses when the moves are.
+template <typename T, int NU>
+bool large_moves() {
+  static signed char known[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return false;
+  }
+  if (known[dev] == 0) {
+    const MoveLaunch one(1, kMoveCluster, nullptr);
+    int fit = 0;
+    const bool yes = large_clusters<evict_move_kernel<T, NU>>() &&
+                     cudaOccupancyMaxActiveClusters(&fit, evict_move_kernel<T, NU>, &one.cfg) == cudaSuccess && fit > 0;
+    cudaGetLastError();
+    known[dev] = yes ? 1 : -1;
+  }
+  return known[dev] > 0;
+}
+
 template <typename T, int NU>
 int launch_move(int rows, int C, cudaStream_t st, const EvictParams& p) {
-  if (C > 8 && !large_clusters<evict_move_kernel<T, NU>>()) return SN_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows) * C);
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(C);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, evict_move_kernel<T, NU>, p) != cudaSuccess) {
+  const MoveLaunch l(rows, C, st);
+  if (cudaLaunchKernelEx(&l.cfg, evict_move_kernel<T, NU>, p) != cudaSuccess) {
     cudaGetLastError();
     return SN_ERR_LAUNCH;
   }
@@ -521,6 +549,26 @@ template <int T>
 int launch_plan(int rows, size_t smem, cudaStream_t st, const EvictParams& p) {
   if (!smem_room<evict_plan_kernel<T>>(kEvictWords * 4)) return SN_ERR_LAUNCH;
   return launch(evict_plan_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(T), smem, st, true, p);
+}
+
+// Both launches; the moves by units of T, NU of them in a position's two rows (0: as row_bytes says).
+template <typename T, int NU>
+int evict(int r, size_t smem, cudaStream_t st, const EvictParams& p) {
+  const int64_t rows = r, room = static_cast<int64_t>(p.map.max_pages) * p.map.page_size;
+  // three CTAs fit on an SM, one beside a plan: all of them start at once (48 rows, 320 moved rows each, 8 CTAs a row 18.3, 7
+  // 16.6); two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM of its own (4
+  // rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)
+  const int C = rows * kMoveCluster <= sm_count() && large_moves<T, NU>()
+                    ? kMoveCluster
+                    : static_cast<int>(std::clamp<int64_t>((3 * sm_count() - 2 * rows) / rows, 2, 8));
+  // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
+  // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512,
+  // and where there are more than two an SM, 256, four CTAs an SM, whose moves fill the waits of one another's plans (4096 rows
+  // of 2112: 191 -> 144, 768 rows 41 -> 35, 144 of them with work 18.4 -> 19.8, 480 of 9000 129 -> 125)
+  const int rc = rows > 2 * sm_count()                 ? launch_plan<256>(r, smem, st, p)
+                 : rows <= sm_count() && room > 4096 ? launch_plan<1024>(r, smem, st, p)
+                                                     : launch_plan<512>(r, smem, st, p);
+  return rc != SN_OK ? rc : launch_move<T, NU>(r, C, st, p);
 }
 
 }  // namespace
@@ -581,25 +629,12 @@ int sn_evict_positions(void* pool, int layers, int num_pages, int page_size, int
   const size_t smem = static_cast<size_t>(sn::bit_words(room) + p.held) * sizeof(uint32_t);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int r = static_cast<int>(rows);
-  // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
-  // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512,
-  // and where there are more than two an SM, 256, four CTAs an SM, whose moves fill the waits of one another's plans (4096 rows
-  // of 2112: 191 -> 144, 768 rows 41 -> 35, 144 of them with work 18.4 -> 19.8, 480 of 9000 129 -> 125)
-  const int rc = rows > 2 * sn::sm_count()                   ? sn::launch_plan<256>(r, smem, st, p)
-                 : rows <= sn::sm_count() && room > 4096 ? sn::launch_plan<1024>(r, smem, st, p)
-                                                         : sn::launch_plan<512>(r, smem, st, p);
-  if (rc != SN_OK) return rc;
-  // three CTAs fit on an SM, one beside a plan: all of them start at once (48 rows, 320 moved rows each, 8 CTAs a row 18.3, 7
-  // 16.6); two a row at least, as not all of the streams may be cut.  Clusters of 16 where each CTA has an SM of its own (4
-  // rows of 30011 positions 41 -> 33 us; 24 rows of 2112, 2.6 CTAs an SM: 16.3 -> 21)
-  const int C = rows * sn::kMoveCluster <= sn::sm_count() ? sn::kMoveCluster
-                                                          : static_cast<int>(std::clamp<int64_t>((3 * sn::sm_count() - 2 * rows) / rows, 2, 8));
   if (p.units) {
-    if (head_dim == 128) return sn::launch_move<uint4, 32>(r, C, st, p);
-    if (head_dim == 64) return sn::launch_move<uint4, 16>(r, C, st, p);
-    return sn::launch_move<uint4, 0>(r, C, st, p);
+    if (head_dim == 128) return sn::evict<uint4, 32>(r, smem, st, p);
+    if (head_dim == 64) return sn::evict<uint4, 16>(r, smem, st, p);
+    return sn::evict<uint4, 0>(r, smem, st, p);
   }
-  return sn::launch_move<uint16_t, 0>(r, C, st, p);
+  return sn::evict<uint16_t, 0>(r, smem, st, p);
 }
 
 }  // extern "C"
