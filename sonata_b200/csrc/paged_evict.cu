@@ -174,9 +174,16 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_plan_kernel(const EvictPara
           bulk_g2s(keys4 + i, value4 + i, bytes, &s_copied, l2_policy_evict_normal());
         }
       if (tid == 0) mbar_arrive(&s_copied);
-      if (!mbar_wait_bounded(&s_copied, 0)) {
+      bool copied = mbar_wait_bounded(&s_copied, 0);
+      if (!copied) {
         record_status(SN_ERR_TIMEOUT);
         mbar_wait_bounded(&s_copied, 0);  // once more, as the copies land in this CTA's memory
+      }
+      if (__syncthreads_or(!copied)) {  // nothing may be planned by masses that have not come: the row is left as it is
+        if (tid == 0) p.head[row] = make_int2(n, -1);
+        if (source)
+          for (int i = tid; i < keep; i += T) source[i] = i;
+        return;
       }
     }
 #pragma unroll 4

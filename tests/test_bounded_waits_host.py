@@ -47,3 +47,18 @@ def test_whole_warp_waits_do_not_branch_on_a_lane(name):
     for m in re.finditer(r"if \([^;{]*!mbar_wait_bounded\(", code):
         scope = code[max(0, m.start() - 400):m.start()]
         assert "lane == 0" in scope, code[m.start():m.start() + 80]
+
+
+def test_eviction_plans_nothing_by_masses_that_have_not_come():
+    """Every thread of a plan waits for the copied masses: if one's time is up, all of them leave the row, before any of its
+    keys is read.  (Lists made of other bytes would send rows and masses to places out of range.)"""
+    code = _code("paged_evict.cu")
+    waits = list(_waits(code))
+    assert len(waits) == 2 and waits[0].split() == ["bool", "copied", "="] and not waits[1].strip()
+    m = re.search(r"bool copied = mbar_wait_bounded\((?P<args>[^)]*)\);\s*if \(!copied\) \{(?P<again>.*?)\}"
+                  r"\s*if \(__syncthreads_or\(!copied\)\) \{(?P<leave>.*?)return;\s*\}", code, re.S)
+    assert m, "the plan's wait has another form"
+    assert "record_status(SN_ERR_TIMEOUT)" in m["again"] and f"mbar_wait_bounded({m['args']})" in m["again"]
+    assert "p.head[row] = make_int2(n, -1)" in m["leave"] and "mass[" not in m["leave"]
+    before, after = code[:m.start()], code[m.end():]
+    assert "keys4[i]" not in before and "keys4[i]" in after
