@@ -27,6 +27,8 @@ __device__ __forceinline__ int length_of(const PageMap& m, const int* seq_lens, 
   }
   return n;
 }
+// Pages that hold n positions (their sum with a page's size need not fit).
+__device__ __forceinline__ int pages_of(const PageMap& m, int n) { return n > 0 ? (n - 1) / m.page_size + 1 : 0; }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

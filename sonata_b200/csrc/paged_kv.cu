@@ -267,13 +267,17 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
   float* const scores = kKind == kMass ? p.scores + (static_cast<int64_t>(b) * p.hkv * p.sets_per_kv + set) * p.room * p.score_heads +
                                              (h - hk * (p.hq / p.hkv)) % p.heads_per_set
                                        : nullptr;
-  // entries of the list that are read; the host has checked that count pages fit
-  const int steps = kKind == kListed ? min(p.count, (len + p.map.page_size - 1) / p.map.page_size) * p.map.page_size : len;
-  for (int t = warp; t < steps; t += 4) {
-    int blk = t / p.map.page_size;
+  // rows of a page that may count; entries of a list that are read, whose pages fit into the page table's reach.  (Listed steps
+  // without a sign: 64 streams of 64 blocks of 16, head size 96, 481 -> 459 us; all positions would take 2004 for 1990.)
+  const int rows = kKind == kListed ? max(1, min(p.map.page_size, len)) : p.map.page_size;
+  const int steps = kKind == kListed ? min(p.count, pages_of(p.map, len)) * rows : len;
+  using Step = typename std::conditional<kKind == kListed, unsigned, int>::type;
+  for (Step step = warp; step < static_cast<Step>(steps); step += 4) {
+    const int t = static_cast<int>(step);
+    int blk = t / rows;
     if constexpr (kKind == kListed) {
       blk = p.blocks[(static_cast<int64_t>(b) * p.hkv + hk) * p.count + blk];
-      if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + t % p.map.page_size >= len) continue;
+      if (blk < 0 || static_cast<int64_t>(blk) * p.map.page_size + t % rows >= len) continue;
     }
     const int pg = page_of(p.map, b, blk);
     if (pg < 0) {
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(128) paged_decode_rows_kernel(const AttendPara
       if (kKind == kMass && lane == 0) scores[static_cast<int64_t>(t) * p.score_heads] = -INFINITY;
       continue;
     }
-    const int at = t % p.map.page_size;
+    const int at = t % rows;
     const __nv_bfloat16* kr = p.kp + pg * p.ks.page + hk * p.ks.head + at * p.ks.tok;
     const __nv_bfloat16* vr = p.vp + pg * p.vs.page + hk * p.vs.head + at * p.vs.tok;
     float s = 0.f;
@@ -437,7 +441,7 @@ __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kT
 template <Kind kKind>
 __device__ __forceinline__ int stream_tiles(const AttendParams& p, int len) {
   if constexpr (kKind == kListed)
-    return min(p.count, (len + p.map.page_size - 1) / p.map.page_size) * (p.map.page_size / kTile);
+    return min(p.count, pages_of(p.map, len)) * (p.map.page_size / kTile);
   return tiles_of(len);
 }
 constexpr int kAbsent = -2;  // a listed block that does not count, in the place of its page

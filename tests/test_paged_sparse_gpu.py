@@ -513,3 +513,17 @@ def test_select_where_64_bits_round(PS, hd, nb, count):
     for h in range(2):
         v = score[:, h].tolist()
         assert got[0, h].tolist() == sorted(sorted(range(nb), key=lambda i: (-v[i], i))[:count])
+
+
+def test_sparse_page_of_nearly_2_31_positions(PS):
+    """A page so long that its size and a length do not add up in 32 bits: the same bits as with a short one."""
+    page, n = 2**31 - 256, 1000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, rows = (torch.randn(s, device="cuda", generator=g).to(BF16) for s in ((1, 2, 1), (1, 1, n, 1)))
+    k = torch.empty(1, 1, page, 1, device="cuda", dtype=BF16)
+    k[:, :, :n] = rows
+    tab, lens, blocks = ints([[0]]), ints([n]), ints([[[0]]])
+    got = PS.paged_sparse_attention(q, k, k, tab, lens, blocks, return_lse=True)
+    want = PS.paged_sparse_attention(q, rows, rows, tab, lens, blocks, return_lse=True)
+    torch.cuda.synchronize()
+    assert want[0].ne(0).any() and all(torch.equal(a, b) for a, b in zip(got, want))
