@@ -569,7 +569,10 @@ int sn_mamba2_prompt(const void *zxbcdt, int64_t ld, void *conv_state, const voi
  * exponentials, -inf for an empty stream) or NULL.  An empty stream gives
  * zeros.  Scores, weights and sums are fp32; the products of head_dim 64 and
  * 128 take 16 bits of the weights, in two bf16 operands, so an infinity in a v
- * that counts may come out as a NaN.  head_dim <= 256.  workspace: sn_paged_decode_workspace_size bytes,
+ * that counts may come out as a NaN.  head_dim <= 256; max_pages * page_size <
+ * 2^31 (< 2^31 - 3 where positions are taken one by one: other head sizes, pages
+ * of no multiple of 16, rows not on 16 bytes).  workspace:
+ * sn_paged_decode_workspace_size bytes,
  * 16-byte aligned, its first 4 SN_PAGED_DECODE_COUNTERS bytes zero before the
  * first call and left ready for the next, whatever its sizes are; calls that
  * share it must not overlap.

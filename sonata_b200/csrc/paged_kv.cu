@@ -1316,6 +1316,8 @@ int attend(AttendParams p, void* workspace, size_t workspace_bytes, void* stream
       return two ? launch_decode<64, 2, kKind>(grid, st, km, vm, p, sp) : launch_decode<64, 1, kKind>(grid, st, km, vm, p, sp);
     return two ? launch_decode<128, 2, kKind>(grid, st, km, vm, p, sp) : launch_decode<128, 1, kKind>(grid, st, km, vm, p, sp);
   }
+  // (four positions a step, counted in 32 bits)
+  if (kKind != kListed && static_cast<int64_t>(p.map.max_pages) * p.map.page_size > INT32_MAX - 3) return SN_ERR_UNSUPPORTED;
   return launch(paged_decode_rows_kernel<kKind>, dim3(static_cast<unsigned>(p.batch * p.hq)), dim3(128), 0, st, true, p);
 }
 

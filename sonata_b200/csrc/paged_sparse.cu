@@ -104,10 +104,10 @@ __global__ void __launch_bounds__(128) page_bounds_kernel(const BoundsParams p) 
     lo.x = lo.y = lo.z = lo.w = 0x7f807f80u;  // infinities
     hi.x = hi.y = hi.z = hi.w = 0xff80ff80u;
     if (c < pieces) {
-      for (int r0 = group; r0 < rows; r0 += 8 * groups) {  // eight loads in flight, the last row's again past the end
+      for (unsigned r0 = group; r0 < rows; r0 += 8 * groups) {  // eight loads in flight, the last row's again past the end
         uint4 k[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const uint4*>(src + min(r0 + j * groups, rows - 1) * p.ks.tok);
+        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const uint4*>(src + min(r0 + j * groups, rows - 1u) * p.ks.tok);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           lo.x = min2(lo.x, k[j].x), lo.y = min2(lo.y, k[j].y), lo.z = min2(lo.z, k[j].z), lo.w = min2(lo.w, k[j].w);

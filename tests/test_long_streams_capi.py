@@ -121,3 +121,14 @@ def test_append_at(L):
              cu=p, pos=p, cos=p, sin=p, max_pos=64, tokens=5, batch=2, hq=16, hkv=4, hd=128, rot=128, inter=0, stream=None)
     for change, rc in ((dict(pos=None), -1), (dict(qkv=None), -1), (dict(rot=130), -1), (dict(tokens=0), 0), (dict(tokens=0, pos=None), 0)):
         assert L.sn_rotary_paged_append_at(*{**a, **change}.values()) == rc
+
+
+@pytest.mark.parametrize("reach", [2**31 - 1, 2**31 - 3])
+def test_steps_past_2_31(L, reach):
+    """Position by position, four at a time, a step from the last of so many would not fit into 32 bits."""
+    few = dict(hd=1, hq=1, hkv=1, batch=1, qb=1, qh=1, page=reach, mp=1, ts=1, kps=reach, khs=reach, kts=1, vps=reach, vhs=reach, vts=1, mh=reach,
+               mb=reach, wsb=1 << 50)
+    assert mass(L, **few) == -3
+    a = dict(q=p, qb=2048, qh=128, **POOLS, out=p, lse=None, scale=0.1, batch=2, hq=16, hkv=4, hd=128, ws=p, wsb=BIG, stream=None)
+    a.update({k: v for k, v in few.items() if k in a})
+    assert L.sn_paged_decode_attention(*a.values()) == -3
