@@ -13,7 +13,8 @@ a prompt or a fork starts another there.
 
 For long streams, either of two: with ``budget`` the cache of a stream stays
 bounded (its attention adds up the positions' weights, and whenever a stream
-has grown past the budget by some pages, those of little weight leave); with
+has grown past the budget by some pages, those of little weight leave it and
+every other stream over the budget); with
 ``attend_blocks`` a step reads only some of a stream's blocks, which bounds of
 their keys choose (the prompts read all of them).
 
@@ -42,7 +43,9 @@ class RaggedZonos:
         positions for all streams, `max_len` positions at most for one.
 
         `budget`: positions of a stream that stay cached, its first `sinks` and last
-        `recent` among them; it is cut when it has four pages more.  `attend_blocks`:
+        `recent` among them.  As soon as a stream has four pages more, every stream
+        that is over the budget is cut, so when a stream loses positions, and with
+        them its logits, depends on the streams beside it.  `attend_blocks`:
         blocks of page_size positions that a step attends to in each key/value head,
         the first and the last two among them."""
         if budget is not None and (attend_blocks is not None or budget < 1 or min(recent, sinks) < 0 or recent + sinks > budget):

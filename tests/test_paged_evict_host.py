@@ -276,3 +276,18 @@ def test_budget_of_a_stream_beside_shared_ones(cpu):
     r._cut()
     assert r.cache.lens == [20, 20, 20, 0]
     r.cache.reserve([1, 1, 1, 0])
+
+
+def test_streams_over_a_budget_are_cut_together(cpu):
+    """No stream is cut before one has four pages more than the budget; then all that are over it are, and no other."""
+    from sonata_b200.kernels import serve
+    r = object.__new__(serve.RaggedZonos)
+    r.budget, r.recent, r.sinks, r.cache = 8, 4, 1, make()
+    for slot, n in enumerate((9, 23, 8, 3)):
+        write(r.cache, slot, [float(i + 1) for i in range(n)])
+    r._cut()
+    assert r.cache.lens == [9, 23, 8, 3]
+    write(r.cache, 1, [24.0])
+    r._cut()
+    assert r.cache.lens == [8, 8, 8, 3]
+    consistent(r.cache)
