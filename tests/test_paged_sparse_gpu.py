@@ -489,8 +489,8 @@ def test_select_with_a_query_that_is_not_finite(PS, hd, value, hq, nb):
 
 
 @pytest.mark.parametrize("hd", [64, 128, 96, 40])
-@pytest.mark.parametrize("nb,count", [(50, 20), (300, 100), (1500, 700)])
-def test_select_where_64_bits_round(PS, hd, nb, count):
+@pytest.mark.parametrize("nb,count,group", [(50, 20, 2), (300, 100, 2), (1500, 700, 2), (300, 100, 1), (50, 20, 7), (300, 100, 7), (300, 100, 16)])
+def test_select_where_64_bits_round(PS, hd, nb, count, group):
     """Sums whose terms span more than 53 bits: each block has the same terms at other places, so that only the rounding of the
     sums tells them apart, and it is that of one order whatever number of blocks is compared: elements d mod 32, then those sums
     in pairs of neighbours."""
@@ -498,8 +498,8 @@ def test_select_where_64_bits_round(PS, hd, nb, count):
     terms = torch.randn(hd, device="cuda", generator=g) * 2.0 ** torch.randint(0, 70, (hd,), device="cuda", generator=g)
     place = torch.rand(nb, 2, hd, device="cuda", generator=g).argsort(-1)
     bounds = terms.to(BF16)[place][:, :, None].expand(-1, -1, 2, -1).contiguous()
-    q = torch.tensor([1.0, -2.0, 0.5, -1.0], device="cuda").to(BF16).view(1, 4, 1).expand(1, 4, hd).contiguous()
-    x = bounds[:, :, 0].double()[:, :, None] * q.view(2, 2, hd).double()  # [nb, hkv, group, hd]
+    q = torch.tensor([1.0, -2.0, 0.5, -1.0], device="cuda").repeat(group)[:2 * group].to(BF16).view(1, -1, 1).expand(1, -1, hd).contiguous()
+    x = bounds[:, :, 0].double()[:, :, None] * q.view(2, group, hd).double()  # [nb, hkv, group, hd]
     x = torch.nn.functional.pad(x, (0, -hd % 32)).unflatten(-1, (-1, 32))
     s = torch.zeros_like(x[..., 0, :])
     for i in range(x.shape[-2]):
