@@ -571,7 +571,9 @@ int evict(int r, size_t smem, cudaStream_t st, const EvictParams& p) {
   // the plan's passes are shorter with more threads, its barriers longer: 48 rows of 8000 positions 26.5 us with 1024 threads a
   // row and 29.5 with 512, of 4096 both 18.9, of 2112 18.8 and 17.7 (moves included); where there are more rows than SMs, 512,
   // and where there are more than two an SM, 256, four CTAs an SM, whose moves fill the waits of one another's plans (4096 rows
-  // of 2112: 191 -> 144, 768 rows 41 -> 35, 144 of them with work 18.4 -> 19.8, 480 of 9000 129 -> 125)
+  // of 2112: 191 -> 144, 768 rows 41 -> 35, 144 of them with work 18.4 -> 19.8, 480 of 9000 129 -> 125).  That holds while four
+  // plans' keys fit an SM, up to some 11500 positions: of tables of 9000 768 rows take 375 us, with 512 threads 379, but of
+  // 16000 and 30000 675 and 687, with 512 threads 615 and 621
   const int rc = rows > 2 * sm_count()                 ? launch_plan<256>(r, smem, st, p)
                  : rows <= sm_count() && room > 4096 ? launch_plan<1024>(r, smem, st, p)
                                                      : launch_plan<512>(r, smem, st, p);

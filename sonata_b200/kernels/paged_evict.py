@@ -30,7 +30,8 @@ def _mass_size(batch: int, nheads: int, nheads_kv: int, head_dim: int, max_posit
 def mass_workspace(batch: int, nheads: int, nheads_kv: int, head_dim: int, max_positions: int, device="cuda") -> torch.Tensor:
     """The workspace of paged_decode_attention_mass for up to `batch` streams
     whose page tables reach max_positions (max_pages * page_size): zeroed once,
-    kept for every step on one stream of calls."""
+    kept for every step on one stream of calls.  Four bytes a query head and
+    position that the tables reach, whatever the streams' lengths."""
     n = _mass_size(batch, nheads, nheads_kv, head_dim, max_positions)
     if n == 0:
         raise ValueError("every size must be positive, and nheads a multiple of nheads_kv")
