@@ -164,8 +164,9 @@ __global__ void __launch_bounds__(128) page_bounds_rows_kernel(const BoundsParam
 // exact, and scores are compared as their sums in 64 bits, which are added in
 // one order wherever it is done (elements d mod 32 by rising d, then these 32 in
 // pairs of neighbours): where terms span more than 53 bits and a sum rounds, the
-// choice is the same all the same.  A block with a bound that is not finite
-// ranks above all, and so do all blocks for a head with a query that is not.
+// choice still does not depend on which step compares a block.  A block with a
+// bound that is not finite ranks above all, and so do all blocks for a head with
+// a query that is not.
 //
 // Sums of all blocks in 64 bits would be bound by the conversions and by shared
 // memory (3 streams of up to 100001 positions, pages of 16: 66 us where reading
@@ -351,8 +352,8 @@ __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int b, in
 // times 2^1023 more, which leaves the order as it is, the products, multiples of 2^-266 times 2^-769, are held exactly, and
 // no sum of them needs a bit below what a double has.  Added in exact_score's order: lane t has the elements 8 t .. 8 t + 7 mod 32.
 // Out of line, as are the few other steps that most calls do not take: what is taken runs once a CTA, and waits for its
-// instructions (16 -> 19 us with all of it inline).
-// 6251 blocks of a row that are all equal: 303 us; 512 rows of 500: 100.
+// instructions (16 -> 19 us with all of it inline).  6251 equal blocks of a row: 303 us; 512 rows of 500: 100; 2048 rows 538, two heads
+// at a time, as four would spill where a thread has 64 registers (835).
 template <int T, int kHeads>
 __device__ __noinline__ void exact_scores(const SelectParams& p, int b, int hk, const int* at, uint32_t many, uint64_t* keys,
                                           SelectShared<T>& s) {
