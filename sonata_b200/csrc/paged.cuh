@@ -27,8 +27,10 @@ __device__ __forceinline__ int length_of(const PageMap& m, const int* seq_lens, 
   }
   return n;
 }
-// Pages that hold n positions (their sum with a page's size need not fit).
-__device__ __forceinline__ int pages_of(const PageMap& m, int n) { return n > 0 ? (n - 1) / m.page_size + 1 : 0; }
+// Pages that hold n >= 0 positions (their sum with a page's size fits without a sign only).
+__device__ __forceinline__ int pages_of(const PageMap& m, int n) {
+  return static_cast<int>((static_cast<unsigned>(n) + static_cast<unsigned>(m.page_size) - 1u) / static_cast<unsigned>(m.page_size));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
